@@ -438,6 +438,79 @@ TSC_API int tsc_dense_scatter(const void* feat, int32_t elem_bytes, int64_t n, i
                               const int32_t spatial[3] /* host */, int32_t channels_first,
                               void* out, int32_t* status, tsc_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Operators of transformer blocks over the rows of a sparse tensor (no
+ * counterpart in the reference).  Strides are in elements; the last
+ * dimension of every tensor is contiguous.  Sums, norms and softmax
+ * statistics are f32; each output is rounded once to `dtype`.
+ *
+ * out[r][o] = act(sum_i x[r][i] weight[o][i] + bias[o]) + residual[r][o].
+ * x (n, c_in) with row stride x_stride, weight (c_out, c_in) with row stride
+ * w_stride, residual (n, c_out) with row stride r_stride or NULL, bias
+ * (c_out) of bias_dtype or NULL; out (n, c_out) contiguous, no input.
+ * GELU is x Phi(x) with the normal distribution function Phi; GELU_TANH its
+ * tanh form; SILU x / (1 + e^-x).
+ * ------------------------------------------------------------------------ */
+enum tsc_activation {
+  TSC_ACT_NONE = 0,
+  TSC_ACT_RELU = 1,
+  TSC_ACT_GELU = 2,
+  TSC_ACT_GELU_TANH = 3,
+  TSC_ACT_SILU = 4
+};
+TSC_API int tsc_linear_act(const void* x, int64_t x_stride, const void* weight, int64_t w_stride,
+                           const void* bias, int32_t bias_dtype, const void* residual,
+                           int64_t r_stride, int32_t dtype, int64_t n, int32_t c_in,
+                           int32_t c_out, int32_t act, void* out, tsc_stream_t stream);
+
+/* Query and key heads, each normalised to unit mean square, scaled by its
+ * gain and rotated by its row's position, in one pass.  For a head x of dim
+ * values: y = x / sqrt(mean(x^2) + eps) * gain; with F = (dim / 2) / axes
+ * (whole pairs), pair a*F + i, a < axes, i < F, turns by
+ * t = positions[row][a] * base^(-i / F): (u, w) -> (u cos t - w sin t,
+ * u sin t + w cos t); pairs from axes*F on stay.  Pair j is (y[j],
+ * y[j + dim/2]), or (y[2j], y[2j + 1]) when interleaved != 0.
+ * q (n, q_heads, dim) with row and head strides, k likewise (either may have
+ * 0 heads); positions (n, axes), axes 1..4, int32 or (pos_float != 0) f32
+ * with row stride pos_row; gains of gain_dtype: (dim), or (heads, dim) when
+ * *_gain_per_head != 0, or NULL for 1.  dim even, 2..256; base > 1.
+ * q_out and k_out are contiguous. */
+TSC_API int tsc_norm_rotate_heads(const void* q, int64_t q_row, int64_t q_head, const void* k,
+                                  int64_t k_row, int64_t k_head, const void* positions,
+                                  int64_t pos_row, int32_t pos_float, int32_t axes,
+                                  const void* q_gain, const void* k_gain, int32_t gain_dtype,
+                                  int32_t q_gain_per_head, int32_t k_gain_per_head, float eps,
+                                  double base, int32_t interleaved, int32_t dtype, int64_t n,
+                                  int32_t q_heads, int32_t k_heads, int32_t dim, void* q_out,
+                                  void* k_out, tsc_stream_t stream);
+
+/* Attention of packed samples in a sliding window with sinks.  Sample b owns
+ * query rows [offsets_q[b], offsets_q[b+1]) and key rows [offsets_k[b],
+ * offsets_k[b+1]) (device int32, samples + 1 each; they start at 0, do not
+ * decrease and end at n_q and n_k: other values give unspecified results,
+ * but nothing outside the tensors is touched).  Its Lq queries are the last
+ * of its Lk positions: query i stands at p = i + Lk - Lq and sees key j when
+ * 0 <= j < Lk, j <= p + right, and j >= p - left or j < sinks (left or right
+ * < 0: no limit on that side).  out = softmax over the seen keys of
+ * scale * q.k, times v; 0 where nothing is seen.  Values of keys that a
+ * query does not see do not reach it, not even NaN or infinities.
+ * q (n_q, q_heads, dim), k and v (n_k, k_heads, dim) with row and head
+ * strides, q_heads a multiple of k_heads (query head h reads key head
+ * h / (q_heads / k_heads)), dim 1..256; out (n_q, q_heads, dim) contiguous.
+ * ws: *_workspace_bytes of scratch. */
+TSC_API int64_t tsc_window_attention_workspace_bytes(int32_t samples, int64_t n_q, int64_t n_k,
+                                                     int32_t q_heads, int32_t k_heads,
+                                                     int32_t dim, int32_t left, int32_t right,
+                                                     int32_t sinks, int32_t dtype);
+TSC_API int tsc_window_attention(const void* q, int64_t q_row, int64_t q_head, const void* k,
+                                 int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                                 int64_t v_head, const int32_t* offsets_q,
+                                 const int32_t* offsets_k, int32_t samples, int64_t n_q,
+                                 int64_t n_k, int32_t q_heads, int32_t k_heads, int32_t dim,
+                                 int32_t left, int32_t right, int32_t sinks, float scale,
+                                 int32_t dtype, void* ws, int64_t ws_bytes, void* out,
+                                 tsc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

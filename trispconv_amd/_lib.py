@@ -88,9 +88,21 @@ _SIGNATURES = {
     "tsc_conv_kernel_name": (ctypes.c_char_p, [_i32, _i32, _i32, _i32, _i64]),
     "tsc_dense_scatter": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _i32, c_i32p, _i32, _vp,
                                          _vp, _vp]),
+    "tsc_linear_act": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _i32, _i64,
+                                      _i32, _i32, _i32, _vp, _vp]),
+    "tsc_norm_rotate_heads": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32,
+                                             _i32, _vp, _vp, _i32, _i32, _i32, ctypes.c_float,
+                                             ctypes.c_double, _i32, _i32, _i64, _i32, _i32, _i32,
+                                             _vp, _vp, _vp]),
+    "tsc_window_attention_workspace_bytes": (_i64, [_i32, _i64, _i64, _i32, _i32, _i32, _i32,
+                                                    _i32, _i32, _i32]),
+    "tsc_window_attention": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                            _vp, _vp, _i32, _i64, _i64, _i32, _i32, _i32, _i32,
+                                            _i32, _i32, ctypes.c_float, _i32, _vp, _i64, _vp,
+                                            _vp]),
 }
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 _lib: Optional[ctypes.CDLL] = None
 

@@ -1,0 +1,154 @@
+// RMS norm of query and key heads with the rotation by position, one pass.
+//
+// For a head vector x of D values (g the gain, 1 without one):
+//   n = x / sqrt(mean(x^2) + eps) * g
+// and with A position axes, F = (D/2) div A pairs per axis, pair i of axis a
+// (pair a*F + i) turns by t = p[a] * base^(-i/F):
+//   (u, w) -> (u cos t - w sin t, u sin t + w cos t);
+// pairs from A*F on stay.  Pair j is (j, j + D/2), or (2j, 2j + 1) interleaved.
+#include "common.hpp"
+
+namespace tsc {
+namespace {
+
+struct RotateArgs {
+  const void* q;
+  int64_t q_row, q_head;
+  const void* k;
+  int64_t k_row, k_head;
+  const void* pos;
+  int64_t pos_row;
+  int pos_float, axes;
+  const void* q_gain;
+  const void* k_gain;
+  int gain_dtype;
+  int q_gain_head, k_gain_head;  // 0, or D for a gain per head
+  float eps;
+  double log2_base;
+  int interleaved;
+  int64_t n;
+  int q_heads, k_heads, dim;
+  void* q_out;
+  void* k_out;
+};
+
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
+  if (dtype == TSC_F32) return static_cast<const float*>(p)[i];
+  if (dtype == TSC_F16) return to_f32(static_cast<const __half*>(p)[i]);
+  return to_f32(static_cast<const __hip_bfloat16*>(p)[i]);
+}
+
+// Cosine and sine of p * base^(-i/F).  The angle is taken in turns in 64
+// bits: positions reach thousands, and an f32 angle of a thousand radians is
+// already 6e-5 off.  What is left after the whole turns fits f32.
+__device__ __forceinline__ float2 turn_of(double p, int i, int F, double log2_base) {
+  const double speed = exp2(-log2_base * i / F) * 0.15915494309189535;
+  const double t = p * speed;
+  const float part = static_cast<float>(2.0 * (t - rint(t)));
+  float2 cs;
+  sincospif(part, &cs.y, &cs.x);
+  return cs;
+}
+
+// A wave per row; a head takes LP lanes (a power of two from D/2 up, at most
+// 64), a lane its pairs l, l + 64.  Any size, stride and alignment.
+template <typename T>
+__global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t r = blockIdx.x * (int64_t)4 + threadIdx.x / kWave;
+  if (r >= a.n) return;
+  const int half = a.dim / 2, F = half / a.axes;
+  const int sub = lane / lp, l = lane % lp, heads = kWave / lp;
+  float2 cs[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = l + u * lp;
+    cs[u] = make_float2(1.f, 0.f);
+    if (j < half && F > 0 && j < a.axes * F) {
+      const int64_t at = r * a.pos_row + j / F;
+      const double p = a.pos_float ? static_cast<const float*>(a.pos)[at]
+                                   : static_cast<const int32_t*>(a.pos)[at];
+      cs[u] = turn_of(p, j % F, F, a.log2_base);
+    }
+  }
+  const int total = a.q_heads + a.k_heads;
+  for (int h0 = 0; h0 < total; h0 += heads) {
+    const int h = h0 + sub;
+    const bool in = h < total, is_q = h < a.q_heads;
+    const int hh = is_q ? h : h - a.q_heads;
+    const T* src = static_cast<const T*>(is_q ? a.q : a.k) +
+                   (is_q ? r * a.q_row + hh * a.q_head : r * a.k_row + hh * a.k_head);
+    T* dst = static_cast<T*>(is_q ? a.q_out : a.k_out) +
+             (r * (is_q ? a.q_heads : a.k_heads) + hh) * a.dim;
+    const void* gain = is_q ? a.q_gain : a.k_gain;
+    const int64_t gain_at = (int64_t)hh * (is_q ? a.q_gain_head : a.k_gain_head);
+    float x[2][2] = {}, sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = l + u * lp;
+      if (in && j < half) {
+        x[u][0] = to_f32(src[a.interleaved ? 2 * j : j]);
+        x[u][1] = to_f32(src[a.interleaved ? 2 * j + 1 : j + half]);
+      }
+      sum += x[u][0] * x[u][0] + x[u][1] * x[u][1];
+    }
+    for (int d = 1; d < lp; d <<= 1) sum += __shfl_xor(sum, d, kWave);
+    const float inv = 1.f / sqrtf(sum / a.dim + a.eps);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = l + u * lp;
+      if (!in || j >= half) continue;
+      const int ia = a.interleaved ? 2 * j : j, ib = a.interleaved ? 2 * j + 1 : j + half;
+      float p = x[u][0] * inv, q = x[u][1] * inv;
+      if (gain) {
+        p *= load_any(gain, a.gain_dtype, gain_at + ia);
+        q *= load_any(gain, a.gain_dtype, gain_at + ib);
+      }
+      dst[ia] = from_f32<T>(p * cs[u].x - q * cs[u].y);
+      dst[ib] = from_f32<T>(p * cs[u].y + q * cs[u].x);
+    }
+  }
+}
+
+template <typename T>
+int launch_rotate(const RotateArgs& a, hipStream_t s) {
+  int lp = 1;
+  while (lp < kWave && lp < a.dim / 2) lp *= 2;
+  rotate_any_kernel<T><<<static_cast<unsigned>(ceil_div(a.n, 4)), 256, 0, s>>>(a, lp);
+  TSC_LAUNCH_CHECK("norm_rotate_heads");
+  return 0;
+}
+
+}  // namespace
+}  // namespace tsc
+
+using namespace tsc;
+
+extern "C" int tsc_norm_rotate_heads(const void* q, int64_t q_row, int64_t q_head, const void* k,
+                                     int64_t k_row, int64_t k_head, const void* positions,
+                                     int64_t pos_row, int32_t pos_float, int32_t axes,
+                                     const void* q_gain, const void* k_gain, int32_t gain_dtype,
+                                     int32_t q_gain_per_head, int32_t k_gain_per_head, float eps,
+                                     double base, int32_t interleaved, int32_t dtype, int64_t n,
+                                     int32_t q_heads, int32_t k_heads, int32_t dim, void* q_out,
+                                     void* k_out, tsc_stream_t stream) {
+  TSC_REQUIRE(dtype_ok(dtype) && dtype_ok(gain_dtype), "norm_rotate_heads: unknown dtype");
+  TSC_REQUIRE(n >= 0 && n < (1ll << 31) && q_heads >= 0 && k_heads >= 0 && q_heads <= 65536 &&
+                  k_heads <= 65536, "norm_rotate_heads: invalid sizes");
+  TSC_REQUIRE(dim >= 2 && dim <= 256 && dim % 2 == 0,
+              "norm_rotate_heads: head size %d is not an even number up to 256", dim);
+  TSC_REQUIRE(axes >= 1 && axes <= 4, "norm_rotate_heads: %d position axes, 1 to 4 are supported", axes);
+  TSC_REQUIRE(base > 1.0 && eps >= 0.f, "norm_rotate_heads: base must be over 1 and eps not negative");
+  if (n == 0 || q_heads + k_heads == 0) return 0;
+  TSC_REQUIRE(positions && (!q_heads || (q && q_out)) && (!k_heads || (k && k_out)),
+              "norm_rotate_heads: null pointer");
+  const RotateArgs a{q, q_row, q_head, k, k_row, k_head, positions, pos_row, pos_float, axes,
+                     q_gain, k_gain, gain_dtype, q_gain_per_head ? dim : 0, k_gain_per_head ? dim : 0,
+                     eps, log2(base), interleaved, n, q_heads, k_heads, dim, q_out, k_out};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case TSC_F32: return launch_rotate<float>(a, s);
+    case TSC_F16: return launch_rotate<__half>(a, s);
+    default: return launch_rotate<__hip_bfloat16>(a, s);
+  }
+}
