@@ -1,0 +1,698 @@
+// Attention of packed sequences in a sliding window, with sinks.
+//
+// Sample b owns queries [oq[b], oq[b+1]) and keys [ok[b], ok[b+1]); its Lq
+// queries are the last of its Lk positions: query i stands at p = i + Lk - Lq
+// and sees key j when 0 <= j < Lk, j <= p + right, and j >= p - left or
+// j < sinks.  Per head (G query heads share a key head)
+//   o = sum_j e^(s_j) v_j / sum_j e^(s_j),  s_j = scale q.k_j  over the seen j,
+// and 0 where there is none.  The seen keys are two ranges:
+//   [lo, hi) with lo = max(0, p - left), hi = min(Lk, p + right + 1), and
+//   [0, min(sinks, lo, hi)).
+// One pass over the keys with the running maximum m and sum l of the
+// exponentials (f32): a new maximum rescales what is there by e^(m_old - m).
+#pragma once
+
+#include "sequence.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace tsc {
+
+struct AttendArgs {
+  const void* q;
+  int64_t q_row, q_head;
+  const void* k;
+  int64_t k_row, k_head;
+  const void* v;
+  int64_t v_row, v_head;
+  const int32_t* off_q;
+  const int32_t* off_k;
+  int samples;
+  int64_t n_q, n_k;
+  int q_heads, k_heads, dim;
+  int left, right, sinks;  // left, right: kNoLimit where there is none
+  float scale_log2;        // |scale| * log2(e), 1 for a scale of 0
+  float q_sign;            // the scale's sign, 0 for a scale of 0
+  void* out;
+  float* part;             // [split][n_q * q_heads][m, l, dim values] when the keys are split
+};
+
+constexpr int kNoLimit = 0x7fffffff;
+
+// How a call is cut up: the rows of a workgroup and the parts its keys are
+// split into.
+struct Cut {
+  int wide;  // 1: four waves a workgroup, 0: one
+  int64_t tiles;
+  int splits;
+};
+
+// Rows of a wave in 32s: two where scores, sums and queries of both fit the
+// registers of two waves a SIMD.
+template <typename T>
+constexpr int row_blocks(int dp) { return kIs16<T> && dp <= 64 ? 2 : 1; }
+// Keys of a tile in 32s: two, unless four tiles of it would not fit the LDS.
+template <typename T>
+constexpr int key_blocks(int dp) { return dp * (int)sizeof(T) <= 512 ? 2 : 1; }
+
+// Waves a SIMD that the registers and the LDS leave room for.
+template <typename T>
+constexpr int waves_per_simd(int dp) { return dp * (int)sizeof(T) <= 256 ? 2 : 1; }
+
+inline int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
+
+template <typename T>
+int rows_of(int dim) { return 128 * row_blocks<T>(padded_dim(dim)); }
+
+// The call on tensors of type T, cut as c says.
+template <typename T>
+int launch_attend(const AttendArgs& a, const Cut& c, hipStream_t s);
+
+namespace {
+
+// [offsets[b], offsets[b+1]) cut to [0, n]: no value of the offsets leads out
+// of the tensors.
+__device__ __forceinline__ void sample_range(const int32_t* off, int b, int64_t n, int64_t& at,
+                                             int& len) {
+  const int64_t lo = min(max((int64_t)off[b], (int64_t)0), n);
+  const int64_t hi = min(max((int64_t)off[b + 1], lo), n);
+  at = lo;
+  len = static_cast<int>(hi - lo);
+}
+
+// The seen keys of position p among lk: [lo, hi) and [0, sink).
+__device__ __forceinline__ void seen_keys(int p, int lk, int left, int right, int sinks, int& lo,
+                                          int& hi, int& sink) {
+  const int64_t h = (int64_t)p + right + 1, l = (int64_t)p - left;
+  hi = static_cast<int>(max((int64_t)0, min(h, (int64_t)lk)));
+  lo = static_cast<int>(min((int64_t)lk, max(l, (int64_t)0)));
+  sink = min(sinks, min(lo, hi));
+}
+
+// One query and head by one wave: a lane scores every 64th key, then the lanes
+// share out the D values and add the 64 keys' values one by one.  Reads no
+// key it does not see, and of those only [s0, s1) among the sinks and [w0,
+// w1) of the window's tiles.  Any size, stride and alignment; q_s: D floats of LDS
+// for this wave.  Returns the running maximum (in units of log2) and sum;
+// lane l holds the sums of values l, l + 64, ...
+template <typename T>
+__device__ void attend_row(const AttendArgs& a, const T* q, const T* k, const T* v, int lo, int hi,
+                           int sink, int s0, int s1, int w0, int w1, float* q_s, float& m_out,
+                           float& l_out, float o[4]) {
+  const int lane = threadIdx.x % kWave;
+  __builtin_amdgcn_wave_barrier();
+  for (int d = lane; d < a.dim; d += kWave) q_s[d] = a.q_sign * to_f32(q[d]);
+  __builtin_amdgcn_wave_barrier();
+  float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) o[u] = 0.f;
+  // sinks of the sink tiles, sinks that lie among the window's tiles, window
+  for (int part = 0; part < 3; ++part) {
+    const int from = part == 0 ? s0 : part == 1 ? w0 : max(lo, w0);
+    const int to = part == 0 ? min(sink, s1) : part == 1 ? min(sink, w1) : min(hi, w1);
+    for (int j0 = from; j0 < to; j0 += kWave) {
+      const int j = j0 + lane;
+      float s = -__builtin_inff();
+      if (j < to) {
+        float dot = 0.f;
+        for (int d = 0; d < a.dim; ++d) dot += q_s[d] * to_f32(k[j * a.k_row + d]);
+        s = dot * a.scale_log2;
+      }
+      float top = s;
+#pragma unroll
+      for (int x = 1; x < kWave; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, kWave));
+      const float m_new = fmaxf(m, top);
+      const float base = m_new == -__builtin_inff() ? 0.f : m_new;
+      const float fix = exp2f(m - base), p = j < to ? exp2f(s - base) : 0.f;
+      l *= fix;
+      m = m_new;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[u] *= fix;
+      const int cnt = min(kWave, to - j0);
+      for (int x = 0; x < cnt; ++x) {
+        const float px = __shfl(p, x, kWave);
+        l += px;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int d = lane + u * kWave;
+          if (d < a.dim) o[u] += px * to_f32(v[(j0 + x) * a.v_row + d]);
+        }
+      }
+    }
+  }
+  m_out = m;
+  l_out = l;
+}
+
+// What 16-byte chunk c of row r of an LDS tile is stored in, so that the reads
+// below find their chunks in different banks.  RB: bytes of a row.
+template <int RB>
+__device__ __forceinline__ int k_slot(int r, int c) {  // 8 rows, the same chunk: 16 bytes a lane
+  return RB % 128 == 0 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+}
+template <int RB>
+__device__ __forceinline__ int v_slot(int r, int c) {  // 4 rows, two chunks each: 8 bytes a lane
+  return RB % 128 == 0 ? c ^ (2 * (r & 3)) : c ^ (2 * ((r >> 1) & 1));
+}
+
+// Source of the chunks that no tensor holds (rows past the last key, values
+// past the head).
+__device__ const uint4 kNothing = {0u, 0u, 0u, 0u};
+
+// A tile of rows [j0, j0 + 32 KB) of one head into LDS, chunk by chunk in the
+// order of the slots; rows from `end` on and values from dim on are 0.
+template <typename T, int DP, int KB, int WAVES, bool ALIGNED, bool IS_V>
+__device__ __forceinline__ void stage_tile(char* tile, const T* src, int64_t stride, int j0, int end,
+                                           int dim) {
+  constexpr int RB = DP * sizeof(T), CH = RB / 16, CHUNKS = 32 * KB * CH;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  static_assert(CHUNKS % (kWave * WAVES) == 0, "whole instructions");
+  constexpr int ROUNDS = CHUNKS / (kWave * WAVES), AT_ONCE = !ALIGNED ? 2 : ROUNDS <= 8 ? ROUNDS : 4;
+  const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(tile) + wave * 1024);
+#pragma unroll AT_ONCE
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int slot = i * kWave * WAVES + wave * kWave + lane;
+    const int r = slot / CH, c = IS_V && kIs16<T> ? v_slot<RB>(r, slot % CH)
+                               : IS_V             ? slot % CH
+                                                  : k_slot<RB>(r, slot % CH);
+    const int j = j0 + r, d = c * kPer16<T>;
+    const T* p = src + j * stride + d;
+    if constexpr (ALIGNED) {
+      const void* g = j < end && d < dim ? static_cast<const void*>(p) : &kNothing;
+      load_to_lds(g, at + i * WAVES * 1024);
+    } else {
+      const int4v x = j < end && d + kPer16<T> <= dim ? load16_unaligned(p)
+                                                       : load16_partial(p, j < end ? dim - d : 0);
+      *reinterpret_cast<int4v*>(tile + slot * 16) = x;
+    }
+  }
+}
+
+__device__ __forceinline__ float max_halves(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// Non-finite values of a V tile: replaced by 0, their keys' bits set in the
+// KB words of LDS at `bad`.  Every thread of the workgroup calls it.
+template <typename T, int DP, int KB, int WAVES>
+__device__ void find_bad(char* vt, uint32_t* bad) {
+  constexpr int RB = DP * sizeof(T), CH = RB / 16, CHUNKS = 32 * KB * CH;
+  if (threadIdx.x < KB) bad[threadIdx.x] = 0u;
+  __syncthreads();
+  for (int slot = threadIdx.x; slot < CHUNKS; slot += kWave * WAVES) {
+    T* e = reinterpret_cast<T*>(vt + slot * 16);
+    bool any = false;
+    for (int i = 0; i < kPer16<T>; ++i) {
+      const float x = to_f32(e[i]) * 0.f;
+      if (x != x) {
+        e[i] = from_f32<T>(0.f);
+        any = true;
+      }
+    }
+    if (any) atomicOr(&bad[slot / CH / 32], 1u << (slot / CH % 32));
+  }
+  __syncthreads();
+}
+
+// The sample and the tile within it of the x-th tile of all: sample b has
+// ceil(Lq * group / rows) of them.  Every wave finds it for itself, 64 samples
+// at a time.  false: past the last.
+__device__ __forceinline__ bool find_tile(const AttendArgs& a, int group, int rows, int x, int64_t& q0,
+                                          int& lq, int& b, int& tile) {
+  const int lane = threadIdx.x % kWave;
+  for (int b0 = 0; b0 < a.samples; b0 += kWave) {
+    int64_t at = 0;
+    int len = 0;
+    if (b0 + lane < a.samples) sample_range(a.off_q, b0 + lane, a.n_q, at, len);
+    const uint32_t tiles = static_cast<uint32_t>(((int64_t)len * group + rows - 1) / rows);
+    const uint32_t inc = wave_inclusive(tiles);
+    const uint64_t past = __ballot(inc > static_cast<uint32_t>(x));
+    if (past) {
+      const int at_lane = __builtin_ctzll(past);
+      b = b0 + at_lane;
+      tile = x - static_cast<int>(__shfl(inc - tiles, at_lane, kWave));
+      lq = __shfl(len, at_lane, kWave);
+      q0 = __shfl(static_cast<int>(at), at_lane, kWave);
+      return true;
+    }
+    x -= static_cast<int>(__shfl(inc, kWave - 1, kWave));
+  }
+  return false;
+}
+
+// What a workgroup computes: rows [row0, ...) of the `rows` (token, head of
+// the group) rows of a sample and key head, against key tiles [t0, t1) of
+// those that it walks: [0, sink_end) in sink_tiles of them, then [start, end).
+struct Walk {
+  int64_t q0;  // the sample's first query row
+  uint32_t row0, rows;
+  int group, hk, lk, shift;  // shift: position of the sample's first query
+  int sink_end, sink_tiles, start, end, t0, t1;
+  int split, splits;
+  // (the host keeps n_q * group within 32 bits)
+  __device__ int token(uint32_t r) const { return static_cast<int>(min(r, rows - 1) / static_cast<uint32_t>(group)); }
+};
+
+// Tiles of 32 RB WAVES rows (a row: one query of one head; the heads that
+// share a key head side by side) against tiles of 32 KB keys.
+//
+// A wave holds 32 RB rows as the columns of the transposed scores S^T = K Q^T:
+// a lane has 16 KB keys of one row per 32, so the row's maximum and sum are a
+// lane's own values and one exchange with the other half, and e^S^T is, as it
+// stands, the right operand of O^T = V^T e^S^T: the product's sum runs over
+// keys in the order that S^T's registers have them, and V is read in the same
+// order (ds_read_b64_tr_b16 transposes it on the way from LDS).  K and V tiles
+// are double buffered: direct-to-LDS loads of the next ones fly while these
+// are used, one barrier a tile.
+//
+// A row's reference maximum m moves only when some score exceeds it by 2^8:
+// exponentials up to 2^8 keep the relative accuracy of the 16-bit type that
+// multiplies V, and the rescale of O almost never runs.
+//
+// A key that a row does not see has weight 0, and 0 times an infinite or NaN
+// value would be NaN.  When a row of the workgroup comes out not finite, the
+// keys are walked once more with such values replaced by 0, which leaves the
+// bits of every row that sees none of them as they would have been; rows that
+// see one are then done key by key.  This is a pass of the walk, false: it has
+// to be done again (CLEAN).
+template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED, bool CLEAN>
+__device__ __forceinline__ bool attend_pass(const AttendArgs& a, const Walk& w, const T* k, const T* v,
+                                            char* lds) {
+  constexpr int KT = 32 * KB, ROW_BYTES = DP * sizeof(T);
+  constexpr int TILE = KT * ROW_BYTES, STEPS = DP * (int)sizeof(T) / 32, DB = DP / 32;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, half = lane / 32, col = lane % 32;
+  int lo_first, hi_first, lo_last, hi_last, none;
+  const uint32_t wave_row = w.row0 + wave * 32 * RB;
+  seen_keys(w.token(wave_row) + w.shift, w.lk, a.left, a.right, a.sinks, lo_first, hi_first, none);
+  seen_keys(w.token(wave_row + 32 * RB - 1) + w.shift, w.lk, a.left, a.right, a.sinks, lo_last, hi_last, none);
+  int lo[RB], hi[RB], sink[RB];
+  int4v qf[RB][STEPS];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const uint32_t r = wave_row + rb * 32 + col;
+    const int t = w.token(r), g = static_cast<int>(min(r, w.rows - 1) - static_cast<uint32_t>(t) * w.group);
+    seen_keys(t + w.shift, w.lk, a.left, a.right, a.sinks, lo[rb], hi[rb], sink[rb]);
+    if (r >= w.rows) hi[rb] = 0;
+    const T* q = static_cast<const T*>(a.q) + (w.q0 + t) * a.q_row + (w.hk * w.group + g) * a.q_head;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      const int d = (2 * st + half) * kPer16<T>;
+      int4v x;
+      if (d + kPer16<T> <= a.dim) x = load16_unaligned(q + d);
+      else x = load16_partial(q + d, a.dim - d);
+      // the scale's sign (0 for a scale of 0) goes into q, exactly
+      if (a.q_sign != 1.f) {
+        T e[kPer16<T>];
+        __builtin_memcpy(e, &x, 16);
+#pragma unroll
+        for (int i = 0; i < kPer16<T>; ++i) e[i] = from_f32<T>(to_f32(e[i]) * a.q_sign);
+        __builtin_memcpy(&x, e, 16);
+      }
+      qf[rb][st] = x;
+    }
+  }
+
+  auto tile_at = [&](int t, int& j0, int& end) {
+    if (t < w.sink_tiles) {
+      j0 = t * KT;
+      end = w.sink_end;
+    } else {
+      j0 = w.start + (t - w.sink_tiles) * KT;
+      end = w.end;
+    }
+  };
+  auto stage = [&](int t, int buf) {
+    int j0, end;
+    tile_at(t, j0, end);
+    stage_tile<T, DP, KB, WAVES, ALIGNED, false>(lds + buf * 2 * TILE, k, a.k_row, j0, end, a.dim);
+    stage_tile<T, DP, KB, WAVES, ALIGNED, true>(lds + buf * 2 * TILE + TILE, v, a.v_row, j0, end, a.dim);
+  };
+
+  f32x16 o[RB][DB];
+  float m[RB], mc[RB], l[RB];
+  int hit = 0;  // bit rb: the row sees a value that is not finite
+  uint32_t* bad = reinterpret_cast<uint32_t*>(lds + 4 * TILE + WAVES * DP * 4);
+  const float c = a.scale_log2;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    m[rb] = -__builtin_inff();
+    mc[rb] = l[rb] = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[rb][db] = f32x16(0.f);
+  }
+
+  if (w.t0 < w.t1) stage(w.t0, 0);
+  for (int t = w.t0; t < w.t1; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t + 1 < w.t1) stage(t + 1, (t + 1 - w.t0) & 1);
+    int j0, end;
+    tile_at(t, j0, end);
+    const char* kt = lds + ((t - w.t0) & 1) * 2 * TILE;
+    const char* vt = kt + TILE;
+    if constexpr (CLEAN) {
+      find_bad<T, DP, KB, WAVES>(lds + ((t - w.t0) & 1) * 2 * TILE + TILE, bad);
+      for (int x = 0; x < KT; ++x) {
+        const int j = j0 + x;
+        if (!(bad[x / 32] >> (x % 32) & 1u)) continue;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          hit |= (j < min(end, hi[rb]) && (j >= lo[rb] || j < a.sinks)) << rb;
+      }
+    }
+    if (j0 >= hi_last || (j0 + KT <= lo_first && j0 >= a.sinks)) continue;
+    const bool whole = j0 + KT <= min(end, hi_first) && (j0 >= lo_last || j0 + KT <= a.sinks) &&
+                       wave_row + 32 * RB <= w.rows;
+
+    f32x16 s[RB][KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) s[rb][kb] = f32x16(0.f);
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        const int r = kb * 32 + col;
+        const int4v x = *reinterpret_cast<const int4v*>(kt + r * ROW_BYTES +
+                                                        k_slot<ROW_BYTES>(r, 2 * st + half) * 16);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) s[rb][kb] = mma32<T>(x, qf[rb][st], s[rb][kb]);
+      }
+    }
+
+    int p16[RB][KB][8];  // e^S^T in 16 bits, two keys a register
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      if (!whole) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = j0 + kb * 32 + 8 * (i / 4) + 4 * half + i % 4;
+            const bool see = j < min(end, hi[rb]) && (j >= lo[rb] || j < a.sinks);
+            s[rb][kb][i] = see ? s[rb][kb][i] : -__builtin_inff();
+          }
+      }
+      float top = s[rb][0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[rb][kb][i]);
+      top = max_halves(top);
+      if (__any((top - m[rb]) * c > 8.f || (m[rb] == -__builtin_inff() && top > m[rb]))) {
+        const float m_new = fmaxf(m[rb], top);
+        const float mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c;
+        const float fix = m[rb] == -__builtin_inff() ? 0.f : exp2f(mc[rb] - mc_new);
+        m[rb] = m_new;
+        mc[rb] = mc_new;
+        l[rb] *= fix;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[rb][db] *= fix;
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][kb][i], c, -mc[rb]));
+          s[rb][kb][i] = p;
+          l[rb] += p;
+        }
+      if constexpr (kIs16<T>) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p16[rb][kb][i] = pack2<T>(s[rb][kb][2 * i], s[rb][kb][2 * i + 1]);
+      }
+    }
+
+    // O^T += V^T e^S^T.  16 bits: 16 keys a step, of which the halves take
+    // keys 0-3, 8-11 and 4-7, 12-15.  f32: two keys a step, 4 apart.
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      if constexpr (kIs16<T>) {
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            int4v x;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = kb * 32 + 16 * st + 8 * h + 4 * half + (lane & 15) / 4;
+              const int d = 32 * db + (lane & 16) + 4 * (lane & 3);
+              const char* p = vt + r * ROW_BYTES + v_slot<ROW_BYTES>(r, d / 8) * 16 + (d % 8) * 2;
+              const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) short4v*)p);
+              const int2v z = __builtin_bit_cast(int2v, y);
+              x[2 * h] = z[0];
+              x[2 * h + 1] = z[1];
+            }
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              const int4v p = {p16[rb][kb][4 * st], p16[rb][kb][4 * st + 1], p16[rb][kb][4 * st + 2],
+                               p16[rb][kb][4 * st + 3]};
+              o[rb][db] = mma32<T>(x, p, o[rb][db]);
+            }
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const int r = kb * 32 + 8 * (i / 4) + 4 * half + i % 4;
+            const float x = *reinterpret_cast<const float*>(vt + r * ROW_BYTES + (32 * db + col) * 4);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+              o[rb][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[rb][kb][i], o[rb][db], 0, 0, 0);
+          }
+      }
+    }
+  }
+
+  if constexpr (!CLEAN) {
+    float off = 0.f;  // NaN when one of the sums is not finite
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) off = __builtin_fmaf(o[rb][db][i], 0.f, off);
+    if (__syncthreads_or(off != off)) return false;
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    l[rb] = sum_halves(l[rb]);
+    const uint32_t r = wave_row + rb * 32 + col;
+    const int t = w.token(r), g = static_cast<int>(min(r, w.rows - 1) - static_cast<uint32_t>(t) * w.group);
+    const int64_t item = (w.q0 + t) * a.q_heads + w.hk * w.group + g;
+    const bool odd = r < w.rows && (hit >> rb & 1);
+    if (r < w.rows && !odd) {
+      const float inv = l[rb] == 0.f ? 0.f : 1.f / l[rb];
+      if (w.splits > 1) {
+        float* part = a.part + (w.split * a.n_q * a.q_heads + item) * (a.dim + 2);
+        if (half == 0) {
+          part[0] = l[rb] == 0.f ? -__builtin_inff() : mc[rb];
+          part[1] = l[rb];
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int d = 32 * db + 8 * (i / 4) + 4 * half + i % 4;
+            if (d < a.dim) part[2 + d] = o[rb][db][i];
+          }
+      } else {
+        T* out = static_cast<T*>(a.out) + item * a.dim;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = 32 * db + 8 * i + 4 * half;
+            T e[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) e[x] = from_f32<T>(o[rb][db][4 * i + x] * inv);
+            if (d + 4 <= a.dim) {
+              __builtin_memcpy(out + d, e, sizeof e);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 3; ++x)
+                if (d + x < a.dim) out[d + x] = e[x];
+            }
+          }
+      }
+    }
+    uint64_t redo = __ballot(odd && half == 0);  // w.rows done key by key
+    if (redo) {
+      // the tiles in LDS may still be read by other waves: each wave takes
+      // its row's scratch from its own D floats behind them
+      float* q_s = reinterpret_cast<float*>(lds + 4 * TILE) + wave * DP;
+      int j0 = 0, end = 0, sink_from = 0, sink_to = 0, from = 0, to = 0;
+      // this w.split's keys: tiles [w.t0, w.t1)
+      if (w.t0 < w.sink_tiles) {
+        tile_at(w.t0, j0, end);
+        sink_from = j0;
+        sink_to = min(min(w.t1, w.sink_tiles) * KT, w.sink_end);
+      }
+      if (w.t1 > w.sink_tiles) {
+        from = w.start + (max(w.t0, w.sink_tiles) - w.sink_tiles) * KT;
+        to = min(w.start + (w.t1 - w.sink_tiles) * KT, w.end);
+      }
+      while (redo) {
+        const int x = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        const uint32_t rx = wave_row + rb * 32 + x;
+        const int tx = w.token(rx), gx = static_cast<int>(rx - static_cast<uint32_t>(tx) * w.group);
+        const int64_t ix = (w.q0 + tx) * a.q_heads + w.hk * w.group + gx;
+        int lx, hx, sx;
+        seen_keys(tx + w.shift, w.lk, a.left, a.right, a.sinks, lx, hx, sx);
+        float mx, lsum, ox[4];
+        attend_row(a, static_cast<const T*>(a.q) + (w.q0 + tx) * a.q_row + (w.hk * w.group + gx) * a.q_head, k, v,
+                   lx, hx, sx, sink_from, sink_to, from, to, q_s, mx, lsum, ox);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int d = lane + u * kWave;
+          if (d >= a.dim) continue;
+          if (w.splits > 1) {
+            float* part = a.part + (w.split * a.n_q * a.q_heads + ix) * (a.dim + 2);
+            part[2 + d] = ox[u];
+            if (d == 0) {
+              part[0] = lsum == 0.f ? -__builtin_inff() : mx;
+              part[1] = lsum;
+            }
+          } else {
+            static_cast<T*>(a.out)[ix * a.dim + d] = from_f32<T>(lsum == 0.f ? 0.f : ox[u] / lsum);
+          }
+        }
+      }
+    }
+  }
+  return true;
+}
+
+template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
+__global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP)) attend_kernel(AttendArgs a, int tiles_max, int splits) {
+  constexpr int ROWS = 32 * RB * WAVES, KT = 32 * KB;
+  extern __shared__ __align__(16) char lds[];  // K, V, K, V tiles; a row of q for each wave; KB words
+  // tiles of one head next to each other on one XCD (workgroups go round the
+  // eight in turn), so that neighbouring windows meet in its L2
+  const int64_t blocks = (int64_t)tiles_max * a.k_heads * splits, per = (blocks + 7) / 8;
+  const int64_t id = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  if (blockIdx.x / 8 >= per || id >= blocks) return;
+  const int group = a.q_heads / a.k_heads;
+  Walk w;
+  w.split = static_cast<int>(id % splits);
+  w.splits = splits;
+  w.hk = static_cast<int>(id / splits / tiles_max);
+  int64_t k0;
+  int lq, b, tile;
+  if (!find_tile(a, group, ROWS, static_cast<int>(id / splits % tiles_max), w.q0, lq, b, tile)) return;
+  sample_range(a.off_k, b, a.n_k, k0, w.lk);
+  const T* k = static_cast<const T*>(a.k) + k0 * a.k_row + w.hk * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + k0 * a.v_row + w.hk * a.v_head;
+
+  w.group = group;
+  w.row0 = static_cast<uint32_t>(tile) * ROWS;
+  w.rows = static_cast<uint32_t>(lq) * group;
+  w.shift = w.lk - lq;
+  int lo, hi, s, lo2, hi2;
+  seen_keys(w.token(w.row0) + w.shift, w.lk, a.left, a.right, a.sinks, lo, hi, s);
+  seen_keys(w.token(w.row0 + ROWS - 1) + w.shift, w.lk, a.left, a.right, a.sinks, lo2, hi2, s);
+  w.sink_end = min(a.sinks, min(lo, hi2));
+  w.start = lo;
+  if (a.sinks >= lo) w.sink_end = w.start = 0;
+  w.end = max(hi2, w.start);
+  w.sink_tiles = (w.sink_end + KT - 1) / KT;
+  const int tiles = w.sink_tiles + (w.end - w.start + KT - 1) / KT, each = (tiles + splits - 1) / splits;
+  w.t0 = min(w.split * each, tiles);
+  w.t1 = min(w.t0 + each, tiles);
+  if (!attend_pass<T, DP, RB, KB, WAVES, ALIGNED, false>(a, w, k, v, lds))
+    attend_pass<T, DP, RB, KB, WAVES, ALIGNED, true>(a, w, k, v, lds);
+}
+
+// Joins the splits of each row: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s
+// in the order of the splits, m the largest m_s.  A wave per row.
+template <typename T>
+__global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a, int splits) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t items = a.n_q * a.q_heads, item = blockIdx.x * (int64_t)4 + threadIdx.x / kWave;
+  if (item >= items) return;
+  const float* part = a.part + item * (a.dim + 2);
+  const int64_t step = items * (a.dim + 2);
+  float m = -__builtin_inff();
+  for (int s = lane; s < splits; s += kWave) m = fmaxf(m, part[s * step]);
+#pragma unroll
+  for (int x = 1; x < kWave; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, kWave));
+  const float base = m == -__builtin_inff() ? 0.f : m;
+  float l = 0.f, o[4] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float* p = part + s * step;
+    // a part that saw nothing counts for nothing; NaN sums stay NaN
+    if (p[1] == 0.f) continue;
+    const float f = exp2f(p[0] - base);
+    l += f * p[1];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int d = lane + u * kWave;
+      if (d < a.dim) o[u] += f * p[2 + d];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int d = lane + u * kWave;
+    if (d < a.dim) static_cast<T*>(a.out)[item * a.dim + d] = from_f32<T>(l == 0.f ? 0.f : o[u] / l);
+  }
+}
+
+template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
+int launch_tiles(const AttendArgs& a, const Cut& c, hipStream_t s) {
+  constexpr int bytes = 4 * 32 * KB * DP * (int)sizeof(T) + WAVES * DP * 4 + KB * 4;
+  auto kernel = &attend_kernel<T, DP, RB, KB, WAVES, ALIGNED>;
+  if (bytes > 65536)
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  const int64_t blocks = align_up(c.tiles * a.k_heads * c.splits, 8);
+  TSC_REQUIRE(blocks < (1ll << 31), "window_attention: too many tiles");
+  kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, static_cast<int>(c.tiles), c.splits);
+  TSC_LAUNCH_CHECK("window_attention");
+  if (c.splits > 1) {
+    attend_join_kernel<T><<<static_cast<unsigned>(ceil_div(a.n_q * a.q_heads, 4)), 256, 0, s>>>(a, c.splits);
+    TSC_LAUNCH_CHECK("window_attention_join");
+  }
+  return 0;
+}
+
+template <typename T, int DP, bool ALIGNED>
+int launch_dim(const AttendArgs& a, const Cut& c, hipStream_t s) {
+  constexpr int RB = row_blocks<T>(DP), KB = key_blocks<T>(DP);
+  return c.wide ? launch_tiles<T, DP, RB, KB, 4, ALIGNED>(a, c, s)
+                : launch_tiles<T, DP, 1, KB, 1, ALIGNED>(a, c, s);
+}
+
+template <typename T, bool ALIGNED>
+int launch_aligned(const AttendArgs& a, const Cut& c, hipStream_t s) {
+  switch (padded_dim(a.dim)) {
+    case 32: return launch_dim<T, 32, ALIGNED>(a, c, s);
+    case 64: return launch_dim<T, 64, ALIGNED>(a, c, s);
+    case 96: return launch_dim<T, 96, ALIGNED>(a, c, s);
+    case 128: return launch_dim<T, 128, ALIGNED>(a, c, s);
+    default: return launch_dim<T, 256, ALIGNED>(a, c, s);
+  }
+}
+
+}  // namespace
+
+template <typename T>
+int launch_attend(const AttendArgs& a, const Cut& c, hipStream_t s) {
+  const int64_t e = kPer16<T>;
+  const bool aligned = a.dim % e == 0 && a.k_row % e == 0 && a.v_row % e == 0 && a.k_head % e == 0 &&
+                       a.v_head % e == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
+  return aligned ? launch_aligned<T, true>(a, c, s) : launch_aligned<T, false>(a, c, s);
+}
+
+}  // namespace tsc
