@@ -156,38 +156,71 @@ __device__ __forceinline__ int v_slot(int r, int c) {  // 4 rows, two chunks eac
   return RB % 128 == 0 ? c ^ (2 * (r & 3)) : c ^ (2 * ((r >> 1) & 1));
 }
 
-// Source of the chunks that no tensor holds (rows past the last key, values
-// past the head).
-__device__ const uint4 kNothing = {0u, 0u, 0u, 0u};
-
-// A tile of rows [j0, j0 + 32 KB) of one head into LDS, chunk by chunk in the
-// order of the slots; rows from `end` on and values from dim on are 0.
+// Brings tiles of rows [j0, j0 + 32 KB) of one key head's K or V into LDS,
+// chunk by chunk in the order of the slots.  Rows from `end` on are not used
+// by anyone: they are row end - 1 again, so nothing past the sample is read.
+// Values from dim on stay the zeros that clear() put there.
 template <typename T, int DP, int KB, int WAVES, bool ALIGNED, bool IS_V>
-__device__ __forceinline__ void stage_tile(char* tile, const T* src, int64_t stride, int j0, int end,
-                                           int dim) {
-  constexpr int RB = DP * sizeof(T), CH = RB / 16, CHUNKS = 32 * KB * CH;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  static_assert(CHUNKS % (kWave * WAVES) == 0, "whole instructions");
-  constexpr int ROUNDS = CHUNKS / (kWave * WAVES), AT_ONCE = !ALIGNED ? 2 : ROUNDS <= 8 ? ROUNDS : 4;
-  const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(tile) + wave * 1024);
-#pragma unroll AT_ONCE
-  for (int i = 0; i < ROUNDS; ++i) {
-    const int slot = i * kWave * WAVES + wave * kWave + lane;
-    const int r = slot / CH, c = IS_V && kIs16<T> ? v_slot<RB>(r, slot % CH)
-                               : IS_V             ? slot % CH
-                                                  : k_slot<RB>(r, slot % CH);
-    const int j = j0 + r, d = c * kPer16<T>;
-    const T* p = src + j * stride + d;
+struct Stager {
+  static constexpr int RB = DP * sizeof(T), CH = RB / 16, CHUNKS = 32 * KB * CH;
+  static constexpr int THREADS = kWave * WAVES, ROUNDS = CHUNKS / THREADS;
+  static_assert(CHUNKS % THREADS == 0, "whole instructions");
+  // the slots of a thread's rounds hold the same chunk of rows a constant apart
+  static constexpr bool SAME = THREADS % (8 * CH) == 0;
+  const T* src;
+  int64_t stride;
+  int dim, lane, wave;
+  uint32_t offset[SAME ? 1 : ROUNDS];  // bytes from row j0 to the thread's chunks
+
+  __device__ static int row(int slot) { return slot / CH; }
+  __device__ static int chunk(int slot) {
+    return IS_V && kIs16<T> ? v_slot<RB>(slot / CH, slot % CH)
+           : IS_V           ? slot % CH
+                            : k_slot<RB>(slot / CH, slot % CH);
+  }
+  __device__ int slot(int i) const { return i * THREADS + wave * kWave + lane; }
+
+  __device__ __forceinline__ void begin(const T* src_, int64_t stride_, int dim_, int wave_) {
+    src = src_, stride = stride_, dim = dim_, wave = wave_, lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int i = 0; i < (SAME ? 1 : ROUNDS); ++i)
+      offset[i] = static_cast<uint32_t>(row(slot(i)) * stride * sizeof(T)) + chunk(slot(i)) * 16;
+  }
+  __device__ void clear(char* tile) const {
+    if (dim >= DP) return;
+    for (int i = 0; i < ROUNDS; ++i)
+      if (chunk(slot(i)) * kPer16<T> >= dim) *reinterpret_cast<int4v*>(tile + slot(i) * 16) = int4v(0);
+  }
+  __device__ __forceinline__ void load(char* tile, int j0, int end) const {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(tile) + wave * 1024);
     if constexpr (ALIGNED) {
-      const void* g = j < end && d < dim ? static_cast<const void*>(p) : &kNothing;
-      load_to_lds(g, at + i * WAVES * 1024);
+      const T* base = src + j0 * stride;
+      if (j0 + 32 * KB <= end && dim >= DP) {
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) {
+          if (SAME) load_to_lds(base + i * (THREADS / CH) * stride, offset[0], at + i * WAVES * 1024);
+          else load_to_lds(base, offset[SAME ? 0 : i], at + i * WAVES * 1024);
+        }
+      } else {
+#pragma unroll 2
+        for (int i = 0; i < ROUNDS; ++i) {
+          const int r = min(row(slot(i)), end - 1 - j0);
+          load_to_lds(base, static_cast<uint32_t>(r * stride * sizeof(T)) + chunk(slot(i)) * 16,
+                      at + i * WAVES * 1024, in(i));
+        }
+      }
     } else {
-      const int4v x = j < end && d + kPer16<T> <= dim ? load16_unaligned(p)
-                                                       : load16_partial(p, j < end ? dim - d : 0);
-      *reinterpret_cast<int4v*>(tile + slot * 16) = x;
+#pragma unroll 2
+      for (int i = 0; i < ROUNDS; ++i) {
+        const int d = chunk(slot(i)) * kPer16<T>;
+        const T* p = src + min(j0 + row(slot(i)), end - 1) * stride + d;
+        const int4v x = d + kPer16<T> <= dim ? load16_unaligned(p) : load16_partial(p, dim - d);
+        *reinterpret_cast<int4v*>(tile + slot(i) * 16) = x;
+      }
     }
   }
-}
+  __device__ __forceinline__ bool in(int i) const { return dim >= DP || chunk(slot(i)) * kPer16<T> < dim; }
+};
 
 __device__ __forceinline__ float max_halves(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
@@ -238,12 +271,12 @@ __device__ __forceinline__ bool find_tile(const AttendArgs& a, int group, int ro
     if (past) {
       const int at_lane = __builtin_ctzll(past);
       b = b0 + at_lane;
-      tile = x - static_cast<int>(__shfl(inc - tiles, at_lane, kWave));
-      lq = __shfl(len, at_lane, kWave);
-      q0 = __shfl(static_cast<int>(at), at_lane, kWave);
+      tile = x - __builtin_amdgcn_readlane(inc - tiles, at_lane);
+      lq = __builtin_amdgcn_readlane(len, at_lane);
+      q0 = __builtin_amdgcn_readlane(static_cast<int>(at), at_lane);
       return true;
     }
-    x -= static_cast<int>(__shfl(inc, kWave - 1, kWave));
+    x -= __builtin_amdgcn_readlane(inc, kWave - 1);
   }
   return false;
 }
@@ -261,6 +294,8 @@ struct Walk {
   __device__ int token(uint32_t r) const { return static_cast<int>(min(r, rows - 1) / static_cast<uint32_t>(group)); }
 };
 
+constexpr float kMostOver = 8.f;
+
 // Tiles of 32 RB WAVES rows (a row: one query of one head; the heads that
 // share a key head side by side) against tiles of 32 KB keys.
 //
@@ -273,22 +308,22 @@ struct Walk {
 // are double buffered: direct-to-LDS loads of the next ones fly while these
 // are used, one barrier a tile.
 //
-// A row's reference maximum m moves only when some score exceeds it by 2^8:
-// exponentials up to 2^8 keep the relative accuracy of the 16-bit type that
-// multiplies V, and the rescale of O almost never runs.
+// A row's reference maximum m moves only when some score exceeds it by
+// 2^kMostOver: weights up to there keep the relative accuracy of f16 and bf16,
+// and the rescale of O almost never runs.
 //
 // A key that a row does not see has weight 0, and 0 times an infinite or NaN
 // value would be NaN.  When a row of the workgroup comes out not finite, the
 // keys are walked once more with such values replaced by 0, which leaves the
 // bits of every row that sees none of them as they would have been; rows that
-// see one are then done key by key.  This is a pass of the walk, false: it has
-// to be done again (CLEAN).
-template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED, bool CLEAN>
-__device__ __forceinline__ bool attend_pass(const AttendArgs& a, const Walk& w, const T* k, const T* v,
+// see one are then done key by key.
+template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
+__device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, const T* k, const T* v,
                                             char* lds) {
   constexpr int KT = 32 * KB, ROW_BYTES = DP * sizeof(T);
   constexpr int TILE = KT * ROW_BYTES, STEPS = DP * (int)sizeof(T) / 32, DB = DP / 32;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, half = lane / 32, col = lane % 32;
+  const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   int lo_first, hi_first, lo_last, hi_last, none;
   const uint32_t wave_row = w.row0 + wave * 32 * RB;
   seen_keys(w.token(wave_row) + w.shift, w.lk, a.left, a.right, a.sinks, lo_first, hi_first, none);
@@ -329,153 +364,175 @@ __device__ __forceinline__ bool attend_pass(const AttendArgs& a, const Walk& w, 
       end = w.end;
     }
   };
-  auto stage = [&](int t, int buf) {
-    int j0, end;
-    tile_at(t, j0, end);
-    stage_tile<T, DP, KB, WAVES, ALIGNED, false>(lds + buf * 2 * TILE, k, a.k_row, j0, end, a.dim);
-    stage_tile<T, DP, KB, WAVES, ALIGNED, true>(lds + buf * 2 * TILE + TILE, v, a.v_row, j0, end, a.dim);
+  Stager<T, DP, KB, WAVES, ALIGNED, false> k_stage;
+  Stager<T, DP, KB, WAVES, ALIGNED, true> v_stage;
+  k_stage.begin(k, a.k_row, a.dim, wave);
+  v_stage.begin(v, a.v_row, a.dim, wave);
+  for (int x = 0; x < 2; ++x) {
+    k_stage.clear(lds + x * 2 * TILE);
+    v_stage.clear(lds + x * 2 * TILE + TILE);
+  }
+  auto stage = [&](int j0, int end, int buf) {
+    k_stage.load(lds + buf * 2 * TILE, j0, end);
+    v_stage.load(lds + buf * 2 * TILE + TILE, j0, end);
   };
 
   f32x16 o[RB][DB];
-  float m[RB], mc[RB], l[RB];
-  int hit = 0;  // bit rb: the row sees a value that is not finite
+  float m[RB], mc[RB], l[RB][2];  // reference maximum, times c, two partial sums
+  int hit = 0;    // bit rb: the row sees a value that is not finite
+  int clean = 0;  // the walk that replaces those values
   uint32_t* bad = reinterpret_cast<uint32_t*>(lds + 4 * TILE + WAVES * DP * 4);
   const float c = a.scale_log2;
+  // 32 keys from row kb * 32 of a tile; whole: every row of the wave sees all
+  auto key_step = [&](bool whole, const char* kt, const char* vt, int kb, int j0, int end) {
+    f32x16 s[RB];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    m[rb] = -__builtin_inff();
-    mc[rb] = l[rb] = 0.f;
+    for (int rb = 0; rb < RB; ++rb) s[rb] = f32x16(0.f);
 #pragma unroll
-    for (int db = 0; db < DB; ++db) o[rb][db] = f32x16(0.f);
-  }
-
-  if (w.t0 < w.t1) stage(w.t0, 0);
-  for (int t = w.t0; t < w.t1; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < w.t1) stage(t + 1, (t + 1 - w.t0) & 1);
-    int j0, end;
-    tile_at(t, j0, end);
-    const char* kt = lds + ((t - w.t0) & 1) * 2 * TILE;
-    const char* vt = kt + TILE;
-    if constexpr (CLEAN) {
-      find_bad<T, DP, KB, WAVES>(lds + ((t - w.t0) & 1) * 2 * TILE + TILE, bad);
-      for (int x = 0; x < KT; ++x) {
-        const int j = j0 + x;
-        if (!(bad[x / 32] >> (x % 32) & 1u)) continue;
+    for (int st = 0; st < STEPS; ++st) {
+      const int4v x = *reinterpret_cast<const int4v*>(kt + (kb * 32 + col) * ROW_BYTES +
+                                                      k_slot<ROW_BYTES>(col, 2 * st + half) * 16);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          hit |= (j < min(end, hi[rb]) && (j >= lo[rb] || j < a.sinks)) << rb;
+      for (int rb = 0; rb < RB; ++rb) s[rb] = mma32<T>(x, qf[rb][st], s[rb]);
+    }
+    if (!whole && j0 < a.sinks) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = j0 + kb * 32 + 8 * (i / 4) + 4 * half + i % 4;
+          const bool see = j < min(end, hi[rb]) && (j >= lo[rb] || j < a.sinks);
+          s[rb][i] = see ? s[rb][i] : -__builtin_inff();
+        }
+    } else if (!whole) {
+      // no sinks here: one comparison for both ends
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const uint32_t from = j0 + kb * 32 + 4 * half - lo[rb], span = max(0, min(end, hi[rb]) - lo[rb]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[rb][i] = from + (8 * (i / 4) + i % 4) < span ? s[rb][i] : -__builtin_inff();
       }
     }
-    if (j0 >= hi_last || (j0 + KT <= lo_first && j0 >= a.sinks)) continue;
-    const bool whole = j0 + KT <= min(end, hi_first) && (j0 >= lo_last || j0 + KT <= a.sinks) &&
-                       wave_row + 32 * RB <= w.rows;
-
-    f32x16 s[RB][KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) s[rb][kb] = f32x16(0.f);
-#pragma unroll
-      for (int st = 0; st < STEPS; ++st) {
-        const int r = kb * 32 + col;
-        const int4v x = *reinterpret_cast<const int4v*>(kt + r * ROW_BYTES +
-                                                        k_slot<ROW_BYTES>(r, 2 * st + half) * 16);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) s[rb][kb] = mma32<T>(x, qf[rb][st], s[rb][kb]);
-      }
-    }
-
-    int p16[RB][KB][8];  // e^S^T in 16 bits, two keys a register
+    float top[RB];
+    bool over = false;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      if (!whole) {
+      top[rb] = fmaxf(s[rb][0], s[rb][1]);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+      for (int i = 2; i < 16; i += 2) top[rb] = fmaxf(fmaxf(top[rb], s[rb][i]), s[rb][i + 1]);
+      top[rb] = max_halves(top[rb]);
+      over |= (top[rb] - m[rb]) * c > kMostOver;  // -inf - -inf is NaN: nothing seen yet, nothing over
+    }
+    if (__any(over)) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = j0 + kb * 32 + 8 * (i / 4) + 4 * half + i % 4;
-            const bool see = j < min(end, hi[rb]) && (j >= lo[rb] || j < a.sinks);
-            s[rb][kb][i] = see ? s[rb][kb][i] : -__builtin_inff();
-          }
-      }
-      float top = s[rb][0][0];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[rb][kb][i]);
-      top = max_halves(top);
-      if (__any((top - m[rb]) * c > 8.f || (m[rb] == -__builtin_inff() && top > m[rb]))) {
-        const float m_new = fmaxf(m[rb], top);
+      for (int rb = 0; rb < RB; ++rb) {
+        const float m_new = fmaxf(m[rb], top[rb]);
         const float mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c;
         const float fix = m[rb] == -__builtin_inff() ? 0.f : exp2f(mc[rb] - mc_new);
         m[rb] = m_new;
         mc[rb] = mc_new;
-        l[rb] *= fix;
+        l[rb][0] *= fix;
+        l[rb][1] *= fix;
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[rb][db] *= fix;
       }
+    }
+    int p16[RB][8];  // e^S^T in 16 bits, two keys a register
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+    for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][kb][i], c, -mc[rb]));
-          s[rb][kb][i] = p;
-          l[rb] += p;
-        }
+      for (int i = 0; i < 16; ++i) {
+        s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], c, -mc[rb]));
+        l[rb][i & 1] += s[rb][i];
+      }
       if constexpr (kIs16<T>) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) p16[rb][kb][i] = pack2<T>(s[rb][kb][2 * i], s[rb][kb][2 * i + 1]);
+        for (int i = 0; i < 8; ++i) p16[rb][i] = pack2<T>(s[rb][2 * i], s[rb][2 * i + 1]);
       }
     }
-
     // O^T += V^T e^S^T.  16 bits: 16 keys a step, of which the halves take
     // keys 0-3, 8-11 and 4-7, 12-15.  f32: two keys a step, 4 apart.
+    if constexpr (kIs16<T>) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      if constexpr (kIs16<T>) {
+      for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int st = 0; st < 2; ++st)
+        for (int db = 0; db < DB; ++db) {
+          int4v x;
 #pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            int4v x;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int r = kb * 32 + 16 * st + 8 * h + 4 * half + (lane & 15) / 4;
-              const int d = 32 * db + (lane & 16) + 4 * (lane & 3);
-              const char* p = vt + r * ROW_BYTES + v_slot<ROW_BYTES>(r, d / 8) * 16 + (d % 8) * 2;
-              const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (__attribute__((address_space(3))) short4v*)p);
-              const int2v z = __builtin_bit_cast(int2v, y);
-              x[2 * h] = z[0];
-              x[2 * h + 1] = z[1];
-            }
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-              const int4v p = {p16[rb][kb][4 * st], p16[rb][kb][4 * st + 1], p16[rb][kb][4 * st + 2],
-                               p16[rb][kb][4 * st + 3]};
-              o[rb][db] = mma32<T>(x, p, o[rb][db]);
-            }
+          for (int h = 0; h < 2; ++h) {
+            const int r = 16 * st + 8 * h + 4 * half + (lane & 15) / 4;
+            const int d = 32 * db + (lane & 16) + 4 * (lane & 3);
+            const char* p = vt + (kb * 32 + r) * ROW_BYTES + v_slot<ROW_BYTES>(r, d / 8) * 16 + (d % 8) * 2;
+            const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) short4v*)p);
+            const int2v z = __builtin_bit_cast(int2v, y);
+            x[2 * h] = z[0];
+            x[2 * h + 1] = z[1];
           }
-      } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const int r = kb * 32 + 8 * (i / 4) + 4 * half + i % 4;
-            const float x = *reinterpret_cast<const float*>(vt + r * ROW_BYTES + (32 * db + col) * 4);
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-              o[rb][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[rb][kb][i], o[rb][db], 0, 0, 0);
+          for (int rb = 0; rb < RB; ++rb) {
+            const int4v p = {p16[rb][4 * st], p16[rb][4 * st + 1], p16[rb][4 * st + 2], p16[rb][4 * st + 3]};
+            o[rb][db] = mma32<T>(x, p, o[rb][db]);
           }
-      }
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const int r = kb * 32 + 8 * (i / 4) + 4 * half + i % 4;
+          const float x = *reinterpret_cast<const float*>(vt + r * ROW_BYTES + (32 * db + col) * 4);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb)
+            o[rb][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[rb][i], o[rb][db], 0, 0, 0);
+        }
     }
-  }
+  };
 
-  if constexpr (!CLEAN) {
+  for (;;) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      m[rb] = -__builtin_inff();
+      mc[rb] = l[rb][0] = l[rb][1] = 0.f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[rb][db] = f32x16(0.f);
+    }
+
+    int j0, end, buf = 0;
+    tile_at(w.t0, j0, end);
+    if (w.t0 < w.t1) stage(j0, end, 0);
+    for (int t = w.t0; t < w.t1; ++t, buf ^= 1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const int j0_now = j0, end_now = end;
+      if (t + 1 < w.t1) {
+        j0 += KT;
+        if (t + 1 == w.sink_tiles) j0 = w.start, end = w.end;
+        stage(j0, end, buf ^ 1);
+      }
+      const char* kt = lds + buf * 2 * TILE;
+      const char* vt = kt + TILE;
+      asm volatile("" : "+v"(clean));  // one loop for both walks
+      if (__builtin_amdgcn_readfirstlane(clean)) {
+        find_bad<T, DP, KB, WAVES>(lds + buf * 2 * TILE + TILE, bad);
+        for (int x = 0; x < KT; ++x) {
+          const int j = j0_now + x;
+          if (!(bad[x / 32] >> (x % 32) & 1u)) continue;
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb)
+            hit |= (j < min(end_now, hi[rb]) && (j >= lo[rb] || j < a.sinks)) << rb;
+        }
+      }
+      if (j0_now >= hi_last || (j0_now + KT <= lo_first && j0_now >= a.sinks)) continue;
+      const bool whole = j0_now + KT <= min(end_now, hi_first) && (j0_now >= lo_last || j0_now + KT <= a.sinks) &&
+                         wave_row + 32 * RB <= w.rows;
+
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) key_step(whole, kt, vt, kb, j0_now, end_now);
+    }
+
+    if (__builtin_amdgcn_readfirstlane(clean)) break;
     float off = 0.f;  // NaN when one of the sums is not finite
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
@@ -483,22 +540,23 @@ __device__ __forceinline__ bool attend_pass(const AttendArgs& a, const Walk& w, 
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) off = __builtin_fmaf(o[rb][db][i], 0.f, off);
-    if (__syncthreads_or(off != off)) return false;
+    clean = __syncthreads_or(off != off);
+    if (!__builtin_amdgcn_readfirstlane(clean)) break;
   }
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    l[rb] = sum_halves(l[rb]);
+    const float sum = sum_halves(l[rb][0] + l[rb][1]);
     const uint32_t r = wave_row + rb * 32 + col;
     const int t = w.token(r), g = static_cast<int>(min(r, w.rows - 1) - static_cast<uint32_t>(t) * w.group);
     const int64_t item = (w.q0 + t) * a.q_heads + w.hk * w.group + g;
     const bool odd = r < w.rows && (hit >> rb & 1);
     if (r < w.rows && !odd) {
-      const float inv = l[rb] == 0.f ? 0.f : 1.f / l[rb];
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       if (w.splits > 1) {
         float* part = a.part + (w.split * a.n_q * a.q_heads + item) * (a.dim + 2);
         if (half == 0) {
-          part[0] = l[rb] == 0.f ? -__builtin_inff() : mc[rb];
-          part[1] = l[rb];
+          part[0] = sum == 0.f ? -__builtin_inff() : mc[rb];
+          part[1] = sum;
         }
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -572,7 +630,6 @@ __device__ __forceinline__ bool attend_pass(const AttendArgs& a, const Walk& w, 
       }
     }
   }
-  return true;
 }
 
 template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
@@ -611,8 +668,7 @@ __global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP)) attend_k
   const int tiles = w.sink_tiles + (w.end - w.start + KT - 1) / KT, each = (tiles + splits - 1) / splits;
   w.t0 = min(w.split * each, tiles);
   w.t1 = min(w.t0 + each, tiles);
-  if (!attend_pass<T, DP, RB, KB, WAVES, ALIGNED, false>(a, w, k, v, lds))
-    attend_pass<T, DP, RB, KB, WAVES, ALIGNED, true>(a, w, k, v, lds);
+  attend_walk<T, DP, RB, KB, WAVES, ALIGNED>(a, w, k, v, lds);
 }
 
 // Joins the splits of each row: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s

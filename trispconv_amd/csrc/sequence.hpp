@@ -56,12 +56,14 @@ __device__ __forceinline__ int pack2(float a, float b) {
     return __builtin_bit_cast(int, __builtin_convertvector(v, bf16x2));
 }
 
-// 16 bytes per lane from each lane's global address into LDS at byte address
-// m0 (wave uniform) + 16 * lane, without passing through registers.  The
-// compiler does not know of the load: the kernels wait for it themselves.
-// Nothing else in these kernels uses M0.
-__device__ __forceinline__ void load_to_lds(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "s"(m0) : "memory");
+// 16 bytes per lane from base (wave uniform) + offset into LDS at byte address
+// m0 (wave uniform) + 16 * lane, without passing through registers; lanes
+// that are not in leave their place as it is.  The compiler does not know of
+// the load: the kernels wait for it themselves.  Nothing else in these
+// kernels uses M0.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t m0, bool in = true) {
+  if (in)
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(m0) : "memory");
 }
 
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
