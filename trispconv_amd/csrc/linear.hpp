@@ -1,0 +1,365 @@
+// y = act(x W^T + bias) + residual for the rows of a feature tensor.
+//
+//   v[r][o] = sum_i x[r][i] w[o][i]  (f32 sums),  v += bias[o],
+//   v = act(v),  v += residual[r][o],  one rounding to the rows' type.
+#pragma once
+
+#include "activation.hpp"
+#include "sequence.hpp"
+
+#include <algorithm>
+
+namespace tsc {
+
+struct LinearArgs {
+  const void* x;
+  int64_t x_stride;
+  const void* w;
+  int64_t w_stride;
+  const void* bias;
+  int bias_dtype;
+  const void* residual;
+  int64_t r_stride;
+  int act;
+  void* out;
+  int64_t n;
+  int c_in, c_out;
+};
+
+template <typename T>
+int launch_linear(const LinearArgs& a, hipStream_t s);
+
+namespace {
+
+__device__ __forceinline__ float activate_any(int act, float v) {
+  switch (act) {
+    case TSC_ACT_RELU: return activate<TSC_ACT_RELU>(v);
+    case TSC_ACT_GELU: return activate<TSC_ACT_GELU>(v);
+    case TSC_ACT_GELU_TANH: return activate<TSC_ACT_GELU_TANH>(v);
+    case TSC_ACT_SILU: return activate<TSC_ACT_SILU>(v);
+    default: return v;
+  }
+}
+
+// ------------------------------------------------------------- few rows --
+// Up to kFewRows rows: a wave per output column, the lanes share out the
+// inputs.  Bound by reading W once.
+constexpr int kFewRows = 8;
+
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(256) linear_few_kernel(LinearArgs a) {
+  constexpr int P = kPer16<T>;
+  const int lane = threadIdx.x % kWave;
+  const int o = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
+  if (o >= a.c_out) return;
+  const T* x = static_cast<const T*>(a.x);
+  const T* w = static_cast<const T*>(a.w) + o * a.w_stride;
+  float acc[ROWS] = {};
+  for (int i = lane * P; i < a.c_in; i += kWave * P) {
+    const bool whole = i + P <= a.c_in;
+    const int4v wv = whole ? load16_unaligned(w + i) : load16_partial(w + i, a.c_in - i);
+    T we[P];
+    __builtin_memcpy(we, &wv, 16);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (r >= a.n) break;
+      const T* xr = x + r * a.x_stride + i;
+      const int4v xv = whole ? load16_unaligned(xr) : load16_partial(xr, a.c_in - i);
+      T xe[P];
+      __builtin_memcpy(xe, &xv, 16);
+#pragma unroll
+      for (int e = 0; e < P; ++e) acc[r] = __builtin_fmaf(to_f32(xe[e]), to_f32(we[e]), acc[r]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) acc[r] += __shfl_xor(acc[r], d, kWave);
+    if (lane == r && r < a.n) {
+      float v = acc[r];
+      if (a.bias) v += load_any(a.bias, a.bias_dtype, o);
+      v = activate_any(a.act, v);
+      if (a.residual) v += to_f32(static_cast<const T*>(a.residual)[r * a.r_stride + o]);
+      static_cast<T*>(a.out)[(int64_t)r * a.c_out + o] = from_f32<T>(v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- tiles --
+// 16-byte chunk c of row r of an operand tile is stored in slot c ^ s(r): the
+// 8 lanes that read one chunk of 8 rows find them in different banks.
+template <int RB>
+__device__ __forceinline__ int tile_slot(int r, int c) {
+  return RB == 64 ? c ^ ((r >> 1) & 3) : c ^ (r & 7);
+}
+
+// ROWS rows of RB bytes of an operand, one k tile after the other.
+template <typename T, int ROWS, int RB, int THREADS, bool ALIGNED>
+struct OperandStage {
+  static constexpr int CH = RB / 16, ROUNDS = ROWS * CH / THREADS;
+  static_assert(ROWS * CH % THREADS == 0 && THREADS % (8 * CH) == 0, "whole rounds of like lanes");
+  const T* src;       // the lane's row in round 0, at its chunk
+  uint32_t offset[ROUNDS];
+  const T* base;
+  int chunk, first_row, rows_left, wave;
+  int64_t stride;
+  int4v held[ALIGNED ? 1 : ROUNDS];
+
+  // rows from `row` on of a tensor with `rows` of them; the ones past the
+  // last are the last again (their products are never stored)
+  __device__ __forceinline__ void begin(const T* p, int64_t stride_, int64_t row, int64_t rows) {
+    const int lane = threadIdx.x % kWave;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    base = p + row * stride_;
+    stride = stride_;
+    rows_left = static_cast<int>(min(rows - row, (int64_t)ROWS));
+    const int slot = wave * kWave + lane;
+    first_row = slot / CH;
+    chunk = tile_slot<RB>(first_row, slot % CH);
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i)
+      offset[i] = static_cast<uint32_t>(min(first_row + i * (THREADS / CH), rows_left - 1) * stride * (int)sizeof(T)) +
+                  chunk * 16;
+  }
+  // k tile kt (of `left` values from its first one on) into LDS (ALIGNED) or registers
+  __device__ __forceinline__ void load(int kt, int left, char* tile) {
+    const T* at = base + (int64_t)kt * (RB / (int)sizeof(T));
+    if constexpr (ALIGNED) {
+      const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_address(tile) + wave * 1024);
+      if (left >= RB / (int)sizeof(T)) {
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) load_to_lds(at, offset[i], m0 + i * THREADS * 16);
+      } else {
+        const bool in = chunk * kPer16<T> < left;
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) {
+          load_to_lds(at, offset[i], m0 + i * THREADS * 16, in);
+          if (!in) *reinterpret_cast<int4v*>(tile + (i * THREADS + threadIdx.x) * 16) = int4v(0);
+        }
+      }
+    } else {
+      const int have = left - chunk * kPer16<T>;
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) {
+        const T* p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(at) + offset[i]);
+        held[i] = have >= kPer16<T> ? load16_unaligned(p) : load16_partial(p, have);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* tile) const {
+    if constexpr (!ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i)
+        *reinterpret_cast<int4v*>(tile + (i * THREADS + threadIdx.x) * 16) = held[i];
+    }
+  }
+};
+
+// A tile of BM rows by BN columns, WM x WN waves, each MW x NW of it in 32x32
+// blocks: columns of W as the rows of the product, rows of x as its columns.
+// Operand tiles of RB bytes a row go round STAGES buffers of LDS through
+// direct-to-LDS loads, one barrier a tile.  The sums leave through LDS, so that
+// rows are written (and the residual read) as whole 16-byte pieces side by
+// side, with a lane's eight columns, and so its bias, the same in every row.
+template <typename T, int BM, int BN, int WM, int WN, int RB, int STAGES, bool ALIGNED, int OCC>
+__global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearArgs a, int tiles_m, int tiles_n) {
+  constexpr int THREADS = kWave * WM * WN, MW = BM / WM, NW = BN / WN, MB = MW / 32, NB = NW / 32;
+  constexpr int STAGE = (BM + BN) * RB, KT = RB / (int)sizeof(T), STEPS = RB / 32;
+  constexpr int LOADS = (BM + BN) * RB / 16 / THREADS;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+
+  // Tiles next to each other run on one XCD (workgroups go round the eight in
+  // turn), eight bands of rows at a time: they share W's tiles and x's bands
+  // in its L2.
+  const int tiles = tiles_m * tiles_n, per = (tiles + 7) / 8;
+  const int id = blockIdx.x % 8 * per + blockIdx.x / 8;
+  if ((int)blockIdx.x / 8 >= per || id >= tiles) return;
+  constexpr int BANDS = 8;
+  const int group = id / (BANDS * tiles_n), in_group = id - group * BANDS * tiles_n;
+  const int bands = min(BANDS, tiles_m - group * BANDS);
+  const int tn = in_group / bands, tm = group * BANDS + in_group - tn * bands;
+  const int64_t row0 = (int64_t)tm * BM;
+  const int col0 = tn * BN;
+
+  OperandStage<T, BM, RB, THREADS, ALIGNED> xs;
+  OperandStage<T, BN, RB, THREADS, ALIGNED> ws;
+  xs.begin(static_cast<const T*>(a.x), a.x_stride, row0, a.n);
+  ws.begin(static_cast<const T*>(a.w), a.w_stride, col0, a.c_out);
+  auto load = [&](int kt) {
+    char* tile = lds + kt % STAGES * STAGE;
+    xs.load(kt, a.c_in - kt * KT, tile);
+    ws.load(kt, a.c_in - kt * KT, tile + BM * RB);
+  };
+  auto store = [&](int kt) {
+    char* tile = lds + kt % STAGES * STAGE;
+    xs.store(tile);
+    ws.store(tile + BM * RB);
+  };
+
+  f32x16 acc[NB][MB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = f32x16(0.f);
+
+  const int kts = (a.c_in + KT - 1) / KT;
+  const int mrow = wave / WN * MW + col, nrow = wave % WN * NW + col;
+  for (int kt = 0; kt < STAGES - 1 && kt < kts; ++kt) {
+    load(kt);
+    if (!ALIGNED) store(kt);
+  }
+  for (int kt = 0; kt < kts; ++kt) {
+    if constexpr (ALIGNED) {
+      // loads finish in order: with STAGES - 2 later tiles of LOADS each in
+      // flight, this one is there; near the end (where a partial tile may be
+      // fewer loads) wait for all
+      if (kt + STAGES - 1 < kts) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 2) * LOADS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    } else {
+      __syncthreads();
+    }
+    const bool more = kt + STAGES - 1 < kts;
+    if (more) load(kt + STAGES - 1);
+    const char* xt = lds + kt % STAGES * STAGE;
+    const char* wt = xt + BM * RB;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      int4v xf[MB], wf[NB];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+        xf[mb] = *reinterpret_cast<const int4v*>(xt + (mrow + mb * 32) * RB + tile_slot<RB>(mrow, 2 * st + half) * 16);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+        wf[nb] = *reinterpret_cast<const int4v*>(wt + (nrow + nb * 32) * RB + tile_slot<RB>(nrow, 2 * st + half) * 16);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mma32<T>(wf[nb], xf[mb], acc[nb][mb]);
+    }
+    if (!ALIGNED && more) store(kt + STAGES - 1);
+  }
+  __syncthreads();
+
+  // 32 rows of the wave at a time through its own LDS
+  constexpr int LINE = NW * 4 + 16, LANES = NW / 8, ROWS = kWave / LANES;
+  char* mine = lds + wave * 32 * LINE;
+  const int o = col0 + wave % WN * NW + lane % LANES * 8;
+  const int have = a.c_out - o;  // of the lane's eight columns
+  float bias[8] = {};
+  if (a.bias) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < have) bias[e] = load_any(a.bias, a.bias_dtype, o + e);
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 v = {acc[nb][mb][4 * i], acc[nb][mb][4 * i + 1], acc[nb][mb][4 * i + 2], acc[nb][mb][4 * i + 3]};
+        *reinterpret_cast<f32x4*>(mine + col * LINE + (nb * 32 + 8 * i + 4 * half) * 4) = v;
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+    for (int i = 0; i < 32 / ROWS; ++i) {
+      const int r = i * ROWS + lane / LANES;
+      const int64_t row = row0 + wave / WN * MW + mb * 32 + r;
+      float v[8];
+      __builtin_memcpy(v, mine + r * LINE + lane % LANES * 32, 32);
+      if (row >= a.n || have <= 0) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] + bias[e];
+      switch (a.act) {
+        case TSC_ACT_RELU: for (float& e : v) e = activate<TSC_ACT_RELU>(e); break;
+        case TSC_ACT_GELU: for (float& e : v) e = activate<TSC_ACT_GELU>(e); break;
+        case TSC_ACT_GELU_TANH: for (float& e : v) e = activate<TSC_ACT_GELU_TANH>(e); break;
+        case TSC_ACT_SILU: for (float& e : v) e = activate<TSC_ACT_SILU>(e); break;
+        default: break;
+      }
+      T y[8];
+      if (a.residual) {
+        const T* res = static_cast<const T*>(a.residual) + row * a.r_stride + o;
+        if (have >= 8) {
+          __builtin_memcpy(y, res, sizeof y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += to_f32(y[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < have) v[e] += to_f32(res[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(v[e]);
+      T* out = static_cast<T*>(a.out) + row * a.c_out + o;
+      if (have >= 8) {
+        __builtin_memcpy(out, y, sizeof y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < have) out[e] = y[e];
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int RB, int STAGES, bool ALIGNED, int OCC>
+int launch_tile(const LinearArgs& a, hipStream_t s) {
+  constexpr int main_bytes = STAGES * (BM + BN) * RB, out_bytes = WM * WN * 32 * (BN / WN * 4 + 16);
+  constexpr int bytes = main_bytes > out_bytes ? main_bytes : out_bytes;
+  auto kernel = &linear_tile_kernel<T, BM, BN, WM, WN, RB, STAGES, ALIGNED, OCC>;
+  if (bytes > 65536)
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  const int64_t tm = ceil_div(a.n, BM), tn = ceil_div(a.c_out, BN), blocks = align_up(tm * tn, 8);
+  TSC_REQUIRE(blocks < (1ll << 31), "linear_act: too many tiles");
+  kernel<<<static_cast<unsigned>(blocks), kWave * WM * WN, bytes, s>>>(a, static_cast<int>(tm), static_cast<int>(tn));
+  TSC_LAUNCH_CHECK("linear_act");
+  return 0;
+}
+
+template <typename T, int ROWS>
+int launch_few(const LinearArgs& a, hipStream_t s) {
+  linear_few_kernel<T, ROWS><<<static_cast<unsigned>(ceil_div(a.c_out, 4)), 256, 0, s>>>(a);
+  TSC_LAUNCH_CHECK("linear_act_few");
+  return 0;
+}
+
+#ifndef TSC_BIG
+#define TSC_BIG 256, 128, 2, 2, 64, 3
+#define TSC_BIG_OCC 2
+#endif
+#ifndef TSC_MID
+#define TSC_MID 128, 128, 2, 2, 64, 3
+#define TSC_MID_OCC 2
+#endif
+
+template <typename T, bool ALIGNED>
+int launch_sized(const LinearArgs& a, hipStream_t s) {
+  const int64_t big = ceil_div(a.n, 256) * ceil_div(a.c_out, 128);
+  if (kIs16<T> && big >= 1024 && a.c_in >= 512) return launch_tile<T, TSC_BIG, ALIGNED, TSC_BIG_OCC>(a, s);
+  const int64_t mid = ceil_div(a.n, 128) * ceil_div(a.c_out, 128);
+  if (mid >= 256) return launch_tile<T, TSC_MID, ALIGNED, TSC_MID_OCC>(a, s);
+  return launch_tile<T, 64, 64, 2, 2, 128, 3, ALIGNED, 2>(a, s);
+}
+
+}  // namespace
+
+template <typename T>
+int launch_linear(const LinearArgs& a, hipStream_t s) {
+  if (a.n <= 1) return launch_few<T, 1>(a, s);
+  if (a.n <= kFewRows) return launch_few<T, kFewRows>(a, s);
+  const int64_t e = kPer16<T>;
+  // 16-byte pieces at 16-byte addresses, rows of a tile within 32-bit offsets
+  const bool aligned = a.c_in % e == 0 && a.x_stride % e == 0 && a.w_stride % e == 0 &&
+                       reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
+  const bool near = std::max(a.x_stride, a.w_stride) < (1 << 21);
+  TSC_REQUIRE(near, "linear_act: row strides over 2^21 elements are not supported");
+  return aligned ? launch_sized<T, true>(a, s) : launch_sized<T, false>(a, s);
+}
+
+}  // namespace tsc

@@ -43,6 +43,14 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+def _matrix(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """``t`` as the product kernels read it, and its row stride: rows
+    contiguous, less than 2^21 elements apart."""
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) >= 1 << 21 and t.shape[0] > 1):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0) if t.shape[0] > 1 else 0
+
+
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                activation: Optional[str] = None,
                residual: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -66,7 +74,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
                          "(N, C_in) and (C_out, C_in)")
     _same(weight, x, what, "weight")
     n, c_out = x.shape[0], weight.shape[0]
-    x, weight = _rows_of(x), _rows_of(weight)
+    (x, x_stride), (weight, w_stride) = _matrix(x), _matrix(weight)
     b_ptr = r_ptr = None
     b_code = r_stride = 0
     if bias is not None:
@@ -81,8 +89,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         residual = _rows_of(residual)
         r_ptr, r_stride = residual.data_ptr(), residual.stride(0)
     out = torch.empty((n, c_out), dtype=x.dtype, device=x.device)
-    L.check(L.lib().tsc_linear_act(x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
-                                   b_ptr, b_code, r_ptr, r_stride, code, n, x.shape[1], c_out,
+    L.check(L.lib().tsc_linear_act(x.data_ptr(), x_stride, weight.data_ptr(), w_stride, b_ptr,
+                                   b_code, r_ptr, r_stride, code, n, x.shape[1], c_out,
                                    _ACTS[activation], out.data_ptr(), L.stream_of(x)), what)
     return out
 
