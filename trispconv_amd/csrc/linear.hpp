@@ -85,6 +85,43 @@ __global__ void __launch_bounds__(256) linear_few_kernel(LinearArgs a) {
   }
 }
 
+// Eight neighbouring values at any alignment, of which `have` exist.
+template <typename T>
+struct Eight {
+  T e[8];
+  __device__ __forceinline__ void load(const T* p, int have) {
+    if (have >= 8) {
+      __builtin_memcpy(e, p, sizeof e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = i < have ? p[i] : from_f32<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int have) const {
+    if (have >= 8) {
+      __builtin_memcpy(p, e, sizeof e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < have) p[i] = e[i];
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load_eight_of(const void* p, int64_t at, int have, float v[8]) {
+  Eight<T> x;
+  x.load(static_cast<const T*>(p) + at, have);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f32(x.e[i]);
+}
+__device__ __forceinline__ void load_eight(const void* p, int dtype, int64_t at, int have, float v[8]) {
+  if (have <= 0) return;
+  if (dtype == TSC_F32) load_eight_of<float>(p, at, have, v);
+  else if (dtype == TSC_F16) load_eight_of<__half>(p, at, have, v);
+  else load_eight_of<__hip_bfloat16>(p, at, have, v);
+}
+
 // ---------------------------------------------------------------- tiles --
 // 16-byte chunk c of row r of an operand tile is stored in slot c ^ s(r): the
 // 8 lanes that read one chunk of 8 rows find them in different banks.
@@ -198,6 +235,13 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
     ws.store(tile + BM * RB);
   };
 
+  // what the epilogue needs of the bias is asked for first, long before its use
+  constexpr int LINE = NW * 4 + 16, LANES = NW / 8, ROWS = kWave / LANES;
+  const int o = col0 + wave % WN * NW + lane % LANES * 8;
+  const int have = a.c_out - o;  // of the lane's eight columns
+  float bias[8] = {};
+  if (a.bias) load_eight(a.bias, a.bias_dtype, o, have, bias);
+
   f32x16 acc[NB][MB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -244,18 +288,24 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
   __syncthreads();
 
   // 32 rows of the wave at a time through its own LDS
-  constexpr int LINE = NW * 4 + 16, LANES = NW / 8, ROWS = kWave / LANES;
   char* mine = lds + wave * 32 * LINE;
-  const int o = col0 + wave % WN * NW + lane % LANES * 8;
-  const int have = a.c_out - o;  // of the lane's eight columns
-  float bias[8] = {};
-  if (a.bias) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < have) bias[e] = load_any(a.bias, a.bias_dtype, o + e);
-  }
+  const int64_t wave_row = row0 + wave / WN * MW;
+  const uint32_t out_step = static_cast<uint32_t>(a.c_out) * sizeof(T);
+  const uint32_t out_at = lane / LANES * out_step + o * (uint32_t)sizeof(T);
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
+    const int64_t first = wave_row + mb * 32;
+    const int rows = static_cast<int>(min((int64_t)32, a.n - first));
+    if (rows <= 0) break;
+    Eight<T> res[32 / ROWS];
+    if (a.residual) {
+      const T* p = static_cast<const T*>(a.residual) + first * a.r_stride + o;
+#pragma unroll
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const int r = i * ROWS + lane / LANES;
+        if (r < rows) res[i].load(p + r * a.r_stride, have);
+      }
+    }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -264,15 +314,14 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
         *reinterpret_cast<f32x4*>(mine + col * LINE + (nb * 32 + 8 * i + 4 * half) * 4) = v;
       }
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
+    char* out = static_cast<char*>(a.out) + first * a.c_out * (int64_t)sizeof(T);
+#pragma unroll
     for (int i = 0; i < 32 / ROWS; ++i) {
       const int r = i * ROWS + lane / LANES;
-      const int64_t row = row0 + wave / WN * MW + mb * 32 + r;
       float v[8];
       __builtin_memcpy(v, mine + r * LINE + lane % LANES * 32, 32);
-      if (row >= a.n || have <= 0) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = v[e] + bias[e];
+      for (int e = 0; e < 8; ++e) v[e] += bias[e];
       switch (a.act) {
         case TSC_ACT_RELU: for (float& e : v) e = activate<TSC_ACT_RELU>(e); break;
         case TSC_ACT_GELU: for (float& e : v) e = activate<TSC_ACT_GELU>(e); break;
@@ -280,29 +329,14 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
         case TSC_ACT_SILU: for (float& e : v) e = activate<TSC_ACT_SILU>(e); break;
         default: break;
       }
-      T y[8];
       if (a.residual) {
-        const T* res = static_cast<const T*>(a.residual) + row * a.r_stride + o;
-        if (have >= 8) {
-          __builtin_memcpy(y, res, sizeof y);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += to_f32(y[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < have) v[e] += to_f32(res[e]);
-        }
+        for (int e = 0; e < 8; ++e) v[e] += to_f32(res[i].e[e]);
       }
+      Eight<T> y;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = from_f32<T>(v[e]);
-      T* out = static_cast<T*>(a.out) + row * a.c_out + o;
-      if (have >= 8) {
-        __builtin_memcpy(out, y, sizeof y);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < have) out[e] = y[e];
-      }
+      for (int e = 0; e < 8; ++e) y.e[e] = from_f32<T>(v[e]);
+      if (r < rows) y.store(reinterpret_cast<T*>(out + (out_at + i * ROWS * out_step)), have);
     }
     __builtin_amdgcn_wave_barrier();
   }
