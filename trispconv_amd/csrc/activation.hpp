@@ -24,7 +24,7 @@ __device__ __forceinline__ float times_sigmoid(float x, float y) {
 // for every output; the library's erff takes several times as many.
 __device__ __forceinline__ float gelu(float x) {
   // erfc is 0 in f32 long before 16: the limit keeps inf * 0 from being formed
-  const float u = fminf(__builtin_fabsf(x), 16.f);
+  const float u = __builtin_amdgcn_fmed3f(__builtin_fabsf(x), 0.f, 16.f);
   const float t = rcp_fast(__builtin_fmaf(0.3275911f * 0.70710678f, u, 1.f));
   // the coefficients, halved
   float p = __builtin_fmaf(0.5307027145f, t, -0.7265760135f);
@@ -33,7 +33,7 @@ __device__ __forceinline__ float gelu(float x) {
   p = __builtin_fmaf(p, t, 0.127414796f);
   // e^(-z^2) = 2^(-x^2 / (2 ln 2)); NaN for NaN
   const float e = exp2_fast(-0.72134752f * x * x);
-  return __builtin_fmaf(-u, p * t * e, fmaxf(x, 0.f));
+  return __builtin_fmaf(-u, p * t * e, __builtin_amdgcn_fmed3f(x, 0.f, __builtin_inff()));
 }
 
 template <int ACT>

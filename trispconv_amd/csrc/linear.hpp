@@ -334,8 +334,7 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
         for (int e = 0; e < 8; ++e) v[e] += to_f32(res[i].e[e]);
       }
       Eight<T> y;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y.e[e] = from_f32<T>(v[e]);
+      round_to<T, 8>(v, y.e);
       if (r < rows) y.store(reinterpret_cast<T*>(out + (out_at + i * ROWS * out_step)), have);
     }
     __builtin_amdgcn_wave_barrier();
@@ -364,18 +363,18 @@ int launch_few(const LinearArgs& a, hipStream_t s) {
 }
 
 #ifndef TSC_BIG
-#define TSC_BIG 256, 128, 2, 2, 64, 3
+#define TSC_BIG 256, 256, 2, 4, 128, 2
 #define TSC_BIG_OCC 2
 #endif
 #ifndef TSC_MID
-#define TSC_MID 128, 128, 2, 2, 64, 3
+#define TSC_MID 128, 128, 2, 2, 64, 2
 #define TSC_MID_OCC 2
 #endif
 
 template <typename T, bool ALIGNED>
 int launch_sized(const LinearArgs& a, hipStream_t s) {
-  const int64_t big = ceil_div(a.n, 256) * ceil_div(a.c_out, 128);
-  if (kIs16<T> && big >= 1024 && a.c_in >= 512) return launch_tile<T, TSC_BIG, ALIGNED, TSC_BIG_OCC>(a, s);
+  const int64_t big = ceil_div(a.n, 256) * ceil_div(a.c_out, 256);
+  if (kIs16<T> && big >= 200 && a.c_in >= 512) return launch_tile<T, TSC_BIG, ALIGNED, TSC_BIG_OCC>(a, s);
   const int64_t mid = ceil_div(a.n, 128) * ceil_div(a.c_out, 128);
   if (mid >= 256) return launch_tile<T, TSC_MID, ALIGNED, TSC_MID_OCC>(a, s);
   return launch_tile<T, 64, 64, 2, 2, 128, 3, ALIGNED, 2>(a, s);

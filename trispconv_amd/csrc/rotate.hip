@@ -6,7 +6,10 @@
 // (pair a*F + i) turns by t = p[a] * base^(-i/F):
 //   (u, w) -> (u cos t - w sin t, u sin t + w cos t);
 // pairs from A*F on stay.  Pair j is (j, j + D/2), or (2j, 2j + 1) interleaved.
-#include "common.hpp"
+#include "sequence.hpp"
+
+#include <algorithm>
+#include <cmath>
 
 namespace tsc {
 namespace {
@@ -32,12 +35,6 @@ struct RotateArgs {
   void* k_out;
 };
 
-__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
-  if (dtype == TSC_F32) return static_cast<const float*>(p)[i];
-  if (dtype == TSC_F16) return to_f32(static_cast<const __half*>(p)[i]);
-  return to_f32(static_cast<const __hip_bfloat16*>(p)[i]);
-}
-
 // Cosine and sine of p * base^(-i/F).  The angle is taken in turns in 64
 // bits: positions reach thousands, and an f32 angle of a thousand radians is
 // already 6e-5 off.  What is left after the whole turns fits f32.
@@ -48,6 +45,21 @@ __device__ __forceinline__ float2 turn_of(double p, int i, int F, double log2_ba
   float2 cs;
   sincospif(part, &cs.y, &cs.x);
   return cs;
+}
+
+// N gains as f32.
+template <int N>
+__device__ __forceinline__ void load_gain(const void* p, int dtype, int64_t at, float g[N]) {
+  auto as = [&](auto tag) {
+    using G = decltype(tag);
+    G e[N];
+    __builtin_memcpy(e, static_cast<const G*>(p) + at, sizeof e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = to_f32(e[i]);
+  };
+  if (dtype == TSC_F32) as(float{});
+  else if (dtype == TSC_F16) as(__half{});
+  else as(__hip_bfloat16{});
 }
 
 // A wave per row; a head takes LP lanes (a power of two from D/2 up, at most
@@ -110,8 +122,116 @@ __global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
   }
 }
 
+// The vector form: a workgroup takes ROWS rows; its threads first share out the
+// rows' angles (cosine and sine of every turning pair, to LDS: they are the
+// same for every head of q and k), then the heads' vectors. A head takes
+// LANES lanes, each two pieces of PIECE bytes: elements [l P, l P + P) of its
+// first and of its second half, which are pairs with each other (or one after
+// the other where pairs are neighbours), so that a pair never leaves its lane.
+// Bound by memory: each vector is read and written once, 16 bytes at a time.
+template <typename T, int DIM, int ROWS>
+__global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
+  constexpr int P = kPer16<T>, HALF = DIM / 2, LANES = DIM / (2 * P), HEADS = 256 / LANES;
+  __shared__ __align__(16) float2 turn[ROWS][HALF];
+  __shared__ double speed[HALF];
+  const int F = HALF / a.axes;
+  if (threadIdx.x < HALF)
+    speed[threadIdx.x] = F > 0 && threadIdx.x < a.axes * F
+                             ? exp2(-a.log2_base * (threadIdx.x % F) / F) * 0.15915494309189535 : 0.0;
+  __syncthreads();
+  const int total = a.q_heads + a.k_heads, l = threadIdx.x % LANES;
+  for (int64_t r0 = blockIdx.x * (int64_t)ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
+    const int rows = static_cast<int>(min((int64_t)ROWS, a.n - r0));
+    for (int x = threadIdx.x; x < rows * HALF; x += 256) {
+      const int r = x / HALF, j = x % HALF;
+      float2 cs = make_float2(1.f, 0.f);
+      if (j < a.axes * F) {
+        const int64_t at = (r0 + r) * a.pos_row + j / F;
+        const double p = a.pos_float ? static_cast<const float*>(a.pos)[at]
+                                     : static_cast<const int32_t*>(a.pos)[at];
+        const double t = p * speed[j];
+        sincospif(static_cast<float>(2.0 * (t - rint(t))), &cs.y, &cs.x);
+      }
+      turn[r][j] = cs;
+    }
+    __syncthreads();
+    for (int v = threadIdx.x / LANES; v < rows * total; v += HEADS) {
+      const int r = v / total, h = v % total;
+      const bool is_q = h < a.q_heads;
+      const int hh = is_q ? h : h - a.q_heads;
+      const int64_t row = r0 + r;
+      const T* src = static_cast<const T*>(is_q ? a.q : a.k) +
+                     (is_q ? row * a.q_row + hh * a.q_head : row * a.k_row + hh * a.k_head);
+      T* dst = static_cast<T*>(is_q ? a.q_out : a.k_out) +
+               (row * (is_q ? a.q_heads : a.k_heads) + hh) * DIM;
+      // the lane's elements: [first, first + P) and [second, second + P)
+      const int first = a.interleaved ? 2 * P * l : P * l, second = first + (a.interleaved ? P : HALF);
+      T e[2 * P];
+      __builtin_memcpy(e, src + first, 16);
+      __builtin_memcpy(e + P, src + second, 16);
+      float x[2 * P], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * P; ++i) {
+        x[i] = to_f32(e[i]);
+        sum = __builtin_fmaf(x[i], x[i], sum);
+      }
+#pragma unroll
+      for (int d = 1; d < LANES; d <<= 1) sum += __shfl_xor(sum, d, kWave);
+      const float inv = 1.f / sqrtf(sum * (1.f / DIM) + a.eps);
+      const void* gain = is_q ? a.q_gain : a.k_gain;
+      if (gain) {
+        const int64_t at = (int64_t)hh * (is_q ? a.q_gain_head : a.k_gain_head);
+        float g[2 * P];
+        load_gain<P>(gain, a.gain_dtype, at + first, g);
+        load_gain<P>(gain, a.gain_dtype, at + second, g + P);
+#pragma unroll
+        for (int i = 0; i < 2 * P; ++i) x[i] *= inv * g[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * P; ++i) x[i] *= inv;
+      }
+      float y[2 * P];
+      const float2* cs = &turn[r][P * l];
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          y[2 * i] = x[2 * i] * cs[i].x - x[2 * i + 1] * cs[i].y;
+          y[2 * i + 1] = x[2 * i] * cs[i].y + x[2 * i + 1] * cs[i].x;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          y[i] = x[i] * cs[i].x - x[P + i] * cs[i].y;
+          y[P + i] = x[i] * cs[i].y + x[P + i] * cs[i].x;
+        }
+      }
+      round_to<T, 2 * P>(y, e);
+      __builtin_memcpy(dst + first, e, 16);
+      __builtin_memcpy(dst + second, e + P, 16);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int DIM>
+int launch_vector(const RotateArgs& a, hipStream_t s) {
+  constexpr int ROWS = 8;
+  const int64_t blocks = std::min<int64_t>(ceil_div(a.n, ROWS), 16384);
+  rotate_vector_kernel<T, DIM, ROWS><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+  TSC_LAUNCH_CHECK("norm_rotate_heads");
+  return 0;
+}
+
 template <typename T>
 int launch_rotate(const RotateArgs& a, hipStream_t s) {
+  // head sizes whose pairs fill whole 16-byte pieces of whole lanes
+  switch (a.dim) {
+    case 32: return launch_vector<T, 32>(a, s);
+    case 64: return launch_vector<T, 64>(a, s);
+    case 128: return launch_vector<T, 128>(a, s);
+    case 256: return launch_vector<T, 256>(a, s);
+    default: break;
+  }
   int lp = 1;
   while (lp < kWave && lp < a.dim / 2) lp *= 2;
   rotate_any_kernel<T><<<static_cast<unsigned>(ceil_div(a.n, 4)), 256, 0, s>>>(a, lp);

@@ -56,6 +56,19 @@ __device__ __forceinline__ int pack2(float a, float b) {
     return __builtin_bit_cast(int, __builtin_convertvector(v, bf16x2));
 }
 
+// N (even) f32 values rounded to T.
+template <typename T, int N>
+__device__ __forceinline__ void round_to(const float* v, T* e) {
+  if constexpr (kIs16<T>) {
+    int w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    __builtin_memcpy(e, w, N * sizeof(T));
+  } else {
+    __builtin_memcpy(e, v, N * sizeof(T));
+  }
+}
+
 // 16 bytes per lane from base (wave uniform) + offset into LDS at byte address
 // m0 (wave uniform) + 16 * lane, without passing through registers; lanes
 // that are not in leave their place as it is.  The compiler does not know of
