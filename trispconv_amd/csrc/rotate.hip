@@ -35,16 +35,18 @@ struct RotateArgs {
   void* k_out;
 };
 
-// Cosine and sine of p * base^(-i/F).  The angle is taken in turns in 64
-// bits: positions reach thousands, and an f32 angle of a thousand radians is
-// already 6e-5 off.  What is left after the whole turns fits f32.
-__device__ __forceinline__ float2 turn_of(double p, int i, int F, double log2_base) {
-  const double speed = exp2(-log2_base * i / F) * 0.15915494309189535;
+// Cosine and sine of position p times a pair's speed, base^(-i/F) / 2 pi turns.
+// The angle is taken in 64 bits: positions reach thousands, and an f32 angle
+// of a thousand radians is already 6e-5 off.  What is left after the whole
+// turns fits f32.
+__device__ __forceinline__ float2 turn_of(double p, double speed) {
   const double t = p * speed;
-  const float part = static_cast<float>(2.0 * (t - rint(t)));
   float2 cs;
-  sincospif(part, &cs.y, &cs.x);
+  sincospif(static_cast<float>(2.0 * (t - rint(t))), &cs.y, &cs.x);
   return cs;
+}
+__device__ __forceinline__ double speed_of(int i, int F, double log2_base) {
+  return exp2(-log2_base * i / F) * 0.15915494309189535;
 }
 
 // N gains as f32.
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
       const int64_t at = r * a.pos_row + j / F;
       const double p = a.pos_float ? static_cast<const float*>(a.pos)[at]
                                    : static_cast<const int32_t*>(a.pos)[at];
-      cs[u] = turn_of(p, j % F, F, a.log2_base);
+      cs[u] = turn_of(p, speed_of(j % F, F, a.log2_base));
     }
   }
   const int total = a.q_heads + a.k_heads;
@@ -122,62 +124,70 @@ __global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
   }
 }
 
-// The vector form: a workgroup takes ROWS rows; its threads first share out the
+// The vector form: a workgroup takes kRows rows; its threads first share out the
 // rows' angles (cosine and sine of every turning pair, to LDS: they are the
-// same for every head of q and k), then the heads' vectors. A head takes
-// LANES lanes, each two pieces of PIECE bytes: elements [l P, l P + P) of its
-// first and of its second half, which are pairs with each other (or one after
-// the other where pairs are neighbours), so that a pair never leaves its lane.
-// Bound by memory: each vector is read and written once, 16 bytes at a time.
-template <typename T, int DIM, int ROWS>
+// same for every head of q and k), then the heads.  A head takes LANES lanes (a
+// power of two; the last may idle), each two pieces of P elements: [l P,
+// l P + P) of its first and of its second half, which are pairs with each other
+// (or one after the other where pairs are neighbours), so that a pair never
+// leaves its lane.  Bound by memory: each vector is read and written once.
+// 500k rows of 12 + 12 heads of 64, bf16: 607 us, 5.07 TB/s (a large copy on
+// this card: 4.86).
+constexpr int kRows = 8, kMaxHalf = 128;
+
+template <typename T, int P, int LANES>
 __global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
-  constexpr int P = kPer16<T>, HALF = DIM / 2, LANES = DIM / (2 * P), HEADS = 256 / LANES;
-  __shared__ __align__(16) float2 turn[ROWS][HALF];
-  __shared__ double speed[HALF];
-  const int F = HALF / a.axes;
-  if (threadIdx.x < HALF)
-    speed[threadIdx.x] = F > 0 && threadIdx.x < a.axes * F
-                             ? exp2(-a.log2_base * (threadIdx.x % F) / F) * 0.15915494309189535 : 0.0;
+  constexpr int HEADS = 256 / LANES, BYTES = P * sizeof(T);
+  __shared__ __align__(16) float2 turn[kRows][kMaxHalf];
+  __shared__ double speed[kMaxHalf];
+  const int half = a.dim / 2, F = half / a.axes;
+  if (threadIdx.x < half)
+    speed[threadIdx.x] = F > 0 && (int)threadIdx.x < a.axes * F
+                             ? speed_of(threadIdx.x % F, F, a.log2_base) : 0.0;
   __syncthreads();
   const int total = a.q_heads + a.k_heads, l = threadIdx.x % LANES;
-  for (int64_t r0 = blockIdx.x * (int64_t)ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
-    const int rows = static_cast<int>(min((int64_t)ROWS, a.n - r0));
-    for (int x = threadIdx.x; x < rows * HALF; x += 256) {
-      const int r = x / HALF, j = x % HALF;
+  const bool in = LANES == 1 || l * P < half;
+  const float over = 1.f / a.dim;
+  // the lane's elements of a head: [first, first + P) and [second, second + P)
+  const int first = in ? (a.interleaved ? 2 * P * l : P * l) : 0, second = first + (a.interleaved ? P : half);
+  for (int64_t r0 = blockIdx.x * (int64_t)kRows; r0 < a.n; r0 += (int64_t)gridDim.x * kRows) {
+    const int rows = static_cast<int>(min((int64_t)kRows, a.n - r0));
+    for (int x = threadIdx.x; x < rows * half; x += 256) {
+      const int r = x / half, j = x - r * half;
       float2 cs = make_float2(1.f, 0.f);
       if (j < a.axes * F) {
         const int64_t at = (r0 + r) * a.pos_row + j / F;
         const double p = a.pos_float ? static_cast<const float*>(a.pos)[at]
                                      : static_cast<const int32_t*>(a.pos)[at];
-        const double t = p * speed[j];
-        sincospif(static_cast<float>(2.0 * (t - rint(t))), &cs.y, &cs.x);
+        cs = turn_of(p, speed[j]);
       }
       turn[r][j] = cs;
     }
     __syncthreads();
     for (int v = threadIdx.x / LANES; v < rows * total; v += HEADS) {
-      const int r = v / total, h = v % total;
+      const int r = v / total, h = v - r * total;
       const bool is_q = h < a.q_heads;
       const int hh = is_q ? h : h - a.q_heads;
       const int64_t row = r0 + r;
       const T* src = static_cast<const T*>(is_q ? a.q : a.k) +
                      (is_q ? row * a.q_row + hh * a.q_head : row * a.k_row + hh * a.k_head);
       T* dst = static_cast<T*>(is_q ? a.q_out : a.k_out) +
-               (row * (is_q ? a.q_heads : a.k_heads) + hh) * DIM;
-      // the lane's elements: [first, first + P) and [second, second + P)
-      const int first = a.interleaved ? 2 * P * l : P * l, second = first + (a.interleaved ? P : HALF);
+               (row * (is_q ? a.q_heads : a.k_heads) + hh) * a.dim;
       T e[2 * P];
-      __builtin_memcpy(e, src + first, 16);
-      __builtin_memcpy(e + P, src + second, 16);
-      float x[2 * P], sum = 0.f;
+      float x[2 * P] = {}, sum = 0.f;
+      if (in) {
+        __builtin_memcpy(e, src + first, BYTES);
+        __builtin_memcpy(e + P, src + second, BYTES);
 #pragma unroll
-      for (int i = 0; i < 2 * P; ++i) {
-        x[i] = to_f32(e[i]);
-        sum = __builtin_fmaf(x[i], x[i], sum);
+        for (int i = 0; i < 2 * P; ++i) {
+          x[i] = to_f32(e[i]);
+          sum = __builtin_fmaf(x[i], x[i], sum);
+        }
       }
 #pragma unroll
       for (int d = 1; d < LANES; d <<= 1) sum += __shfl_xor(sum, d, kWave);
-      const float inv = 1.f / sqrtf(sum * (1.f / DIM) + a.eps);
+      if (!in) continue;
+      const float inv = 1.f / sqrtf(sum * over + a.eps);
       const void* gain = is_q ? a.q_gain : a.k_gain;
       if (gain) {
         const int64_t at = (int64_t)hh * (is_q ? a.q_gain_head : a.k_gain_head);
@@ -206,32 +216,40 @@ __global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
         }
       }
       round_to<T, 2 * P>(y, e);
-      __builtin_memcpy(dst + first, e, 16);
-      __builtin_memcpy(dst + second, e + P, 16);
+      __builtin_memcpy(dst + first, e, BYTES);
+      __builtin_memcpy(dst + second, e + P, BYTES);
     }
     __syncthreads();
   }
 }
 
-template <typename T, int DIM>
+template <typename T, int P, int LANES>
 int launch_vector(const RotateArgs& a, hipStream_t s) {
-  constexpr int ROWS = 8;
-  const int64_t blocks = std::min<int64_t>(ceil_div(a.n, ROWS), 16384);
-  rotate_vector_kernel<T, DIM, ROWS><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+  const int64_t blocks = std::min<int64_t>(ceil_div(a.n, kRows), 16384);
+  rotate_vector_kernel<T, P, LANES><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
   TSC_LAUNCH_CHECK("norm_rotate_heads");
   return 0;
 }
 
+template <typename T, int P>
+int launch_lanes(const RotateArgs& a, hipStream_t s) {
+  const int lanes = a.dim / 2 / P;
+  if (lanes <= 1) return launch_vector<T, P, 1>(a, s);
+  if (lanes <= 2) return launch_vector<T, P, 2>(a, s);
+  if (lanes <= 4) return launch_vector<T, P, 4>(a, s);
+  if (lanes <= 8) return launch_vector<T, P, 8>(a, s);
+  if (lanes <= 16) return launch_vector<T, P, 16>(a, s);
+  return launch_vector<T, P, 32>(a, s);
+}
+
 template <typename T>
 int launch_rotate(const RotateArgs& a, hipStream_t s) {
-  // head sizes whose pairs fill whole 16-byte pieces of whole lanes
-  switch (a.dim) {
-    case 32: return launch_vector<T, 32>(a, s);
-    case 64: return launch_vector<T, 64>(a, s);
-    case 128: return launch_vector<T, 128>(a, s);
-    case 256: return launch_vector<T, 256>(a, s);
-    default: break;
-  }
+  // half a head in whole pieces of 16 bytes, or 8 for 16-bit values; head
+  // sizes that are neither (2, 6, 250) go value by value
+  const int half = a.dim / 2;
+  if (half % kPer16<T> == 0) return launch_lanes<T, kPer16<T>>(a, s);
+  if constexpr (kIs16<T>)
+    if (half % 4 == 0) return launch_lanes<T, 4>(a, s);
   int lp = 1;
   while (lp < kWave && lp < a.dim / 2) lp *= 2;
   rotate_any_kernel<T><<<static_cast<unsigned>(ceil_div(a.n, 4)), 256, 0, s>>>(a, lp);

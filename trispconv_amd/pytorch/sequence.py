@@ -33,7 +33,7 @@ _MOST = 2 ** 31 - 1
 
 
 def _same(t: torch.Tensor, like: torch.Tensor, what: str, name: str) -> None:
-    if t.dtype != like.dtype or t.device != like.device:
+    if t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{what}: {name} is {t.dtype} on {t.device}, expected {like.dtype} on "
                          f"{like.device}")
 
@@ -78,7 +78,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     b_ptr = r_ptr = None
     b_code = r_stride = 0
     if bias is not None:
-        if bias.dim() != 1 or bias.shape[0] != c_out or bias.device != x.device:
+        if bias.dim() != 1 or bias.shape[0] != c_out or bias.get_device() != x.get_device():
             raise ValueError(f"{what}: bias must have {c_out} entries on {x.device}")
         bias = bias.contiguous()
         b_ptr, b_code = bias.data_ptr(), L.dtype_code(bias.dtype)
@@ -88,7 +88,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         _same(residual, x, what, "residual")
         residual = _rows_of(residual)
         r_ptr, r_stride = residual.data_ptr(), residual.stride(0)
-    out = torch.empty((n, c_out), dtype=x.dtype, device=x.device)
+    out = x.new_empty((n, c_out))
     L.check(L.lib().tsc_linear_act(x.data_ptr(), x_stride, weight.data_ptr(), w_stride, b_ptr,
                                    b_code, r_ptr, r_stride, code, n, x.shape[1], c_out,
                                    _ACTS[activation], out.data_ptr(), L.stream_of(x)), what)
@@ -120,7 +120,7 @@ def norm_rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     _same(k, q, what, "k")
     n, hq, dim = q.shape
     hk = k.shape[1]
-    if positions.dim() != 2 or positions.shape[0] != n or positions.device != q.device or \
+    if positions.dim() != 2 or positions.shape[0] != n or positions.get_device() != q.get_device() or \
             positions.dtype not in (torch.int32, torch.float32):
         raise ValueError(f"{what}: positions must be ({n}, axes) int32 or float32 on {q.device}")
     gains, per_head, g_code = [], [], 0
@@ -129,7 +129,7 @@ def norm_rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
         g_code = L.dtype_code(g_dtype)
         for w, h, name in ((q_weight, hq, "q_weight"), (k_weight, hk, "k_weight")):
             if w is not None:
-                if w.shape not in ((dim,), (h, dim)) or w.device != q.device or w.dtype != g_dtype:
+                if w.shape not in ((dim,), (h, dim)) or w.get_device() != q.get_device() or w.dtype != g_dtype:
                     raise ValueError(f"{what}: {name} must be ({dim},) or ({h}, {dim}) {g_dtype} "
                                      f"on {q.device}")
                 w = w.contiguous()
@@ -138,8 +138,7 @@ def norm_rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     else:
         gains, per_head = [None, None], [0, 0]
     q, k, positions = _rows_of(q), _rows_of(k), _rows_of(positions)
-    q_out = torch.empty((n, hq, dim), dtype=q.dtype, device=q.device)
-    k_out = torch.empty((n, hk, dim), dtype=q.dtype, device=q.device)
+    q_out, k_out = q.new_empty((n, hq, dim)), q.new_empty((n, hk, dim))
     L.check(L.lib().tsc_norm_rotate_heads(
         q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
         positions.data_ptr(), positions.stride(0), int(positions.dtype == torch.float32),
@@ -194,7 +193,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         raise ValueError(f"{what}: offsets must be (B + 1,) for queries and keys, got "
                          f"{tuple(offsets.shape)} and {tuple(offsets_k.shape)}")
     for t in (offsets, offsets_k):
-        if t.dtype != torch.int32 or t.device != q.device:
+        if t.dtype is not torch.int32 or t.get_device() != q.get_device():
             raise ValueError(f"{what}: offsets must be int32 on {q.device}, got {t.dtype} on "
                              f"{t.device}")
     left, right = (_limit(side, what) for side in window)
@@ -202,7 +201,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         raise ValueError(f"{what}: sinks must not be negative, got {sinks}")
     q, k, v = _rows_of(q), _rows_of(k), _rows_of(v)
     offsets, offsets_k = offsets.contiguous(), offsets_k.contiguous()
-    out = torch.empty((n_q, hq, dim), dtype=q.dtype, device=q.device)
+    out = q.new_empty((n_q, hq, dim))
     lib, samples, sinks = L.lib(), offsets.shape[0] - 1, min(int(sinks), _MOST)
     nbytes = lib.tsc_window_attention_workspace_bytes(samples, n_q, n_k, hq, hk, dim, left, right,
                                                       sinks, code)
