@@ -33,6 +33,11 @@ Cut attend_cut(int64_t samples, int64_t n_q, int64_t n_k, int q_heads, int k_hea
   return c;
 }
 
+// Scratch of a call: the splits' maxima, sums and values.
+int64_t part_bytes(const Cut& c, int64_t rows, int dim) {
+  return c.splits > 1 ? (align_up(c.splits * rows * 2, 4) + c.splits * rows * dim) * 4 : 0;
+}
+
 int rows_of_type(int dtype, int dim) {
   return dtype == TSC_F32 ? rows_of<float>(dim) : rows_of<__half>(dim);
 }
@@ -50,7 +55,7 @@ extern "C" int64_t tsc_window_attention_workspace_bytes(int32_t samples, int64_t
       dim > 256)
     return -1;
   const Cut c = attend_cut(samples, n_q, n_k, q_heads, k_heads, left, right, sinks, rows_of_type(dtype, dim));
-  return c.splits > 1 ? (int64_t)c.splits * n_q * q_heads * (dim + 2) * 4 : 0;
+  return part_bytes(c, n_q * q_heads, dim);
 }
 
 extern "C" int tsc_window_attention(const void* q, int64_t q_row, int64_t q_head, const void* k,
@@ -75,7 +80,7 @@ extern "C" int tsc_window_attention(const void* q, int64_t q_row, int64_t q_head
               "window_attention: null pointer");
   TSC_REQUIRE(std::isfinite(scale), "window_attention: scale is not finite");
   const Cut c = attend_cut(samples, n_q, n_k, q_heads, k_heads, left, right, sinks, rows_of_type(dtype, dim));
-  const int64_t need = c.splits > 1 ? (int64_t)c.splits * n_q * q_heads * (dim + 2) * 4 : 0;
+  const int64_t need = part_bytes(c, n_q * q_heads, dim);
   TSC_REQUIRE(need == 0 || (ws && ws_bytes >= need), "window_attention: a workspace of %lld bytes is needed",
               static_cast<long long>(need));
   const AttendArgs a{q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, offsets_q, offsets_k,

@@ -35,7 +35,10 @@ struct AttendArgs {
   float scale_log2;        // |scale| * log2(e), 1 for a scale of 0
   float q_sign;            // the scale's sign, 0 for a scale of 0
   void* out;
-  float* part;             // [split][n_q * q_heads][m, l, dim values] when the keys are split
+  float* part;             // when the keys are split: [split][n_q * q_heads][m, l], then
+                           // [split][n_q * q_heads][dim] sums from part_values() on
+  __host__ __device__ int64_t rows() const { return n_q * q_heads; }
+  __host__ __device__ int64_t part_values(int splits) const { return (splits * rows() * 2 + 3) / 4 * 4; }
 };
 
 constexpr int kNoLimit = 0x7fffffff;
@@ -56,6 +59,11 @@ constexpr int row_blocks(int dp) { return kIs16<T> && dp <= 64 ? 2 : 1; }
 template <typename T>
 constexpr int key_blocks(int dp) { return dp * (int)sizeof(T) <= 512 ? 2 : 1; }
 
+// Tiles of K and V in LDS: the one in use and those on their way.  A wave that
+// is a workgroup of its own walks a few tiles, and asks for most of them at
+// once.
+template <typename T>
+constexpr int tile_buffers(int dp, int waves) { return waves == 1 && dp * (int)sizeof(T) <= 128 ? 4 : 2; }
 // Waves a SIMD that the registers and the LDS leave room for.
 template <typename T>
 constexpr int waves_per_simd(int dp) { return dp * (int)sizeof(T) <= 256 ? 2 : 1; }
@@ -257,23 +265,28 @@ __device__ void find_bad(char* vt, uint32_t* bad) {
 
 // The sample and the tile within it of the x-th tile of all: sample b has
 // ceil(Lq * group / rows) of them.  Every wave finds it for itself, 64 samples
-// at a time.  false: past the last.
+// at a time, the keys' offsets on the way so that nothing waits for them
+// later.  false: past the last.
 __device__ __forceinline__ bool find_tile(const AttendArgs& a, int group, int rows, int x, int64_t& q0,
-                                          int& lq, int& b, int& tile) {
+                                          int& lq, int64_t& k0, int& lk, int& tile) {
   const int lane = threadIdx.x % kWave;
   for (int b0 = 0; b0 < a.samples; b0 += kWave) {
-    int64_t at = 0;
-    int len = 0;
-    if (b0 + lane < a.samples) sample_range(a.off_q, b0 + lane, a.n_q, at, len);
+    int64_t at = 0, at_k = 0;
+    int len = 0, len_k = 0;
+    if (b0 + lane < a.samples) {
+      sample_range(a.off_q, b0 + lane, a.n_q, at, len);
+      sample_range(a.off_k, b0 + lane, a.n_k, at_k, len_k);
+    }
     const uint32_t tiles = static_cast<uint32_t>(((int64_t)len * group + rows - 1) / rows);
     const uint32_t inc = wave_inclusive(tiles);
     const uint64_t past = __ballot(inc > static_cast<uint32_t>(x));
     if (past) {
       const int at_lane = __builtin_ctzll(past);
-      b = b0 + at_lane;
       tile = x - __builtin_amdgcn_readlane(inc - tiles, at_lane);
       lq = __builtin_amdgcn_readlane(len, at_lane);
       q0 = __builtin_amdgcn_readlane(static_cast<int>(at), at_lane);
+      k0 = __builtin_amdgcn_readlane(static_cast<int>(at_k), at_lane);
+      lk = __builtin_amdgcn_readlane(len_k, at_lane);
       return true;
     }
     x -= __builtin_amdgcn_readlane(inc, kWave - 1);
@@ -321,7 +334,7 @@ template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
 __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, const T* k, const T* v,
                                             char* lds) {
   constexpr int KT = 32 * KB, ROW_BYTES = DP * sizeof(T);
-  constexpr int TILE = KT * ROW_BYTES, STEPS = DP * (int)sizeof(T) / 32, DB = DP / 32;
+  constexpr int BUFFERS = tile_buffers<T>(DP, WAVES), TILE = KT * ROW_BYTES, STEPS = DP * (int)sizeof(T) / 32, DB = DP / 32;
   const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   int lo_first, hi_first, lo_last, hi_last, none;
@@ -368,7 +381,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
   Stager<T, DP, KB, WAVES, ALIGNED, true> v_stage;
   k_stage.begin(k, a.k_row, a.dim, wave);
   v_stage.begin(v, a.v_row, a.dim, wave);
-  for (int x = 0; x < 2; ++x) {
+  for (int x = 0; x < BUFFERS; ++x) {
     k_stage.clear(lds + x * 2 * TILE);
     v_stage.clear(lds + x * 2 * TILE + TILE);
   }
@@ -381,7 +394,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
   float m[RB], mc[RB], l[RB][2];  // reference maximum, times c, two partial sums
   int hit = 0;    // bit rb: the row sees a value that is not finite
   int clean = 0;  // the walk that replaces those values
-  uint32_t* bad = reinterpret_cast<uint32_t*>(lds + 4 * TILE + WAVES * DP * 4);
+  uint32_t* bad = reinterpret_cast<uint32_t*>(lds + 2 * BUFFERS * TILE + WAVES * DP * 4);
   const float c = a.scale_log2;
   // 32 keys from row kb * 32 of a tile; whole: every row of the wave sees all
   auto key_step = [&](bool whole, const char* kt, const char* vt, int kb, int j0, int end) {
@@ -499,17 +512,32 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
       for (int db = 0; db < DB; ++db) o[rb][db] = f32x16(0.f);
     }
 
-    int j0, end, buf = 0;
+    // tile t is in buffer t - t0 modulo BUFFERS
+    int j0 = 0, end = 0, buf = 0;
     tile_at(w.t0, j0, end);
     if (w.t0 < w.t1) stage(j0, end, 0);
-    for (int t = w.t0; t < w.t1; ++t, buf ^= 1) {
+    if constexpr (BUFFERS > 2) {
+#pragma unroll 1
+      for (int t = 1; t < BUFFERS - 1 && w.t0 + t < w.t1; ++t) {
+        int j0_then, end_then;
+        tile_at(w.t0 + t, j0_then, end_then);
+        stage(j0_then, end_then, t);
+      }
+    }
+    for (int t = w.t0; t < w.t1; ++t, buf = buf + 1 == BUFFERS ? 0 : buf + 1) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       const int j0_now = j0, end_now = end;
       if (t + 1 < w.t1) {
         j0 += KT;
         if (t + 1 == w.sink_tiles) j0 = w.start, end = w.end;
-        stage(j0, end, buf ^ 1);
+      }
+      if constexpr (BUFFERS == 2) {
+        if (t + 1 < w.t1) stage(j0, end, buf ^ 1);
+      } else if (t + BUFFERS - 1 < w.t1) {
+        int j0_then, end_then;
+        tile_at(t + BUFFERS - 1, j0_then, end_then);
+        stage(j0_then, end_then, buf == 0 ? BUFFERS - 1 : buf - 1);
       }
       const char* kt = lds + buf * 2 * TILE;
       const char* vt = kt + TILE;
@@ -553,17 +581,18 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
     if (r < w.rows && !odd) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       if (w.splits > 1) {
-        float* part = a.part + (w.split * a.n_q * a.q_heads + item) * (a.dim + 2);
+        const int64_t at = w.split * a.rows() + item;
+        float* part = a.part + a.part_values(w.splits) + at * a.dim;
         if (half == 0) {
-          part[0] = sum == 0.f ? -__builtin_inff() : mc[rb];
-          part[1] = sum;
+          a.part[2 * at] = sum == 0.f ? -__builtin_inff() : mc[rb];
+          a.part[2 * at + 1] = sum;
         }
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int d = 32 * db + 8 * (i / 4) + 4 * half + i % 4;
-            if (d < a.dim) part[2 + d] = o[rb][db][i];
+            if (d < a.dim) part[d] = o[rb][db][i];
           }
       } else {
         T* out = static_cast<T*>(a.out) + item * a.dim;
@@ -589,7 +618,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
     if (redo) {
       // the tiles in LDS may still be read by other waves: each wave takes
       // its row's scratch from its own D floats behind them
-      float* q_s = reinterpret_cast<float*>(lds + 4 * TILE) + wave * DP;
+      float* q_s = reinterpret_cast<float*>(lds + 2 * BUFFERS * TILE) + wave * DP;
       int j0 = 0, end = 0, sink_from = 0, sink_to = 0, from = 0, to = 0;
       // this w.split's keys: tiles [w.t0, w.t1)
       if (w.t0 < w.sink_tiles) {
@@ -617,11 +646,11 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
           const int d = lane + u * kWave;
           if (d >= a.dim) continue;
           if (w.splits > 1) {
-            float* part = a.part + (w.split * a.n_q * a.q_heads + ix) * (a.dim + 2);
-            part[2 + d] = ox[u];
+            const int64_t at = w.split * a.rows() + ix;
+            a.part[a.part_values(w.splits) + at * a.dim + d] = ox[u];
             if (d == 0) {
-              part[0] = lsum == 0.f ? -__builtin_inff() : mx;
-              part[1] = lsum;
+              a.part[2 * at] = lsum == 0.f ? -__builtin_inff() : mx;
+              a.part[2 * at + 1] = lsum;
             }
           } else {
             static_cast<T*>(a.out)[ix * a.dim + d] = from_f32<T>(lsum == 0.f ? 0.f : ox[u] / lsum);
@@ -647,9 +676,8 @@ __global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP)) attend_k
   w.splits = splits;
   w.hk = static_cast<int>(id / splits / tiles_max);
   int64_t k0;
-  int lq, b, tile;
-  if (!find_tile(a, group, ROWS, static_cast<int>(id / splits % tiles_max), w.q0, lq, b, tile)) return;
-  sample_range(a.off_k, b, a.n_k, k0, w.lk);
+  int lq, tile;
+  if (!find_tile(a, group, ROWS, static_cast<int>(id / splits % tiles_max), w.q0, lq, k0, w.lk, tile)) return;
   const T* k = static_cast<const T*>(a.k) + k0 * a.k_row + w.hk * a.k_head;
   const T* v = static_cast<const T*>(a.v) + k0 * a.v_row + w.hk * a.v_head;
 
@@ -671,43 +699,75 @@ __global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP)) attend_k
   attend_walk<T, DP, RB, KB, WAVES, ALIGNED>(a, w, k, v, lds);
 }
 
-// Joins the splits of each row: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s
-// in the order of the splits, m the largest m_s.  A wave per row.
-template <typename T>
+// Joins the splits of each row: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s,
+// m the largest m_s; always in the same order.  A workgroup per row: every
+// wave works out the splits' weights for itself, then VALUES / 4 threads take
+// four values each of every (1024 / VALUES)th split, and the groups' sums meet
+// in LDS.
+constexpr int kMostSplits = 768;
+
+template <typename T, int VALUES>
 __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a, int splits) {
-  const int lane = threadIdx.x % kWave;
-  const int64_t items = a.n_q * a.q_heads, item = blockIdx.x * (int64_t)4 + threadIdx.x / kWave;
-  if (item >= items) return;
-  const float* part = a.part + item * (a.dim + 2);
-  const int64_t step = items * (a.dim + 2);
-  float m = -__builtin_inff();
-  for (int s = lane; s < splits; s += kWave) m = fmaxf(m, part[s * step]);
+  constexpr int LANES = VALUES / 4, GROUPS = 256 / LANES;
+  __shared__ float weight[kMostSplits];
+  __shared__ __align__(16) f32x4 sums[GROUPS][LANES];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t item = blockIdx.x, step = a.rows();
+  const float* ml = a.part + 2 * item;
+  float m = -__builtin_inff(), l = 0.f;
+  for (int s = lane; s < splits; s += kWave) m = fmaxf(m, ml[2 * s * step]);
 #pragma unroll
   for (int x = 1; x < kWave; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, kWave));
   const float base = m == -__builtin_inff() ? 0.f : m;
-  float l = 0.f, o[4] = {};
-  for (int s = 0; s < splits; ++s) {
-    const float* p = part + s * step;
+  for (int s = lane; s < splits; s += kWave) {
+    const float ls = ml[2 * s * step + 1];
     // a part that saw nothing counts for nothing; NaN sums stay NaN
-    if (p[1] == 0.f) continue;
-    const float f = exp2f(p[0] - base);
-    l += f * p[1];
+    const float f = ls == 0.f ? 0.f : exp2f(ml[2 * s * step] - base);
+    if (wave == 0) weight[s] = f;
+    l += f * ls;
+  }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int d = lane + u * kWave;
-      if (d < a.dim) o[u] += f * p[2 + d];
+  for (int x = 1; x < kWave; x <<= 1) l += __shfl_xor(l, x, kWave);
+  __syncthreads();
+  const int c = threadIdx.x % LANES, g = threadIdx.x / LANES, d = 4 * c;
+  const float* o = a.part + a.part_values(splits) + item * a.dim;
+  f32x4 sum = f32x4(0.f);
+  if (d < a.dim) {
+#pragma unroll 2
+    for (int s = g; s < splits; s += GROUPS) {
+      const float f = weight[s];
+      f32x4 x = f32x4(0.f);
+      const float* p = o + s * step * a.dim + d;
+      if (d + 4 <= a.dim) __builtin_memcpy(&x, p, 16);
+      else
+        for (int i = 0; i < 3; ++i) x[i] = d + i < a.dim ? p[i] : 0.f;
+      if (f != 0.f) sum += f * x;
     }
   }
+  sums[g][c] = sum;
+  __syncthreads();
+  if (threadIdx.x >= LANES) return;
+  sum = f32x4(0.f);
+  for (int x = 0; x < GROUPS; ++x) sum += sums[x][c];
+  T* out = static_cast<T*>(a.out) + item * a.dim;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int d = lane + u * kWave;
-    if (d < a.dim) static_cast<T*>(a.out)[item * a.dim + d] = from_f32<T>(l == 0.f ? 0.f : o[u] / l);
-  }
+  for (int i = 0; i < 4; ++i)
+    if (d + i < a.dim) out[d + i] = from_f32<T>(l == 0.f ? 0.f : sum[i] / l);
+}
+
+template <typename T>
+int launch_join(const AttendArgs& a, int splits, hipStream_t s) {
+  const unsigned blocks = static_cast<unsigned>(a.rows());
+  if (a.dim <= 64) attend_join_kernel<T, 64><<<blocks, 256, 0, s>>>(a, splits);
+  else if (a.dim <= 128) attend_join_kernel<T, 128><<<blocks, 256, 0, s>>>(a, splits);
+  else attend_join_kernel<T, 256><<<blocks, 256, 0, s>>>(a, splits);
+  TSC_LAUNCH_CHECK("window_attention_join");
+  return 0;
 }
 
 template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
 int launch_tiles(const AttendArgs& a, const Cut& c, hipStream_t s) {
-  constexpr int bytes = 4 * 32 * KB * DP * (int)sizeof(T) + WAVES * DP * 4 + KB * 4;
+  constexpr int bytes = tile_buffers<T>(DP, WAVES) * 2 * 32 * KB * DP * (int)sizeof(T) + WAVES * DP * 4 + KB * 4;
   auto kernel = &attend_kernel<T, DP, RB, KB, WAVES, ALIGNED>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
@@ -715,10 +775,7 @@ int launch_tiles(const AttendArgs& a, const Cut& c, hipStream_t s) {
   TSC_REQUIRE(blocks < (1ll << 31), "window_attention: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, static_cast<int>(c.tiles), c.splits);
   TSC_LAUNCH_CHECK("window_attention");
-  if (c.splits > 1) {
-    attend_join_kernel<T><<<static_cast<unsigned>(ceil_div(a.n_q * a.q_heads, 4)), 256, 0, s>>>(a, c.splits);
-    TSC_LAUNCH_CHECK("window_attention_join");
-  }
+  if (c.splits > 1) return launch_join<T>(a, c.splits, s);
   return 0;
 }
 
