@@ -192,104 +192,35 @@ struct OperandStage {
   }
 };
 
-// A tile of BM rows by BN columns, WM x WN waves, each MW x NW of it in 32x32
-// blocks: columns of W as the rows of the product, rows of x as its columns.
-// Operand tiles of RB bytes a row go round STAGES buffers of LDS through
-// direct-to-LDS loads, one barrier a tile.  The sums leave through LDS, so that
-// rows are written (and the residual read) as whole 16-byte pieces side by
-// side, with a lane's eight columns, and so its bias, the same in every row.
-template <typename T, int BM, int BN, int WM, int WN, int RB, int STAGES, bool ALIGNED, int OCC>
-__global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearArgs a, int tiles_m, int tiles_n) {
-  constexpr int THREADS = kWave * WM * WN, MW = BM / WM, NW = BN / WN, MB = MW / 32, NB = NW / 32;
-  constexpr int STAGE = (BM + BN) * RB, KT = RB / (int)sizeof(T), STEPS = RB / 32;
-  constexpr int LOADS = (BM + BN) * RB / 16 / THREADS;
-  extern __shared__ __align__(16) char lds[];
-  const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-
-  // Tiles next to each other run on one XCD (workgroups go round the eight in
-  // turn), eight bands of rows at a time: they share W's tiles and x's bands
-  // in its L2.
+// The workgroup's tile: false for the few workgroups that have none.  Tiles next
+// to each other run on one XCD (workgroups go round the eight in turn), eight
+// bands of rows at a time: they share W's tiles and x's bands in its L2.
+__device__ __forceinline__ bool find_tile(int tiles_m, int tiles_n, int& tm, int& tn) {
   const int tiles = tiles_m * tiles_n, per = (tiles + 7) / 8;
   const int id = blockIdx.x % 8 * per + blockIdx.x / 8;
-  if ((int)blockIdx.x / 8 >= per || id >= tiles) return;
+  if ((int)blockIdx.x / 8 >= per || id >= tiles) return false;
   constexpr int BANDS = 8;
   const int group = id / (BANDS * tiles_n), in_group = id - group * BANDS * tiles_n;
   const int bands = min(BANDS, tiles_m - group * BANDS);
-  const int tn = in_group / bands, tm = group * BANDS + in_group - tn * bands;
-  const int64_t row0 = (int64_t)tm * BM;
-  const int col0 = tn * BN;
+  tn = in_group / bands;
+  tm = group * BANDS + in_group - tn * bands;
+  return true;
+}
 
-  OperandStage<T, BM, RB, THREADS, ALIGNED> xs;
-  OperandStage<T, BN, RB, THREADS, ALIGNED> ws;
-  xs.begin(static_cast<const T*>(a.x), a.x_stride, row0, a.n);
-  ws.begin(static_cast<const T*>(a.w), a.w_stride, col0, a.c_out);
-  auto load = [&](int kt) {
-    char* tile = lds + kt % STAGES * STAGE;
-    xs.load(kt, a.c_in - kt * KT, tile);
-    ws.load(kt, a.c_in - kt * KT, tile + BM * RB);
-  };
-  auto store = [&](int kt) {
-    char* tile = lds + kt % STAGES * STAGE;
-    xs.store(tile);
-    ws.store(tile + BM * RB);
-  };
+// Bytes of a row of 32-bit sums on their way out.
+constexpr int leave_line(int columns) { return columns * 4 + 16; }
 
-  // what the epilogue needs of the bias is asked for first, long before its use
-  constexpr int LINE = NW * 4 + 16, LANES = NW / 8, ROWS = kWave / LANES;
-  const int o = col0 + wave % WN * NW + lane % LANES * 8;
-  const int have = a.c_out - o;  // of the lane's eight columns
-  float bias[8] = {};
-  if (a.bias) load_eight(a.bias, a.bias_dtype, o, have, bias);
-
-  f32x16 acc[NB][MB];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = f32x16(0.f);
-
-  const int kts = (a.c_in + KT - 1) / KT;
-  const int mrow = wave / WN * MW + col, nrow = wave % WN * NW + col;
-  for (int kt = 0; kt < STAGES - 1 && kt < kts; ++kt) {
-    load(kt);
-    if (!ALIGNED) store(kt);
-  }
-  for (int kt = 0; kt < kts; ++kt) {
-    if constexpr (ALIGNED) {
-      // loads finish in order: with STAGES - 2 later tiles of LOADS each in
-      // flight, this one is there; near the end (where a partial tile may be
-      // fewer loads) wait for all
-      if (kt + STAGES - 1 < kts) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 2) * LOADS) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    } else {
-      __syncthreads();
-    }
-    const bool more = kt + STAGES - 1 < kts;
-    if (more) load(kt + STAGES - 1);
-    const char* xt = lds + kt % STAGES * STAGE;
-    const char* wt = xt + BM * RB;
-#pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-      int4v xf[MB], wf[NB];
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-        xf[mb] = *reinterpret_cast<const int4v*>(xt + (mrow + mb * 32) * RB + tile_slot<RB>(mrow, 2 * st + half) * 16);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-        wf[nb] = *reinterpret_cast<const int4v*>(wt + (nrow + nb * 32) * RB + tile_slot<RB>(nrow, 2 * st + half) * 16);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mma32<T>(wf[nb], xf[mb], acc[nb][mb]);
-    }
-    if (!ALIGNED && more) store(kt + STAGES - 1);
-  }
-  __syncthreads();
-
+// A wave's sums leave: rows wave_row on, 32 MB of them, by NW columns, of which
+// the lane's eight begin at column o.  Through `mine`, 32 lines of the wave's
+// own LDS, so that rows are written (and the residual read) as whole 16-byte
+// pieces side by side, with a lane's columns, and so its bias, the same in
+// every row.
+template <typename T, int NW, int NB, int MB>
+__device__ __forceinline__ void leave(const LinearArgs& a, const f32x16 (&acc)[NB][MB], char* mine,
+                                      int64_t wave_row, int o, const float (&bias)[8]) {
   // 32 rows of the wave at a time through its own LDS
-  char* mine = lds + wave * 32 * LINE;
-  const int64_t wave_row = row0 + wave / WN * MW;
+  constexpr int LINE = leave_line(NW), LANES = NW / 8, ROWS = kWave / LANES;
+  const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32, have = a.c_out - o;
   const uint32_t out_step = static_cast<uint32_t>(a.c_out) * sizeof(T);
   const uint32_t out_at = lane / LANES * out_step + o * (uint32_t)sizeof(T);
 #pragma unroll
@@ -341,6 +272,93 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
   }
 }
 
+// A tile of BM rows by BN columns, WM x WN waves, each MW x NW of it in 32x32
+// blocks: columns of W as the rows of the product, rows of x as its columns.
+// Operand tiles of RB bytes a row go round STAGES buffers of LDS through
+// direct-to-LDS loads, one barrier a tile.
+template <typename T, int BM, int BN, int WM, int WN, int RB, int STAGES, bool ALIGNED, int OCC>
+__global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearArgs a, int tiles_m, int tiles_n) {
+  constexpr int THREADS = kWave * WM * WN, MW = BM / WM, NW = BN / WN, MB = MW / 32, NB = NW / 32;
+  constexpr int STAGE = (BM + BN) * RB, KT = RB / (int)sizeof(T), STEPS = RB / 32;
+  constexpr int LOADS = (BM + BN) * RB / 16 / THREADS;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+
+  int tm, tn;
+  if (!find_tile(tiles_m, tiles_n, tm, tn)) return;
+  const int64_t row0 = (int64_t)tm * BM;
+  const int col0 = tn * BN;
+
+  OperandStage<T, BM, RB, THREADS, ALIGNED> xs;
+  OperandStage<T, BN, RB, THREADS, ALIGNED> ws;
+  xs.begin(static_cast<const T*>(a.x), a.x_stride, row0, a.n);
+  ws.begin(static_cast<const T*>(a.w), a.w_stride, col0, a.c_out);
+  auto load = [&](int kt) {
+    char* tile = lds + kt % STAGES * STAGE;
+    xs.load(kt, a.c_in - kt * KT, tile);
+    ws.load(kt, a.c_in - kt * KT, tile + BM * RB);
+  };
+  auto store = [&](int kt) {
+    char* tile = lds + kt % STAGES * STAGE;
+    xs.store(tile);
+    ws.store(tile + BM * RB);
+  };
+
+  // what the epilogue needs of the bias is asked for first, long before its use
+  constexpr int LINE = leave_line(NW), LANES = NW / 8;
+  const int o = col0 + wave % WN * NW + lane % LANES * 8;
+  float bias[8] = {};  // of the lane's eight columns
+  if (a.bias) load_eight(a.bias, a.bias_dtype, o, a.c_out - o, bias);
+
+  f32x16 acc[NB][MB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = f32x16(0.f);
+
+  const int kts = (a.c_in + KT - 1) / KT;
+  const int mrow = wave / WN * MW + col, nrow = wave % WN * NW + col;
+  for (int kt = 0; kt < STAGES - 1 && kt < kts; ++kt) {
+    load(kt);
+    if (!ALIGNED) store(kt);
+  }
+  for (int kt = 0; kt < kts; ++kt) {
+    if constexpr (ALIGNED) {
+      // loads finish in order: with STAGES - 2 later tiles of LOADS each in
+      // flight, this one is there; near the end (where a partial tile may be
+      // fewer loads) wait for all
+      if (kt + STAGES - 1 < kts) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 2) * LOADS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    } else {
+      __syncthreads();
+    }
+    const bool more = kt + STAGES - 1 < kts;
+    if (more) load(kt + STAGES - 1);
+    const char* xt = lds + kt % STAGES * STAGE;
+    const char* wt = xt + BM * RB;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      int4v xf[MB], wf[NB];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+        xf[mb] = *reinterpret_cast<const int4v*>(xt + (mrow + mb * 32) * RB + tile_slot<RB>(mrow, 2 * st + half) * 16);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+        wf[nb] = *reinterpret_cast<const int4v*>(wt + (nrow + nb * 32) * RB + tile_slot<RB>(nrow, 2 * st + half) * 16);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mma32<T>(wf[nb], xf[mb], acc[nb][mb]);
+    }
+    if (!ALIGNED && more) store(kt + STAGES - 1);
+  }
+  __syncthreads();
+
+  leave<T, NW>(a, acc, lds + wave * 32 * LINE, row0 + wave / WN * MW, o, bias);
+}
+
 template <typename T, int BM, int BN, int WM, int WN, int RB, int STAGES, bool ALIGNED, int OCC>
 int launch_tile(const LinearArgs& a, hipStream_t s) {
   constexpr int main_bytes = STAGES * (BM + BN) * RB, out_bytes = WM * WN * 32 * (BN / WN * 4 + 16);
@@ -355,6 +373,199 @@ int launch_tile(const LinearArgs& a, hipStream_t s) {
   return 0;
 }
 
+// ------------------------------------------------------ f32 on bf16 units --
+// An f32 value is the sum of three bf16 values exactly (8 bits each of its 24):
+// hi + mid + lo, mid within 2^-8 and lo within 2^-16 of it.  Of the nine
+// products of two such sums the three of 2^-24 and less are left out (together
+// at most 2^-23 of the whole, an f32 rounding or two), and six bf16 matrix
+// instructions take the place of eight f32 ones that each last twice as long.
+struct Split8 {
+  int4v hi, mid, lo;
+};
+
+__device__ __forceinline__ Split8 split8(const float v[8]) {
+  Split8 s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x = v[2 * i], y = v[2 * i + 1];
+    auto part = [&] {  // both rounded to bf16 and taken off
+      const int p = pack2<__hip_bfloat16>(x, y);
+      x -= __builtin_bit_cast(float, p << 16);
+      y -= __builtin_bit_cast(float, p & 0xffff0000);
+      return p;
+    };
+    s.hi[i] = part();
+    s.mid[i] = part();
+    s.lo[i] = pack2<__hip_bfloat16>(x, y);
+  }
+  return s;
+}
+
+// c += a b, both in three parts, the small products first.
+__device__ __forceinline__ f32x16 mma32_split(const int4v a[3], const int4v b[3], f32x16 c) {
+  using B = __hip_bfloat16;
+  c = mma32<B>(a[2], b[0], c);
+  c = mma32<B>(a[0], b[2], c);
+  c = mma32<B>(a[1], b[1], c);
+  c = mma32<B>(a[1], b[0], c);
+  c = mma32<B>(a[0], b[1], c);
+  return mma32<B>(a[0], b[0], c);
+}
+
+// ROWS rows of 32 values of an operand: from memory to registers, and from
+// there, split, to LDS (three planes of 64 bytes a row).
+template <int ROWS, int THREADS>
+struct SplitStage {
+  static constexpr int ROUNDS = ROWS * 4 / THREADS, PLANE = ROWS * 64;
+  static_assert(ROWS * 4 % THREADS == 0, "whole rounds");
+  const char* base;
+  uint32_t offset[ROUNDS];
+  float held[ROUNDS][8];
+  __device__ __forceinline__ void begin(const float* p, int64_t stride, int64_t row, int64_t rows) {
+    base = reinterpret_cast<const char*>(p + row * stride);
+    const int last = static_cast<int>(min(rows - row, (int64_t)ROWS)) - 1;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int r = (i * THREADS + threadIdx.x) / 4;
+      offset[i] = static_cast<uint32_t>(min(r, last) * stride * 4) + threadIdx.x % 4 * 32;
+    }
+  }
+  __device__ __forceinline__ void load(int kt, int left) {
+    const int have = left - (int)threadIdx.x % 4 * 8;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const float* p = reinterpret_cast<const float*>(base + kt * 128ll + offset[i]);
+      if (have >= 8) {
+        __builtin_memcpy(held[i], p, 32);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) held[i][e] = e < have ? p[e] : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int r = (i * THREADS + threadIdx.x) / 4;
+      char* at = tile + r * 64 + tile_slot<64>(r, threadIdx.x % 4) * 16;
+      const Split8 s = split8(held[i]);
+      *reinterpret_cast<int4v*>(at) = s.hi;
+      *reinterpret_cast<int4v*>(at + PLANE) = s.mid;
+      *reinterpret_cast<int4v*>(at + 2 * PLANE) = s.lo;
+    }
+  }
+};
+
+// Results that the split cannot be trusted with: not finite (an infinity has no
+// parts, and 0 times it would be NaN), or under 2^-64 (parts of the smallest
+// values are lost).  They are summed again on the f32 unit, a block of 32 x 32 at
+// a time, and no other result changes.
+__device__ __forceinline__ bool doubtful(float v) {
+  const float m = __builtin_fabsf(v);
+  return !(m >= 0x1p-64f && m < __builtin_inff()) && v != 0.f;
+}
+
+// Tiles as in linear_tile_kernel, for f32 tensors: split on the way into LDS,
+// with the next k tile's values on their way to registers meanwhile.
+template <int BM, int BN, int WM, int WN, int OCC>
+__global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(LinearArgs a, int tiles_m, int tiles_n) {
+  constexpr int THREADS = kWave * WM * WN, MW = BM / WM, NW = BN / WN, MB = MW / 32, NB = NW / 32;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  int tm, tn;
+  if (!find_tile(tiles_m, tiles_n, tm, tn)) return;
+  const int64_t row0 = (int64_t)tm * BM;
+  const int col0 = tn * BN;
+  SplitStage<BM, THREADS> xs;
+  SplitStage<BN, THREADS> ws;
+  xs.begin(static_cast<const float*>(a.x), a.x_stride, row0, a.n);
+  ws.begin(static_cast<const float*>(a.w), a.w_stride, col0, a.c_out);
+  constexpr int LINE = leave_line(NW), LANES = NW / 8;
+  const int o = col0 + wave % WN * NW + lane % LANES * 8;
+  float bias[8] = {};
+  if (a.bias) load_eight(a.bias, a.bias_dtype, o, a.c_out - o, bias);
+
+  f32x16 acc[NB][MB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = f32x16(0.f);
+  const int kts = (a.c_in + 31) / 32;
+  const int mrow = wave / WN * MW + col, nrow = wave % WN * NW + col;
+  const char *xt = lds, *wt = lds + 3 * BM * 64;
+  if (kts > 0) {
+    xs.load(0, a.c_in);
+    ws.load(0, a.c_in);
+  }
+  for (int kt = 0; kt < kts; ++kt) {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    xs.store(lds);
+    ws.store(lds + 3 * BM * 64);
+    if (kt + 1 < kts) {
+      xs.load(kt + 1, a.c_in - (kt + 1) * 32);
+      ws.load(kt + 1, a.c_in - (kt + 1) * 32);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      int4v xf[MB][3], wf[NB][3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+          xf[mb][p] = *reinterpret_cast<const int4v*>(xt + p * BM * 64 + (mrow + mb * 32) * 64 +
+                                                      tile_slot<64>(mrow, 2 * st + half) * 16);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          wf[nb][p] = *reinterpret_cast<const int4v*>(wt + p * BN * 64 + (nrow + nb * 32) * 64 +
+                                                      tile_slot<64>(nrow, 2 * st + half) * 16);
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mma32_split(wf[nb], xf[mb], acc[nb][mb]);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) odd |= doubtful(acc[nb][mb][i]);
+      if (!__any(odd)) continue;
+      const float* x = static_cast<const float*>(a.x) +
+                       min(row0 + wave / WN * MW + mb * 32 + col, a.n - 1) * a.x_stride;
+      const float* w = static_cast<const float*>(a.w) +
+                       min(col0 + wave % WN * NW + nb * 32 + col, a.c_out - 1) * a.w_stride;
+      f32x16 sum = f32x16(0.f);
+#pragma unroll 4
+      for (int k = half; k < a.c_in + half; k += 2) {
+        const bool in = k < a.c_in;
+        sum = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? w[k] : 0.f, in ? x[k] : 0.f, sum, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[nb][mb][i] = doubtful(acc[nb][mb][i]) ? sum[i] : acc[nb][mb][i];
+    }
+  leave<float, NW>(a, acc, lds + wave * 32 * LINE, row0 + wave / WN * MW, o, bias);
+}
+
+template <int BM, int BN, int WM, int WN, int OCC>
+int launch_split(const LinearArgs& a, hipStream_t s) {
+  constexpr int main_bytes = 3 * (BM + BN) * 64, out_bytes = WM * WN * 32 * leave_line(BN / WN);
+  constexpr int bytes = main_bytes > out_bytes ? main_bytes : out_bytes;
+  auto kernel = &linear_split_kernel<BM, BN, WM, WN, OCC>;
+  if (bytes > 65536)
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  const int64_t tm = ceil_div(a.n, BM), tn = ceil_div(a.c_out, BN), blocks = align_up(tm * tn, 8);
+  TSC_REQUIRE(blocks < (1ll << 31), "linear_act: too many tiles");
+  kernel<<<static_cast<unsigned>(blocks), kWave * WM * WN, bytes, s>>>(a, static_cast<int>(tm), static_cast<int>(tn));
+  TSC_LAUNCH_CHECK("linear_act_split");
+  return 0;
+}
+
 template <typename T, int ROWS>
 int launch_few(const LinearArgs& a, hipStream_t s) {
   linear_few_kernel<T, ROWS><<<static_cast<unsigned>(ceil_div(a.c_out, 4)), 256, 0, s>>>(a);
@@ -362,22 +573,24 @@ int launch_few(const LinearArgs& a, hipStream_t s) {
   return 0;
 }
 
-#ifndef TSC_BIG
-#define TSC_BIG 256, 256, 2, 4, 128, 2
-#define TSC_BIG_OCC 2
+#ifndef TSC_SMALL
+#define TSC_SMALL 64, 64, 2, 2, 128, 3
 #endif
-#ifndef TSC_MID
-#define TSC_MID 128, 128, 2, 2, 64, 2
-#define TSC_MID_OCC 2
-#endif
+
+inline bool half_empty(int columns) { return (columns - 1) % 128 < 64; }
 
 template <typename T, bool ALIGNED>
 int launch_sized(const LinearArgs& a, hipStream_t s) {
-  const int64_t big = ceil_div(a.n, 256) * ceil_div(a.c_out, 256);
-  if (kIs16<T> && big >= 200 && a.c_in >= 512) return launch_tile<T, TSC_BIG, ALIGNED, TSC_BIG_OCC>(a, s);
-  const int64_t mid = ceil_div(a.n, 128) * ceil_div(a.c_out, 128);
-  if (mid >= 256) return launch_tile<T, TSC_MID, ALIGNED, TSC_MID_OCC>(a, s);
-  return launch_tile<T, 64, 64, 2, 2, 128, 3, ALIGNED, 2>(a, s);
+  auto tiles = [&](int rows, int columns) { return ceil_div(a.n, rows) * ceil_div(a.c_out, columns); };
+  // 256 x 256 reads least per product, but one workgroup fills a CU, with
+  // nothing beside it while its sums leave: for long sums, and enough tiles
+  if (a.c_in >= 512 && tiles(256, 256) >= 200) return launch_tile<T, 256, 256, 2, 4, 128, 2, ALIGNED, 2>(a, s);
+  if (tiles(128, 128) >= 256) {
+    // 64 columns where tiles of 128 would leave half of the last one empty
+    if (half_empty(a.c_out)) return launch_tile<T, 128, 64, 2, 2, 64, 2, ALIGNED, 2>(a, s);
+    return launch_tile<T, 128, 128, 2, 2, 64, 2, ALIGNED, 2>(a, s);
+  }
+  return launch_tile<T, TSC_SMALL, ALIGNED, 2>(a, s);
 }
 
 }  // namespace
@@ -392,7 +605,12 @@ int launch_linear(const LinearArgs& a, hipStream_t s) {
                        reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
   const bool near = std::max(a.x_stride, a.w_stride) < (1 << 21);
   TSC_REQUIRE(near, "linear_act: row strides over 2^21 elements are not supported");
-  return aligned ? launch_sized<T, true>(a, s) : launch_sized<T, false>(a, s);
+  if constexpr (!kIs16<T>) {
+    if (ceil_div(a.n, 128) * ceil_div(a.c_out, 128) < 256) return launch_split<64, 64, 2, 2, 3>(a, s);
+    return half_empty(a.c_out) ? launch_split<128, 64, 2, 2, 3>(a, s) : launch_split<128, 128, 2, 2, 2>(a, s);
+  } else {
+    return aligned ? launch_sized<T, true>(a, s) : launch_sized<T, false>(a, s);
+  }
 }
 
 }  // namespace tsc

@@ -38,17 +38,25 @@ def _same(t: torch.Tensor, like: torch.Tensor, what: str, name: str) -> None:
                          f"{like.device}")
 
 
-def _rows_of(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with its last dimension contiguous (any strides before it)."""
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+def _rows_of(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, ...]]:
+    """``t`` with its last dimension contiguous (any strides before it), and its strides."""
+    strides = t.stride()
+    if strides[-1] != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+        strides = t.stride()
+    return t, strides
 
 
 def _matrix(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """``t`` as the product kernels read it, and its row stride: rows
     contiguous, less than 2^21 elements apart."""
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) >= 1 << 21 and t.shape[0] > 1):
+    row, column = t.stride()
+    if (column != 1 and t.shape[1] > 1) or row >= 1 << 21:
+        if t.shape[0] <= 1 and (column == 1 or t.shape[1] <= 1):
+            return t, 0  # one row: its stride means nothing
         t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride(0) if t.shape[0] > 1 else 0
+        row = t.stride(0)
+    return t, row
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -64,16 +72,18 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     rounded once to x's dtype.
     """
     what = "linear_act"
-    L.require_gpu(x, what)
+    if not x.is_cuda:
+        L.require_gpu(x, what)
     code = L.dtype_code(x.dtype)
-    if activation not in _ACTS:
+    act = _ACTS.get(activation)
+    if act is None:
         raise ValueError(f"{what}: unknown activation {activation!r}; one of "
                          f"{sorted(a for a in _ACTS if a)}")
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"{what}: x {tuple(x.shape)} and weight {tuple(weight.shape)} are not "
                          "(N, C_in) and (C_out, C_in)")
     _same(weight, x, what, "weight")
-    n, c_out = x.shape[0], weight.shape[0]
+    (n, c_in), c_out = x.shape, weight.shape[0]
     (x, x_stride), (weight, w_stride) = _matrix(x), _matrix(weight)
     b_ptr = r_ptr = None
     b_code = r_stride = 0
@@ -86,12 +96,14 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         if residual.shape != (n, c_out):
             raise ValueError(f"{what}: residual {tuple(residual.shape)}, expected {(n, c_out)}")
         _same(residual, x, what, "residual")
-        residual = _rows_of(residual)
-        r_ptr, r_stride = residual.data_ptr(), residual.stride(0)
+        residual, (r_stride, _) = _rows_of(residual)
+        r_ptr = residual.data_ptr()
     out = x.new_empty((n, c_out))
-    L.check(L.lib().tsc_linear_act(x.data_ptr(), x_stride, weight.data_ptr(), w_stride, b_ptr,
-                                   b_code, r_ptr, r_stride, code, n, x.shape[1], c_out,
-                                   _ACTS[activation], out.data_ptr(), L.stream_of(x)), what)
+    rc = L.lib().tsc_linear_act(x.data_ptr(), x_stride, weight.data_ptr(), w_stride, b_ptr, b_code,
+                                r_ptr, r_stride, code, n, c_in, c_out, act, out.data_ptr(),
+                                L.stream_of(x))
+    if rc:
+        L.check(rc, what)
     return out
 
 
@@ -112,39 +124,44 @@ def norm_rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     (y[2j], y[2j+1]) with ``interleaved``.  Returns new contiguous tensors.
     """
     what = "norm_rotate_heads"
-    L.require_gpu(q, what)
+    if not q.is_cuda:
+        L.require_gpu(q, what)
     code = L.dtype_code(q.dtype)
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} are not (N, Hq, D) "
                          "and (N, Hk, D)")
     _same(k, q, what, "k")
     n, hq, dim = q.shape
-    hk = k.shape[1]
-    if positions.dim() != 2 or positions.shape[0] != n or positions.get_device() != q.get_device() or \
-            positions.dtype not in (torch.int32, torch.float32):
+    hk, device = k.shape[1], q.get_device()
+    in_f32 = positions.dtype is torch.float32
+    if positions.dim() != 2 or positions.shape[0] != n or positions.get_device() != device or \
+            not (in_f32 or positions.dtype is torch.int32):
         raise ValueError(f"{what}: positions must be ({n}, axes) int32 or float32 on {q.device}")
-    gains, per_head, g_code = [], [], 0
+    qg_ptr = kg_ptr = None
+    qg_heads = kg_heads = g_code = 0
     if q_weight is not None or k_weight is not None:
         g_dtype = (k_weight if q_weight is None else q_weight).dtype
         g_code = L.dtype_code(g_dtype)
         for w, h, name in ((q_weight, hq, "q_weight"), (k_weight, hk, "k_weight")):
-            if w is not None:
-                if w.shape not in ((dim,), (h, dim)) or w.get_device() != q.get_device() or w.dtype != g_dtype:
-                    raise ValueError(f"{what}: {name} must be ({dim},) or ({h}, {dim}) {g_dtype} "
-                                     f"on {q.device}")
-                w = w.contiguous()
-            gains.append(w)
-            per_head.append(int(w is not None and w.dim() == 2))
-    else:
-        gains, per_head = [None, None], [0, 0]
-    q, k, positions = _rows_of(q), _rows_of(k), _rows_of(positions)
+            if w is not None and (w.shape not in ((dim,), (h, dim)) or w.get_device() != device
+                                  or w.dtype is not g_dtype):
+                raise ValueError(f"{what}: {name} must be ({dim},) or ({h}, {dim}) {g_dtype} on "
+                                 f"{q.device}")
+        if q_weight is not None:
+            q_weight = q_weight.contiguous()
+            qg_ptr, qg_heads = q_weight.data_ptr(), q_weight.dim() - 1
+        if k_weight is not None:
+            k_weight = k_weight.contiguous()
+            kg_ptr, kg_heads = k_weight.data_ptr(), k_weight.dim() - 1
+    (q, (q_row, q_head, _)), (k, (k_row, k_head, _)) = _rows_of(q), _rows_of(k)
+    positions, (p_row, _) = _rows_of(positions)
     q_out, k_out = q.new_empty((n, hq, dim)), q.new_empty((n, hk, dim))
-    L.check(L.lib().tsc_norm_rotate_heads(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        positions.data_ptr(), positions.stride(0), int(positions.dtype == torch.float32),
-        positions.shape[1], L.ptr(gains[0]), L.ptr(gains[1]), g_code, per_head[0], per_head[1],
-        float(eps), float(base), int(bool(interleaved)), code, n, hq, hk, dim, q_out.data_ptr(),
-        k_out.data_ptr(), L.stream_of(q)), what)
+    rc = L.lib().tsc_norm_rotate_heads(
+        q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, positions.data_ptr(), p_row,
+        in_f32, positions.shape[1], qg_ptr, kg_ptr, g_code, qg_heads, kg_heads, eps, base,
+        interleaved, code, n, hq, hk, dim, q_out.data_ptr(), k_out.data_ptr(), L.stream_of(q))
+    if rc:
+        L.check(rc, what)
     return q_out, k_out
 
 
@@ -176,7 +193,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     and sums are float32.
     """
     what = "window_attention"
-    L.require_gpu(q, what)
+    if not q.is_cuda:
+        L.require_gpu(q, what)
     code = L.dtype_code(q.dtype)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} are "
@@ -184,7 +202,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     _same(k, q, what, "k")
     _same(v, q, what, "v")
     n_q, hq, dim = q.shape
-    n_k, hk = k.shape[:2]
+    n_k, hk, _ = k.shape
     if offsets_k is None:
         offsets_k = offsets
         if n_q != n_k:
@@ -196,22 +214,27 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         if t.dtype is not torch.int32 or t.get_device() != q.get_device():
             raise ValueError(f"{what}: offsets must be int32 on {q.device}, got {t.dtype} on "
                              f"{t.device}")
-    left, right = (_limit(side, what) for side in window)
+    left, right = window
+    left, right = _limit(left, what), _limit(right, what)
     if sinks < 0:
         raise ValueError(f"{what}: sinks must not be negative, got {sinks}")
-    q, k, v = _rows_of(q), _rows_of(k), _rows_of(v)
+    (q, (q_row, q_head, _)), (k, (k_row, k_head, _)) = _rows_of(q), _rows_of(k)
+    v, (v_row, v_head, _) = _rows_of(v)
     offsets, offsets_k = offsets.contiguous(), offsets_k.contiguous()
     out = q.new_empty((n_q, hq, dim))
-    lib, samples, sinks = L.lib(), offsets.shape[0] - 1, min(int(sinks), _MOST)
+    lib, samples, sinks = L.lib(), offsets.shape[0] - 1, min(sinks, _MOST)
     nbytes = lib.tsc_window_attention_workspace_bytes(samples, n_q, n_k, hq, hk, dim, left, right,
                                                       sinks, code)
-    ws = L.workspace(nbytes, q.device) if nbytes > 0 else None
-    L.check(lib.tsc_window_attention(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        v.data_ptr(), v.stride(0), v.stride(1), offsets.data_ptr(), offsets_k.data_ptr(), samples,
-        n_q, n_k, hq, hk, dim, left, right, sinks,
-        float(dim ** -0.5 if scale is None else scale), code, L.ptr(ws), max(nbytes, 0),
-        out.data_ptr(), L.stream_of(q)), what)
+    ws = None
+    if nbytes > 0:
+        ws = offsets.new_empty(-(-nbytes // 4))
+    rc = lib.tsc_window_attention(
+        q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+        offsets.data_ptr(), offsets_k.data_ptr(), samples, n_q, n_k, hq, hk, dim, left, right,
+        sinks, dim ** -0.5 if scale is None else scale, code,
+        None if ws is None else ws.data_ptr(), nbytes, out.data_ptr(), L.stream_of(q))
+    if rc:
+        L.check(rc, what)
     return out
 
 
