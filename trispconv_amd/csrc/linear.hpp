@@ -108,19 +108,43 @@ struct Eight {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ void load_eight_of(const void* p, int64_t at, int have, float v[8]) {
-  Eight<T> x;
-  x.load(static_cast<const T*>(p) + at, have);
+// Eight of the bias, as they lie in memory until they are used: asked for before
+// the products, converted after them.
+struct BiasEight {
+  int4v raw[2] = {int4v(0), int4v(0)};
+  template <typename B>
+  __device__ __forceinline__ void load_as(const void* p, int64_t at, int have) {
+    Eight<B> e;
+    e.load(static_cast<const B*>(p) + at, have);
+    __builtin_memcpy(raw, e.e, sizeof e.e);
+  }
+  __device__ __forceinline__ void load(const void* p, int dtype, int64_t at, int have) {
+    if (!p || have <= 0) return;
+    if (dtype == TSC_F32) load_as<float>(p, at, have);
+    else if (dtype == TSC_F16) load_as<__half>(p, at, have);
+    else load_as<__hip_bfloat16>(p, at, have);
+  }
+  template <typename B>
+  __device__ __forceinline__ void values_as(float v[8]) const {
+    Eight<B> e;
+    __builtin_memcpy(e.e, raw, sizeof e.e);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f32(x.e[i]);
-}
-__device__ __forceinline__ void load_eight(const void* p, int dtype, int64_t at, int have, float v[8]) {
-  if (have <= 0) return;
-  if (dtype == TSC_F32) load_eight_of<float>(p, at, have, v);
-  else if (dtype == TSC_F16) load_eight_of<__half>(p, at, have, v);
-  else load_eight_of<__hip_bfloat16>(p, at, have, v);
-}
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(e.e[i]);
+  }
+  __device__ __forceinline__ void values(const void* p, int dtype, float v[8]) {
+    asm volatile("" : "+v"(raw[0]), "+v"(raw[1]));  // not before here
+    if (!p) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    } else if (dtype == TSC_F32) {
+      values_as<float>(v);
+    } else if (dtype == TSC_F16) {
+      values_as<__half>(v);
+    } else {
+      values_as<__hip_bfloat16>(v);
+    }
+  }
+};
 
 // ---------------------------------------------------------------- tiles --
 // 16-byte chunk c of row r of an operand tile is stored in slot c ^ s(r): the
@@ -217,10 +241,12 @@ constexpr int leave_line(int columns) { return columns * 4 + 16; }
 // every row.
 template <typename T, int NW, int NB, int MB>
 __device__ __forceinline__ void leave(const LinearArgs& a, const f32x16 (&acc)[NB][MB], char* mine,
-                                      int64_t wave_row, int o, const float (&bias)[8]) {
+                                      int64_t wave_row, int o, BiasEight& bias_raw) {
   // 32 rows of the wave at a time through its own LDS
   constexpr int LINE = leave_line(NW), LANES = NW / 8, ROWS = kWave / LANES;
   const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32, have = a.c_out - o;
+  float bias[8];
+  bias_raw.values(a.bias, a.bias_dtype, bias);
   const uint32_t out_step = static_cast<uint32_t>(a.c_out) * sizeof(T);
   const uint32_t out_at = lane / LANES * out_step + o * (uint32_t)sizeof(T);
 #pragma unroll
@@ -305,11 +331,9 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
     ws.store(tile + BM * RB);
   };
 
-  // what the epilogue needs of the bias is asked for first, long before its use
   constexpr int LINE = leave_line(NW), LANES = NW / 8;
   const int o = col0 + wave % WN * NW + lane % LANES * 8;
-  float bias[8] = {};  // of the lane's eight columns
-  if (a.bias) load_eight(a.bias, a.bias_dtype, o, a.c_out - o, bias);
+  BiasEight bias;  // of the lane's eight columns
 
   f32x16 acc[NB][MB];
 #pragma unroll
@@ -323,6 +347,7 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
     load(kt);
     if (!ALIGNED) store(kt);
   }
+  bias.load(a.bias, a.bias_dtype, o, a.c_out - o);
   for (int kt = 0; kt < kts; ++kt) {
     if constexpr (ALIGNED) {
       // loads finish in order: with STAGES - 2 later tiles of LOADS each in
@@ -483,8 +508,7 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
   ws.begin(static_cast<const float*>(a.w), a.w_stride, col0, a.c_out);
   constexpr int LINE = leave_line(NW), LANES = NW / 8;
   const int o = col0 + wave % WN * NW + lane % LANES * 8;
-  float bias[8] = {};
-  if (a.bias) load_eight(a.bias, a.bias_dtype, o, a.c_out - o, bias);
+  BiasEight bias;  // of the lane's eight columns
 
   f32x16 acc[NB][MB];
 #pragma unroll
@@ -498,6 +522,7 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
     xs.load(0, a.c_in);
     ws.load(0, a.c_in);
   }
+  bias.load(a.bias, a.bias_dtype, o, a.c_out - o);
   for (int kt = 0; kt < kts; ++kt) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     xs.store(lds);
