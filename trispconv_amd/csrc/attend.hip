@@ -14,32 +14,34 @@ namespace {
 
 constexpr int kCus = 256;
 
-Cut attend_cut(int64_t samples, int64_t n_q, int64_t n_k, int q_heads, int k_heads, int left, int right,
-               int sinks, int rows_wide) {
+Cut attend_cut(int64_t samples, int64_t n_q, int64_t n_k, int q_heads, int k_heads, int dim, int elem,
+               int left, int right, int sinks) {
   const int64_t group = q_heads / k_heads;
   auto tiles = [&](int64_t rows) { return n_q * group / rows + std::min(samples, n_q); };
-  Cut c{1, tiles(rows_wide), 1};
-  // Fewer workgroups than CUs: one wave each, 32 rows, and the keys that a
-  // tile can see at most split so that there are about three per CU, but not
-  // under 128 keys.
-  if (c.tiles * k_heads < kCus) {
-    c.wide = 0;
-    c.tiles = tiles(32);
-    int64_t span = n_k;
-    if (left >= 0 && right >= 0) span = std::min<int64_t>(span, (int64_t)left + right + 32 + sinks);
-    const int64_t most = std::max<int64_t>(1, span / 128);
-    c.splits = static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, 3 * kCus / (c.tiles * k_heads))));
-  }
-  return c;
+  // keys that a tile can see at most
+  int64_t span = n_k;
+  if (left >= 0 && right >= 0) span = std::min<int64_t>(span, (int64_t)left + right + 32 + sinks);
+  // 64 rows a wave for long walks: 8k voxels, 16 heads of 64, bf16, all seeing
+  // one another: 308 us, with 32 rows 330 us; in a window of 1025 keys, four
+  // scans of 60k: 435 us against 391 (the wider tile walks more that it masks)
+  if (can_pair(padded_dim(dim), elem) && span >= 4096 && tiles(256) * k_heads >= 2 * kCus)
+    return Cut{2, tiles(256), 1};
+  if (tiles(128) * k_heads >= kCus) return Cut{1, tiles(128), 1};
+  // Fewer workgroups than CUs: the keys are split so that there are about two per
+  // CU, with 256 keys and more each (2k voxels, 8 heads of 64, all seeing one
+  // another: 52 us, unsplit in lone waves 60 us; three per CU: 56 us).
+  // Where the samples have few rows, workgroups of one wave and 32 rows share
+  // nothing that four could, and 128 keys do (one token over 60k keys, 16 heads
+  // on 4: 28 us, three per CU 35 us)
+  const bool lone = n_q * group < 64 * samples;
+  const int64_t few = tiles(lone ? 32 : 128), least = lone ? 128 : 256;
+  const int64_t splits = std::min<int64_t>(span / least, 2 * kCus / (few * k_heads));
+  return Cut{lone ? 0 : 1, few, static_cast<int>(std::max<int64_t>(1, splits))};
 }
 
 // Scratch of a call: the splits' maxima, sums and values.
 int64_t part_bytes(const Cut& c, int64_t rows, int dim) {
   return c.splits > 1 ? (align_up(c.splits * rows * 2, 4) + c.splits * rows * dim) * 4 : 0;
-}
-
-int rows_of_type(int dtype, int dim) {
-  return dtype == TSC_F32 ? rows_of<float>(dim) : rows_of<__half>(dim);
 }
 
 }  // namespace
@@ -54,7 +56,7 @@ extern "C" int64_t tsc_window_attention_workspace_bytes(int32_t samples, int64_t
   if (!dtype_ok(dtype) || samples < 0 || n_q < 0 || n_k < 0 || q_heads <= 0 || k_heads <= 0 || dim < 1 ||
       dim > 256)
     return -1;
-  const Cut c = attend_cut(samples, n_q, n_k, q_heads, k_heads, left, right, sinks, rows_of_type(dtype, dim));
+  const Cut c = attend_cut(samples, n_q, n_k, q_heads, k_heads, dim, dtype_bytes(dtype), left, right, sinks);
   return part_bytes(c, n_q * q_heads, dim);
 }
 
@@ -79,7 +81,7 @@ extern "C" int tsc_window_attention(const void* q, int64_t q_row, int64_t q_head
   TSC_REQUIRE(q && out && offsets_q && offsets_k && (n_k == 0 || (k && v)),
               "window_attention: null pointer");
   TSC_REQUIRE(std::isfinite(scale), "window_attention: scale is not finite");
-  const Cut c = attend_cut(samples, n_q, n_k, q_heads, k_heads, left, right, sinks, rows_of_type(dtype, dim));
+  const Cut c = attend_cut(samples, n_q, n_k, q_heads, k_heads, dim, dtype_bytes(dtype), left, right, sinks);
   const int64_t need = part_bytes(c, n_q * q_heads, dim);
   TSC_REQUIRE(need == 0 || (ws && ws_bytes >= need), "window_attention: a workspace of %lld bytes is needed",
               static_cast<long long>(need));

@@ -46,15 +46,14 @@ constexpr int kNoLimit = 0x7fffffff;
 // How a call is cut up: the rows of a workgroup and the parts its keys are
 // split into.
 struct Cut {
-  int wide;  // 1: four waves a workgroup, 0: one
+  int wave_rows;  // rows of a workgroup of four waves in 128s, 0: one wave, 32 rows
   int64_t tiles;
   int splits;
 };
 
-// Rows of a wave in 32s: two where scores, sums and queries of both fit the
-// registers of two waves a SIMD.
-template <typename T>
-constexpr int row_blocks(int dp) { return kIs16<T> && dp <= 64 ? 2 : 1; }
+// Whether a wave may take 64 rows (two blocks of 32): halves the reads of K and
+// V from LDS, but leaves room for two waves a SIMD instead of four.
+constexpr bool can_pair(int dp, int elem) { return elem == 2 && dp <= 64; }
 // Keys of a tile in 32s: two, unless four tiles of it would not fit the LDS.
 template <typename T>
 constexpr int key_blocks(int dp) { return dp * (int)sizeof(T) <= 512 ? 2 : 1; }
@@ -66,12 +65,11 @@ template <typename T>
 constexpr int tile_buffers(int dp, int waves) { return waves == 1 && dp * (int)sizeof(T) <= 128 ? 4 : 2; }
 // Waves a SIMD that the registers and the LDS leave room for.
 template <typename T>
-constexpr int waves_per_simd(int dp) { return dp * (int)sizeof(T) <= 256 ? 2 : 1; }
+constexpr int waves_per_simd(int dp, int row_blocks) {
+  return dp * (int)sizeof(T) <= 128 ? 4 / row_blocks : dp * (int)sizeof(T) <= 256 ? 2 : 1;
+}
 
 inline int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
-
-template <typename T>
-int rows_of(int dim) { return 128 * row_blocks<T>(padded_dim(dim)); }
 
 // The call on tensors of type T, cut as c says.
 template <typename T>
@@ -408,7 +406,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) s[rb] = mma32<T>(x, qf[rb][st], s[rb]);
     }
-    if (!whole && j0 < a.sinks) {
+    if (!whole && j0 + kb * 32 < a.sinks) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -552,12 +550,15 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
             hit |= (j < min(end_now, hi[rb]) && (j >= lo[rb] || j < a.sinks)) << rb;
         }
       }
-      if (j0_now >= hi_last || (j0_now + KT <= lo_first && j0_now >= a.sinks)) continue;
-      const bool whole = j0_now + KT <= min(end_now, hi_first) && (j0_now >= lo_last || j0_now + KT <= a.sinks) &&
-                         wave_row + 32 * RB <= w.rows;
-
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) key_step(whole, kt, vt, kb, j0_now, end_now);
+      for (int kb = 0; kb < KB; ++kb) {
+        // 32 keys that no row of the wave sees, or that all of them see
+        const int jk = j0_now + kb * 32;
+        if (jk >= min(hi_last, end_now) || (jk + 32 <= lo_first && jk >= a.sinks)) continue;
+        const bool whole = jk + 32 <= min(end_now, hi_first) && (jk >= lo_last || jk + 32 <= a.sinks) &&
+                           wave_row + 32 * RB <= w.rows;
+        key_step(whole, kt, vt, kb, j0_now, end_now);
+      }
     }
 
     if (__builtin_amdgcn_readfirstlane(clean)) break;
@@ -662,7 +663,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
 }
 
 template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
-__global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP)) attend_kernel(AttendArgs a, int tiles_max, int splits) {
+__global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP, RB)) attend_kernel(AttendArgs a, int tiles_max, int splits) {
   constexpr int ROWS = 32 * RB * WAVES, KT = 32 * KB;
   extern __shared__ __align__(16) char lds[];  // K, V, K, V tiles; a row of q for each wave; KB words
   // tiles of one head next to each other on one XCD (workgroups go round the
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP)) attend_k
 // wave works out the splits' weights for itself, then VALUES / 4 threads take
 // four values each of every (1024 / VALUES)th split, and the groups' sums meet
 // in LDS.
-constexpr int kMostSplits = 768;
+constexpr int kMostSplits = 512;  // two workgroups per CU (attend_cut)
 
 template <typename T, int VALUES>
 __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a, int splits) {
@@ -781,9 +782,11 @@ int launch_tiles(const AttendArgs& a, const Cut& c, hipStream_t s) {
 
 template <typename T, int DP, bool ALIGNED>
 int launch_dim(const AttendArgs& a, const Cut& c, hipStream_t s) {
-  constexpr int RB = row_blocks<T>(DP), KB = key_blocks<T>(DP);
-  return c.wide ? launch_tiles<T, DP, RB, KB, 4, ALIGNED>(a, c, s)
-                : launch_tiles<T, DP, 1, KB, 1, ALIGNED>(a, c, s);
+  constexpr int KB = key_blocks<T>(DP);
+  if constexpr (can_pair(DP, sizeof(T)))
+    if (c.wave_rows == 2) return launch_tiles<T, DP, 2, KB, 4, ALIGNED>(a, c, s);
+  return c.wave_rows ? launch_tiles<T, DP, 1, KB, 4, ALIGNED>(a, c, s)
+                     : launch_tiles<T, DP, 1, KB, 1, ALIGNED>(a, c, s);
 }
 
 template <typename T, bool ALIGNED>
