@@ -550,14 +550,24 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
             hit |= (j < min(end_now, hi[rb]) && (j >= lo[rb] || j < a.sinks)) << rb;
         }
       }
+      // keys that no row of the wave sees, or that all of them see: by 32 keys,
+      // or by the tile where a wave has so many rows that it sees nearly all
+      // (the blocks of keys then follow each other without a branch)
+      if constexpr (RB == 1) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        // 32 keys that no row of the wave sees, or that all of them see
-        const int jk = j0_now + kb * 32;
-        if (jk >= min(hi_last, end_now) || (jk + 32 <= lo_first && jk >= a.sinks)) continue;
-        const bool whole = jk + 32 <= min(end_now, hi_first) && (jk >= lo_last || jk + 32 <= a.sinks) &&
-                           wave_row + 32 * RB <= w.rows;
-        key_step(whole, kt, vt, kb, j0_now, end_now);
+        for (int kb = 0; kb < KB; ++kb) {
+          const int jk = j0_now + kb * 32;
+          if (jk >= min(hi_last, end_now) || (jk + 32 <= lo_first && jk >= a.sinks)) continue;
+          const bool whole = jk + 32 <= min(end_now, hi_first) && (jk >= lo_last || jk + 32 <= a.sinks) &&
+                             wave_row + 32 * RB <= w.rows;
+          key_step(whole, kt, vt, kb, j0_now, end_now);
+        }
+      } else {
+        if (j0_now >= hi_last || (j0_now + KT <= lo_first && j0_now >= a.sinks)) continue;
+        const bool whole = j0_now + KT <= min(end_now, hi_first) &&
+                           (j0_now >= lo_last || j0_now + KT <= a.sinks) && wave_row + 32 * RB <= w.rows;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) key_step(whole, kt, vt, kb, j0_now, end_now);
       }
     }
 
