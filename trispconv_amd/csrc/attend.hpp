@@ -305,7 +305,7 @@ struct Walk {
   __device__ int token(uint32_t r) const { return static_cast<int>(min(r, rows - 1) / static_cast<uint32_t>(group)); }
 };
 
-constexpr float kMostOver = 8.f;
+constexpr float kMostWeight = 1024.f;
 
 // Tiles of 32 RB WAVES rows (a row: one query of one head; the heads that
 // share a key head side by side) against tiles of 32 KB keys.
@@ -319,9 +319,11 @@ constexpr float kMostOver = 8.f;
 // are double buffered: direct-to-LDS loads of the next ones fly while these
 // are used, one barrier a tile.
 //
-// A row's reference maximum m moves only when some score exceeds it by
-// 2^kMostOver: weights up to there keep the relative accuracy of f16 and bf16,
-// and the rescale of O almost never runs.
+// A row's reference m is the largest score of its first 32 keys, and moves (with
+// a rescale of what is there, and the weights made again) only when 32 weights
+// sum to over kMostWeight.  Up to there they keep the relative accuracy of f16
+// and bf16, so that most keys need no maximum at all; m is a score of the row,
+// so the largest weight is at least 1 and nothing that counts underflows.
 //
 // A key that a row does not see has weight 0, and 0 times an infinite or NaN
 // value would be NaN.  When a row of the workgroup comes out not finite, the
@@ -425,20 +427,40 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
           s[rb][i] = from + (8 * (i / 4) + i % 4) < span ? s[rb][i] : -__builtin_inff();
       }
     }
-    float top[RB];
+    // weights e^S^T with the rows' references, and their sums
+    int p16[RB][8];     // 16 bits: two keys a register
+    float p32[RB][16];  // f32
+    float sum[RB][2];
+    auto weights = [&] {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        sum[rb][0] = sum[rb][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][2 * i], c, -mc[rb]));
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][2 * i + 1], c, -mc[rb]));
+          sum[rb][0] += x;
+          sum[rb][1] += y;
+          if constexpr (kIs16<T>) {
+            p16[rb][i] = pack2<T>(x, y);
+          } else {
+            p32[rb][2 * i] = x;
+            p32[rb][2 * i + 1] = y;
+          }
+        }
+      }
+    };
+    weights();
     bool over = false;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      top[rb] = fmaxf(s[rb][0], s[rb][1]);
-#pragma unroll
-      for (int i = 2; i < 16; i += 2) top[rb] = fmaxf(fmaxf(top[rb], s[rb][i]), s[rb][i + 1]);
-      top[rb] = max_halves(top[rb]);
-      over |= (top[rb] - m[rb]) * c > kMostOver;  // -inf - -inf is NaN: nothing seen yet, nothing over
-    }
+    for (int rb = 0; rb < RB; ++rb) over |= m[rb] == -__builtin_inff() || sum[rb][0] + sum[rb][1] > kMostWeight;
     if (__any(over)) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        const float m_new = fmaxf(m[rb], top[rb]);
+        float top = fmaxf(s[rb][0], s[rb][1]);
+#pragma unroll
+        for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[rb][i]), s[rb][i + 1]);
+        const float m_new = fmaxf(m[rb], max_halves(top));
         const float mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c;
         const float fix = m[rb] == -__builtin_inff() ? 0.f : exp2f(mc[rb] - mc_new);
         m[rb] = m_new;
@@ -448,19 +470,12 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[rb][db] *= fix;
       }
+      weights();
     }
-    int p16[RB][8];  // e^S^T in 16 bits, two keys a register
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], c, -mc[rb]));
-        l[rb][i & 1] += s[rb][i];
-      }
-      if constexpr (kIs16<T>) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p16[rb][i] = pack2<T>(s[rb][2 * i], s[rb][2 * i + 1]);
-      }
+      l[rb][0] += sum[rb][0];
+      l[rb][1] += sum[rb][1];
     }
     // O^T += V^T e^S^T.  16 bits: 16 keys a step, of which the halves take
     // keys 0-3, 8-11 and 4-7, 12-15.  f32: two keys a step, 4 apart.
@@ -496,7 +511,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
           const float x = *reinterpret_cast<const float*>(vt + r * ROW_BYTES + (32 * db + col) * 4);
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb)
-            o[rb][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[rb][i], o[rb][db], 0, 0, 0);
+            o[rb][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p32[rb][i], o[rb][db], 0, 0, 0);
         }
     }
   };
@@ -504,7 +519,8 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
   for (;;) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      m[rb] = -__builtin_inff();
+      // (rows past the last need none: their scores are all -inf)
+      m[rb] = wave_row + rb * 32 + col < w.rows ? -__builtin_inff() : 0.f;
       mc[rb] = l[rb][0] = l[rb][1] = 0.f;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[rb][db] = f32x16(0.f);
