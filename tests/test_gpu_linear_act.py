@@ -149,3 +149,33 @@ def test_refusals():
         spconv.linear_act(x, w, b, None, r[:9])
     with pytest.raises(ValueError, match="residual is"):
         spconv.linear_act(x, w, b, None, r.float())
+
+
+def test_f32_values_that_three_parts_do_not_carry():
+    """f32 products run as three bf16 parts of each value: rows of the smallest
+    and the largest values, zeros, and infinities against weights whose lower
+    parts are zero must come out as from f32 sums."""
+    n, c_in, c_out = 140, 96, 130
+    x, w, b, _ = _tensors(n, c_in, c_out, torch.float32)
+    w = w.bfloat16().float()
+    x[3] *= 1e-33
+    x[40] *= 2.0 ** -100
+    x[70] = 0
+    x[100] *= 1e35
+    w[5] *= 1e-30
+    check(spconv.linear_act(x.to(DEV), w.to(DEV)), *linear64(x, w))
+    x[9], x[130, 7] = float("inf"), float("inf")
+    got = spconv.linear_act(x.to(DEV), w.to(DEV)).cpu()
+    want, _ = linear64(x, w)
+    rows = [9, 130]
+    assert torch.equal(torch.isnan(got[rows]), torch.isnan(want[rows]))
+    fine = ~torch.isnan(want[rows])
+    assert torch.equal(got[rows][fine], want[rows][fine].float())
+
+
+def test_one_wide_row_stride():
+    """Rows further apart than a tile's 32-bit offsets reach are copied first."""
+    x, w, b, _ = _tensors(20, 64, 96, torch.float16)
+    room = torch.zeros(20, 1 << 21, dtype=torch.float16, device=DEV)
+    room[:, :64] = x.to(DEV)
+    check(spconv.linear_act(room[:, :64], w.to(DEV), b.to(DEV)), *linear64(x, w, b))

@@ -240,3 +240,21 @@ def test_refusals():
     big = torch.zeros(8, 1, 257, dtype=torch.float16, device=DEV)
     with pytest.raises(ValueError, match="head size"):
         f(big, big, big, off)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_that_outgrow_their_reference(dtype):
+    """Keys in rising blocks: each block's scores exceed all before by more than
+    the weights may grow, then fall back; split keys as well."""
+    steps = torch.tensor([0.0, 3.0, 9.0, 4.0, 20.0, 19.0, 40.0, 0.0]).repeat_interleave(70)
+    for lq, lk in (([560], [560]), ([2], [560])):
+        q, k, v = _qkv(lq, lk, 2, 2, 64, dtype)
+        q = torch.full_like(q, 0.5)
+        k = (0.1 * k.float() + steps[:, None, None] / 4).to(dtype)
+        check(_run(q, k, v, lq, lk, (None, None), 0), *attend64(q, k, v, lq, lk, (None, None), 0))
+
+
+def test_many_streams_of_one_token():
+    lq, lk = [1] * 300, [5 + (i * 37) % 200 for i in range(300)]
+    q, k, v = _qkv(lq, lk, 8, 2, 64, torch.bfloat16)
+    check(_run(q, k, v, lq, lk, (63, 0), 2), *attend64(q, k, v, lq, lk, (63, 0), 2))

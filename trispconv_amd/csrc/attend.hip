@@ -21,22 +21,22 @@ Cut attend_cut(int64_t samples, int64_t n_q, int64_t n_k, int q_heads, int k_hea
   // keys that a tile can see at most
   int64_t span = n_k;
   if (left >= 0 && right >= 0) span = std::min<int64_t>(span, (int64_t)left + right + 32 + sinks);
+  auto splits = [&](int64_t tiles, int64_t least) {  // about two workgroups per CU
+    return static_cast<int>(std::max<int64_t>(1, std::min(span / least, 2 * kCus / (tiles * k_heads))));
+  };
+  // Samples of few rows (one new token each): workgroups of one wave and 32
+  // rows, for four waves would share nothing.  When they leave CUs idle, the keys
+  // are split, down to 128 (one token over 60k keys, 16 heads on 4: 28 us,
+  // three workgroups per CU 35 us).
+  if (n_q * group < 64 * samples) return Cut{0, tiles(32), splits(tiles(32), 128)};
   // 64 rows a wave for long walks: 8k voxels, 16 heads of 64, bf16, all seeing
-  // one another: 308 us, with 32 rows 330 us; in a window of 1025 keys, four
+  // one another: 303 us, with 32 rows 331 us; in a window of 1025 keys, four
   // scans of 60k: 435 us against 391 (the wider tile walks more that it masks)
   if (can_pair(padded_dim(dim), elem) && span >= 4096 && tiles(256) * k_heads >= 2 * kCus)
     return Cut{2, tiles(256), 1};
-  if (tiles(128) * k_heads >= kCus) return Cut{1, tiles(128), 1};
-  // Fewer workgroups than CUs: the keys are split so that there are about two per
-  // CU, with 256 keys and more each (2k voxels, 8 heads of 64, all seeing one
-  // another: 52 us, unsplit in lone waves 60 us; three per CU: 56 us).
-  // Where the samples have few rows, workgroups of one wave and 32 rows share
-  // nothing that four could, and 128 keys do (one token over 60k keys, 16 heads
-  // on 4: 28 us, three per CU 35 us)
-  const bool lone = n_q * group < 64 * samples;
-  const int64_t few = tiles(lone ? 32 : 128), least = lone ? 128 : 256;
-  const int64_t splits = std::min<int64_t>(span / least, 2 * kCus / (few * k_heads));
-  return Cut{lone ? 0 : 1, few, static_cast<int>(std::max<int64_t>(1, splits))};
+  // Fewer workgroups than CUs: the keys are split, down to 256 (2k voxels, 8
+  // heads of 64, all seeing one another: 52 us, unsplit in lone waves 60 us)
+  return Cut{1, tiles(128), tiles(128) * k_heads < kCus ? splits(tiles(128), 256) : 1};
 }
 
 // Scratch of a call: the splits' maxima, sums and values.

@@ -831,7 +831,8 @@ int launch_aligned(const AttendArgs& a, const Cut& c, hipStream_t s) {
 template <typename T>
 int launch_attend(const AttendArgs& a, const Cut& c, hipStream_t s) {
   const int64_t e = kPer16<T>;
-  const bool aligned = a.dim % e == 0 && a.k_row % e == 0 && a.v_row % e == 0 && a.k_head % e == 0 &&
+  // 16-byte pieces at 16-byte addresses, rows of a tile within 32-bit offsets
+  const bool aligned = a.k_row < (1 << 24) && a.v_row < (1 << 24) && a.dim % e == 0 && a.k_row % e == 0 && a.v_row % e == 0 && a.k_head % e == 0 &&
                        a.v_head % e == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&
                        reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
   return aligned ? launch_aligned<T, true>(a, c, s) : launch_aligned<T, false>(a, c, s);

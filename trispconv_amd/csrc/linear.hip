@@ -15,7 +15,8 @@ extern "C" int tsc_linear_act(const void* x, int64_t x_stride, const void* weigh
                               int32_t c_in, int32_t c_out, int32_t act, void* out,
                               tsc_stream_t stream) {
   TSC_REQUIRE(dtype_ok(dtype) && dtype_ok(bias_dtype), "linear_act: unknown dtype");
-  TSC_REQUIRE(n >= 0 && n < (1ll << 31) && c_in >= 0 && c_out >= 0, "linear_act: invalid sizes");
+  TSC_REQUIRE(n >= 0 && n < (1ll << 31) && c_in >= 0 && c_out >= 0 && c_out < (1 << 24),
+              "linear_act: invalid sizes");
   TSC_REQUIRE(act >= TSC_ACT_NONE && act <= TSC_ACT_SILU, "linear_act: unknown activation");
   if (n == 0 || c_out == 0) return 0;
   TSC_REQUIRE(out && (c_in == 0 || (x && weight)), "linear_act: null pointer");

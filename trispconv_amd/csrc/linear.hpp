@@ -598,10 +598,6 @@ int launch_few(const LinearArgs& a, hipStream_t s) {
   return 0;
 }
 
-#ifndef TSC_SMALL
-#define TSC_SMALL 64, 64, 2, 2, 128, 3
-#endif
-
 inline bool half_empty(int columns) { return (columns - 1) % 128 < 64; }
 
 template <typename T, bool ALIGNED>
@@ -615,7 +611,7 @@ int launch_sized(const LinearArgs& a, hipStream_t s) {
     if (half_empty(a.c_out)) return launch_tile<T, 128, 64, 2, 2, 64, 2, ALIGNED, 2>(a, s);
     return launch_tile<T, 128, 128, 2, 2, 64, 2, ALIGNED, 2>(a, s);
   }
-  return launch_tile<T, TSC_SMALL, ALIGNED, 2>(a, s);
+  return launch_tile<T, 64, 64, 2, 2, 128, 3, ALIGNED, 2>(a, s);
 }
 
 }  // namespace
