@@ -151,11 +151,24 @@ def test_refusals():
         spconv.linear_act(x, w, b, None, r.float())
 
 
-def test_f32_values_that_three_parts_do_not_carry():
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,c_in,c_out", [(16_400, 40, 256), (33_000, 33, 64), (16_500, 72, 190),
+                                          (1000, 100, 900), (12_900, 520, 1100),
+                                          (12_850, 513, 1031)])
+def test_every_tile_size(n, c_in, c_out, dtype):
+    """Calls large enough for the larger tiles, whole and ragged, aligned and not."""
+    say("linear_act tiles:", n, c_in, c_out, dtype)
+    x, w, b, r = _tensors(n, c_in, c_out, dtype)
+    got = spconv.linear_act(x.to(DEV), w.to(DEV), b.to(DEV), "gelu", r.to(DEV))
+    check(got, *linear64(x, w, b, "gelu", r), what=f"{n} {c_in} {c_out}")
+
+
+@pytest.mark.parametrize("n,c_out", [(140, 130), (1000, 900)])
+def test_f32_values_that_three_parts_do_not_carry(n, c_out):
     """f32 products run as three bf16 parts of each value: rows of the smallest
     and the largest values, zeros, and infinities against weights whose lower
     parts are zero must come out as from f32 sums."""
-    n, c_in, c_out = 140, 96, 130
+    c_in = 96
     x, w, b, _ = _tensors(n, c_in, c_out, torch.float32)
     w = w.bfloat16().float()
     x[3] *= 1e-33

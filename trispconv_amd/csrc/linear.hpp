@@ -591,6 +591,72 @@ int launch_split(const LinearArgs& a, hipStream_t s) {
   return 0;
 }
 
+// ------------------------------------------------------------- some rows --
+// Tiles of 32 x 32 for calls whose larger tiles would leave most CUs idle: the
+// eight waves of a workgroup share out the inputs (wave w takes steps w, w + 8,
+// ...), read their operands straight into registers, and their sums meet in
+// LDS, always in the same order.  Bound by the latency of a few dependent
+// reads.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(512, 2) linear_rows_kernel(LinearArgs a) {
+  constexpr int P = kPer16<T>, STEP = 2 * P;
+  __shared__ __align__(16) float sums[8][32][36];  // [wave][row][column]
+  const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t row0 = blockIdx.y * 32ll;
+  const int col0 = blockIdx.x * 32;
+  const T* x = static_cast<const T*>(a.x) + min(row0 + col, a.n - 1) * a.x_stride;
+  const T* w = static_cast<const T*>(a.w) + min(col0 + col, a.c_out - 1) * a.w_stride;
+  f32x16 acc = f32x16(0.f);
+  const int whole = a.c_in / STEP;  // steps that end within the inputs
+#pragma unroll 4
+  for (int st = wave; st < whole; st += 8) {
+    const int i = st * STEP + half * P;
+    int4v wf, xf;
+    if constexpr (ALIGNED) {
+      wf = *reinterpret_cast<const int4v*>(w + i);
+      xf = *reinterpret_cast<const int4v*>(x + i);
+    } else {
+      wf = load16_unaligned(w + i);
+      xf = load16_unaligned(x + i);
+    }
+    acc = mma32<T>(wf, xf, acc);
+  }
+  if (whole % 8 == wave && whole * STEP < a.c_in) {
+    const int i = whole * STEP + half * P, have = max(0, min(P, a.c_in - i));
+    acc = mma32<T>(load16_partial(w + i, have), load16_partial(x + i, have), acc);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 v = {acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
+    *reinterpret_cast<f32x4*>(&sums[wave][col][8 * i + 4 * half]) = v;
+  }
+  __syncthreads();
+  const int r = threadIdx.x / 16, c = threadIdx.x % 16 * 2;
+  const int64_t row = row0 + r;
+  if (row >= a.n) return;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int o = col0 + c + e;
+    if (o >= a.c_out) return;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += sums[k][r][c + e];
+    if (a.bias) v += load_any(a.bias, a.bias_dtype, o);
+    v = activate_any(a.act, v);
+    if (a.residual) v += to_f32(static_cast<const T*>(a.residual)[row * a.r_stride + o]);
+    static_cast<T*>(a.out)[row * a.c_out + o] = from_f32<T>(v);
+  }
+}
+
+template <typename T, bool ALIGNED>
+int launch_rows(const LinearArgs& a, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.c_out, 32)), static_cast<unsigned>(ceil_div(a.n, 32)));
+  linear_rows_kernel<T, ALIGNED><<<grid, 512, 0, s>>>(a);
+  TSC_LAUNCH_CHECK("linear_act_rows");
+  return 0;
+}
+
 template <typename T, int ROWS>
 int launch_few(const LinearArgs& a, hipStream_t s) {
   linear_few_kernel<T, ROWS><<<static_cast<unsigned>(ceil_div(a.c_out, 4)), 256, 0, s>>>(a);
@@ -626,6 +692,12 @@ int launch_linear(const LinearArgs& a, hipStream_t s) {
                        reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
   const bool near = std::max(a.x_stride, a.w_stride) < (1 << 21);
   TSC_REQUIRE(near, "linear_act: row strides over 2^21 elements are not supported");
+  // Tiles of 64 x 64 on fewer than half the CUs (f32, whose waves wait longer
+  // between barriers: up to 200): 16 x 2048 -> 4096 bf16 8.6 us, in tiles 13.3;
+  // 100 x 1024 -> 4096 (128 tiles) 9.9 against 8.5, f32 20.4 against 27.4;
+  // 1000 x 1024 -> 1024 (256 tiles) 17.9 against 9.0, f32 35.9 against 29.3
+  if (ceil_div(a.n, 64) * ceil_div(a.c_out, 64) < (kIs16<T> ? 128 : 200))
+    return aligned ? launch_rows<T, true>(a, s) : launch_rows<T, false>(a, s);
   if constexpr (!kIs16<T>) {
     if (ceil_div(a.n, 128) * ceil_div(a.c_out, 128) < 256) return launch_split<64, 64, 2, 2, 3>(a, s);
     return half_empty(a.c_out) ? launch_split<128, 64, 2, 2, 3>(a, s) : launch_split<128, 128, 2, 2, 2>(a, s);
