@@ -65,8 +65,8 @@ template <typename T>
 constexpr int tile_buffers(int dp, int waves) { return waves == 1 && dp * (int)sizeof(T) <= 128 ? 4 : 2; }
 // Waves a SIMD that the registers and the LDS leave room for.
 template <typename T>
-constexpr int waves_per_simd(int dp, int row_blocks) {
-  return dp * (int)sizeof(T) <= 128 ? 4 / row_blocks : dp * (int)sizeof(T) <= 256 ? 2 : 1;
+constexpr int waves_per_simd(int dp, int row_blocks, int waves) {
+  return dp * (int)sizeof(T) <= 128 && waves > 1 ? 4 / row_blocks : dp * (int)sizeof(T) <= 256 ? 2 : 1;
 }
 
 inline int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
@@ -151,15 +151,16 @@ __device__ void attend_row(const AttendArgs& a, const T* q, const T* k, const T*
   l_out = l;
 }
 
-// What 16-byte chunk c of row r of an LDS tile is stored in, so that the reads
-// below find their chunks in different banks.  RB: bytes of a row.
+// What 16-byte slot chunk c of row r of an LDS tile is stored in, so that the
+// reads below find their pieces in different columns of the 256 bytes that LDS
+// serves a cycle.  RB: bytes of a row.
 template <int RB>
-__device__ __forceinline__ int k_slot(int r, int c) {  // 8 rows, the same chunk: 16 bytes a lane
-  return RB % 128 == 0 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+__device__ __forceinline__ int k_slot(int r, int c) {  // 16 rows, the same chunk: 16 bytes a lane
+  return RB % 256 == 0 ? c ^ (r & 15) : RB % 128 == 0 ? c ^ ((r >> 1) & 7) : c ^ ((r >> 2) & 3);
 }
 template <int RB>
-__device__ __forceinline__ int v_slot(int r, int c) {  // 4 rows, two chunks each: 8 bytes a lane
-  return RB % 128 == 0 ? c ^ (2 * (r & 3)) : c ^ (2 * ((r >> 1) & 1));
+__device__ __forceinline__ int v_slot(int r, int c) {  // 4 rows, four chunks each: 8 bytes a lane
+  return RB % 256 == 0 ? c ^ (4 * (r & 3)) : RB % 128 == 0 ? c ^ (2 * (r & 3)) : c;
 }
 
 // Brings tiles of rows [j0, j0 + 32 KB) of one key head's K or V into LDS,
@@ -172,7 +173,7 @@ struct Stager {
   static constexpr int THREADS = kWave * WAVES, ROUNDS = CHUNKS / THREADS;
   static_assert(CHUNKS % THREADS == 0, "whole instructions");
   // the slots of a thread's rounds hold the same chunk of rows a constant apart
-  static constexpr bool SAME = THREADS % (8 * CH) == 0;
+  static constexpr bool SAME = THREADS % (16 * CH) == 0;
   const T* src;
   int64_t stride;
   int dim, lane, wave;
@@ -689,7 +690,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
 }
 
 template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
-__global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP, RB)) attend_kernel(AttendArgs a, int tiles_max, int splits) {
+__global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP, RB, WAVES)) attend_kernel(AttendArgs a, int tiles_max, int splits) {
   constexpr int ROWS = 32 * RB * WAVES, KT = 32 * KB;
   extern __shared__ __align__(16) char lds[];  // K, V, K, V tiles; a row of q for each wave; KB words
   // tiles of one head next to each other on one XCD (workgroups go round the

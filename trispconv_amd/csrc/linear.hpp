@@ -147,18 +147,19 @@ struct BiasEight {
 };
 
 // ---------------------------------------------------------------- tiles --
-// 16-byte chunk c of row r of an operand tile is stored in slot c ^ s(r): the
-// 8 lanes that read one chunk of 8 rows find them in different banks.
+// 16-byte chunk c of row r of an operand tile is stored in slot c ^ s(r), so
+// that the 16 lanes LDS serves at a time (one chunk of 16 rows) find them in
+// different 16-byte columns of its 256 bytes a cycle.
 template <int RB>
 __device__ __forceinline__ int tile_slot(int r, int c) {
-  return RB == 64 ? c ^ ((r >> 1) & 3) : c ^ (r & 7);
+  return RB == 64 ? c ^ ((r >> 2) & 3) : c ^ ((r >> 1) & 7);
 }
 
 // ROWS rows of RB bytes of an operand, one k tile after the other.
 template <typename T, int ROWS, int RB, int THREADS, bool ALIGNED>
 struct OperandStage {
   static constexpr int CH = RB / 16, ROUNDS = ROWS * CH / THREADS;
-  static_assert(ROWS * CH % THREADS == 0 && THREADS % (8 * CH) == 0, "whole rounds of like lanes");
+  static_assert(ROWS * CH % THREADS == 0 && THREADS % (16 * CH) == 0, "whole rounds of like lanes");
   const T* src;       // the lane's row in round 0, at its chunk
   uint32_t offset[ROUNDS];
   const T* base;
