@@ -137,3 +137,15 @@ def test_graph_replays(rows):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, block(inputs).features), i
+
+
+def test_document_example():
+    """The network shown in the boundary document, as written there."""
+    import re
+    from pathlib import Path
+    text = (Path(__file__).resolve().parent.parent / "INTEGRATION.md").read_text()
+    block = re.findall(r"```python\n(.*?)```", text.split("## Voxel blocks", 1)[1], flags=re.S)[0]
+    names: dict = {}
+    exec(compile(block, "INTEGRATION.md", "exec"), names)
+    y = names["net"](_input(channels=16, dtype=torch.float16))
+    assert y.features.shape == (471, 64) and torch.isfinite(y.features).all()

@@ -258,3 +258,16 @@ def test_many_streams_of_one_token():
     lq, lk = [1] * 300, [5 + (i * 37) % 200 for i in range(300)]
     q, k, v = _qkv(lq, lk, 8, 2, 64, torch.bfloat16)
     check(_run(q, k, v, lq, lk, (63, 0), 2), *attend64(q, k, v, lq, lk, (63, 0), 2))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries", [1, 200])
+def test_long_tail_of_small_weights(queries, dtype):
+    """One key 12 above thousands of others, which together still make up a
+    thirtieth of the sum: their weights keep their accuracy in 16 bits."""
+    n = 6000
+    q, k, v = _qkv([queries], [n], 1, 1, 32, dtype)
+    q, k, v = torch.zeros_like(q), torch.zeros_like(k), torch.ones_like(v)
+    q[..., 0], k[3, 0, 0], v[3] = 1.0, 12.0, 0.0
+    check(_run(q, k, v, [queries], [n], (None, None), 0, scale=1.0),
+          *attend64(q, k, v, [queries], [n], (None, None), 0, scale=1.0))

@@ -306,7 +306,7 @@ struct Walk {
   __device__ int token(uint32_t r) const { return static_cast<int>(min(r, rows - 1) / static_cast<uint32_t>(group)); }
 };
 
-constexpr float kMostWeight = 1024.f;
+constexpr float kLift = 8.f, kMostWeight = 32768.f;
 
 // Tiles of 32 RB WAVES rows (a row: one query of one head; the heads that
 // share a key head side by side) against tiles of 32 KB keys.
@@ -317,14 +317,16 @@ constexpr float kMostWeight = 1024.f;
 // stands, the right operand of O^T = V^T e^S^T: the product's sum runs over
 // keys in the order that S^T's registers have them, and V is read in the same
 // order (ds_read_b64_tr_b16 transposes it on the way from LDS).  K and V tiles
-// are double buffered: direct-to-LDS loads of the next ones fly while these
+// have BUFFERS buffers: direct-to-LDS loads of the next ones fly while these
 // are used, one barrier a tile.
 //
-// A row's reference m is the largest score of its first 32 keys, and moves (with
-// a rescale of what is there, and the weights made again) only when 32 weights
-// sum to over kMostWeight.  Up to there they keep the relative accuracy of f16
-// and bf16, so that most keys need no maximum at all; m is a score of the row,
-// so the largest weight is at least 1 and nothing that counts underflows.
+// A row's reference m is the largest score of its first 32 keys; a key of that
+// score has weight 2^kLift.  m moves (with a rescale of what is there, and the
+// weights made again) only when a lane's 16 weights sum to over kMostWeight,
+// which f16 still holds, so that most keys need no maximum at all.  m is a
+// score of the row, so its largest weight is at least 2^kLift: the lift keeps
+// weights down to 2^-22 of it normal numbers of f16, for long rows where many
+// such keys make up a share of the sum.
 //
 // A key that a row does not see has weight 0, and 0 times an infinite or NaN
 // value would be NaN.  When a row of the workgroup comes out not finite, the
@@ -342,13 +344,13 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
   const uint32_t wave_row = w.row0 + wave * 32 * RB;
   seen_keys(w.token(wave_row) + w.shift, w.lk, a.left, a.right, a.sinks, lo_first, hi_first, none);
   seen_keys(w.token(wave_row + 32 * RB - 1) + w.shift, w.lk, a.left, a.right, a.sinks, lo_last, hi_last, none);
-  int lo[RB], hi[RB], sink[RB];
+  int lo[RB], hi[RB];
   int4v qf[RB][STEPS];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const uint32_t r = wave_row + rb * 32 + col;
     const int t = w.token(r), g = static_cast<int>(min(r, w.rows - 1) - static_cast<uint32_t>(t) * w.group);
-    seen_keys(t + w.shift, w.lk, a.left, a.right, a.sinks, lo[rb], hi[rb], sink[rb]);
+    seen_keys(t + w.shift, w.lk, a.left, a.right, a.sinks, lo[rb], hi[rb], none);
     if (r >= w.rows) hi[rb] = 0;
     const T* q = static_cast<const T*>(a.q) + (w.q0 + t) * a.q_row + (w.hk * w.group + g) * a.q_head;
 #pragma unroll
@@ -392,7 +394,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
   };
 
   f32x16 o[RB][DB];
-  float m[RB], mc[RB], l[RB][2];  // reference maximum, times c, two partial sums
+  float m[RB], mc[RB], l[RB][2];  // reference score, its exponent, two partial sums
   int hit = 0;    // bit rb: the row sees a value that is not finite
   int clean = 0;  // the walk that replaces those values
   uint32_t* bad = reinterpret_cast<uint32_t*>(lds + 2 * BUFFERS * TILE + WAVES * DP * 4);
@@ -462,7 +464,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
 #pragma unroll
         for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[rb][i]), s[rb][i + 1]);
         const float m_new = fmaxf(m[rb], max_halves(top));
-        const float mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c;
+        const float mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c - kLift;
         const float fix = m[rb] == -__builtin_inff() ? 0.f : exp2f(mc[rb] - mc_new);
         m[rb] = m_new;
         mc[rb] = mc_new;
@@ -642,13 +644,13 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
           }
       }
     }
-    uint64_t redo = __ballot(odd && half == 0);  // w.rows done key by key
+    uint64_t redo = __ballot(odd && half == 0);  // rows done key by key
     if (redo) {
       // the tiles in LDS may still be read by other waves: each wave takes
       // its row's scratch from its own D floats behind them
       float* q_s = reinterpret_cast<float*>(lds + 2 * BUFFERS * TILE) + wave * DP;
       int j0 = 0, end = 0, sink_from = 0, sink_to = 0, from = 0, to = 0;
-      // this w.split's keys: tiles [w.t0, w.t1)
+      // this split's keys: tiles [t0, t1)
       if (w.t0 < w.sink_tiles) {
         tile_at(w.t0, j0, end);
         sink_from = j0;
