@@ -672,9 +672,11 @@ int launch_sized(const LinearArgs& a, hipStream_t s) {
   auto tiles = [&](int rows, int columns) { return ceil_div(a.n, rows) * ceil_div(a.c_out, columns); };
   // 256 x 256 reads least per product, but one workgroup fills a CU, with
   // nothing beside it while its sums leave: for long sums, and enough tiles
+  // (65536 x 1024 -> 4096 f16 610 us, in 128 x 128 tiles 800)
   if (a.c_in >= 512 && tiles(256, 256) >= 200) return launch_tile<T, 256, 256, 2, 4, 128, 2, ALIGNED, 2>(a, s);
   if (tiles(128, 128) >= 256) {
     // 64 columns where tiles of 128 would leave half of the last one empty
+    // (100000 x 64 -> 64 16.7 us, in 128 x 128 tiles 25.7)
     if (half_empty(a.c_out)) return launch_tile<T, 128, 64, 2, 2, 64, 2, ALIGNED, 2>(a, s);
     return launch_tile<T, 128, 128, 2, 2, 64, 2, ALIGNED, 2>(a, s);
   }
@@ -700,6 +702,7 @@ int launch_linear(const LinearArgs& a, hipStream_t s) {
   if (ceil_div(a.n, 64) * ceil_div(a.c_out, 64) < (kIs16<T> ? 128 : 200))
     return aligned ? launch_rows<T, true>(a, s) : launch_rows<T, false>(a, s);
   if constexpr (!kIs16<T>) {
+    // as for 16 bits (60000 x 768 -> 192: 128 x 64 129 us, 128 x 128 147)
     if (ceil_div(a.n, 128) * ceil_div(a.c_out, 128) < 256) return launch_split<64, 64, 2, 2, 3>(a, s);
     return half_empty(a.c_out) ? launch_split<128, 64, 2, 2, 3>(a, s) : launch_split<128, 128, 2, 2, 2>(a, s);
   } else {
