@@ -192,3 +192,15 @@ def test_one_wide_row_stride():
     room = torch.zeros(20, 1 << 21, dtype=torch.float16, device=DEV)
     room[:, :64] = x.to(DEV)
     check(spconv.linear_act(room[:, :64], w.to(DEV), b.to(DEV)), *linear64(x, w, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,c_in,c_out", [(10_700, 520, 1100), (10_500, 513, 1031), (10_497, 576, 1152)])
+def test_tiles_of_192_columns(n, c_in, c_out, dtype):
+    """Calls that 192 columns a tile cut with less left empty than 256."""
+    say("linear_act tiles of 192:", n, c_in, c_out, dtype)
+    x, w, b, r = _tensors(n, c_in, c_out, dtype)
+    for bias, act, res in ((None, None, r), (b, "gelu", None)):
+        got = spconv.linear_act(x.to(DEV), w.to(DEV), None if bias is None else bias.to(DEV), act,
+                                None if res is None else res.to(DEV))
+        check(got, *linear64(x, w, bias, act, res), what=f"{n} {c_in} {c_out} {act}")

@@ -244,7 +244,7 @@ template <typename T, int NW, int NB, int MB>
 __device__ __forceinline__ void leave(const LinearArgs& a, const f32x16 (&acc)[NB][MB], char* mine,
                                       int64_t wave_row, int o, BiasEight& bias_raw) {
   // 32 rows of the wave at a time through its own LDS
-  constexpr int LINE = leave_line(NW), LANES = NW / 8, ROWS = kWave / LANES;
+  constexpr int LINE = leave_line(NW), LANES = NW / 8, ROWS = kWave / LANES, ROUNDS = (32 + ROWS - 1) / ROWS;
   const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32, have = a.c_out - o;
   float bias[8];
   bias_raw.values(a.bias, a.bias_dtype, bias);
@@ -255,13 +255,15 @@ __device__ __forceinline__ void leave(const LinearArgs& a, const f32x16 (&acc)[N
     const int64_t first = wave_row + mb * 32;
     const int rows = static_cast<int>(min((int64_t)32, a.n - first));
     if (rows <= 0) break;
-    Eight<T> res[32 / ROWS];
+    // (lanes past a whole number of rows have none)
+    const int mine_to = kWave % LANES == 0 || lane < ROWS * LANES ? rows : 0;
+    Eight<T> res[ROUNDS];
     if (a.residual) {
       const T* p = static_cast<const T*>(a.residual) + first * a.r_stride + o;
 #pragma unroll
-      for (int i = 0; i < 32 / ROWS; ++i) {
+      for (int i = 0; i < ROUNDS; ++i) {
         const int r = i * ROWS + lane / LANES;
-        if (r < rows) res[i].load(p + r * a.r_stride, have);
+        if (r < mine_to) res[i].load(p + r * a.r_stride, have);
       }
     }
 #pragma unroll
@@ -274,10 +276,10 @@ __device__ __forceinline__ void leave(const LinearArgs& a, const f32x16 (&acc)[N
     __builtin_amdgcn_wave_barrier();
     char* out = static_cast<char*>(a.out) + first * a.c_out * (int64_t)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 32 / ROWS; ++i) {
+    for (int i = 0; i < ROUNDS; ++i) {
       const int r = i * ROWS + lane / LANES;
       float v[8];
-      __builtin_memcpy(v, mine + r * LINE + lane % LANES * 32, 32);
+      __builtin_memcpy(v, mine + (kWave % LANES ? min(r, 31) : r) * LINE + lane % LANES * 32, 32);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += bias[e];
       switch (a.act) {
@@ -293,7 +295,7 @@ __device__ __forceinline__ void leave(const LinearArgs& a, const f32x16 (&acc)[N
       }
       Eight<T> y;
       round_to<T, 8>(v, y.e);
-      if (r < rows) y.store(reinterpret_cast<T*>(out + (out_at + i * ROWS * out_step)), have);
+      if (r < mine_to) y.store(reinterpret_cast<T*>(out + (out_at + i * ROWS * out_step)), have);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -670,10 +672,20 @@ inline bool half_empty(int columns) { return (columns - 1) % 128 < 64; }
 template <typename T, bool ALIGNED>
 int launch_sized(const LinearArgs& a, hipStream_t s) {
   auto tiles = [&](int rows, int columns) { return ceil_div(a.n, rows) * ceil_div(a.c_out, columns); };
-  // 256 x 256 reads least per product, but one workgroup fills a CU, with
-  // nothing beside it while its sums leave: for long sums, and enough tiles
-  // (65536 x 1024 -> 4096 f16 610 us, in 128 x 128 tiles 800)
-  if (a.c_in >= 512 && tiles(256, 256) >= 200) return launch_tile<T, 256, 256, 2, 4, 128, 2, ALIGNED, 2>(a, s);
+  // Tiles of 256 rows read least per product, but one workgroup fills a CU: the
+  // last round of the 256 CUs takes as long as the others, with nothing beside
+  // it while its sums leave.  Smaller tiles follow each other, at 1.3 times the
+  // time a product (65536 x 1024 -> 4096 f16 610 us, in 128 x 128 tiles 800).
+  // So the products of a CU decide, for sums long enough to be most of the time
+  // (f16, us, 256 x 256, 256 x 192, small: 60013 x 768 -> 192 37.1 31.7 46.5;
+  // 60000 x 2048 -> 256 84.5 122 109; 10000 x 2048 -> 2048 123 102 122;
+  // 16000 x 1024 -> 1024 42.8 61.5 51.2; 100000 x 512 -> 384 99 86 73)
+  if (a.c_in >= 512) {
+    const auto rounds = [&](int columns) { return ceil_div(tiles(256, columns), 256) * 256 * columns; };
+    const int64_t small = a.n * align_up(a.c_out, 64) / 256 * 13 / 10;
+    if (rounds(256) <= std::min(rounds(192), small)) return launch_tile<T, 256, 256, 2, 4, 128, 2, ALIGNED, 2>(a, s);
+    if (rounds(192) < small) return launch_tile<T, 256, 192, 4, 2, 128, 2, ALIGNED, 2>(a, s);
+  }
   if (tiles(128, 128) >= 256) {
     // 64 columns where tiles of 128 would leave half of the last one empty
     // (100000 x 64 -> 64 16.7 us, in 128 x 128 tiles 25.7)
