@@ -149,3 +149,8 @@ def test_document_example():
     exec(compile(block, "INTEGRATION.md", "exec"), names)
     y = names["net"](_input(channels=16, dtype=torch.float16))
     assert y.features.shape == (471, 64) and torch.isfinite(y.features).all()
+
+
+def test_block_of_no_voxels():
+    net = spconv.SparseSequential(spconv.SerialOrder("o"), spconv.VoxelBlock(32, 2, "o")).to(DEV)
+    assert net(_input(per_sample=(0, 0))).features.shape == (0, 32)

@@ -271,3 +271,9 @@ def test_long_tail_of_small_weights(queries, dtype):
     q[..., 0], k[3, 0, 0], v[3] = 1.0, 12.0, 0.0
     check(_run(q, k, v, [queries], [n], (None, None), 0, scale=1.0),
           *attend64(q, k, v, [queries], [n], (None, None), 0, scale=1.0))
+
+
+@pytest.mark.parametrize("lq,lk", [([0], [0]), ([0, 0], [5, 3]), ([], [])])
+def test_no_queries(lq, lk):
+    q, k, v = _qkv(lq, lk, 4, 2, 16, torch.float16)
+    assert _run(q, k, v, lq, lk, (None, None), 0).shape == (0, 4, 16)

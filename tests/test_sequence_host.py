@@ -115,3 +115,8 @@ def test_serial_order_sorts_by_sample_and_interleaved_bits():
     y = spconv.SerialOrder("o")(x)
     assert y.features.flatten().tolist() == [3.0, 2.0, 1.0, 5.0, 4.0, 0.0]
     assert y.indice_dict["o"].offsets.tolist() == [0, 5, 6, 6]
+
+
+@pytest.mark.parametrize("samples,n_q,n_k", [(1, 0, 0), (3, 0, 10), (0, 0, 0), (0, 5, 5), (1, 5, 0)])
+def test_attention_of_nothing_needs_no_scratch(samples, n_q, n_k):
+    assert L.lib().tsc_window_attention_workspace_bytes(samples, n_q, n_k, 4, 2, 16, -1, -1, 0, 1) == 0

@@ -56,6 +56,7 @@ extern "C" int64_t tsc_window_attention_workspace_bytes(int32_t samples, int64_t
   if (!dtype_ok(dtype) || samples < 0 || n_q < 0 || n_k < 0 || q_heads <= 0 || k_heads <= 0 || dim < 1 ||
       dim > 256)
     return -1;
+  if (n_q == 0 || samples == 0) return 0;
   const Cut c = attend_cut(samples, n_q, n_k, q_heads, k_heads, dim, dtype_bytes(dtype), left, right, sinks);
   return part_bytes(c, n_q * q_heads, dim);
 }
