@@ -486,9 +486,10 @@ TSC_API int tsc_norm_rotate_heads(const void* q, int64_t q_row, int64_t q_head, 
 
 /* Attention of packed samples in a sliding window with sinks.  Sample b owns
  * query rows [offsets_q[b], offsets_q[b+1]) and key rows [offsets_k[b],
- * offsets_k[b+1]) (device int32, samples + 1 each; they start at 0, do not
- * decrease and end at n_q and n_k: other values give unspecified results,
- * but nothing outside the tensors is touched).  Its Lq queries are the last
+ * offsets_k[b+1]) (device int32, samples + 1 each, not decreasing; offsets
+ * that do, or that lie outside the tensors, give unspecified results, but
+ * nothing outside the tensors is touched).  Rows of out before the first
+ * sample and behind the last are 0; without samples nothing is written.  Its Lq queries are the last
  * of its Lk positions: query i stands at p = i + Lk - Lq and sees key j when
  * 0 <= j < Lk, j <= p + right, and j >= p - left or j < sinks (left or right
  * < 0: no limit on that side).  out = softmax over the seen keys of

@@ -277,3 +277,27 @@ def test_long_tail_of_small_weights(queries, dtype):
 def test_no_queries(lq, lk):
     q, k, v = _qkv(lq, lk, 4, 2, 16, torch.float16)
     assert _run(q, k, v, lq, lk, (None, None), 0).shape == (0, 4, 16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lq,lk", [([300, 70], [300, 70]), ([2, 1], [900, 4000])])
+def test_rows_of_no_sample(lq, lk, dtype):
+    """Rows before the first sample and behind the last give zeros, with the
+    keys split and without; the samples' rows are as they would be alone."""
+    q, k, v = _qkv(lq, lk, 4, 2, 64, dtype)
+    want = _run(q, k, v, lq, lk, (900, 30), 2)
+    pad = torch.full((5, 4, 64), float("nan"), dtype=dtype)
+    wide = torch.cat([pad, q, pad, pad]).to(DEV)
+    torch.full_like(wide, float("nan"))  # what the outputs' memory may hold
+    got = spconv.window_attention(wide, k.to(DEV), v.to(DEV), _offsets(lq) + 5, _offsets(lk),
+                                  window=(900, 30), sinks=2)
+    assert (got[:5] == 0).all() and (got[-10:] == 0).all()
+    check(got[5:-10], *attend64(q, k, v, lq, lk, (900, 30), 2))
+    check(want, *attend64(q, k, v, lq, lk, (900, 30), 2))
+
+
+def test_no_samples():
+    q, k, v = (t.to(DEV) for t in _qkv([40], [40], 4, 2, 64, torch.float16))
+    torch.full_like(q, float("nan"))
+    off = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert (spconv.window_attention(q, k, v, off) == 0).all()

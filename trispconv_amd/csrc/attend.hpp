@@ -8,8 +8,8 @@
 // and 0 where there is none.  The seen keys are two ranges:
 //   [lo, hi) with lo = max(0, p - left), hi = min(Lk, p + right + 1), and
 //   [0, min(sinks, lo, hi)).
-// One pass over the keys with the running maximum m and sum l of the
-// exponentials (f32): a new maximum rescales what is there by e^(m_old - m).
+// One pass over the keys with a running reference score m and the sum l of the
+// exponentials (f32): a new reference rescales what is there by e^(m_old - m).
 #pragma once
 
 #include "sequence.hpp"
@@ -85,6 +85,21 @@ __device__ __forceinline__ void sample_range(const int32_t* off, int b, int64_t 
   const int64_t hi = min(max((int64_t)off[b + 1], lo), n);
   at = lo;
   len = static_cast<int>(hi - lo);
+}
+
+// The query rows [first, last) from the first sample's to the last one's; the
+// others belong to no sample, and their outputs are 0.
+__device__ __forceinline__ void sample_rows(const AttendArgs& a, int64_t& first, int64_t& last) {
+  first = min(max((int64_t)a.off_q[0], (int64_t)0), a.n_q);
+  last = min(max((int64_t)a.off_q[a.samples], first), a.n_q);
+}
+
+// Zeros for the rows outside [first, last), shared out over the grid.
+template <typename T>
+__device__ __noinline__ void zero_outside(T* out, int64_t row, int64_t first, int64_t last, int64_t n) {
+  const int64_t before = first * row, all = before + (n - last) * row;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x)
+    out[i < before ? i : i - before + last * row] = from_f32<T>(0.f);
 }
 
 // The seen keys of position p among lk: [lo, hi) and [0, sink).
@@ -697,6 +712,12 @@ __global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP, RB, WAVES
   extern __shared__ __align__(16) char lds[];  // K, V, K, V tiles; a row of q for each wave; KB words
   // tiles of one head next to each other on one XCD (workgroups go round the
   // eight in turn), so that neighbouring windows meet in its L2
+  if (splits == 1) {  // (the join does it otherwise)
+    int64_t first, last;
+    sample_rows(a, first, last);
+    if (first > 0 || last < a.n_q)
+      zero_outside(static_cast<T*>(a.out), (int64_t)a.q_heads * a.dim, first, last, a.n_q);
+  }
   const int64_t blocks = (int64_t)tiles_max * a.k_heads * splits, per = (blocks + 7) / 8;
   const int64_t id = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (blockIdx.x / 8 >= per || id >= blocks) return;
@@ -779,10 +800,14 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a, int spli
   if (threadIdx.x >= LANES) return;
   sum = f32x4(0.f);
   for (int x = 0; x < GROUPS; ++x) sum += sums[x][c];
+  int64_t first, last;
+  sample_rows(a, first, last);
+  // (a row of no sample has no parts: what was read for it means nothing)
+  const bool none = l == 0.f || item < first * a.q_heads || item >= last * a.q_heads;
   T* out = static_cast<T*>(a.out) + item * a.dim;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (d + i < a.dim) out[d + i] = from_f32<T>(l == 0.f ? 0.f : sum[i] / l);
+    if (d + i < a.dim) out[d + i] = from_f32<T>(none ? 0.f : sum[i] / l);
 }
 
 template <typename T>

@@ -188,7 +188,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     as q and everything kept as k and v.  It sees the keys j with
     p - left <= j <= p + right (window = (left, right), None for no limit)
     and, up to p + right, the sample's first ``sinks`` keys.  scale defaults
-    to D^-0.5.  A query that sees no key gives zeros; what lies at keys a
+    to D^-0.5.  A query that sees no key gives zeros, as rows outside every
+    sample do (before offsets[0], from offsets[-1] on); what lies at keys a
     query does not see (NaN, infinities) does not reach it.  Scores, softmax
     and sums are float32.
     """
@@ -221,6 +222,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     (q, (q_row, q_head, _)), (k, (k_row, k_head, _)) = _rows_of(q), _rows_of(k)
     v, (v_row, v_head, _) = _rows_of(v)
     offsets, offsets_k = offsets.contiguous(), offsets_k.contiguous()
+    if offsets.shape[0] == 1:  # no samples
+        return q.new_zeros((n_q, hq, dim))
     out = q.new_empty((n_q, hq, dim))
     lib, samples, sinks = L.lib(), offsets.shape[0] - 1, min(sinks, _MOST)
     nbytes = lib.tsc_window_attention_workspace_bytes(samples, n_q, n_k, hq, hk, dim, left, right,
