@@ -10,11 +10,9 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // x * sigmoid(y): x / (1 + e^-y).  e^-y is infinite for y below about -89,
-// where 1/inf = 0 gives the limit; an x of -infinity is the lowest finite value
-// there, for 0 * infinity is NaN (a NaN x has a NaN y).
+// where 1/inf = 0 gives the limit.
 __device__ __forceinline__ float times_sigmoid(float x, float y) {
-  const float finite = __builtin_amdgcn_fmed3f(x, -3.4028235e38f, __builtin_inff());
-  return finite * rcp_fast(1.f + exp2_fast(-1.442695041f * y));
+  return x * rcp_fast(1.f + exp2_fast(-1.442695041f * y));
 }
 
 // x * Phi(x), Phi the normal distribution function.  With z = |x| / sqrt(2)
@@ -45,9 +43,9 @@ __device__ __forceinline__ float activate(float v) {
   if constexpr (ACT == TSC_ACT_GELU_TANH) {
     // 0.5 v (1 + tanh u) = v sigmoid(2u), u = sqrt(2/pi) (v + 0.044715 v^3)
     const float y = 1.5957691216f * v * __builtin_fmaf(0.044715f * v, v, 1.f);
-    return times_sigmoid(v, y);
+    return v == -__builtin_inff() ? 0.f : times_sigmoid(v, y);
   }
-  if constexpr (ACT == TSC_ACT_SILU) return times_sigmoid(v, v);
+  if constexpr (ACT == TSC_ACT_SILU) return v == -__builtin_inff() ? 0.f : times_sigmoid(v, v);
   return v;
 }
 

@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_tile_kernel(LinearA
     // The reads of a step between the matrix instructions of the one before,
     // for tiles of four steps (us, both orders in turn, bf16: 10000 x 2048 ->
     // 2048 86 against 91, 16000 x 1024 -> 1024 42.1 against 43.1, 65536 x 1024
-    // -> 4096 545 against 549; with the two steps of 64-byte rows nothing, or
+    // -> 4096 with SiLU 608 against 621; with the two steps of 64-byte rows nothing, or
     // 1% more at 100000 x 512 -> 384)
     if constexpr (RB == 128) __builtin_amdgcn_iglp_opt(0);
 #pragma unroll
