@@ -1,0 +1,28 @@
+"""Waits that inline assembly has to bring itself: the compiler's own hazard
+handling ends at its border."""
+import re
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parent.parent / "trispconv_amd" / "csrc"
+
+
+def _blocks():
+    """(file, the lines of instructions) of every inline assembly statement."""
+    for path in sorted([*CSRC.glob("*.hip"), *CSRC.glob("*.hpp")]):
+        for text in re.findall(r'\basm\s*volatile\s*\(\s*((?:"[^"]*"\s*)+)', path.read_text()):
+            code = "".join(re.findall(r'"([^"]*)"', text))
+            lines = [s.strip() for s in re.split(r"\\n|;", code.replace("\\t", " "))]
+            yield path.name, [s for s in lines if s]
+
+
+def test_m0_settles_before_a_load_to_lds():
+    """A load to LDS takes its LDS address from M0 and may not be the next
+    instruction behind the one that writes M0 (one wait state on CDNA; the
+    compiler puts an s_nop there around its own loads)."""
+    seen = 0
+    for name, lines in _blocks():
+        for i, line in enumerate(lines):
+            if re.match(r"s_\w+\s+m0\b", line):
+                seen += 1
+                assert i + 1 < len(lines) and lines[i + 1].startswith("s_nop"), (name, lines)
+    assert seen >= 3

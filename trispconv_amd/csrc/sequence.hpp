@@ -76,7 +76,7 @@ __device__ __forceinline__ void round_to(const float* v, T* e) {
 // kernels uses M0.
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t m0, bool in = true) {
   if (in)
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(m0) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(m0) : "memory");
 }
 
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
