@@ -26,3 +26,19 @@ def test_m0_settles_before_a_load_to_lds():
                 seen += 1
                 assert i + 1 < len(lines) and lines[i + 1].startswith("s_nop"), (name, lines)
     assert seen >= 3
+
+
+def test_a_base_in_scalar_registers_settles_before_a_load():
+    """A scalar register that a vector instruction wrote may be read by a memory
+    instruction five wait states later (CDNA).  Base addresses come back from
+    spilled registers through v_readlane right before the statement, so it has
+    to bring the five itself."""
+    seen = 0
+    for name, lines in _blocks():
+        for i, line in enumerate(lines):
+            if re.match(r"(global|buffer|scratch)_", line) and not line.endswith("off"):
+                seen += 1
+                waits = sum(1 + int(re.match(r"s_nop\s+(\d+)", s)[1]) if s.startswith("s_nop") else 1
+                            for s in lines[:i])
+                assert waits >= 5, (name, lines)
+    assert seen >= 1

@@ -73,10 +73,12 @@ __device__ __forceinline__ void round_to(const float* v, T* e) {
 // m0 (wave uniform) + 16 * lane, without passing through registers; lanes
 // that are not in leave their place as it is.  The compiler does not know of
 // the load: the kernels wait for it themselves.  Nothing else in these
-// kernels uses M0.
+// kernels uses M0.  Nor does it know the load's hazards: one wait state after
+// M0's write, and five after a vector instruction that wrote the base (a
+// spilled base comes back through v_readlane): the move and four more.
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t m0, bool in = true) {
   if (in)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(m0) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(m0) : "memory");
 }
 
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
