@@ -11,6 +11,8 @@ def _blocks():
     for path in sorted([*CSRC.glob("*.hip"), *CSRC.glob("*.hpp")]):
         for text in re.findall(r'\basm\s*volatile\s*\(\s*((?:"[^"]*"\s*)+)', path.read_text()):
             code = "".join(re.findall(r'"([^"]*)"', text))
+            # s_nop may be written as its word
+            code = re.sub(r"\.long 0xbf8000(\d\d)", lambda m: f"s_nop {int(m[1], 16)}", code)
             lines = [s.strip() for s in re.split(r"\\n|;", code.replace("\\t", " "))]
             yield path.name, [s for s in lines if s]
 

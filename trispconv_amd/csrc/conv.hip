@@ -1011,11 +1011,14 @@ __device__ __attribute__((aligned(16))) int32_t g_no_row[4] = {-1, -1, -1, -1};
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p));  // low 32 bits of a shared pointer
 }
+// A load that reads M0 must not be the next instruction behind the one that
+// writes it: one wait state, here as its word (0xbf800000 is s_nop 0), so that
+// the write and its load stay the only instructions of the statement.
 __device__ __forceinline__ void dma_b128(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "s"(m0) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\t.long 0xbf800000\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "s"(m0) : "memory");
 }
 __device__ __forceinline__ void dma_b32(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(g), "s"(m0) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\t.long 0xbf800000\n\tglobal_load_lds_dword %0, off" : : "v"(g), "s"(m0) : "memory");
 }
 
 // Dynamic LDS of conv_dma_kernel: two weight slabs, each wave's operand rows
