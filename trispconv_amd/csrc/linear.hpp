@@ -408,7 +408,8 @@ int launch_tile(const LinearArgs& a, hipStream_t s) {
 }
 
 // ------------------------------------------------------ f32 on bf16 units --
-// An f32 value is the sum of three bf16 values exactly (8 bits each of its 24):
+// An f32 value of 2^-110 or more is the sum of three bf16 values exactly (8 bits
+// each of its 24; subnormal ones, which the unit keeps, end at 2^-133):
 // hi + mid + lo, mid within 2^-8 and lo within 2^-16 of it.  Of the nine
 // products of two such sums the three of 2^-24 and less are left out (together
 // at most 2^-23 of the whole, an f32 rounding or two), and six bf16 matrix
@@ -446,6 +447,33 @@ __device__ __forceinline__ f32x16 mma32_split(const int4v a[3], const int4v b[3]
   return mma32<B>(a[0], b[0], c);
 }
 
+// Sums that the split cannot be trusted with are computed again on the f32 unit, a
+// block of 32 x 32 at a time; which they are goes by a sum's own row and column,
+// so that no other sum changes and the tile does not matter.
+//   * Not finite (an infinity has no parts, and 0 times it would be NaN), or under
+//     2^-64 without being zero (products of small parts are lost).
+//   * A value below 2^-110 leaves up to 2^-134, times the other operand.  Where a
+//     row of x has such values, that adds up to at most c_in max|w| 2^-134 over
+//     the column's weights w, and likewise for a row of W: sums below 2^28 times
+//     that, zeros as well.
+// Whether a tile has any such value is known from the split's registers (1.5
+// operations a value: 20,011 x 96 -> 384 23.5 us, without 22.8; 20,000 x 1024 ->
+// 1024 236 against 229); the ranges of its rows are looked for only then.
+__device__ __forceinline__ bool doubtful(float v) {
+  const float m = __builtin_fabsf(v);
+  return !(m >= 0x1p-64f && m < __builtin_inff()) && v != 0.f;
+}
+
+// A row's values: the largest, and whether one other than zero is below 2^-110.
+struct RowRange {
+  float most;
+  uint32_t small;
+};
+// A value's magnitude as a number that orders them, zero last: the bits without
+// the sign, shifted left, minus one.
+__device__ __forceinline__ uint32_t place(float v) { return (__builtin_bit_cast(uint32_t, v) << 1) - 1u; }
+constexpr uint32_t kSplitHolds = ((127u - 110u) << 24) - 1u;  // 2^-110's
+
 // ROWS rows of 32 values of an operand: from memory to registers, and from
 // there, split, to LDS (three planes of 64 bytes a row).
 template <int ROWS, int THREADS>
@@ -477,9 +505,12 @@ struct SplitStage {
       }
     }
   }
-  __device__ __forceinline__ void store(char* tile) const {
+  // least: the smallest place() of the values so far
+  __device__ __forceinline__ void store(char* tile, uint32_t& least) const {
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) least = min(least, place(held[i][e]));
       const int r = (i * THREADS + threadIdx.x) / 4;
       char* at = tile + r * 64 + tile_slot<64>(r, threadIdx.x % 4) * 16;
       const Split8 s = split8(held[i]);
@@ -490,13 +521,10 @@ struct SplitStage {
   }
 };
 
-// Results that the split cannot be trusted with: not finite (an infinity has no
-// parts, and 0 times it would be NaN), or under 2^-64 (parts of the smallest
-// values are lost).  They are summed again on the f32 unit, a block of 32 x 32 at
-// a time, and no other result changes.
-__device__ __forceinline__ bool doubtful(float v) {
-  const float m = __builtin_fabsf(v);
-  return !(m >= 0x1p-64f && m < __builtin_inff()) && v != 0.f;
+// LDS for the parts of two operand tiles, and for the sums on their way out.
+constexpr int split_pool_bytes(int bm, int bn, int wm, int wn) {
+  const int parts = 3 * (bm + bn) * 64, out = wm * wn * 32 * leave_line(bn / wn);
+  return parts > out ? parts : out;
 }
 
 // Tiles as in linear_tile_kernel, for f32 tensors: split on the way into LDS,
@@ -527,6 +555,7 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
   const int kts = (a.c_in + 31) / 32;
   const int mrow = wave / WN * MW + col, nrow = wave % WN * NW + col;
   const char *xt = lds, *wt = lds + 3 * BM * 64;
+  uint32_t least = 0xffffffffu;
   if (kts > 0) {
     xs.load(0, a.c_in);
     ws.load(0, a.c_in);
@@ -534,8 +563,9 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
   bias.load(a.bias, a.bias_dtype, o, a.c_out - o);
   for (int kt = 0; kt < kts; ++kt) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    xs.store(lds);
-    ws.store(lds + 3 * BM * 64);
+    xs.store(lds, least);
+    ws.store(lds + 3 * BM * 64, least);
+    asm volatile("" : "+v"(least));  // before the next values take registers
     if (kt + 1 < kts) {
       xs.load(kt + 1, a.c_in - (kt + 1) * 32);
       ws.load(kt + 1, a.c_in - (kt + 1) * 32);
@@ -561,15 +591,40 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
         for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mma32_split(wf[nb], xf[mb], acc[nb][mb]);
     }
   }
-  __syncthreads();
+  RowRange* ranges = reinterpret_cast<RowRange*>(lds + split_pool_bytes(BM, BN, WM, WN));
+  const bool small = __syncthreads_or(least < kSplitHolds);
+  if (small) {  // the ranges of the tile's rows, read once more: a thread each
+    for (int r = threadIdx.x; r < BM + BN; r += THREADS) {
+      const float* p = r < BM ? static_cast<const float*>(a.x) + min(row0 + r, a.n - 1) * a.x_stride
+                              : static_cast<const float*>(a.w) + min(col0 + r - BM, a.c_out - 1) * a.w_stride;
+      uint32_t first = 0xffffffffu;
+      float most = 0.f;
+#pragma unroll 1
+      for (int k = 0; k < a.c_in; ++k) {
+        first = min(first, place(p[k]));
+        most = fmaxf(most, __builtin_fabsf(p[k]));
+      }
+      ranges[r] = RowRange{most, first < kSplitHolds};
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-      bool odd = false;
+      uint32_t redo = 0;  // bit i: sum i is computed again
 #pragma unroll
-      for (int i = 0; i < 16; ++i) odd |= doubtful(acc[nb][mb][i]);
-      if (!__any(odd)) continue;
+      for (int i = 0; i < 16; ++i) redo |= (doubtful(acc[nb][mb][i]) ? 1u : 0u) << i;
+      if (small) {
+        const RowRange xr = ranges[mrow + mb * 32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const RowRange wr = ranges[BM + wave % WN * NW + nb * 32 + 8 * (i / 4) + 4 * half + i % 4];
+          const float loss = (xr.small ? wr.most : 0.f) + (wr.small ? xr.most : 0.f);
+          redo |= (__builtin_fabsf(acc[nb][mb][i]) < loss * (a.c_in * 0x1p-106f) ? 1u : 0u) << i;
+        }
+      }
+      if (!__any(redo)) continue;
       const float* x = static_cast<const float*>(a.x) +
                        min(row0 + wave / WN * MW + mb * 32 + col, a.n - 1) * a.x_stride;
       const float* w = static_cast<const float*>(a.w) +
@@ -581,15 +636,14 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
         sum = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? w[k] : 0.f, in ? x[k] : 0.f, sum, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[nb][mb][i] = doubtful(acc[nb][mb][i]) ? sum[i] : acc[nb][mb][i];
+      for (int i = 0; i < 16; ++i) acc[nb][mb][i] = redo >> i & 1u ? sum[i] : acc[nb][mb][i];
     }
   leave<float, NW>(a, acc, lds + wave * 32 * LINE, row0 + wave / WN * MW, o, bias);
 }
 
 template <int BM, int BN, int WM, int WN, int OCC>
 int launch_split(const LinearArgs& a, hipStream_t s) {
-  constexpr int main_bytes = 3 * (BM + BN) * 64, out_bytes = WM * WN * 32 * leave_line(BN / WN);
-  constexpr int bytes = main_bytes > out_bytes ? main_bytes : out_bytes;
+  constexpr int bytes = split_pool_bytes(BM, BN, WM, WN) + (BM + BN) * (int)sizeof(RowRange);
   auto kernel = &linear_split_kernel<BM, BN, WM, WN, OCC>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
