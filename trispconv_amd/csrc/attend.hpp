@@ -321,7 +321,13 @@ struct Walk {
   __device__ int token(uint32_t r) const { return static_cast<int>(min(r, rows - 1) / static_cast<uint32_t>(group)); }
 };
 
-constexpr float kLift = 8.f, kMostWeight = 32768.f;
+// The weight of a key at its row's reference score (in log2), and what a lane's 16
+// weights may sum to before the reference moves: 2^7 times as much.  f16 needs
+// the place below, and its values are too small for an f32 sum to overflow.  bf16
+// and f32 reach as far as the sums: their weights are at most 1, so that sums of
+// large values overflow no earlier than with the largest score as the reference.
+template <typename T> constexpr float kLift = std::is_same_v<T, __half> ? 8.f : -7.f;
+template <typename T> constexpr float kMostWeight = std::is_same_v<T, __half> ? 32768.f : 1.f;
 
 // Tiles of 32 RB WAVES rows (a row: one query of one head; the heads that
 // share a key head side by side) against tiles of 32 KB keys.
@@ -337,11 +343,17 @@ constexpr float kLift = 8.f, kMostWeight = 32768.f;
 //
 // A row's reference m is the largest score of its first 32 keys; a key of that
 // score has weight 2^kLift.  m moves (with a rescale of what is there, and the
-// weights made again) only when a lane's 16 weights sum to over kMostWeight,
-// which f16 still holds, so that most keys need no maximum at all.  m is a
-// score of the row, so its largest weight is at least 2^kLift: the lift keeps
-// weights down to 2^-22 of it normal numbers of f16, for long rows where many
-// such keys make up a share of the sum.
+// weights made again) only when a lane's 16 weights sum to over kMostWeight, so
+// that most keys need no maximum at all.  m is a score of the row, so its largest
+// weight is at least 2^kLift.  For f16, whose numbers end at 2^15 and are
+// normal from 2^-14 on, that keeps weights down to 2^-22 of it normal, for long rows
+// where many such keys make up a share of the sum.
+//
+// 16-bit tensors have their weights rounded to 16 bits for the product with V:
+// on the f32 unit, or split into parts, that product would take several times
+// as long.  It adds up to half a unit in the last place of the type to each
+// weight (errors against 64 bits 1.4 times those with f32 weights); scores,
+// references and both sums stay f32.
 //
 // A key that a row does not see has weight 0, and 0 times an infinite or NaN
 // value would be NaN.  When a row of the workgroup comes out not finite, the
@@ -471,7 +483,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
     weights();
     bool over = false;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) over |= m[rb] == -__builtin_inff() || sum[rb][0] + sum[rb][1] > kMostWeight;
+    for (int rb = 0; rb < RB; ++rb) over |= m[rb] == -__builtin_inff() || sum[rb][0] + sum[rb][1] > kMostWeight<T>;
     if (__any(over)) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
@@ -479,7 +491,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
 #pragma unroll
         for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[rb][i]), s[rb][i + 1]);
         const float m_new = fmaxf(m[rb], max_halves(top));
-        const float mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c - kLift;
+        const float mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c - kLift<T>;
         const float fix = m[rb] == -__builtin_inff() ? 0.f : exp2f(mc[rb] - mc_new);
         m[rb] = m_new;
         mc[rb] = mc_new;

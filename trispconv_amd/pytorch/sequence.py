@@ -190,8 +190,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     and, up to p + right, the sample's first ``sinks`` keys.  scale defaults
     to D^-0.5.  A query that sees no key gives zeros, as rows outside every
     sample do (before offsets[0], from offsets[-1] on); what lies at keys a
-    query does not see (NaN, infinities) does not reach it.  Scores, softmax
-    and sums are float32.
+    query does not see (NaN, infinities) does not reach it.  Scores, maxima and
+    sums are float32; for float16 and bfloat16 the softmax weights are rounded
+    to that type for the product with v.
     """
     what = "window_attention"
     if not q.is_cuda:
