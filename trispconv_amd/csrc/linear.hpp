@@ -31,12 +31,13 @@ int launch_linear(const LinearArgs& a, hipStream_t s);
 
 namespace {
 
+template <typename T>
 __device__ __forceinline__ float activate_any(int act, float v) {
   switch (act) {
-    case TSC_ACT_RELU: return activate<TSC_ACT_RELU>(v);
-    case TSC_ACT_GELU: return activate<TSC_ACT_GELU>(v);
-    case TSC_ACT_GELU_TANH: return activate<TSC_ACT_GELU_TANH>(v);
-    case TSC_ACT_SILU: return activate<TSC_ACT_SILU>(v);
+    case TSC_ACT_RELU: return activate<TSC_ACT_RELU, T>(v);
+    case TSC_ACT_GELU: return activate<TSC_ACT_GELU, T>(v);
+    case TSC_ACT_GELU_TANH: return activate<TSC_ACT_GELU_TANH, T>(v);
+    case TSC_ACT_SILU: return activate<TSC_ACT_SILU, T>(v);
     default: return v;
   }
 }
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(256) linear_few_kernel(LinearArgs a) {
     if (lane == r && r < a.n) {
       float v = acc[r];
       if (a.bias) v += load_any(a.bias, a.bias_dtype, o);
-      v = activate_any(a.act, v);
+      v = activate_any<T>(a.act, v);
       if (a.residual) v += to_f32(static_cast<const T*>(a.residual)[r * a.r_stride + o]);
       static_cast<T*>(a.out)[(int64_t)r * a.c_out + o] = from_f32<T>(v);
     }
@@ -283,10 +284,10 @@ __device__ __forceinline__ void leave(const LinearArgs& a, const f32x16 (&acc)[N
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += bias[e];
       switch (a.act) {
-        case TSC_ACT_RELU: for (float& e : v) e = activate<TSC_ACT_RELU>(e); break;
-        case TSC_ACT_GELU: for (float& e : v) e = activate<TSC_ACT_GELU>(e); break;
-        case TSC_ACT_GELU_TANH: for (float& e : v) e = activate<TSC_ACT_GELU_TANH>(e); break;
-        case TSC_ACT_SILU: for (float& e : v) e = activate<TSC_ACT_SILU>(e); break;
+        case TSC_ACT_RELU: for (float& e : v) e = activate<TSC_ACT_RELU, T>(e); break;
+        case TSC_ACT_GELU: for (float& e : v) e = activate<TSC_ACT_GELU, T>(e); break;
+        case TSC_ACT_GELU_TANH: for (float& e : v) e = activate<TSC_ACT_GELU_TANH, T>(e); break;
+        case TSC_ACT_SILU: for (float& e : v) e = activate<TSC_ACT_SILU, T>(e); break;
         default: break;
       }
       if (a.residual) {
@@ -706,7 +707,7 @@ __global__ void __launch_bounds__(512, 2) linear_rows_kernel(LinearArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v += sums[k][r][c + e];
     if (a.bias) v += load_any(a.bias, a.bias_dtype, o);
-    v = activate_any(a.act, v);
+    v = activate_any<T>(a.act, v);
     if (a.residual) v += to_f32(static_cast<const T*>(a.residual)[row * a.r_stride + o]);
     static_cast<T*>(a.out)[row * a.c_out + o] = from_f32<T>(v);
   }
