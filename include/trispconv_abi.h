@@ -498,6 +498,7 @@ TSC_API int tsc_norm_rotate_heads(const void* q, int64_t q_row, int64_t q_head, 
  * q (n_q, q_heads, dim), k and v (n_k, k_heads, dim) with row and head
  * strides, q_heads a multiple of k_heads (query head h reads key head
  * h / (q_heads / k_heads)), dim 1..256; out (n_q, q_heads, dim) contiguous.
+ * n_q < 2^31, n_k < 2^31 - 1024.
  * Scores, softmax statistics and sums are f32; for 16-bit dtypes the weights
  * are rounded to `dtype` for the product with v.
  * ws: *_workspace_bytes of scratch. */

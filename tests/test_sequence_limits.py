@@ -1,0 +1,16 @@
+"""Sizes at which the voxel-block operators' C entries refuse (nothing is launched)."""
+from trispconv_amd import _lib as L
+
+
+def test_attention_refuses_key_counts_that_its_tiles_would_pass():
+    """Key numbers are 32-bit, and a walk looks up to a tile past the last key:
+    the last of 2^31 - 1 keys would send it to negative ones."""
+    lib = L.lib()
+
+    def call(n_k, n_q=8):
+        return lib.tsc_window_attention(16, 64, 16, 16, 0, 16, 16, 0, 16, 16, 16, 1, n_q, n_k, 4, 2,
+                                        16, 100, 0, 0, 1.0, 1, None, 0, 16, None)
+
+    for n_k in (2 ** 31 - 1, 2 ** 31 - 1024):
+        assert call(n_k) == 1 and b"keys" in lib.tsc_last_error(), lib.tsc_last_error()
+    assert call(2 ** 31 - 1025, n_q=0) == 0  # accepted (without queries nothing is launched)

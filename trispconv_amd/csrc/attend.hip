@@ -76,6 +76,8 @@ extern "C" int tsc_window_attention(const void* q, int64_t q_row, int64_t q_head
               "window_attention: %d query heads do not share %d key heads evenly", q_heads, k_heads);
   TSC_REQUIRE(n_q * (q_heads / k_heads) < (1ll << 32) - 1024,
               "window_attention: over 2^32 rows of queries and the heads that share a key head");
+  // key numbers are 32-bit, and a walk looks up to a tile past the last
+  TSC_REQUIRE(n_k < (1ll << 31) - 1024, "window_attention: over 2^31 - 1025 keys");
   TSC_REQUIRE(dim >= 1 && dim <= 256, "window_attention: head size %d, 1 to 256 are supported", dim);
   TSC_REQUIRE(sinks >= 0, "window_attention: negative number of sinks");
   if (n_q == 0 || samples == 0) return 0;
