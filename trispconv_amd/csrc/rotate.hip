@@ -64,15 +64,11 @@ __device__ __forceinline__ void load_gain(const void* p, int dtype, int64_t at, 
   else as(__hip_bfloat16{});
 }
 
-// A wave per row; a head takes LP lanes (a power of two from D/2 up, at most
-// 64), a lane its pairs l, l + 64.  Any size, stride and alignment.
+// One row by one wave: lane l of a head (its pairs l and l + lp), group `sub` of
+// `heads` heads at a time.
 template <typename T>
-__global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
-  const int lane = threadIdx.x % kWave;
-  const int64_t r = blockIdx.x * (int64_t)4 + threadIdx.x / kWave;
-  if (r >= a.n) return;
-  const int half = a.dim / 2, F = half / a.axes;
-  const int sub = lane / lp, l = lane % lp, heads = kWave / lp;
+__device__ __forceinline__ void rotate_any_row(const RotateArgs& a, int64_t r, int lp, int half, int F, int sub,
+                                               int l, int heads) {
   float2 cs[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -122,6 +118,17 @@ __global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
       dst[ib] = from_f32<T>(p * cs[u].y + q * cs[u].x);
     }
   }
+}
+
+// A wave per row and turn; a head takes LP lanes (a power of two from D/2 up, at most
+// 64), a lane its pairs l, l + 64.  Any size, stride and alignment.
+template <typename T>
+__global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
+  const int lane = threadIdx.x % kWave;
+  const int half = a.dim / 2, F = half / a.axes;
+  const int sub = lane / lp, l = lane % lp, heads = kWave / lp;
+  for (int64_t r = blockIdx.x * (int64_t)4 + threadIdx.x / kWave; r < a.n; r += (int64_t)gridDim.x * 4)
+    rotate_any_row<T>(a, r, lp, half, F, sub, l, heads);
 }
 
 // The vector form: a workgroup takes kRows rows; its threads first share out the
@@ -252,7 +259,9 @@ int launch_rotate(const RotateArgs& a, hipStream_t s) {
     if (half % 4 == 0) return launch_lanes<T, 4>(a, s);
   int lp = 1;
   while (lp < kWave && lp < a.dim / 2) lp *= 2;
-  rotate_any_kernel<T><<<static_cast<unsigned>(ceil_div(a.n, 4)), 256, 0, s>>>(a, lp);
+  // (a launch holds fewer than 2^32 threads, 2^26 waves)
+  const int64_t blocks = std::min<int64_t>(ceil_div(a.n, 4), 1 << 20);
+  rotate_any_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, lp);
   TSC_LAUNCH_CHECK("norm_rotate_heads");
   return 0;
 }
