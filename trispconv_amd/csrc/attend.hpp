@@ -839,7 +839,7 @@ int launch_tiles(const AttendArgs& a, const Cut& c, hipStream_t s) {
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
   const int64_t blocks = align_up(c.tiles * a.k_heads * c.splits, 8);
-  TSC_REQUIRE(blocks < (1ll << 31), "window_attention: too many tiles");
+  TSC_REQUIRE(blocks * kWave * WAVES < (1ll << 32), "window_attention: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, static_cast<int>(c.tiles), c.splits);
   TSC_LAUNCH_CHECK("window_attention");
   if (c.splits > 1) return launch_join<T>(a, c.splits, s);

@@ -402,7 +402,7 @@ int launch_tile(const LinearArgs& a, hipStream_t s) {
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
   const int64_t tm = ceil_div(a.n, BM), tn = ceil_div(a.c_out, BN), blocks = align_up(tm * tn, 8);
-  TSC_REQUIRE(blocks < (1ll << 31), "linear_act: too many tiles");
+  TSC_REQUIRE(blocks * kWave * WM * WN < (1ll << 32), "linear_act: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * WM * WN, bytes, s>>>(a, static_cast<int>(tm), static_cast<int>(tn));
   TSC_LAUNCH_CHECK("linear_act");
   return 0;
@@ -649,7 +649,7 @@ int launch_split(const LinearArgs& a, hipStream_t s) {
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
   const int64_t tm = ceil_div(a.n, BM), tn = ceil_div(a.c_out, BN), blocks = align_up(tm * tn, 8);
-  TSC_REQUIRE(blocks < (1ll << 31), "linear_act: too many tiles");
+  TSC_REQUIRE(blocks * kWave * WM * WN < (1ll << 32), "linear_act: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * WM * WN, bytes, s>>>(a, static_cast<int>(tm), static_cast<int>(tn));
   TSC_LAUNCH_CHECK("linear_act_split");
   return 0;
