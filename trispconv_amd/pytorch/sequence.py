@@ -20,9 +20,10 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from .. import _lib as L
-from .modules import SparseModule
+from .modules import SparseModule, _plain
 from .tensor import SparseConvTensor
 
 __all__ = ["linear_act", "norm_rotate_heads", "window_attention", "VoxelOrder", "SerialOrder",
@@ -287,6 +288,20 @@ class SerialOrder(SparseModule):
                                 indice_dict={self.order_key: order})
 
 
+_ACT_MODULES = {None: lambda v: v, "none": lambda v: v, "relu": F.relu, "gelu": F.gelu,
+                "gelu_tanh": lambda v: F.gelu(v, approximate="tanh"), "silu": F.silu}
+
+
+def _project(m: nn.Module, x: torch.Tensor, activation: Optional[str] = None,
+             residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(m(x)) + residual: one launch where ``m`` is an nn.Linear as it is;
+    a subclass, a module in its place or one with hooks runs by itself."""
+    if type(m) is nn.Linear and _plain(m):
+        return linear_act(x, m.weight, m.bias, activation, residual)
+    v = _ACT_MODULES[activation](m(x))
+    return v if residual is None else v + residual
+
+
 class VoxelBlock(SparseModule):
     """A transformer block over the voxels of each sample, in the order that a
     SerialOrder with the same ``order_key`` left them:
@@ -329,13 +344,13 @@ class VoxelBlock(SparseModule):
         with torch.no_grad():
             f = x.features
             hq, hk = self.heads, self.kv_heads
-            qkv = linear_act(self.norm1(f), self.qkv.weight, self.qkv.bias)
-            qkv = qkv.view(f.shape[0], hq + 2 * hk, self.dim)
+            qkv = _project(self.qkv, self.norm1(f))
+            qkv = qkv.reshape(f.shape[0], hq + 2 * hk, self.dim)
             q, k = norm_rotate_heads(qkv[:, :hq], qkv[:, hq:hq + hk], x.indices[:, 1:],
                                      self.q_gain, self.k_gain, self.eps, self.base)
             a = window_attention(q, k, qkv[:, hq + hk:], order.offsets, window=self.window,
                                  sinks=self.sinks)
-            f = linear_act(a.view(f.shape), self.proj.weight, self.proj.bias, residual=f)
-            h = linear_act(self.norm2(f), self.up.weight, self.up.bias, self.activation)
-            f = linear_act(h, self.down.weight, self.down.bias, residual=f)
+            f = _project(self.proj, a.view(f.shape), residual=f)
+            h = _project(self.up, self.norm2(f), self.activation)
+            f = _project(self.down, h, residual=f)
         return x.replace_feature(f)
