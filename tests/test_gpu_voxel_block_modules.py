@@ -80,3 +80,34 @@ def test_subclass_runs_its_own_forward():
     plain = block(x).features
     block.up.__class__ = Twice
     assert not torch.allclose(block(x).features, plain, rtol=1e-3, atol=1e-3)
+
+
+@pytest.mark.parametrize("features,parameters", [
+    (torch.float16, torch.float32), (torch.bfloat16, torch.float32), (torch.float64, torch.float32),
+    (torch.float32, torch.float16), (torch.float16, torch.bfloat16), (torch.float64, torch.float64)])
+def test_features_of_another_type(features, parameters):
+    """As in the convolutions: f32 copies compute it, and the result has the
+    features' type."""
+    block = _block(kv_heads=1).to(parameters)
+    x = _input(features)
+    got = block(x)
+    assert got.features.dtype is features and got.indices is x.indices
+    want = copy.deepcopy(block).float()(x.replace_feature(x.features.float()))
+    assert torch.equal(got.features, want.features.to(features))
+    assert all(p.dtype is parameters for p in block.parameters())
+
+
+def test_one_parameter_of_another_type():
+    """A block in f16 whose norms are kept in f32, as mixed precision leaves it."""
+    block = _block().half()
+    block.norm1.float(), block.norm2.float()
+    x = _input(torch.float16)
+    want = copy.deepcopy(block).float()(x.replace_feature(x.features.float()))
+    assert torch.equal(block(x).features, want.features.half())
+
+
+def test_hooks_run_on_features_of_another_type():
+    block, calls = _block(), []
+    block.up.register_forward_hook(lambda m, args, out: calls.append(out.dtype))
+    block(_input(torch.bfloat16))
+    assert calls == [torch.float32]

@@ -23,6 +23,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import _lib as L
+from .functional import compute_dtype
 from .modules import SparseModule, _plain
 from .tensor import SparseConvTensor
 
@@ -332,6 +333,17 @@ class VoxelBlock(SparseModule):
         self.proj = nn.Linear(channels, channels)
         self.up, self.down = nn.Linear(channels, hidden), nn.Linear(hidden, channels)
 
+    def _computes_in(self, dtype: torch.dtype) -> bool:
+        """Whether the kernels take ``dtype`` and the layers' weights have it."""
+        if compute_dtype(dtype, dtype) is not dtype:
+            return False
+        layers = self._modules
+        for name in ("norm1", "qkv", "proj", "norm2", "up", "down"):
+            w = layers[name]._parameters.get("weight")
+            if w is not None and w.dtype is not dtype:
+                return False
+        return True
+
     def forward(self, x: SparseConvTensor) -> SparseConvTensor:
         order = x.indice_dict.get(self.order_key)
         if not isinstance(order, VoxelOrder):
@@ -341,8 +353,13 @@ class VoxelBlock(SparseModule):
             raise ValueError(f"VoxelBlock: the rows are not those that SerialOrder "
                              f"'{self.order_key}' ordered (a layer since then changed the "
                              "coordinates); run a SerialOrder on them first")
+        f = x.features
+        if not self._computes_in(f.dtype):
+            # on f32 copies, as the convolutions do
+            wide = {n: p.float() for n, p in self.named_parameters() if p.is_floating_point()}
+            y = torch.func.functional_call(self, wide, (x.replace_feature(f.float()),))
+            return x.replace_feature(y.features.to(f.dtype))
         with torch.no_grad():
-            f = x.features
             hq, hk = self.heads, self.kv_heads
             qkv = _project(self.qkv, self.norm1(f))
             qkv = qkv.reshape(f.shape[0], hq + 2 * hk, self.dim)
