@@ -237,7 +237,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     rc = lib.tsc_window_attention(
         q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
         offsets.data_ptr(), offsets_k.data_ptr(), samples, n_q, n_k, hq, hk, dim, left, right,
-        sinks, dim ** -0.5 if scale is None else scale, code,
+        sinks, max(dim, 1) ** -0.5 if scale is None else scale, code,
         None if ws is None else ws.data_ptr(), nbytes, out.data_ptr(), L.stream_of(q))
     if rc:
         L.check(rc, what)
