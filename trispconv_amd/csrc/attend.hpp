@@ -59,8 +59,9 @@ template <typename T>
 constexpr int key_blocks(int dp) { return dp * (int)sizeof(T) <= 512 ? 2 : 1; }
 
 // Tiles of K and V in LDS: the one in use and those on their way.  A wave that
-// is a workgroup of its own walks a few tiles, and asks for most of them at
-// once.
+// is a workgroup of its own asks for three tiles at once, which is most of a
+// split walk; every tile then waits for all that is on the way, so that over a
+// longer walk four buffers hide no more than two.
 template <typename T>
 constexpr int tile_buffers(int dp, int waves) { return waves == 1 && dp * (int)sizeof(T) <= 128 ? 4 : 2; }
 // Waves a SIMD that the registers and the LDS leave room for.
