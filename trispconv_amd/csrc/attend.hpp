@@ -329,6 +329,7 @@ struct Walk {
 // large values overflow no earlier than with the largest score as the reference.
 template <typename T> constexpr float kLift = std::is_same_v<T, __half> ? 8.f : -7.f;
 template <typename T> constexpr float kMostWeight = std::is_same_v<T, __half> ? 32768.f : 1.f;
+constexpr float kFar = 0x1p24f;  // exponents from here on have no fractions in f32
 
 // Tiles of 32 RB WAVES rows (a row: one query of one head; the heads that
 // share a key head side by side) against tiles of 32 KB keys.
@@ -355,6 +356,10 @@ template <typename T> constexpr float kMostWeight = std::is_same_v<T, __half> ? 
 // as long.  It adds up to half a unit in the last place of the type to each
 // weight (errors against 64 bits 1.4 times those with f32 weights); scores,
 // references and both sums stay f32.
+//
+// The exponents are s c - mc with mc = m c rounded: a row's weights have a factor in
+// common that the division takes out again, unless the rounding is of whole
+// exponents.  Rows whose reference was ever that far from 0 are done key by key.
 //
 // A key that a row does not see has weight 0, and 0 times an infinite or NaN
 // value would be NaN.  When a row of the workgroup comes out not finite, the
@@ -423,7 +428,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
 
   f32x16 o[RB][DB];
   float m[RB], mc[RB], l[RB][2];  // reference score, its exponent, two partial sums
-  int hit = 0;    // bit rb: the row sees a value that is not finite
+  int hit = 0;    // bit rb: the row is done key by key
   int clean = 0;  // the walk that replaces those values
   uint32_t* bad = reinterpret_cast<uint32_t*>(lds + 2 * BUFFERS * TILE + WAVES * DP * 4);
   const float c = a.scale_log2;
@@ -496,6 +501,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
         const float fix = m[rb] == -__builtin_inff() ? 0.f : exp2f(mc[rb] - mc_new);
         m[rb] = m_new;
         mc[rb] = mc_new;
+        hit |= (__builtin_fabsf(mc_new) >= kFar) << rb;
         l[rb][0] *= fix;
         l[rb][1] *= fix;
 #pragma unroll
