@@ -278,6 +278,8 @@ class SerialOrder(SparseModule):
     def forward(self, x: SparseConvTensor) -> SparseConvTensor:
         if max(x.spatial_shape) > 1 << 16:
             raise ValueError(f"SerialOrder: {list(x.spatial_shape)} has an axis over 65536 cells")
+        if x.batch_size > (1 << 15) - 1:  # with 48 bits of a cell a key fills 63
+            raise ValueError(f"SerialOrder: over 32767 samples ({x.batch_size})")
         b, zc, yc, xc = (c.long() for c in x.indices.unbind(1))
         key = (b << 48) | (_spread(zc) << 2) | (_spread(yc) << 1) | _spread(xc)
         key, rows = torch.sort(key, stable=True)
