@@ -457,9 +457,12 @@ __device__ __forceinline__ f32x16 mma32_split(const int4v a[3], const int4v b[3]
 //     row of x has such values, that adds up to at most c_in max|w| 2^-134 over
 //     the column's weights w, and likewise for a row of W: sums below 2^28 times
 //     that, zeros as well.
-// Whether a tile has any such value is known from the split's registers (1.5
-// operations a value: 20,011 x 96 -> 384 23.5 us, without 22.8; 20,000 x 1024 ->
-// 1024 236 against 229); the ranges of its rows are looked for only then.
+// Whether a tile has such a value, and its largest, is known from the split's
+// registers (2 operations a value: 20,000 x 1024 -> 1024 with GELU 244 us, without
+// 235; 60,000 x 768 -> 192 131 against 125).  The ranges of its rows are read only
+// where one of its sums is below what the tile's largest value could cost (a value of
+// 1e-36 in every row: the same times; with the ranges read for all tiles 1540 and
+// 1030).
 __device__ __forceinline__ bool doubtful(float v) {
   const float m = __builtin_fabsf(v);
   return !(m >= 0x1p-64f && m < __builtin_inff()) && v != 0.f;
@@ -506,12 +509,15 @@ struct SplitStage {
       }
     }
   }
-  // least: the smallest place() of the values so far
-  __device__ __forceinline__ void store(char* tile, uint32_t& least) const {
+  // least, most: the smallest place() and the largest magnitude so far
+  __device__ __forceinline__ void store(char* tile, uint32_t& least, float& most) const {
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) least = min(least, place(held[i][e]));
+      for (int e = 0; e < 8; ++e) {
+        least = min(least, place(held[i][e]));
+        most = fmaxf(most, __builtin_fabsf(held[i][e]));
+      }
       const int r = (i * THREADS + threadIdx.x) / 4;
       char* at = tile + r * 64 + tile_slot<64>(r, threadIdx.x % 4) * 16;
       const Split8 s = split8(held[i]);
@@ -557,6 +563,7 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
   const int mrow = wave / WN * MW + col, nrow = wave % WN * NW + col;
   const char *xt = lds, *wt = lds + 3 * BM * 64;
   uint32_t least = 0xffffffffu;
+  float most = 0.f;
   if (kts > 0) {
     xs.load(0, a.c_in);
     ws.load(0, a.c_in);
@@ -564,9 +571,9 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
   bias.load(a.bias, a.bias_dtype, o, a.c_out - o);
   for (int kt = 0; kt < kts; ++kt) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    xs.store(lds, least);
-    ws.store(lds + 3 * BM * 64, least);
-    asm volatile("" : "+v"(least));  // before the next values take registers
+    xs.store(lds, least, most);
+    ws.store(lds + 3 * BM * 64, least, most);
+    asm volatile("" : "+v"(least), "+v"(most));  // before the next values take registers
     if (kt + 1 < kts) {
       xs.load(kt + 1, a.c_in - (kt + 1) * 32);
       ws.load(kt + 1, a.c_in - (kt + 1) * 32);
@@ -593,19 +600,43 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
     }
   }
   RowRange* ranges = reinterpret_cast<RowRange*>(lds + split_pool_bytes(BM, BN, WM, WN));
-  const bool small = __syncthreads_or(least < kSplitHolds);
-  if (small) {  // the ranges of the tile's rows, read once more: a thread each
-    for (int r = threadIdx.x; r < BM + BN; r += THREADS) {
+  const float weight = a.c_in * 0x1p-106f;
+  bool small = __syncthreads_or(least < kSplitHolds);
+  if (small) {  // does a sum come near what any row or column of the tile may lose?
+#pragma unroll
+    for (int x = 1; x < kWave; x <<= 1) most = fmaxf(most, __shfl_xor(most, x, kWave));
+    if (lane == 0) ranges[wave].most = most;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < WM * WN; ++x) most = fmaxf(most, ranges[x].most);
+    bool near = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) near |= __builtin_fabsf(acc[nb][mb][i]) < 2.f * most * weight;
+    small = __syncthreads_or(near);
+  }
+  if (small) {  // the ranges of the tile's rows, read once more: eight lanes a row
+    static_assert((BM + BN) % (THREADS / 8) == 0, "whole rounds");
+#pragma unroll 2
+    for (int r = threadIdx.x / 8; r < BM + BN; r += THREADS / 8) {
       const float* p = r < BM ? static_cast<const float*>(a.x) + min(row0 + r, a.n - 1) * a.x_stride
                               : static_cast<const float*>(a.w) + min(col0 + r - BM, a.c_out - 1) * a.w_stride;
       uint32_t first = 0xffffffffu;
-      float most = 0.f;
-#pragma unroll 1
-      for (int k = 0; k < a.c_in; ++k) {
+      float top = 0.f;
+#pragma unroll 4
+      for (int k = lane % 8; k < a.c_in; k += 8) {
         first = min(first, place(p[k]));
-        most = fmaxf(most, __builtin_fabsf(p[k]));
+        top = fmaxf(top, __builtin_fabsf(p[k]));
       }
-      ranges[r] = RowRange{most, first < kSplitHolds};
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) {
+        first = min(first, static_cast<uint32_t>(__shfl_xor(static_cast<int>(first), x, kWave)));
+        top = fmaxf(top, __shfl_xor(top, x, kWave));
+      }
+      if (lane % 8 == 0) ranges[r] = RowRange{top, first < kSplitHolds};
     }
     __syncthreads();
   }
@@ -622,7 +653,7 @@ __global__ void __launch_bounds__(kWave* WM* WN, OCC) linear_split_kernel(Linear
         for (int i = 0; i < 16; ++i) {
           const RowRange wr = ranges[BM + wave % WN * NW + nb * 32 + 8 * (i / 4) + 4 * half + i % 4];
           const float loss = (xr.small ? wr.most : 0.f) + (wr.small ? xr.most : 0.f);
-          redo |= (__builtin_fabsf(acc[nb][mb][i]) < loss * (a.c_in * 0x1p-106f) ? 1u : 0u) << i;
+          redo |= (__builtin_fabsf(acc[nb][mb][i]) < loss * weight ? 1u : 0u) << i;
         }
       }
       if (!__any(redo)) continue;
