@@ -515,6 +515,57 @@ TSC_API int tsc_window_attention(const void* q, int64_t q_row, int64_t q_head, c
                                  int32_t dtype, void* ws, int64_t ws_bytes, void* out,
                                  tsc_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Keys and values kept in pages (no counterpart in the reference).  k_pages
+ * and v_pages hold `pages` pages of page_rows rows (1 to 2^20) of k_heads heads
+ * of dim values, with any page, row and head strides.  Position t of sample b
+ * is row t % page_rows of page table[b * table_row + t / page_rows] (device
+ * int32; table_pages entries a sample), and lengths[b] (device int32) is how
+ * many positions the sample has, its new rows among them: of the Lq rows
+ * offsets[b] .. offsets[b+1] (as above) row i stands at position
+ * lengths[b] - Lq + i.  Lengths over the table's room, or negative, are cut.
+ *
+ * tsc_norm_rotate_append is tsc_norm_rotate_heads with the keys written to their
+ * rows of k_pages, and the values v (n, k_heads, dim; copied as they are) to
+ * those of v_pages.  Nothing else of the pages is written.  A row of no sample,
+ * or one whose position or page there is not, writes its q_out only.  No two
+ * samples' new rows may share a page's row.
+ * ------------------------------------------------------------------------ */
+TSC_API int tsc_norm_rotate_append(
+    const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+    const void* v, int64_t v_row, int64_t v_head, const void* positions, int64_t pos_row,
+    int32_t pos_float, int32_t axes, const void* q_gain, const void* k_gain, int32_t gain_dtype,
+    int32_t q_gain_per_head, int32_t k_gain_per_head, float eps, double base, int32_t interleaved,
+    int32_t dtype, int64_t n, int32_t q_heads, int32_t k_heads, int32_t dim, void* k_pages,
+    int64_t k_page, int64_t k_page_row, int64_t k_page_head, void* v_pages, int64_t v_page,
+    int64_t v_page_row, int64_t v_page_head, int64_t pages, int64_t page_rows,
+    const int32_t* table, int64_t table_row, int64_t table_pages, const int32_t* offsets,
+    const int32_t* lengths, int32_t samples, void* q_out, tsc_stream_t stream);
+
+/* tsc_window_attention of the new rows q (n_q, q_heads, dim) over what their
+ * samples keep: query i of Lq stands at p = i + Lk - Lq of its sample's Lk =
+ * lengths[b] positions.  prefix_pages > 0: the first prefix_pages * page_rows
+ * positions of every sample are the pages prefix[0 ..] (device int32; these
+ * entries of the table are not read), and are read once for all samples.  Pages
+ * that a query sees have to be there; other numbers are cut to those there are.
+ * Rows of out before the first sample and behind the last are 0.
+ * `longest` of the workspace query: table_pages * page_rows; its prefix_rows:
+ * prefix_pages * page_rows. */
+TSC_API int64_t tsc_cache_attention_workspace_bytes(int32_t samples, int64_t n_q, int64_t longest,
+                                                    int64_t prefix_rows, int32_t q_heads,
+                                                    int32_t k_heads, int32_t dim, int32_t left,
+                                                    int32_t right, int32_t sinks, int32_t dtype);
+TSC_API int tsc_cache_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages,
+                                int64_t k_page, int64_t k_page_row, int64_t k_page_head,
+                                const void* v_pages, int64_t v_page, int64_t v_page_row,
+                                int64_t v_page_head, int64_t pages, int64_t page_rows,
+                                const int32_t* table, int64_t table_row, int64_t table_pages,
+                                const int32_t* offsets, const int32_t* lengths, int32_t samples,
+                                const int32_t* prefix, int64_t prefix_pages, int64_t n_q,
+                                int32_t q_heads, int32_t k_heads, int32_t dim, int32_t left,
+                                int32_t right, int32_t sinks, float scale, int32_t dtype, void* ws,
+                                int64_t ws_bytes, void* out, tsc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

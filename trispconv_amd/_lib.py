@@ -100,9 +100,21 @@ _SIGNATURES = {
                                             _vp, _vp, _i32, _i64, _i64, _i32, _i32, _i32, _i32,
                                             _i32, _i32, ctypes.c_float, _i32, _vp, _i64, _vp,
                                             _vp]),
+    "tsc_norm_rotate_append": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                              _vp, _i64, _i32, _i32, _vp, _vp, _i32, _i32, _i32,
+                                              ctypes.c_float, ctypes.c_double, _i32, _i32, _i64,
+                                              _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp, _i64,
+                                              _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                                              _i32, _vp, _vp]),
+    "tsc_cache_attention_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+                                                   _i32, _i32, _i32]),
+    "tsc_cache_attention": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
+                                           _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp,
+                                           _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32,
+                                           ctypes.c_float, _i32, _vp, _i64, _vp, _vp]),
 }
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _lib: Optional[ctypes.CDLL] = None
 

@@ -112,14 +112,23 @@ __device__ __forceinline__ void seen_keys(int p, int lk, int left, int right, in
   sink = min(sinks, min(lo, hi));
 }
 
+// The keys or values of one sample and head: row j is stride elements behind row
+// j - 1.
+template <typename T>
+struct DenseRows {
+  const T* base;
+  int64_t stride;
+  __device__ __forceinline__ const T* row(int j) const { return base + j * stride; }
+};
+
 // One query and head by one wave: a lane scores every 64th key, then the lanes
 // share out the D values and add the 64 keys' values one by one.  Reads no
 // key it does not see, and of those only [s0, s1) among the sinks and [w0,
 // w1) of the window's tiles.  Any size, stride and alignment; q_s: D floats of LDS
 // for this wave.  Returns the running maximum (in units of log2) and sum;
 // lane l holds the sums of values l, l + 64, ...
-template <typename T>
-__device__ void attend_row(const AttendArgs& a, const T* q, const T* k, const T* v, int lo, int hi,
+template <typename T, typename Rows>
+__device__ void attend_row(const AttendArgs& a, const T* q, const Rows& k, const Rows& v, int lo, int hi,
                            int sink, int s0, int s1, int w0, int w1, float* q_s, float& m_out,
                            float& l_out, float o[4]) {
   const int lane = threadIdx.x % kWave;
@@ -138,7 +147,8 @@ __device__ void attend_row(const AttendArgs& a, const T* q, const T* k, const T*
       float s = -__builtin_inff();
       if (j < to) {
         float dot = 0.f;
-        for (int d = 0; d < a.dim; ++d) dot += q_s[d] * to_f32(k[j * a.k_row + d]);
+        const T* kj = k.row(j);
+        for (int d = 0; d < a.dim; ++d) dot += q_s[d] * to_f32(kj[d]);
         s = dot * a.scale_log2;
       }
       float top = s;
@@ -155,10 +165,11 @@ __device__ void attend_row(const AttendArgs& a, const T* q, const T* k, const T*
       for (int x = 0; x < cnt; ++x) {
         const float px = __shfl(p, x, kWave);
         l += px;
+        const T* vj = v.row(j0 + x);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int d = lane + u * kWave;
-          if (d < a.dim) o[u] += px * to_f32(v[(j0 + x) * a.v_row + d]);
+          if (d < a.dim) o[u] += px * to_f32(vj[d]);
         }
       }
     }
@@ -703,8 +714,8 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
         int lx, hx, sx;
         seen_keys(tx + w.shift, w.lk, a.left, a.right, a.sinks, lx, hx, sx);
         float mx, lsum, ox[4];
-        attend_row(a, static_cast<const T*>(a.q) + (w.q0 + tx) * a.q_row + (w.hk * w.group + gx) * a.q_head, k, v,
-                   lx, hx, sx, sink_from, sink_to, from, to, q_s, mx, lsum, ox);
+        attend_row(a, static_cast<const T*>(a.q) + (w.q0 + tx) * a.q_row + (w.hk * w.group + gx) * a.q_head,
+                   DenseRows<T>{k, a.k_row}, DenseRows<T>{v, a.v_row}, lx, hx, sx, sink_from, sink_to, from, to, q_s, mx, lsum, ox);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int d = lane + u * kWave;

@@ -1,0 +1,67 @@
+// Entry points of the attention over pages: argument checks.
+#include <cmath>
+
+#include "cache.hpp"
+
+namespace tsc {
+extern template int launch_cache<float>(const CacheArgs&, hipStream_t);
+extern template int launch_cache<__half>(const CacheArgs&, hipStream_t);
+extern template int launch_cache<__hip_bfloat16>(const CacheArgs&, hipStream_t);
+}  // namespace tsc
+
+using namespace tsc;
+
+extern "C" int64_t tsc_cache_attention_workspace_bytes(int32_t samples, int64_t n_q, int64_t longest,
+                                                       int64_t prefix_rows, int32_t q_heads, int32_t k_heads,
+                                                       int32_t dim, int32_t left, int32_t right, int32_t sinks,
+                                                       int32_t dtype) {
+  if (!dtype_ok(dtype) || samples < 0 || n_q < 0 || longest < 0 || prefix_rows < 0 || q_heads <= 0 ||
+      k_heads <= 0 || dim < 1 || dim > 256)
+    return -1;
+  return 0;
+}
+
+extern "C" int tsc_cache_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages,
+                                   int64_t k_page, int64_t k_page_row, int64_t k_page_head, const void* v_pages,
+                                   int64_t v_page, int64_t v_page_row, int64_t v_page_head, int64_t pages,
+                                   int64_t page_rows, const int32_t* table, int64_t table_row, int64_t table_pages,
+                                   const int32_t* offsets, const int32_t* lengths, int32_t samples,
+                                   const int32_t* prefix, int64_t prefix_pages, int64_t n_q, int32_t q_heads,
+                                   int32_t k_heads, int32_t dim, int32_t left, int32_t right, int32_t sinks,
+                                   float scale, int32_t dtype, void* ws, int64_t ws_bytes, void* out,
+                                   tsc_stream_t stream) {
+  const char* what = "cache_attention";
+  TSC_REQUIRE(dtype_ok(dtype), "%s: unknown dtype", what);
+  TSC_REQUIRE(n_q >= 0 && n_q < (1ll << 31), "%s: invalid sizes", what);
+  TSC_REQUIRE(q_heads > 0 && k_heads > 0 && q_heads % k_heads == 0 && q_heads <= 65535,
+              "%s: %d query heads do not share %d key heads evenly", what, q_heads, k_heads);
+  TSC_REQUIRE(n_q * (q_heads / k_heads) < (1ll << 32) - 1024,
+              "%s: over 2^32 rows of queries and the heads that share a key head", what);
+  TSC_REQUIRE(dim >= 1 && dim <= 256, "%s: head size %d, 1 to 256 are supported", what, dim);
+  TSC_REQUIRE(sinks >= 0, "%s: negative number of sinks", what);
+  TSC_REQUIRE(std::isfinite(scale), "%s: scale is not finite", what);
+  CacheArgs a{};
+  if (int rc = a.pages.set(what, table, table_row, table_pages, lengths, samples, pages, page_rows)) return rc;
+  TSC_REQUIRE(prefix_pages >= 0 && prefix_pages <= table_pages, "%s: a prefix of %lld pages, the table has %lld",
+              what, static_cast<long long>(prefix_pages), static_cast<long long>(table_pages));
+  if (n_q == 0 || samples == 0) return 0;
+  TSC_REQUIRE(q && out && offsets && (pages == 0 || (k_pages && v_pages)) && (prefix_pages == 0 || prefix),
+              "%s: null pointer", what);
+  if (pages == 0) a.pages.table_pages = 0, prefix_pages = 0;  // nothing is kept anywhere
+  a.q = q, a.q_row = q_row, a.q_head = q_head;
+  a.k = k_pages, a.k_at = {k_page, k_page_row, k_page_head};
+  a.v = v_pages, a.v_at = {v_page, v_page_row, v_page_head};
+  a.off_q = offsets, a.samples = samples, a.n_q = n_q;
+  a.q_heads = q_heads, a.k_heads = k_heads, a.dim = dim;
+  a.left = left < 0 ? kNoLimit : left, a.right = right < 0 ? kNoLimit : right, a.sinks = sinks;
+  a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504f;
+  a.q_sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
+  a.out = out, a.part = static_cast<float*>(ws);
+  a.prefix = prefix, a.prefix_pages = static_cast<int>(prefix_pages);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case TSC_F32: return launch_cache<float>(a, s);
+    case TSC_F16: return launch_cache<__half>(a, s);
+    default: return launch_cache<__hip_bfloat16>(a, s);
+  }
+}

@@ -1,0 +1,6 @@
+// The paged attention kernels on f16 tensors.
+#include "cache.hpp"
+
+namespace tsc {
+template int launch_cache<__half>(const CacheArgs&, hipStream_t);
+}  // namespace tsc

@@ -6,6 +6,10 @@
 // (pair a*F + i) turns by t = p[a] * base^(-i/F):
 //   (u, w) -> (u cos t - w sin t, u sin t + w cos t);
 // pairs from A*F on stay.  Pair j is (j, j + D/2), or (2j, 2j + 1) interleaved.
+//
+// The queries go to a tensor of their own, the keys too, or with the values
+// (copied as they are) to the pages that hold what a sample keeps.
+#include "pages.hpp"
 #include "sequence.hpp"
 
 #include <algorithm>
@@ -33,7 +37,39 @@ struct RotateArgs {
   int q_heads, k_heads, dim;
   void* q_out;
   void* k_out;
+  // the paged form: values and where keys and values go
+  const void* v;
+  int64_t v_row, v_head;
+  void* k_pages;
+  PageStrides k_at;
+  void* v_pages;
+  PageStrides v_at;
+  PageTable pages;
+  const int32_t* offsets;
 };
+
+// The page and its row that input row r goes to: r is one of the last rows of
+// the sample whose offsets enclose it.  A page of -1: nowhere (a row of no
+// sample, a position or a page that there is not).
+struct Place {
+  int32_t page, row;
+};
+__device__ __forceinline__ Place place_of(const RotateArgs& a, int64_t r) {
+  int lo = 0, hi = a.pages.samples + 1;  // offsets up to r: [0, lo) are, [hi, ...) are not
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (a.offsets[mid] <= r) lo = mid + 1;
+    else hi = mid;
+  }
+  const int b = lo - 1;
+  if (b < 0 || b >= a.pages.samples) return Place{-1, 0};
+  const int64_t pos = a.pages.lengths[b] - (a.offsets[b + 1] - r);
+  if (pos < 0 || pos >= a.pages.most()) return Place{-1, 0};
+  const uint32_t at = a.pages.page_of(static_cast<uint32_t>(pos));
+  const int32_t page = a.pages.table[b * a.pages.table_row + at];
+  if (page < 0 || page >= a.pages.pages) return Place{-1, 0};
+  return Place{page, static_cast<int32_t>(pos - (int64_t)at * a.pages.page_rows)};
+}
 
 // Cosine and sine of position p times a pair's speed, base^(-i/F) / 2 pi turns.
 // The angle is taken in 64 bits: positions reach thousands, and an f32 angle
@@ -66,7 +102,7 @@ __device__ __forceinline__ void load_gain(const void* p, int dtype, int64_t at, 
 
 // One row by one wave: lane l of a head (its pairs l and l + lp), group `sub` of
 // `heads` heads at a time.
-template <typename T>
+template <typename T, bool PAGED>
 __device__ __forceinline__ void rotate_any_row(const RotateArgs& a, int64_t r, int lp, int half, int F, int sub,
                                                int l, int heads) {
   float2 cs[2];
@@ -81,15 +117,18 @@ __device__ __forceinline__ void rotate_any_row(const RotateArgs& a, int64_t r, i
       cs[u] = turn_of(p, speed_of(j % F, F, a.log2_base));
     }
   }
+  Place to{0, 0};
+  if constexpr (PAGED) to = place_of(a, r);
   const int total = a.q_heads + a.k_heads;
   for (int h0 = 0; h0 < total; h0 += heads) {
     const int h = h0 + sub;
-    const bool in = h < total, is_q = h < a.q_heads;
+    const bool is_q = h < a.q_heads, in = h < total && (is_q || to.page >= 0);
     const int hh = is_q ? h : h - a.q_heads;
     const T* src = static_cast<const T*>(is_q ? a.q : a.k) +
                    (is_q ? r * a.q_row + hh * a.q_head : r * a.k_row + hh * a.k_head);
-    T* dst = static_cast<T*>(is_q ? a.q_out : a.k_out) +
-             (r * (is_q ? a.q_heads : a.k_heads) + hh) * a.dim;
+    T* dst;
+    if (PAGED && !is_q) dst = static_cast<T*>(a.k_pages) + a.k_at.at(to.page, to.row, hh);
+    else dst = static_cast<T*>(is_q ? a.q_out : a.k_out) + (r * (is_q ? a.q_heads : a.k_heads) + hh) * a.dim;
     const void* gain = is_q ? a.q_gain : a.k_gain;
     const int64_t gain_at = (int64_t)hh * (is_q ? a.q_gain_head : a.k_gain_head);
     float x[2][2] = {}, sum = 0.f;
@@ -118,17 +157,25 @@ __device__ __forceinline__ void rotate_any_row(const RotateArgs& a, int64_t r, i
       dst[ib] = from_f32<T>(p * cs[u].y + q * cs[u].x);
     }
   }
+  if constexpr (PAGED) {
+    if (to.page < 0) return;
+    for (int h = sub; h < a.k_heads; h += heads) {
+      const T* src = static_cast<const T*>(a.v) + r * a.v_row + h * a.v_head;
+      T* dst = static_cast<T*>(a.v_pages) + a.v_at.at(to.page, to.row, h);
+      for (int d = l; d < a.dim; d += lp) dst[d] = src[d];
+    }
+  }
 }
 
 // A wave per row and turn; a head takes LP lanes (a power of two from D/2 up, at most
 // 64), a lane its pairs l, l + 64.  Any size, stride and alignment.
-template <typename T>
+template <typename T, bool PAGED>
 __global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
   const int lane = threadIdx.x % kWave;
   const int half = a.dim / 2, F = half / a.axes;
   const int sub = lane / lp, l = lane % lp, heads = kWave / lp;
   for (int64_t r = blockIdx.x * (int64_t)4 + threadIdx.x / kWave; r < a.n; r += (int64_t)gridDim.x * 4)
-    rotate_any_row<T>(a, r, lp, half, F, sub, l, heads);
+    rotate_any_row<T, PAGED>(a, r, lp, half, F, sub, l, heads);
 }
 
 // The vector form: a workgroup takes kRows rows; its threads first share out the
@@ -142,9 +189,10 @@ __global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
 // this card: 4.86).
 constexpr int kRows = 8, kMaxHalf = 128;
 
-template <typename T, int P, int LANES>
+template <typename T, int P, int LANES, bool PAGED>
 __global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
   constexpr int HEADS = 256 / LANES, BYTES = P * sizeof(T);
+  __shared__ Place place[PAGED ? kRows : 1];
   __shared__ __align__(16) float2 turn[kRows][kMaxHalf];
   __shared__ double speed[kMaxHalf];
   const int half = a.dim / 2, F = half / a.axes;
@@ -152,13 +200,15 @@ __global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
     speed[threadIdx.x] = F > 0 && (int)threadIdx.x < a.axes * F
                              ? speed_of(threadIdx.x % F, F, a.log2_base) : 0.0;
   __syncthreads();
-  const int total = a.q_heads + a.k_heads, l = threadIdx.x % LANES;
+  const int turning = a.q_heads + a.k_heads, total = turning + (PAGED ? a.k_heads : 0), l = threadIdx.x % LANES;
   const bool in = LANES == 1 || l * P < half;
   const float over = 1.f / a.dim;
   // the lane's elements of a head: [first, first + P) and [second, second + P)
   const int first = in ? (a.interleaved ? 2 * P * l : P * l) : 0, second = first + (a.interleaved ? P : half);
   for (int64_t r0 = blockIdx.x * (int64_t)kRows; r0 < a.n; r0 += (int64_t)gridDim.x * kRows) {
     const int rows = static_cast<int>(min((int64_t)kRows, a.n - r0));
+    if constexpr (PAGED)
+      if ((int)threadIdx.x >= 256 - rows) place[255 - threadIdx.x] = place_of(a, r0 + 255 - threadIdx.x);
     for (int x = threadIdx.x; x < rows * half; x += 256) {
       const int r = x / half, j = x - r * half;
       float2 cs = make_float2(1.f, 0.f);
@@ -176,11 +226,25 @@ __global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
       const bool is_q = h < a.q_heads;
       const int hh = is_q ? h : h - a.q_heads;
       const int64_t row = r0 + r;
+      if (PAGED && !is_q && place[r].page < 0) continue;
+      T e[2 * P];
+      if (PAGED && h >= turning) {
+        const int hv = h - turning;
+        const T* src = static_cast<const T*>(a.v) + row * a.v_row + hv * a.v_head;
+        T* dst = static_cast<T*>(a.v_pages) + a.v_at.at(place[r].page, place[r].row, hv);
+        if (in) {
+          __builtin_memcpy(e, src + first, BYTES);
+          __builtin_memcpy(e + P, src + second, BYTES);
+          __builtin_memcpy(dst + first, e, BYTES);
+          __builtin_memcpy(dst + second, e + P, BYTES);
+        }
+        continue;
+      }
       const T* src = static_cast<const T*>(is_q ? a.q : a.k) +
                      (is_q ? row * a.q_row + hh * a.q_head : row * a.k_row + hh * a.k_head);
-      T* dst = static_cast<T*>(is_q ? a.q_out : a.k_out) +
-               (row * (is_q ? a.q_heads : a.k_heads) + hh) * a.dim;
-      T e[2 * P];
+      T* dst;
+      if (PAGED && !is_q) dst = static_cast<T*>(a.k_pages) + a.k_at.at(place[r].page, place[r].row, hh);
+      else dst = static_cast<T*>(is_q ? a.q_out : a.k_out) + (row * (is_q ? a.q_heads : a.k_heads) + hh) * a.dim;
       float x[2 * P] = {}, sum = 0.f;
       if (in) {
         __builtin_memcpy(e, src + first, BYTES);
@@ -230,39 +294,61 @@ __global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
   }
 }
 
-template <typename T, int P, int LANES>
-int launch_vector(const RotateArgs& a, hipStream_t s) {
+template <typename T, bool PAGED, int P, int LANES>
+int launch_vector(const RotateArgs& a, const char* what, hipStream_t s) {
   const int64_t blocks = std::min<int64_t>(ceil_div(a.n, kRows), 16384);
-  rotate_vector_kernel<T, P, LANES><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-  TSC_LAUNCH_CHECK("norm_rotate_heads");
+  rotate_vector_kernel<T, P, LANES, PAGED><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+  TSC_LAUNCH_CHECK(what);
   return 0;
 }
 
-template <typename T, int P>
-int launch_lanes(const RotateArgs& a, hipStream_t s) {
+template <typename T, bool PAGED, int P>
+int launch_lanes(const RotateArgs& a, const char* what, hipStream_t s) {
   const int lanes = a.dim / 2 / P;
-  if (lanes <= 1) return launch_vector<T, P, 1>(a, s);
-  if (lanes <= 2) return launch_vector<T, P, 2>(a, s);
-  if (lanes <= 4) return launch_vector<T, P, 4>(a, s);
-  if (lanes <= 8) return launch_vector<T, P, 8>(a, s);
-  if (lanes <= 16) return launch_vector<T, P, 16>(a, s);
-  return launch_vector<T, P, 32>(a, s);
+  if (lanes <= 1) return launch_vector<T, PAGED, P, 1>(a, what, s);
+  if (lanes <= 2) return launch_vector<T, PAGED, P, 2>(a, what, s);
+  if (lanes <= 4) return launch_vector<T, PAGED, P, 4>(a, what, s);
+  if (lanes <= 8) return launch_vector<T, PAGED, P, 8>(a, what, s);
+  if (lanes <= 16) return launch_vector<T, PAGED, P, 16>(a, what, s);
+  return launch_vector<T, PAGED, P, 32>(a, what, s);
 }
 
-template <typename T>
-int launch_rotate(const RotateArgs& a, hipStream_t s) {
+template <typename T, bool PAGED>
+int launch_rotate(const RotateArgs& a, const char* what, hipStream_t s) {
   // half a head in whole pieces of 16 bytes, or 8 for 16-bit values; head
   // sizes that are neither (2, 6, 250) go value by value
   const int half = a.dim / 2;
-  if (half % kPer16<T> == 0) return launch_lanes<T, kPer16<T>>(a, s);
+  if (half % kPer16<T> == 0) return launch_lanes<T, PAGED, kPer16<T>>(a, what, s);
   if constexpr (kIs16<T>)
-    if (half % 4 == 0) return launch_lanes<T, 4>(a, s);
+    if (half % 4 == 0) return launch_lanes<T, PAGED, 4>(a, what, s);
   int lp = 1;
   while (lp < kWave && lp < a.dim / 2) lp *= 2;
   // (a launch holds fewer than 2^32 threads, 2^26 waves)
   const int64_t blocks = std::min<int64_t>(ceil_div(a.n, 4), 1 << 20);
-  rotate_any_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, lp);
-  TSC_LAUNCH_CHECK("norm_rotate_heads");
+  rotate_any_kernel<T, PAGED><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, lp);
+  TSC_LAUNCH_CHECK(what);
+  return 0;
+}
+
+template <bool PAGED>
+int launch(const RotateArgs& a, int dtype, const char* what, hipStream_t s) {
+  switch (dtype) {
+    case TSC_F32: return launch_rotate<float, PAGED>(a, what, s);
+    case TSC_F16: return launch_rotate<__half, PAGED>(a, what, s);
+    default: return launch_rotate<__hip_bfloat16, PAGED>(a, what, s);
+  }
+}
+
+// What both forms ask of their arguments; 0 or an error code.
+int check(const char* what, int dtype, int gain_dtype, int64_t n, int q_heads, int k_heads, int dim, int axes,
+          double base, float eps) {
+  TSC_REQUIRE(dtype_ok(dtype) && dtype_ok(gain_dtype), "%s: unknown dtype", what);
+  TSC_REQUIRE(n >= 0 && n < (1ll << 31) && q_heads >= 0 && k_heads >= 0 && q_heads <= 65536 &&
+                  k_heads <= 65536, "%s: invalid sizes", what);
+  TSC_REQUIRE(dim >= 2 && dim <= 256 && dim % 2 == 0,
+              "%s: head size %d is not an even number up to 256", what, dim);
+  TSC_REQUIRE(axes >= 1 && axes <= 4, "%s: %d position axes, 1 to 4 are supported", what, axes);
+  TSC_REQUIRE(base > 1.0 && eps >= 0.f, "%s: base must be over 1 and eps not negative", what);
   return 0;
 }
 
@@ -279,23 +365,37 @@ extern "C" int tsc_norm_rotate_heads(const void* q, int64_t q_row, int64_t q_hea
                                      double base, int32_t interleaved, int32_t dtype, int64_t n,
                                      int32_t q_heads, int32_t k_heads, int32_t dim, void* q_out,
                                      void* k_out, tsc_stream_t stream) {
-  TSC_REQUIRE(dtype_ok(dtype) && dtype_ok(gain_dtype), "norm_rotate_heads: unknown dtype");
-  TSC_REQUIRE(n >= 0 && n < (1ll << 31) && q_heads >= 0 && k_heads >= 0 && q_heads <= 65536 &&
-                  k_heads <= 65536, "norm_rotate_heads: invalid sizes");
-  TSC_REQUIRE(dim >= 2 && dim <= 256 && dim % 2 == 0,
-              "norm_rotate_heads: head size %d is not an even number up to 256", dim);
-  TSC_REQUIRE(axes >= 1 && axes <= 4, "norm_rotate_heads: %d position axes, 1 to 4 are supported", axes);
-  TSC_REQUIRE(base > 1.0 && eps >= 0.f, "norm_rotate_heads: base must be over 1 and eps not negative");
+  const char* what = "norm_rotate_heads";
+  if (int rc = check(what, dtype, gain_dtype, n, q_heads, k_heads, dim, axes, base, eps)) return rc;
   if (n == 0 || q_heads + k_heads == 0) return 0;
   TSC_REQUIRE(positions && (!q_heads || (q && q_out)) && (!k_heads || (k && k_out)),
               "norm_rotate_heads: null pointer");
   const RotateArgs a{q, q_row, q_head, k, k_row, k_head, positions, pos_row, pos_float, axes,
                      q_gain, k_gain, gain_dtype, q_gain_per_head ? dim : 0, k_gain_per_head ? dim : 0,
                      eps, log2(base), interleaved, n, q_heads, k_heads, dim, q_out, k_out};
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case TSC_F32: return launch_rotate<float>(a, s);
-    case TSC_F16: return launch_rotate<__half>(a, s);
-    default: return launch_rotate<__hip_bfloat16>(a, s);
-  }
+  return launch<false>(a, dtype, what, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int tsc_norm_rotate_append(
+    const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
+    int64_t v_row, int64_t v_head, const void* positions, int64_t pos_row, int32_t pos_float, int32_t axes,
+    const void* q_gain, const void* k_gain, int32_t gain_dtype, int32_t q_gain_per_head, int32_t k_gain_per_head,
+    float eps, double base, int32_t interleaved, int32_t dtype, int64_t n, int32_t q_heads, int32_t k_heads,
+    int32_t dim, void* k_pages, int64_t k_page, int64_t k_page_row, int64_t k_page_head, void* v_pages,
+    int64_t v_page, int64_t v_page_row, int64_t v_page_head, int64_t pages, int64_t page_rows,
+    const int32_t* table, int64_t table_row, int64_t table_pages, const int32_t* offsets, const int32_t* lengths,
+    int32_t samples, void* q_out, tsc_stream_t stream) {
+  const char* what = "norm_rotate_append";
+  if (int rc = check(what, dtype, gain_dtype, n, q_heads, k_heads, dim, axes, base, eps)) return rc;
+  PageTable t;
+  if (int rc = t.set(what, table, table_row, table_pages, lengths, samples, pages, page_rows)) return rc;
+  if (n == 0 || q_heads + k_heads == 0) return 0;
+  TSC_REQUIRE(positions && offsets && (!q_heads || (q && q_out)), "%s: null pointer", what);
+  TSC_REQUIRE(!k_heads || (k && v && (pages == 0 || (k_pages && v_pages))), "%s: null pointer", what);
+  const RotateArgs a{q, q_row, q_head, k, k_row, k_head, positions, pos_row, pos_float, axes,
+                     q_gain, k_gain, gain_dtype, q_gain_per_head ? dim : 0, k_gain_per_head ? dim : 0,
+                     eps, log2(base), interleaved, n, q_heads, k_heads, dim, q_out, nullptr, v, v_row, v_head,
+                     k_pages, {k_page, k_page_row, k_page_head}, v_pages, {v_page, v_page_row, v_page_head},
+                     t, offsets};
+  return launch<true>(a, dtype, what, static_cast<hipStream_t>(stream));
 }

@@ -3,6 +3,7 @@
 Export list of trispconv/pytorch/__init__.py:13-21, then the operators and
 modules of transformer blocks over the voxels.
 """
+from .cache import VoxelCache, cache_attention, norm_rotate_append
 from .compat import ConvAlgo
 from .modules import (SparseConv3d, SparseConvolution, SparseInverseConv3d, SparseModule,
                       SparseSequential, SubMConv3d)
@@ -25,4 +26,7 @@ __all__ = [
     "VoxelOrder",
     "SerialOrder",
     "VoxelBlock",
+    "norm_rotate_append",
+    "cache_attention",
+    "VoxelCache",
 ]

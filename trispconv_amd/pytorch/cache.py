@@ -1,0 +1,320 @@
+"""Streams of voxels: keys and values kept in pages from step to step.
+
+A stream brings a sample's voxels in steps (sweeps of a scan, what a generator
+has drawn so far); the blocks' attention sees the new rows and everything the
+sample keeps.  Two operators work on pages of rows (no counterpart in the
+reference; inference, as everything here):
+
+``norm_rotate_append``  norm_rotate_heads, with the keys and the values written
+                        to the pages of their samples
+``cache_attention``     window_attention over those pages; pages that all
+                        samples begin with are read once for all
+
+``VoxelCache`` holds the pages of a network's blocks, hands them out and shares
+them; a VoxelBlock called with one streams.
+"""
+from __future__ import annotations
+
+from typing import Callable, List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from .. import _lib as L
+from .sequence import _head_gains, _limit, _MOST, _position_rows, _rows_of, _same
+
+__all__ = ["norm_rotate_append", "cache_attention", "VoxelCache"]
+
+
+def _launch(device: int, call: Callable, *args) -> int:
+    """``call`` with ``device`` as the current one, as launches on its streams need."""
+    if torch.cuda.current_device() == device:
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
+
+
+def _check_pages(what: str, like: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 table: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor) -> None:
+    """Pages and tables beside ``like``, whose device they have to be on."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != like.shape[2]:
+        raise ValueError(f"{what}: pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} are not "
+                         f"(pages, rows, heads, {like.shape[2]})")
+    _same(k_pages, like, what, "k_pages")
+    _same(v_pages, like, what, "v_pages")
+    if k_pages.shape[3] > 1 and (k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
+        raise ValueError(f"{what}: the values of a head must lie one behind the other in the pages")
+    if table.dim() != 2 or lengths.shape != table.shape[:1] or \
+            offsets.shape != (table.shape[0] + 1,):
+        raise ValueError(f"{what}: table {tuple(table.shape)}, offsets {tuple(offsets.shape)} and "
+                         f"lengths {tuple(lengths.shape)} are not (B, pages), (B + 1,) and (B,)")
+    device = like.get_device()
+    for t in (table, offsets, lengths):
+        if t.dtype is not torch.int32 or t.get_device() != device:
+            raise ValueError(f"{what}: table, offsets and lengths must be int32 on {like.device}, "
+                             f"got {t.dtype} on {t.device}")
+
+
+def norm_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                       k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                       offsets: torch.Tensor, lengths: torch.Tensor,
+                       q_weight: Optional[torch.Tensor] = None,
+                       k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       base: float = 10000.0, interleaved: bool = False) -> torch.Tensor:
+    """norm_rotate_heads whose keys, and the values beside them, go to pages.
+
+    q (N, Hq, D), k and v (N, Hk, D) and the arguments of the norm and the
+    rotation as in ``norm_rotate_heads``; returns the queries as it does.
+    k_pages and v_pages (P, R, Hk, D), R rows a page, any strides with D
+    contiguous, are written in place: sample b's new rows are rows offsets[b]
+    to offsets[b+1], the last of its lengths[b] positions, and position t is row
+    t % R of page table[b, t // R].  offsets (B + 1,), lengths (B,) and table
+    (B, pages) are int32 on the GPU.  Nothing else in the pages is written; a row
+    of no sample, or one whose position or page there is not, is written nowhere.
+    No row of a page may be that of two new rows, and no input may lie in the pages.
+    """
+    what = "norm_rotate_append"
+    if not q.is_cuda:
+        L.require_gpu(q, what)
+    code = L.dtype_code(q.dtype)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or \
+            q.shape[2] != k.shape[2]:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} are "
+                         "not (N, Hq, D), (N, Hk, D), (N, Hk, D)")
+    _same(k, q, what, "k")
+    _same(v, q, what, "v")
+    _check_pages(what, q, k_pages, v_pages, table, offsets, lengths)
+    n, hq, dim = q.shape
+    hk = k.shape[1]
+    if k_pages.shape[2] != hk:
+        raise ValueError(f"{what}: {hk} key heads, the pages have {k_pages.shape[2]}")
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if 0 in t.stride()[:3] and any(s == 0 and e > 1 for s, e in zip(t.stride(), t.shape)):
+            raise ValueError(f"{what}: {name} is expanded: its rows share memory")
+    positions, p_row, in_f32 = _position_rows(positions, q, what)
+    q_weight, k_weight, gains = _head_gains(q_weight, k_weight, q, hk, what)
+    (q, (q_row, q_head, _)), (k, (k_row, k_head, _)) = _rows_of(q), _rows_of(k)
+    (v, (v_row, v_head, _)), (table, (t_row, _)) = _rows_of(v), _rows_of(table)
+    offsets, lengths = offsets.contiguous(), lengths.contiguous()
+    q_out = q.new_empty((n, hq, dim))
+    pages, rows = k_pages.shape[:2]
+    rc = _launch(
+        q.get_device(), L.lib().tsc_norm_rotate_append, q.data_ptr(), q_row, q_head, k.data_ptr(),
+        k_row, k_head, v.data_ptr(), v_row, v_head, positions.data_ptr(), p_row, in_f32,
+        positions.shape[1], *gains, eps, base, interleaved, code, n, hq, hk, dim,
+        k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3], pages,
+        rows, table.data_ptr(), t_row, table.shape[1], offsets.data_ptr(), lengths.data_ptr(),
+        table.shape[0], q_out.data_ptr(), L.stream_of(q))
+    if rc:
+        L.check(rc, what)
+    return q_out
+
+
+def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    table: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor,
+                    prefix: Optional[torch.Tensor] = None,
+                    window: Tuple[Optional[int], Optional[int]] = (None, None), sinks: int = 0,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """window_attention of new rows over what their samples keep in pages.
+
+    q (Nq, Hq, D), the pages, table, offsets and lengths as in
+    ``norm_rotate_append``, Hq a multiple of the pages' heads, D at most 256:
+    query i of a sample's Lq stands at p = i + lengths[b] - Lq and sees of its
+    positions what ``window_attention`` with the same window, sinks and scale
+    would let it see.  Which pages a table names beyond a sample's length, and
+    what they hold, means nothing.  prefix (int32 on the GPU, page numbers):
+    every sample's first positions lie in these pages; they are then read once
+    for the queries of all samples, and the table's entries for them not at all.
+    A query that sees no key gives zeros, as rows outside every sample do.
+    Scores, maxima and sums are float32.
+    """
+    what = "cache_attention"
+    if not q.is_cuda:
+        L.require_gpu(q, what)
+    code = L.dtype_code(q.dtype)
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q {tuple(q.shape)} is not (Nq, Hq, D)")
+    _check_pages(what, q, k_pages, v_pages, table, offsets, lengths)
+    n_q, hq, dim = q.shape
+    pages, rows, hk, _ = k_pages.shape
+    samples, entries = table.shape
+    p_ptr, p_pages = None, 0
+    if prefix is not None:
+        if prefix.dim() != 1 or prefix.dtype is not torch.int32 or \
+                prefix.get_device() != q.get_device() or prefix.shape[0] > entries:
+            raise ValueError(f"{what}: prefix must be up to {entries} page numbers, int32 on "
+                             f"{q.device}, got {tuple(prefix.shape)} {prefix.dtype} on "
+                             f"{prefix.device}")
+        prefix = prefix.contiguous()
+        p_ptr, p_pages = prefix.data_ptr(), prefix.shape[0]
+    left, right = window
+    left, right = _limit(left, what), _limit(right, what)
+    if sinks < 0:
+        raise ValueError(f"{what}: sinks must not be negative, got {sinks}")
+    (q, (q_row, q_head, _)), (table, (t_row, _)) = _rows_of(q), _rows_of(table)
+    offsets, lengths = offsets.contiguous(), lengths.contiguous()
+    if samples == 0:
+        return q.new_zeros((n_q, hq, dim))
+    out = q.new_empty((n_q, hq, dim))
+    lib, sinks = L.lib(), min(sinks, _MOST)
+    nbytes = lib.tsc_cache_attention_workspace_bytes(samples, n_q, entries * rows, p_pages * rows,
+                                                     hq, hk, dim, left, right, sinks, code)
+    ws = None
+    if nbytes > 0:
+        ws = offsets.new_empty(-(-nbytes // 4))
+    rc = _launch(
+        q.get_device(), lib.tsc_cache_attention, q.data_ptr(), q_row, q_head, k_pages.data_ptr(),
+        *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3], pages, rows,
+        table.data_ptr(), t_row, entries, offsets.data_ptr(), lengths.data_ptr(), samples, p_ptr,
+        p_pages, n_q, hq, hk, dim, left, right, sinks, max(dim, 1) ** -0.5 if scale is None else scale,
+        code, None if ws is None else ws.data_ptr(), nbytes, out.data_ptr(), L.stream_of(q))
+    if rc:
+        L.check(rc, what)
+    return out
+
+
+class VoxelCache:
+    """What the samples of a stream keep: pages of ``page_rows`` rows for the keys
+    and the values of every layer, and which of them each sample has.
+
+    ``positions`` is the most rows that one sample may keep, ``pages`` how many
+    there are for all samples (default: enough for all to keep that many).  Every
+    layer has pages of its own under the same numbers: ``k[layer]`` and
+    ``v[layer]`` (pages, page_rows, kv_heads, dim).  ``lengths`` (samples,) and
+    ``table`` (samples, pages of a sample) are int32 on the device and keep their
+    memory, so that a captured step finds there what later steps have changed.
+
+    A step takes room for its new rows (``extend``), then runs the blocks with
+    the cache: ``block(x, cache, layer)``.
+    """
+
+    def __init__(self, samples: int, positions: int, kv_heads: int, dim: int, layers: int = 1,
+                 pages: Optional[int] = None, page_rows: int = 64,
+                 dtype: torch.dtype = torch.float32,
+                 device: Union[str, torch.device] = "cuda"):
+        if min(samples, kv_heads, dim, layers) < 1 or positions < 0 or \
+                not 1 <= page_rows <= 1 << 20:
+            raise ValueError("VoxelCache: samples, kv_heads, dim and layers must be 1 or more, "
+                             "page_rows 1 to 2^20")
+        L.dtype_code(dtype)
+        self.samples, self.positions, self.page_rows = samples, positions, page_rows
+        entries = max(1, -(-positions // page_rows))
+        pages = samples * entries if pages is None else pages
+        if pages < 0:
+            raise ValueError(f"VoxelCache: {pages} pages")
+        # the rows of a head lie together in a page
+        shape = (layers, pages, kv_heads, page_rows, dim)
+        self.k, self.v = (list(torch.empty(shape, dtype=dtype, device=device).transpose(2, 3))
+                          for _ in range(2))
+        self.table = torch.zeros(samples, entries, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(samples, dtype=torch.int32, device=device)
+        self._entries = torch.zeros(samples, entries, dtype=torch.int32)
+        self._kept = [0] * samples
+        self._pages: List[List[int]] = [[] for _ in range(samples)]
+        self._users = [0] * pages
+        self._free = list(range(pages - 1, -1, -1))
+        self._common = 0
+
+    def _publish(self, pages_changed: bool) -> None:
+        """The host's state to the device."""
+        if pages_changed:
+            self.table.copy_(self._entries)
+            held = [p for p in self._pages if p]
+            n = 0
+            if len(held) > 1:
+                for column in zip(*held):
+                    if len(set(column)) > 1:
+                        break
+                    n += 1
+            self._common = n
+        kept = torch.tensor(self._kept, dtype=torch.int32)
+        if self.lengths.is_cuda:
+            self.lengths.copy_(kept.pin_memory(), non_blocking=True)
+        else:
+            self.lengths.copy_(kept)
+
+    def rows(self) -> List[int]:
+        """The rows that each sample keeps."""
+        return list(self._kept)
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def extend(self, rows: Union[Sequence[int], torch.Tensor]) -> None:
+        """Room for ``rows[b]`` new rows behind what sample b keeps, for instance
+        ``order.offsets.diff()``.  A ValueError leaves everything as it was."""
+        rows = rows.tolist() if isinstance(rows, torch.Tensor) else [int(n) for n in rows]
+        if len(rows) != self.samples or any(n < 0 for n in rows):
+            raise ValueError(f"VoxelCache: {rows} new rows for {self.samples} samples")
+        kept = [a + b for a, b in zip(self._kept, rows)]
+        if max(kept) > self.positions:
+            raise ValueError(f"VoxelCache: {max(kept)} rows of a sample, it has room for "
+                             f"{self.positions}")
+        need = [-(-n // self.page_rows) - len(p) for n, p in zip(kept, self._pages)]
+        if sum(need) > len(self._free):
+            raise ValueError(f"VoxelCache: {sum(need)} pages are needed, {len(self._free)} are free")
+        for b, n in enumerate(need):
+            for _ in range(n):
+                page = self._free.pop()
+                self._users[page] = 1
+                self._entries[b, len(self._pages[b])] = page
+                self._pages[b].append(page)
+        self._kept = kept
+        self._publish(sum(need) > 0)
+
+    def share(self, source: int, targets: Sequence[int], rows: int) -> None:
+        """Lets samples that keep nothing begin with the first ``rows`` rows of
+        ``source``, in the same pages: whole pages, so a multiple of page_rows."""
+        if rows % self.page_rows or not 0 <= rows <= self._kept[source]:
+            raise ValueError(f"VoxelCache: {rows} rows of sample {source}, which keeps "
+                             f"{self._kept[source]}, are not whole pages of {self.page_rows}")
+        targets = list(targets)
+        if len(set(targets)) < len(targets) or any(self._kept[b] for b in targets):
+            raise ValueError(f"VoxelCache: samples {targets} must be different and keep nothing")
+        pages = self._pages[source][:rows // self.page_rows]
+        for b in targets:
+            for i, page in enumerate(pages):
+                self._users[page] += 1
+                self._entries[b, i] = page
+            self._pages[b] = list(pages)
+            self._kept[b] = rows
+        self._publish(True)
+
+    def drop(self, samples: Sequence[int]) -> None:
+        """Forgets what these samples keep; pages that no other sample has are free again."""
+        for b in samples:
+            for page in reversed(self._pages[b]):
+                self._users[page] -= 1
+                if not self._users[page]:
+                    self._free.append(page)
+            self._pages[b], self._kept[b] = [], 0
+        self._publish(True)
+
+    def _tables(self) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """The table as far as it is used, and the pages that all samples begin
+        with; a captured step takes the whole table, which later steps fill."""
+        if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            return self.table, None
+        used = max(len(p) for p in self._pages)
+        table = self.table[:, :used]
+        if not self._common:
+            return table, None
+        first = next(b for b, p in enumerate(self._pages) if p)
+        return table, self.table[first, :self._common]
+
+    def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               positions: torch.Tensor, offsets: torch.Tensor,
+               q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+               eps: float = 1e-6, base: float = 10000.0, interleaved: bool = False) -> torch.Tensor:
+        """``norm_rotate_append`` to a layer's pages: the rows that the last ``extend`` made
+        room for, sample after sample."""
+        return norm_rotate_append(q, k, v, positions, self.k[layer], self.v[layer],
+                                  self._tables()[0], offsets, self.lengths, q_weight, k_weight,
+                                  eps, base, interleaved)
+
+    def attend(self, layer: int, q: torch.Tensor, offsets: torch.Tensor,
+               window: Tuple[Optional[int], Optional[int]] = (None, None), sinks: int = 0,
+               scale: Optional[float] = None) -> torch.Tensor:
+        """``cache_attention`` over a layer's pages."""
+        table, prefix = self._tables()
+        return cache_attention(q, self.k[layer], self.v[layer], table, offsets, self.lengths,
+                               prefix, window, sinks, scale)

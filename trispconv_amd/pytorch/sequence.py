@@ -16,7 +16,7 @@ is the block: both are SparseModules for a SparseSequential.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Tuple
+from typing import TYPE_CHECKING, NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -26,6 +26,9 @@ from .. import _lib as L
 from .functional import compute_dtype
 from .modules import SparseModule, _plain
 from .tensor import SparseConvTensor
+
+if TYPE_CHECKING:
+    from .cache import VoxelCache
 
 __all__ = ["linear_act", "norm_rotate_heads", "window_attention", "VoxelOrder", "SerialOrder",
            "VoxelBlock"]
@@ -109,6 +112,44 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     return out
 
 
+def _position_rows(positions: torch.Tensor, q: torch.Tensor,
+                   what: str) -> Tuple[torch.Tensor, int, bool]:
+    """Checked positions, their row stride and whether they are float32."""
+    in_f32 = positions.dtype is torch.float32
+    if positions.dim() != 2 or positions.shape[0] != q.shape[0] or \
+            positions.get_device() != q.get_device() or \
+            not (in_f32 or positions.dtype is torch.int32):
+        raise ValueError(f"{what}: positions must be ({q.shape[0]}, axes) int32 or float32 on "
+                         f"{q.device}")
+    positions, (row, _) = _rows_of(positions)
+    return positions, row, in_f32
+
+
+def _head_gains(q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                q: torch.Tensor, hk: int, what: str):
+    """Checked gains, and their arguments of a C entry: two pointers, the
+    dtype's code and whether each has a gain per head."""
+    qg_ptr = kg_ptr = None
+    qg_heads = kg_heads = g_code = 0
+    if q_weight is not None or k_weight is not None:
+        hq, dim = q.shape[1:]
+        device = q.get_device()
+        g_dtype = (k_weight if q_weight is None else q_weight).dtype
+        g_code = L.dtype_code(g_dtype)
+        for w, h, name in ((q_weight, hq, "q_weight"), (k_weight, hk, "k_weight")):
+            if w is not None and (w.shape not in ((dim,), (h, dim)) or w.get_device() != device
+                                  or w.dtype is not g_dtype):
+                raise ValueError(f"{what}: {name} must be ({dim},) or ({h}, {dim}) {g_dtype} on "
+                                 f"{q.device}")
+        if q_weight is not None:
+            q_weight = q_weight.contiguous()
+            qg_ptr, qg_heads = q_weight.data_ptr(), q_weight.dim() - 1
+        if k_weight is not None:
+            k_weight = k_weight.contiguous()
+            kg_ptr, kg_heads = k_weight.data_ptr(), k_weight.dim() - 1
+    return q_weight, k_weight, (qg_ptr, kg_ptr, g_code, qg_heads, kg_heads)
+
+
 def norm_rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
                       q_weight: Optional[torch.Tensor] = None,
                       k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -134,34 +175,15 @@ def norm_rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
                          "and (N, Hk, D)")
     _same(k, q, what, "k")
     n, hq, dim = q.shape
-    hk, device = k.shape[1], q.get_device()
-    in_f32 = positions.dtype is torch.float32
-    if positions.dim() != 2 or positions.shape[0] != n or positions.get_device() != device or \
-            not (in_f32 or positions.dtype is torch.int32):
-        raise ValueError(f"{what}: positions must be ({n}, axes) int32 or float32 on {q.device}")
-    qg_ptr = kg_ptr = None
-    qg_heads = kg_heads = g_code = 0
-    if q_weight is not None or k_weight is not None:
-        g_dtype = (k_weight if q_weight is None else q_weight).dtype
-        g_code = L.dtype_code(g_dtype)
-        for w, h, name in ((q_weight, hq, "q_weight"), (k_weight, hk, "k_weight")):
-            if w is not None and (w.shape not in ((dim,), (h, dim)) or w.get_device() != device
-                                  or w.dtype is not g_dtype):
-                raise ValueError(f"{what}: {name} must be ({dim},) or ({h}, {dim}) {g_dtype} on "
-                                 f"{q.device}")
-        if q_weight is not None:
-            q_weight = q_weight.contiguous()
-            qg_ptr, qg_heads = q_weight.data_ptr(), q_weight.dim() - 1
-        if k_weight is not None:
-            k_weight = k_weight.contiguous()
-            kg_ptr, kg_heads = k_weight.data_ptr(), k_weight.dim() - 1
+    hk = k.shape[1]
+    positions, p_row, in_f32 = _position_rows(positions, q, what)
+    q_weight, k_weight, gains = _head_gains(q_weight, k_weight, q, hk, what)
     (q, (q_row, q_head, _)), (k, (k_row, k_head, _)) = _rows_of(q), _rows_of(k)
-    positions, (p_row, _) = _rows_of(positions)
     q_out, k_out = q.new_empty((n, hq, dim)), q.new_empty((n, hk, dim))
     rc = L.lib().tsc_norm_rotate_heads(
         q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, positions.data_ptr(), p_row,
-        in_f32, positions.shape[1], qg_ptr, kg_ptr, g_code, qg_heads, kg_heads, eps, base,
-        interleaved, code, n, hq, hk, dim, q_out.data_ptr(), k_out.data_ptr(), L.stream_of(q))
+        in_f32, positions.shape[1], *gains, eps, base, interleaved, code, n, hq, hk, dim,
+        q_out.data_ptr(), k_out.data_ptr(), L.stream_of(q))
     if rc:
         L.check(rc, what)
     return q_out, k_out
@@ -313,7 +335,12 @@ class VoxelBlock(SparseModule):
 
     Queries and keys are normalised per head and rotated by the voxel's
     (z, y, x); the attention sees ``window`` rows on either side and the first
-    ``sinks`` of the sample.  kv_heads (default: heads) shares key heads."""
+    ``sinks`` of the sample.  kv_heads (default: heads) shares key heads.
+
+    With a VoxelCache, as ``block(x, cache, layer)``, the tensor's voxels are the
+    new ones of a stream: they go behind what their samples keep in that layer
+    of the cache (which ``cache.extend`` has made room for), and the attention
+    runs over all of it."""
 
     def __init__(self, channels: int, heads: int, order_key: str, kv_heads: Optional[int] = None,
                  window: Tuple[Optional[int], Optional[int]] = (None, None), sinks: int = 0,
@@ -346,7 +373,8 @@ class VoxelBlock(SparseModule):
                 return False
         return True
 
-    def forward(self, x: SparseConvTensor) -> SparseConvTensor:
+    def forward(self, x: SparseConvTensor, cache: Optional["VoxelCache"] = None,
+                layer: int = 0) -> SparseConvTensor:
         order = x.indice_dict.get(self.order_key)
         if not isinstance(order, VoxelOrder):
             raise KeyError(f"order_key '{self.order_key}' not found in indice_dict. "
@@ -355,20 +383,27 @@ class VoxelBlock(SparseModule):
             raise ValueError(f"VoxelBlock: the rows are not those that SerialOrder "
                              f"'{self.order_key}' ordered (a layer since then changed the "
                              "coordinates); run a SerialOrder on them first")
+        if cache is not None and cache.samples != x.batch_size:
+            raise ValueError(f"VoxelBlock: {x.batch_size} samples, the cache has {cache.samples}")
         f = x.features
         if not self._computes_in(f.dtype):
             # on f32 copies, as the convolutions do
             wide = {n: p.float() for n, p in self.named_parameters() if p.is_floating_point()}
-            y = torch.func.functional_call(self, wide, (x.replace_feature(f.float()),))
+            y = torch.func.functional_call(self, wide, (x.replace_feature(f.float()), cache, layer))
             return x.replace_feature(y.features.to(f.dtype))
         with torch.no_grad():
             hq, hk = self.heads, self.kv_heads
             qkv = _project(self.qkv, self.norm1(f))
             qkv = qkv.reshape(f.shape[0], hq + 2 * hk, self.dim)
-            q, k = norm_rotate_heads(qkv[:, :hq], qkv[:, hq:hq + hk], x.indices[:, 1:],
-                                     self.q_gain, self.k_gain, self.eps, self.base)
-            a = window_attention(q, k, qkv[:, hq + hk:], order.offsets, window=self.window,
-                                 sinks=self.sinks)
+            q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+            coords = x.indices[:, 1:]
+            if cache is None:
+                q, k = norm_rotate_heads(q, k, coords, self.q_gain, self.k_gain, self.eps, self.base)
+                a = window_attention(q, k, v, order.offsets, window=self.window, sinks=self.sinks)
+            else:
+                q = cache.append(layer, q, k, v, coords, order.offsets, self.q_gain, self.k_gain,
+                                 self.eps, self.base)
+                a = cache.attend(layer, q, order.offsets, self.window, self.sinks)
             f = _project(self.proj, a.view(f.shape), residual=f)
             h = _project(self.up, self.norm2(f), self.activation)
             f = _project(self.down, h, residual=f)
