@@ -1,12 +1,55 @@
-// Entry points of the attention over pages: argument checks.
+// Entry points of the attention over pages: argument checks and how a call is
+// cut into workgroups.
+#include <algorithm>
 #include <cmath>
 
 #include "cache.hpp"
 
 namespace tsc {
-extern template int launch_cache<float>(const CacheArgs&, hipStream_t);
-extern template int launch_cache<__half>(const CacheArgs&, hipStream_t);
-extern template int launch_cache<__hip_bfloat16>(const CacheArgs&, hipStream_t);
+extern template int launch_cache<float>(const CacheArgs&, const CachePlan&, hipStream_t);
+extern template int launch_cache<__half>(const CacheArgs&, const CachePlan&, hipStream_t);
+extern template int launch_cache<__hip_bfloat16>(const CacheArgs&, const CachePlan&, hipStream_t);
+
+namespace {
+
+constexpr int kCus = 256;
+
+// longest: positions a sample may have, prefix_rows of them shared.
+CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t prefix_rows, int q_heads, int k_heads,
+                     int dim, int elem, int left, int right, int sinks) {
+  CachePlan p;
+  const int64_t group = q_heads / k_heads, mean = n_q * group / samples;
+  const int row_bytes = padded_dim(dim) * elem, kt = cache_keys(row_bytes);
+  p.row_blocks = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
+  while (p.row_blocks > cache_row_blocks(row_bytes)) p.row_blocks /= 2;
+  const int64_t rows = 16 * p.row_blocks;
+  // keys that a tile of a sample's rows can see at most
+  int64_t span = std::max<int64_t>(longest - prefix_rows, 0);
+  if (left >= 0) span = std::min<int64_t>(span, (int64_t)left + n_q + sinks + kt);
+  auto cut = [&](int64_t keys, int64_t tiles) {
+    CacheCut c;
+    if (sinks > 0) keys += kt;  // (a tile of their own)
+    c.tiles = tiles;
+    // about four workgroups per CU, of 256 keys and more
+    const int64_t most = std::max<int64_t>(1, 4 * kCus / std::max<int64_t>(1, tiles * k_heads));
+    const int64_t least = std::max<int64_t>(256, ceil_div(keys, std::min<int64_t>(most, kMostSplits / 2)));
+    c.chunk = static_cast<int>(align_up(std::min<int64_t>(least, 1ll << 30), 4 * kt));
+    c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
+    return c;
+  };
+  p.own = cut(span, n_q * group / rows + std::min(samples, n_q));
+  if (prefix_rows) p.prefix = cut(prefix_rows, ceil_div(n_q * group, rows));
+  p.own.first_split = p.prefix.splits;
+  return p;
+}
+
+// Scratch of a call: the parts' references, sums and values.
+int64_t part_bytes(const CachePlan& p, int64_t rows, int dim) {
+  const int64_t s = p.splits();
+  return s > 1 ? (align_up(s * rows * 2, 4) + s * rows * dim) * 4 : 0;
+}
+
+}  // namespace
 }  // namespace tsc
 
 using namespace tsc;
@@ -18,7 +61,10 @@ extern "C" int64_t tsc_cache_attention_workspace_bytes(int32_t samples, int64_t 
   if (!dtype_ok(dtype) || samples < 0 || n_q < 0 || longest < 0 || prefix_rows < 0 || q_heads <= 0 ||
       k_heads <= 0 || dim < 1 || dim > 256)
     return -1;
-  return 0;
+  if (n_q == 0 || samples == 0) return 0;
+  return part_bytes(cache_plan(samples, n_q, longest, prefix_rows, q_heads, k_heads, dim, dtype_bytes(dtype), left,
+                               right, sinks),
+                    n_q * q_heads, dim);
 }
 
 extern "C" int tsc_cache_attention(const void* q, int64_t q_row, int64_t q_head, const void* k_pages,
@@ -47,6 +93,11 @@ extern "C" int tsc_cache_attention(const void* q, int64_t q_row, int64_t q_head,
   if (n_q == 0 || samples == 0) return 0;
   TSC_REQUIRE(q && out && offsets && (pages == 0 || (k_pages && v_pages)) && (prefix_pages == 0 || prefix),
               "%s: null pointer", what);
+  const CachePlan p = cache_plan(samples, n_q, a.pages.most(), prefix_pages * page_rows, q_heads, k_heads, dim,
+                                 dtype_bytes(dtype), left, right, sinks);
+  const int64_t need = part_bytes(p, n_q * q_heads, dim);
+  TSC_REQUIRE(need == 0 || (ws && ws_bytes >= need), "%s: a workspace of %lld bytes is needed", what,
+              static_cast<long long>(need));
   if (pages == 0) a.pages.table_pages = 0, prefix_pages = 0;  // nothing is kept anywhere
   a.q = q, a.q_row = q_row, a.q_head = q_head;
   a.k = k_pages, a.k_at = {k_page, k_page_row, k_page_head};
@@ -60,8 +111,8 @@ extern "C" int tsc_cache_attention(const void* q, int64_t q_row, int64_t q_head,
   a.prefix = prefix, a.prefix_pages = static_cast<int>(prefix_pages);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case TSC_F32: return launch_cache<float>(a, s);
-    case TSC_F16: return launch_cache<__half>(a, s);
-    default: return launch_cache<__hip_bfloat16>(a, s);
+    case TSC_F32: return launch_cache<float>(a, p, s);
+    case TSC_F16: return launch_cache<__half>(a, p, s);
+    default: return launch_cache<__hip_bfloat16>(a, p, s);
   }
 }

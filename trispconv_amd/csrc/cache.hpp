@@ -4,7 +4,11 @@
 // its Lq queries are the last of them.  What a query sees, and what comes out,
 // is as for packed keys (attend.hpp), with the keys and values fetched page by
 // page.  With a prefix of P pages every sample's first P R positions are those
-// pages, and their keys are read for all queries at once.
+// pages: their keys are read once, for the queries of all samples (one list of
+// rows), and the rest sample by sample.  A call is cut into parts, the prefix's
+// and each sample's own keys in chunks of their own; a part leaves its reference
+// score m, the sum l of the exponentials and the sums o of the values, and
+//   out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
 #pragma once
 
 #include "attend.hpp"
@@ -17,12 +21,58 @@ struct CacheArgs : AttendArgs {
   PageStrides k_at, v_at;
   const int32_t* prefix;  // its pages, or none
   int prefix_pages;
+  __host__ __device__ int prefix_rows() const { return prefix_pages * pages.page_rows; }
+};
+
+// How the prefix's or the samples' own keys are cut: tiles of query rows (at
+// most), and chunks of `chunk` keys, numbered from first_split on.
+struct CacheCut {
+  int64_t tiles = 0;
+  int splits = 0, first_split = 0;
+  int chunk = 0;
+};
+struct CachePlan {
+  int row_blocks = 1;  // rows of a tile in 16s
+  CacheCut prefix, own;
+  int splits() const { return prefix.splits + own.splits; }
 };
 
 template <typename T>
-int launch_cache(const CacheArgs& a, hipStream_t s);
+int launch_cache(const CacheArgs& a, const CachePlan& p, hipStream_t s);
+
+// Keys of a wave's tile, and waves of a workgroup: what the LDS has room for.
+constexpr int cache_keys(int row_bytes) { return row_bytes <= 512 ? 32 : 16; }
+constexpr int cache_waves(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
+// Rows of a tile in 16s at most: queries and sums stay in the registers.
+constexpr int cache_row_blocks(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
 
 namespace {
+
+constexpr int kTileBuffers = 2;
+
+// c += a b for a 16x16 tile: lane l holds row (a) or column (b) l % 16, and of the
+// sum's terms the 16 bytes' elements of its quarter l / 16, the same for a and b.
+// c: lane l holds column l % 16, rows 4 (l / 16) + 0..3.
+template <typename T>
+__device__ __forceinline__ f32x4 mma16(int4v a, int4v b, f32x4 c) {
+  if constexpr (std::is_same_v<T, __half>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                  0, 0);
+  } else if constexpr (std::is_same_v<T, __hip_bfloat16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                   0, 0, 0);
+  } else {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+    return c;
+  }
+}
+
+// 16 bytes per lane from an address of its own; otherwise as load_to_lds.
+__device__ __forceinline__ void load_to_lds_from(const void* p, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(m0) : "memory");
+}
 
 // The keys or values of one head in the pages of one row of the table.  Page
 // numbers that there are not are cut to those there are.
@@ -39,70 +89,581 @@ struct PagedRows {
   }
 };
 
+// 64 page numbers from `from` on, a lane each.
+struct PageIds {
+  const int32_t* ids;
+  int entries;  // of the table's row
+  int pages, from, id;
+  __device__ __forceinline__ void begin(const int32_t* ids_, int entries_, int pages_) {
+    ids = ids_, entries = entries_, pages = pages_, from = -1, id = 0;
+  }
+  // Pages first to last (at most 63 further) are among them.
+  __device__ __forceinline__ void seek(int first, int last) {
+    if (from >= 0 && first >= from && last < from + kWave) return;
+    from = first;
+    id = min(max(ids[min(from + (int)(threadIdx.x % kWave), entries - 1)], 0), pages - 1);
+  }
+};
+
 // Positions of sample b.
 __device__ __forceinline__ int kept(const CacheArgs& a, int b) {
   return static_cast<int>(min(max((int64_t)a.pages.lengths[b], (int64_t)0), a.pages.most()));
 }
 
-// The sample of query row t (the last whose offset is not behind it), -1 for none.
+// The sample of query row t (the last whose offset is not behind it); t is one
+// of the rows from the first sample's to the last one's.
 __device__ __forceinline__ int sample_of(const CacheArgs& a, int64_t t) {
-  int lo = 0, hi = a.samples + 1;
+  int lo = 0, hi = a.samples;  // offsets up to t: [0, lo) are, [hi, ...) are not
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     if (a.off_q[mid] <= t) lo = mid + 1;
     else hi = mid;
   }
-  return lo - 1 < a.samples ? lo - 1 : -1;
+  return max(lo - 1, 0);
 }
 
-// A wave per query and head.
-template <typename T>
-__global__ void __launch_bounds__(256) cache_row_kernel(CacheArgs a) {
-  __shared__ float q_s[4][256];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  for (int64_t item = blockIdx.x * (int64_t)4 + wave; item < a.rows(); item += gridDim.x * (int64_t)4) {
-    const int64_t t = item / a.q_heads;
-    const int h = static_cast<int>(item % a.q_heads), hk = h / (a.q_heads / a.k_heads);
-    const int b = sample_of(a, t);
-    T* out = static_cast<T*>(a.out) + item * a.dim;
-    float m = 0.f, l = 0.f, o[4] = {};
+// The sample and the tile of query rows within it of the x-th tile of all (as
+// find_tile).  false: past the last.
+__device__ __forceinline__ bool find_rows(const CacheArgs& a, int group, int rows, int x, int& b, int64_t& q0,
+                                          int& lq, int& tile) {
+  const int lane = threadIdx.x % kWave;
+  for (int b0 = 0; b0 < a.samples; b0 += kWave) {
+    int64_t at = 0;
+    int len = 0;
+    if (b0 + lane < a.samples) sample_range(a.off_q, b0 + lane, a.n_q, at, len);
+    const uint32_t tiles = static_cast<uint32_t>(((int64_t)len * group + rows - 1) / rows);
+    const uint32_t inc = wave_inclusive(tiles);
+    const uint64_t past = __ballot(inc > static_cast<uint32_t>(x));
+    if (past) {
+      const int at_lane = __builtin_ctzll(past);
+      b = b0 + at_lane;
+      tile = x - __builtin_amdgcn_readlane(inc - tiles, at_lane);
+      lq = __builtin_amdgcn_readlane(len, at_lane);
+      q0 = __builtin_amdgcn_readlane(static_cast<int>(at), at_lane);
+      return true;
+    }
+    x -= __builtin_amdgcn_readlane(inc, kWave - 1);
+  }
+  return false;
+}
+
+// A list of query rows (token, head of the group) and the keys that it walks.
+struct CacheRows {
+  int64_t q0;          // its first query
+  uint32_t rows;       // (queries) * group; the host keeps it within 32 bits
+  int group, hk;
+  int b, lq, lk;       // its sample; -1: the rows of all samples, each with a position of its own
+  int from, to;        // the keys of this part
+  __device__ int token(uint32_t r) const { return static_cast<int>(min(r, rows - 1) / static_cast<uint32_t>(group)); }
+  __device__ int head(uint32_t r) const {
+    r = min(r, rows - 1);
+    return hk * group + static_cast<int>(r % static_cast<uint32_t>(group));
+  }
+  // What row r sees: [lo, hi) and the sinks below both.
+  __device__ __forceinline__ void seen(const CacheArgs& a, uint32_t r, int& lo, int& hi, int& sink) const {
+    const int64_t t = q0 + token(r);
+    int p, keys = lk;
     if (b >= 0) {
-      const int lk = kept(a, b), first = a.prefix_pages * a.pages.page_rows;
-      const int p = static_cast<int>(max(t - a.off_q[b + 1] + lk, -(int64_t)1 << 30));
-      int lo, hi, sink;
-      seen_keys(p, lk, a.left, a.right, a.sinks, lo, hi, sink);
-      const T* q = static_cast<const T*>(a.q) + t * a.q_row + h * a.q_head;
-      PagedRows<T> k{static_cast<const T*>(a.k) + hk * a.k_at.head, a.k_at.page, a.k_at.row, nullptr, &a.pages};
-      PagedRows<T> v{static_cast<const T*>(a.v) + hk * a.v_at.head, a.v_at.page, a.v_at.row, nullptr, &a.pages};
-      if (first) {
-        k.ids = v.ids = a.prefix;
-        attend_row(a, q, k, v, min(lo, first), min(hi, first), sink, 0, 0, 0, first, q_s[wave], m, l, o);
-      }
-      k.ids = v.ids = a.pages.table + b * a.pages.table_row;
-      float m2, l2, o2[4];
-      attend_row(a, q, k, v, max(lo, first), hi, sink, 0, 0, first, lk, q_s[wave], m2, l2, o2);
-      const float top = l == 0.f ? m2 : l2 == 0.f ? m : fmaxf(m, m2);
-      const float f = l == 0.f ? 0.f : exp2f(m - top), f2 = l2 == 0.f ? 0.f : exp2f(m2 - top);
-      l = f * l + f2 * l2;
+      p = token(r) + lk - lq;
+    } else {
+      const int s = sample_of(a, t);
+      keys = kept(a, s);
+      p = static_cast<int>(max(t - a.off_q[s + 1] + keys, -(int64_t)(1 << 30)));
+    }
+    seen_keys(p, keys, a.left, a.right, a.sinks, lo, hi, sink);
+  }
+};
+
+// What 16-byte slot chunk c of row r of a V tile is stored in: the 16 lanes that
+// read b64 pieces of four rows, twice (16 bits), and the 64 that read words of
+// four rows four apart (f32), find them in different columns of 256 bytes.
+template <int RB, bool F32>
+__device__ __forceinline__ int v_slot16(int r, int c) {
+  if constexpr (F32) return RB % 256 == 0 ? c ^ (4 * ((r >> 2) & 3)) : RB % 128 == 0 ? c ^ (4 * ((r >> 2) & 1)) : c;
+  return RB % 256 == 0 ? c ^ (2 * (r & 7)) : RB % 128 == 0 ? c ^ (2 * ((r >> 1) & 3)) : c ^ (2 * ((r >> 2) & 1));
+}
+
+// Brings tiles of KT rows of one head's K and V into a wave's LDS, chunk by chunk
+// in the order of the slots.  Rows before `first` or from `to` on are those
+// nearest to them again, and chunks past the head's last are its first again (q
+// is 0 there): nothing is read that no query sees, and every tile takes the
+// same number of loads, which the waits count on.
+template <typename T, int DP, int KT, bool ALIGNED>
+struct PagedStager {
+  static constexpr int RB = DP * sizeof(T), CH = RB / 16, ROUNDS = KT * CH / kWave;
+  static constexpr int LOADS = 2 * ROUNDS;
+  static_assert(KT * CH % kWave == 0, "whole instructions");
+  const T* k;
+  const T* v;
+  PageStrides k_at, v_at;
+  const PageTable* pages;
+  PageIds ids;
+  int dim, first, to;
+  bool whole_pages;  // tiles from multiples of KT on lie in one page
+  uint32_t k_offset[ROUNDS], v_offset[ROUNDS];
+
+  __device__ static int slot(int i) { return i * kWave + (int)(threadIdx.x % kWave); }
+  __device__ static int row(int i) { return slot(i) / CH; }
+  __device__ static int k_chunk(int i) { return k_slot<RB>(slot(i) / CH, slot(i) % CH); }
+  __device__ static int v_chunk(int i) { return v_slot16<RB, !kIs16<T>>(slot(i) / CH, slot(i) % CH); }
+  __device__ int there(int c) const { return c * kPer16<T> < dim ? c : 0; }
+
+  __device__ __forceinline__ void begin(const CacheArgs& a, int hk, const int32_t* table, int entries, int first_,
+                                        int to_) {
+    k = static_cast<const T*>(a.k) + hk * a.k_at.head, v = static_cast<const T*>(a.v) + hk * a.v_at.head;
+    k_at = a.k_at, v_at = a.v_at, pages = &a.pages, dim = a.dim, first = first_, to = to_;
+    ids.begin(table, entries, a.pages.pages);
+    whole_pages = a.pages.page_rows % KT == 0;
+    if constexpr (ALIGNED) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) o[u] = f * o[u] + f2 * o2[u];
+      for (int i = 0; i < ROUNDS; ++i) {
+        k_offset[i] = static_cast<uint32_t>(row(i) * k_at.row * sizeof(T)) + there(k_chunk(i)) * 16;
+        v_offset[i] = static_cast<uint32_t>(row(i) * v_at.row * sizeof(T)) + there(v_chunk(i)) * 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void load(char* tile, int j0) {
+    const int j_first = max(j0, first), j_last = min(j0 + KT, to) - 1;
+    const int p_first = __builtin_amdgcn_readfirstlane(pages->page_of(j_first));
+    ids.seek(p_first, __builtin_amdgcn_readfirstlane(pages->page_of(j_last)));
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(tile));
+    if (ALIGNED && whole_pages && j_first == j0 && j_last == j0 + KT - 1) {
+      const int64_t id = __builtin_amdgcn_readlane(ids.id, p_first - ids.from);
+      const int64_t r = j0 - p_first * pages->page_rows;
+      const T* kp = k + id * k_at.page + r * k_at.row;
+      const T* vp = v + id * v_at.page + r * v_at.row;
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) load_to_lds(kp, k_offset[i], at + i * 1024);
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) load_to_lds(vp, v_offset[i], at + KT * RB + i * 1024);
+      return;
+    }
+#pragma unroll 2
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int j = min(max(j0 + row(i), j_first), j_last), p = static_cast<int>(pages->page_of(j));
+      const int64_t id = __shfl(ids.id, p - ids.from, kWave), r = j - p * pages->page_rows;
+      const T* kp = k + id * k_at.page + r * k_at.row;
+      const T* vp = v + id * v_at.page + r * v_at.row;
+      if constexpr (ALIGNED) {
+        load_to_lds_from(kp + there(k_chunk(i)) * kPer16<T>, at + i * 1024);
+        load_to_lds_from(vp + there(v_chunk(i)) * kPer16<T>, at + KT * RB + i * 1024);
+      } else {
+        auto chunk = [&](const T* p, int c) {
+          const int d = c * kPer16<T>;
+          return d + kPer16<T> <= dim ? load16_unaligned(p + d) : load16_partial(p + d, dim - d);
+        };
+        *reinterpret_cast<int4v*>(tile + slot(i) * 16) = chunk(kp, k_chunk(i));
+        *reinterpret_cast<int4v*>(tile + KT * RB + slot(i) * 16) = chunk(vp, v_chunk(i));
+      }
+    }
+  }
+};
+
+// Few query rows (16 NR) against many keys: the keys of a workgroup's chunk are
+// shared out over its waves, each with tiles of its own in LDS and no barrier
+// between them, and the waves' sums meet in LDS at the end.
+//
+// Scores are kept transposed as in attend.hpp, S^T = K Q^T, in 16x16 tiles: a lane
+// has four keys of one row per 16, which are, as they stand, the right operand of
+// O^T = V^T e^S^T.  The reference is the running maximum; weights of 16-bit tensors
+// go into the product as two parts (value and remainder), so that they lose
+// nothing against f32: the walk is bound by memory, and the products are idle.
+template <typename T, int DP, int NR, bool ALIGNED>
+__global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
+    cache_few_kernel(CacheArgs a, CacheCut prefix, CacheCut own, int splits) {
+  constexpr int RB = DP * sizeof(T), KT = cache_keys(RB), WAVES = cache_waves(RB), KB = KT / 16;
+  constexpr int STEPS = RB / 64, DB = DP / 16, TILE = 2 * KT * RB, ROWS = 16 * NR;
+  constexpr float LIFT = std::is_same_v<T, __half> ? 8.f : 0.f;  // small f16 weights stay normal
+  using Stager = PagedStager<T, DP, KT, ALIGNED>;
+  static_assert(Stager::LOADS <= 63, "the wait counts to 63");
+  static_assert(ROWS * DP * 4 <= kTileBuffers * TILE, "a wave's sums take the place of its tiles");
+  extern __shared__ __align__(16) char lds[];  // the waves' tiles, then m and l of the waves' rows
+  float* ml = reinterpret_cast<float*>(lds + WAVES * kTileBuffers * TILE);
+  const int lane = threadIdx.x % kWave, col = lane % 16, quarter = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int group = a.q_heads / a.k_heads;
+  if (splits == 1) {  // (the join does it otherwise)
+    int64_t first, last;
+    sample_rows(a, first, last);
+    if (first > 0 || last < a.n_q)
+      zero_outside(static_cast<T*>(a.out), (int64_t)a.q_heads * a.dim, first, last, a.n_q);
+  }
+
+  // rows next to each other, then heads, then chunks
+  const int64_t prefix_blocks = prefix.tiles * a.k_heads * prefix.splits;
+  const bool is_prefix = blockIdx.x < prefix_blocks;
+  const CacheCut& cut = is_prefix ? prefix : own;
+  const int64_t id = is_prefix ? blockIdx.x : blockIdx.x - prefix_blocks;
+  CacheRows w;
+  w.group = group;
+  w.hk = static_cast<int>(id / cut.tiles % a.k_heads);
+  const int split = static_cast<int>(id / cut.tiles / a.k_heads);
+  int tile;
+  const int32_t* table;
+  if (is_prefix) {
+    int64_t last;
+    sample_rows(a, w.q0, last);
+    tile = static_cast<int>(id % cut.tiles);
+    w.rows = static_cast<uint32_t>((last - w.q0) * group);
+    if ((uint32_t)tile * ROWS >= w.rows) return;
+    w.b = -1, w.lq = w.lk = 0, w.from = 0, w.to = a.prefix_rows();
+    table = a.prefix;
+  } else {
+    if (!find_rows(a, group, ROWS, static_cast<int>(id % cut.tiles), w.b, w.q0, w.lq, tile)) return;
+    w.rows = static_cast<uint32_t>(w.lq) * group;
+    w.lk = kept(a, w.b), w.from = a.prefix_rows(), w.to = w.lk;
+    table = a.pages.table + w.b * a.pages.table_row;
+  }
+  const uint32_t row0 = static_cast<uint32_t>(tile) * ROWS;
+
+  // rows past the last are copies of it
+  int lo[NR], hi[NR], lo_min = kNoLimit, lo_max = 0, hi_min = kNoLimit, hi_max = 0;
+#pragma unroll
+  for (int x = 0; x < NR; ++x) {
+    int sink;
+    w.seen(a, row0 + 16 * x + col, lo[x], hi[x], sink);
+    lo_min = min(lo_min, lo[x]), lo_max = max(lo_max, lo[x]);
+    hi_min = min(hi_min, hi[x]), hi_max = max(hi_max, hi[x]);
+  }
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) {
+    lo_min = min(lo_min, __shfl_xor(lo_min, x, kWave)), lo_max = max(lo_max, __shfl_xor(lo_max, x, kWave));
+    hi_min = min(hi_min, __shfl_xor(hi_min, x, kWave)), hi_max = max(hi_max, __shfl_xor(hi_max, x, kWave));
+  }
+  lo_min = __builtin_amdgcn_readfirstlane(lo_min), lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+  hi_min = __builtin_amdgcn_readfirstlane(hi_min), hi_max = __builtin_amdgcn_readfirstlane(hi_max);
+  // the window's tiles begin where pages of whole tiles have theirs
+  int start = lo_min;
+  if (a.pages.page_rows % KT == 0) start = start / KT * KT;
+  int sink_end = min(a.sinks, hi_max);
+  if (a.sinks > start) start = sink_end = 0;
+  start = max(start, w.from);
+  const int end = min(hi_max, w.to);
+  sink_end = min(sink_end, w.to);
+  const int sink_tiles = max(sink_end - w.from + KT - 1, 0) / KT, tiles = sink_tiles + max(end - start + KT - 1, 0) / KT;
+  // this chunk's tiles, and this wave's
+  const int chunk_tiles = cut.chunk / KT, c0 = min(split * (int64_t)chunk_tiles, (int64_t)tiles);
+  const int c1 = split == cut.splits - 1 ? tiles : min(c0 + chunk_tiles, tiles), each = (c1 - c0 + WAVES - 1) / WAVES;
+  const int t0 = min(c0 + wave * each, c1), t1 = min(t0 + each, c1);
+  auto item_of = [&](uint32_t r) { return (w.q0 + w.token(r)) * a.q_heads + w.head(r); };
+  const int part = cut.first_split + split;
+  if (c0 == c1 && splits > 1) {  // nothing to see here
+    for (uint32_t r = threadIdx.x; r < ROWS; r += kWave * WAVES)
+      if (row0 + r < w.rows) {
+        const int64_t at = part * a.rows() + item_of(row0 + r);
+        a.part[2 * at] = -__builtin_inff();
+        a.part[2 * at + 1] = 0.f;
+      }
+    return;
+  }
+
+  Stager stager;
+  const int table_pages = is_prefix ? a.prefix_pages : a.pages.table_pages;
+  stager.begin(a, w.hk, table, table_pages, 0, 0);
+  char* mine = lds + wave * kTileBuffers * TILE;
+  auto place = [&](int t) { return t < sink_tiles ? w.from + t * KT : start + (t - sink_tiles) * KT; };
+  auto stage = [&](int t, int buf) {
+    const bool sinks = t < sink_tiles;
+    stager.first = sinks ? w.from : max(start, min(lo_min, end - 1));
+    if (!sinks && start == w.from) stager.first = start;
+    stager.to = sinks ? sink_end : end;
+    stager.load(mine + buf * TILE, place(t));
+  };
+  if (t0 < t1) stage(t0, 0);
+
+  int4v qf[NR][STEPS];
+#pragma unroll
+  for (int x = 0; x < NR; ++x) {
+    const uint32_t r = row0 + 16 * x + col;
+    const T* q = static_cast<const T*>(a.q) + (w.q0 + w.token(r)) * a.q_row + w.head(r) * a.q_head;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      const int d = (4 * st + quarter) * kPer16<T>;
+      int4v y;
+      if (d + kPer16<T> <= a.dim) y = load16_unaligned(q + d);
+      else y = load16_partial(q + d, a.dim - d);
+      if (a.q_sign != 1.f) {  // (as in attend_walk)
+        T e[kPer16<T>];
+        __builtin_memcpy(e, &y, 16);
+#pragma unroll
+        for (int i = 0; i < kPer16<T>; ++i) e[i] = from_f32<T>(to_f32(e[i]) * a.q_sign);
+        __builtin_memcpy(&y, e, 16);
+      }
+      qf[x][st] = y;
+    }
+  }
+
+  f32x4 o[NR][DB];
+  float m[NR], l[NR];  // reference; this lane's share of the sum
+#pragma unroll
+  for (int x = 0; x < NR; ++x) {
+    m[x] = -__builtin_inff(), l[x] = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[x][db] = f32x4(0.f);
+  }
+  const float c = a.scale_log2;
+  for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
+    if (t + 1 < t1) {
+      // (what was read from that buffer has arrived)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      stage(t + 1, buf ^ 1);
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(ALIGNED ? Stager::LOADS : 0) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const char* kt = mine + buf * TILE;
+    const char* vt = kt + KT * RB;
+    const int j0 = place(t), last = t < sink_tiles ? sink_end : end;
+    f32x4 s[NR][KB];
+#pragma unroll
+    for (int x = 0; x < NR; ++x)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) s[x][kb] = f32x4(0.f);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        const int4v k = *reinterpret_cast<const int4v*>(kt + (16 * kb + col) * RB +
+                                                        k_slot<RB>(16 * kb + col, 4 * st + quarter) * 16);
+#pragma unroll
+        for (int x = 0; x < NR; ++x) s[x][kb] = mma16<T>(k, qf[x][st], s[x][kb]);
+      }
+    const bool whole = j0 + KT <= min(last, hi_min) && (j0 >= lo_max || j0 + KT <= a.sinks);
+    if (!whole) {
+#pragma unroll
+      for (int x = 0; x < NR; ++x)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = j0 + 16 * kb + 4 * quarter + i;
+            const bool see = j < min(last, hi[x]) && (j >= lo[x] || j < a.sinks);
+            s[x][kb][i] = see ? s[x][kb][i] : -__builtin_inff();
+          }
+    }
+    // weights, and their sums; a new reference rescales what is there
+    float top[NR];
+    bool moves = false;
+#pragma unroll
+    for (int x = 0; x < NR; ++x) {
+      top[x] = s[x][0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[x] = fmaxf(top[x], s[x][kb][i]);
+      top[x] = fmaxf(top[x], __shfl_xor(top[x], 16, kWave));
+      top[x] = fmaxf(top[x], __shfl_xor(top[x], 32, kWave));
+      moves |= top[x] > m[x];
+    }
+    if (__any(moves)) {
+#pragma unroll
+      for (int x = 0; x < NR; ++x) {
+        const float m_new = fmaxf(m[x], top[x]);
+        const float fix = m[x] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m[x] - m_new) * c);
+        m[x] = m_new;
+        l[x] *= fix;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[x][db] *= fix;
+      }
+    }
+    float p[NR][KB][4];
+#pragma unroll
+    for (int x = 0; x < NR; ++x) {
+      const float base = m[x] == -__builtin_inff() ? 0.f : m[x];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[x][kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][kb][i] - base, c, LIFT));
+          l[x] += p[x][kb][i];
+        }
+    }
+    if constexpr (kIs16<T>) {
+      static_assert(KB == 2, "a product of 32 keys");
+      int4v ph[NR], pl[NR];  // the weights, and what their rounding leaves
+#pragma unroll
+      for (int x = 0; x < NR; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u = p[x][i / 2][i % 2 * 2], v = p[x][i / 2][i % 2 * 2 + 1];
+          ph[x][i] = pack2<T>(u, v);
+          T e[2];
+          const int both = ph[x][i];
+          __builtin_memcpy(e, &both, 4);
+          pl[x][i] = pack2<T>(u - to_f32(e[0]), v - to_f32(e[1]));
+        }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        int4v y;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 16 * h + 4 * quarter + col / 4, d = 16 * db + 4 * (col % 4);
+          const char* at = vt + r * RB + v_slot16<RB, false>(r, d / 8) * 16 + d % 8 * 2;
+          const int2v z = __builtin_bit_cast(int2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                        (__attribute__((address_space(3))) short4v*)at));
+          y[2 * h] = z[0], y[2 * h + 1] = z[1];
+        }
+#pragma unroll
+        for (int x = 0; x < NR; ++x) {
+          o[x][db] = mma16<T>(y, ph[x], o[x][db]);
+          o[x][db] = mma16<T>(y, pl[x], o[x][db]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * kb + 4 * quarter + i;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const int ch = 4 * db + col / 4;
+            const float y = *reinterpret_cast<const float*>(vt + r * RB + v_slot16<RB, true>(r, ch) * 16 + col % 4 * 4);
+#pragma unroll
+            for (int x = 0; x < NR; ++x)
+              o[x][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(y, p[x][kb][i], o[x][db], 0, 0, 0);
+          }
+        }
+    }
+  }
+
+  // the waves' sums meet
+  float off = 0.f;  // NaN when one of them is not finite
+#pragma unroll
+  for (int x = 0; x < NR; ++x) {
+    l[x] += __shfl_xor(l[x], 16, kWave);
+    l[x] += __shfl_xor(l[x], 32, kWave);
+    off = __builtin_fmaf(l[x], 0.f, off);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) off = __builtin_fmaf(o[x][db][i], 0.f, off);
+    if (quarter == 0) {
+      ml[2 * (wave * ROWS + 16 * x + col)] = m[x];
+      ml[2 * (wave * ROWS + 16 * x + col) + 1] = l[x];
+    }
+  }
+  const int odd = __syncthreads_or(off != off);
+  if (!odd) {
+    float* sums = reinterpret_cast<float*>(mine);
+#pragma unroll
+    for (int x = 0; x < NR; ++x) {
+      float all = -__builtin_inff();
+#pragma unroll
+      for (int y = 0; y < WAVES; ++y) all = fmaxf(all, ml[2 * (y * ROWS + 16 * x + col)]);
+      const float f = m[x] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m[x] - all) * c);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        *reinterpret_cast<f32x4*>(sums + (16 * x + col) * DP + 16 * db + 4 * quarter) = f * o[x][db];
+    }
+    __syncthreads();
+    constexpr int PIECES = DP / 4;
+    for (int x = threadIdx.x; x < ROWS * PIECES; x += kWave * WAVES) {
+      const int r = x / PIECES, d = x % PIECES * 4;
+      if (row0 + r >= w.rows || d >= a.dim) continue;
+      float all = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+      for (int y = 0; y < WAVES; ++y) all = fmaxf(all, ml[2 * (y * ROWS + r)]);
+      f32x4 v = f32x4(0.f);
+#pragma unroll
+      for (int y = 0; y < WAVES; ++y) {
+        const float my = ml[2 * (y * ROWS + r)], ly = ml[2 * (y * ROWS + r) + 1];
+        sum += my == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((my - all) * c) * ly;
+        v += *reinterpret_cast<const f32x4*>(lds + y * kTileBuffers * TILE + (r * DP + d) * 4);
+      }
+      const int64_t item = item_of(row0 + r);
+      const int cnt = min(4, a.dim - d);
+      if (splits > 1) {
+        const int64_t at = part * a.rows() + item;
+        float* to = a.part + a.part_values(splits) + at * a.dim + d;
+        if (d == 0) {
+          a.part[2 * at] = sum == 0.f ? -__builtin_inff() : all * c - LIFT;
+          a.part[2 * at + 1] = sum;
+        }
+        for (int i = 0; i < cnt; ++i) to[i] = v[i];
+      } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T* to = static_cast<T*>(a.out) + item * a.dim + d;
+        for (int i = 0; i < cnt; ++i) to[i] = from_f32<T>(v[i] * inv);
+      }
+    }
+    return;
+  }
+  // a value that is not finite, seen or not: key by key, of the seen ones only
+  PagedRows<T> kr{static_cast<const T*>(a.k) + w.hk * a.k_at.head, a.k_at.page, a.k_at.row, table, &a.pages};
+  PagedRows<T> vr{static_cast<const T*>(a.v) + w.hk * a.v_at.head, a.v_at.page, a.v_at.row, table, &a.pages};
+  const int s0 = min(w.from + c0 * KT, sink_end), s1 = min(w.from + c1 * KT, sink_end);
+  const int w0 = start + max(c0 - sink_tiles, 0) * KT, w1 = min(start + max(c1 - sink_tiles, 0) * KT, end);
+  float* q_s = reinterpret_cast<float*>(mine);
+  for (int r = wave; r < ROWS && row0 + r < w.rows; r += WAVES) {
+    int lo_r, hi_r, sink;
+    w.seen(a, row0 + r, lo_r, hi_r, sink);
+    const T* q = static_cast<const T*>(a.q) + (w.q0 + w.token(row0 + r)) * a.q_row + w.head(row0 + r) * a.q_head;
+    float m_r, l_r, o_r[4];
+    attend_row(a, q, kr, vr, lo_r, hi_r, sink, s0, s1, w0, w1, q_s, m_r, l_r, o_r);
+    const int64_t item = item_of(row0 + r), at = part * a.rows() + item;
+    if (splits > 1 && lane == 0) {
+      a.part[2 * at] = l_r == 0.f ? -__builtin_inff() : m_r;
+      a.part[2 * at + 1] = l_r;
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int d = lane + u * kWave;
-      if (d < a.dim) out[d] = from_f32<T>(l == 0.f ? 0.f : o[u] / l);
+      if (d >= a.dim) continue;
+      if (splits > 1) a.part[a.part_values(splits) + at * a.dim + d] = o_r[u];
+      else static_cast<T*>(a.out)[item * a.dim + d] = from_f32<T>(l_r == 0.f ? 0.f : o_r[u] / l_r);
     }
+  }
+}
+
+template <typename T, int DP, int NR, bool ALIGNED>
+int launch_few(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
+  constexpr int RB = DP * sizeof(T), WAVES = cache_waves(RB);
+  constexpr int bytes = WAVES * (kTileBuffers * 2 * cache_keys(RB) * RB + 16 * NR * 8);
+  auto kernel = &cache_few_kernel<T, DP, NR, ALIGNED>;
+  if (bytes > 65536)
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  const int64_t blocks = (p.prefix.tiles * p.prefix.splits + p.own.tiles * p.own.splits) * a.k_heads;
+  TSC_REQUIRE(blocks * kWave * WAVES < (1ll << 32), "cache_attention: too many tiles");
+  kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, p.prefix, p.own, p.splits());
+  TSC_LAUNCH_CHECK("cache_attention");
+  return 0;
+}
+
+template <typename T, int DP, bool ALIGNED>
+int launch_rows(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
+  constexpr int MOST = cache_row_blocks(DP * sizeof(T));
+  if constexpr (MOST >= 4)
+    if (p.row_blocks == 4) return launch_few<T, DP, 4, ALIGNED>(a, p, s);
+  if constexpr (MOST >= 2)
+    if (p.row_blocks == 2) return launch_few<T, DP, 2, ALIGNED>(a, p, s);
+  return launch_few<T, DP, 1, ALIGNED>(a, p, s);
+}
+
+template <typename T, bool ALIGNED>
+int launch_dims(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
+  switch (padded_dim(a.dim)) {
+    case 32: return launch_rows<T, 32, ALIGNED>(a, p, s);
+    case 64: return launch_rows<T, 64, ALIGNED>(a, p, s);
+    case 96: return launch_rows<T, 96, ALIGNED>(a, p, s);
+    case 128: return launch_rows<T, 128, ALIGNED>(a, p, s);
+    default: return launch_rows<T, 256, ALIGNED>(a, p, s);
   }
 }
 
 }  // namespace
 
 template <typename T>
-int launch_cache(const CacheArgs& a, hipStream_t s) {
-  const int64_t blocks = std::min<int64_t>(ceil_div(a.rows(), 4), 1 << 20);
-  cache_row_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-  TSC_LAUNCH_CHECK("cache_attention");
-  return 0;
+int launch_cache(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
+  const int64_t e = kPer16<T>;
+  // 16-byte pieces at 16-byte addresses, rows of a tile within 32-bit offsets
+  auto whole = [&](const void* base, const PageStrides& at) {
+    return at.row < (1 << 24) && at.row % e == 0 && at.page % e == 0 && at.head % e == 0 &&
+           reinterpret_cast<uintptr_t>(base) % 16 == 0;
+  };
+  const bool aligned = a.dim % e == 0 && whole(a.k, a.k_at) && whole(a.v, a.v_at);
+  if (int rc = aligned ? launch_dims<T, true>(a, p, s) : launch_dims<T, false>(a, p, s)) return rc;
+  return p.splits() > 1 ? launch_join<T>(a, p.splits(), s) : 0;
 }
 
 }  // namespace tsc

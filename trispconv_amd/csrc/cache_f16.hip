@@ -2,5 +2,5 @@
 #include "cache.hpp"
 
 namespace tsc {
-template int launch_cache<__half>(const CacheArgs&, hipStream_t);
+template int launch_cache<__half>(const CacheArgs&, const CachePlan&, hipStream_t);
 }  // namespace tsc
