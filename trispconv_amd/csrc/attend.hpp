@@ -225,8 +225,12 @@ struct Stager {
     for (int i = 0; i < ROUNDS; ++i)
       if (chunk(slot(i)) * kPer16<T> >= dim) *reinterpret_cast<int4v*>(tile + slot(i) * 16) = int4v(0);
   }
+  // Where this wave's part of a tile begins in LDS.
+  __device__ __forceinline__ uint32_t place(const char* tile) const {
+    return __builtin_amdgcn_readfirstlane(lds_address(tile) + wave * 1024);
+  }
   __device__ __forceinline__ void load(char* tile, int j0, int end) const {
-    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(tile) + wave * 1024);
+    const uint32_t at = place(tile);
     if constexpr (ALIGNED) {
       const T* base = src + j0 * stride;
       if (j0 + 32 * KB <= end && dim >= DP) {
@@ -246,14 +250,40 @@ struct Stager {
     } else {
 #pragma unroll 2
       for (int i = 0; i < ROUNDS; ++i) {
-        const int d = chunk(slot(i)) * kPer16<T>;
-        const T* p = src + min(j0 + row(slot(i)), end - 1) * stride + d;
-        const int4v x = d + kPer16<T> <= dim ? load16_unaligned(p) : load16_partial(p, dim - d);
-        *reinterpret_cast<int4v*>(tile + slot(i) * 16) = x;
+        load_chunk(tile, src + min(j0 + row(slot(i)), end - 1) * stride, i);
       }
     }
   }
+  // Round i's chunk of a row at any address, through registers.
+  __device__ __forceinline__ void load_chunk(char* tile, const T* p, int i) const {
+    const int d = chunk(slot(i)) * kPer16<T>;
+    const int4v x = d + kPer16<T> <= dim ? load16_unaligned(p + d) : load16_partial(p + d, dim - d);
+    *reinterpret_cast<int4v*>(tile + slot(i) * 16) = x;
+  }
   __device__ __forceinline__ bool in(int i) const { return dim >= DP || chunk(slot(i)) * kPer16<T> < dim; }
+};
+
+// Tiles of one head's K and V, one behind the other in LDS, from rows of a
+// constant distance.
+template <typename T, int DP, int KB, int WAVES, bool ALIGNED>
+struct DenseTiles {
+  static constexpr int TILE = 32 * KB * DP * (int)sizeof(T);  // bytes of K, and of V
+  Stager<T, DP, KB, WAVES, ALIGNED, false> k;
+  Stager<T, DP, KB, WAVES, ALIGNED, true> v;
+  __device__ __forceinline__ void begin(const T* k_, int64_t k_row, const T* v_, int64_t v_row, int dim, int wave) {
+    k.begin(k_, k_row, dim, wave);
+    v.begin(v_, v_row, dim, wave);
+  }
+  __device__ __forceinline__ void clear(char* tile) const {
+    k.clear(tile);
+    v.clear(tile + TILE);
+  }
+  __device__ __forceinline__ void load(char* tile, int j0, int end) const {
+    k.load(tile, j0, end);
+    v.load(tile + TILE, j0, end);
+  }
+  __device__ DenseRows<T> k_rows() const { return {k.src, k.stride}; }
+  __device__ DenseRows<T> v_rows() const { return {v.src, v.stride}; }
 };
 
 __device__ __forceinline__ float max_halves(float x) {
@@ -322,15 +352,27 @@ __device__ __forceinline__ bool find_tile(const AttendArgs& a, int group, int ro
 
 // What a workgroup computes: rows [row0, ...) of the `rows` (token, head of
 // the group) rows of a sample and key head, against key tiles [t0, t1) of
-// those that it walks: [0, sink_end) in sink_tiles of them, then [start, end).
+// those that it walks: [sink_start, sink_end) in sink_tiles of them, then
+// [start, end).
 struct Walk {
   int64_t q0;  // the sample's first query row
   uint32_t row0, rows;
   int group, hk, lk, shift;  // shift: position of the sample's first query
-  int sink_end, sink_tiles, start, end, t0, t1;
+  int sink_start = 0, sink_end, sink_tiles, start, end, t0, t1;
   int split, splits;
   // (the host keeps n_q * group within 32 bits)
   __device__ int token(uint32_t r) const { return static_cast<int>(min(r, rows - 1) / static_cast<uint32_t>(group)); }
+  // The keys that row r sees (seen_keys).
+  __device__ __forceinline__ void seen(const AttendArgs& a, uint32_t r, int& lo, int& hi, int& sink) const {
+    seen_keys(token(r) + shift, lk, a.left, a.right, a.sinks, lo, hi, sink);
+  }
+  // The least and the most of the rows [first, last]: later positions see later keys.
+  __device__ __forceinline__ void bounds(const AttendArgs& a, uint32_t first, uint32_t last, int& lo_first,
+                                         int& hi_first, int& lo_last, int& hi_last) const {
+    int none;
+    seen(a, first, lo_first, hi_first, none);
+    seen(a, last, lo_last, hi_last, none);
+  }
 };
 
 // The weight of a key at its row's reference score (in log2), and what a lane's 16
@@ -377,24 +419,22 @@ constexpr float kFar = 0x1p24f;  // exponents from here on have no fractions in 
 // keys are walked once more with such values replaced by 0, which leaves the
 // bits of every row that sees none of them as they would have been; rows that
 // see one are then done key by key.
-template <typename T, int DP, int RB, int KB, int WAVES, bool ALIGNED>
-__device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, const T* k, const T* v,
-                                            char* lds) {
+template <typename T, int DP, int RB, int KB, int WAVES, typename Tiles, typename Rows>
+__device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, Tiles& tiles, char* lds) {
   constexpr int KT = 32 * KB, ROW_BYTES = DP * sizeof(T);
   constexpr int BUFFERS = tile_buffers<T>(DP, WAVES), TILE = KT * ROW_BYTES, STEPS = DP * (int)sizeof(T) / 32, DB = DP / 32;
   const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   int lo_first, hi_first, lo_last, hi_last, none;
   const uint32_t wave_row = w.row0 + wave * 32 * RB;
-  seen_keys(w.token(wave_row) + w.shift, w.lk, a.left, a.right, a.sinks, lo_first, hi_first, none);
-  seen_keys(w.token(wave_row + 32 * RB - 1) + w.shift, w.lk, a.left, a.right, a.sinks, lo_last, hi_last, none);
+  w.bounds(a, wave_row, wave_row + 32 * RB - 1, lo_first, hi_first, lo_last, hi_last);
   int lo[RB], hi[RB];
   int4v qf[RB][STEPS];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const uint32_t r = wave_row + rb * 32 + col;
     const int t = w.token(r), g = static_cast<int>(min(r, w.rows - 1) - static_cast<uint32_t>(t) * w.group);
-    seen_keys(t + w.shift, w.lk, a.left, a.right, a.sinks, lo[rb], hi[rb], none);
+    w.seen(a, r, lo[rb], hi[rb], none);
     if (r >= w.rows) hi[rb] = 0;
     const T* q = static_cast<const T*>(a.q) + (w.q0 + t) * a.q_row + (w.hk * w.group + g) * a.q_head;
 #pragma unroll
@@ -417,25 +457,15 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
 
   auto tile_at = [&](int t, int& j0, int& end) {
     if (t < w.sink_tiles) {
-      j0 = t * KT;
+      j0 = w.sink_start + t * KT;
       end = w.sink_end;
     } else {
       j0 = w.start + (t - w.sink_tiles) * KT;
       end = w.end;
     }
   };
-  Stager<T, DP, KB, WAVES, ALIGNED, false> k_stage;
-  Stager<T, DP, KB, WAVES, ALIGNED, true> v_stage;
-  k_stage.begin(k, a.k_row, a.dim, wave);
-  v_stage.begin(v, a.v_row, a.dim, wave);
-  for (int x = 0; x < BUFFERS; ++x) {
-    k_stage.clear(lds + x * 2 * TILE);
-    v_stage.clear(lds + x * 2 * TILE + TILE);
-  }
-  auto stage = [&](int j0, int end, int buf) {
-    k_stage.load(lds + buf * 2 * TILE, j0, end);
-    v_stage.load(lds + buf * 2 * TILE + TILE, j0, end);
-  };
+  for (int x = 0; x < BUFFERS; ++x) tiles.clear(lds + x * 2 * TILE);
+  auto stage = [&](int j0, int end, int buf) { tiles.load(lds + buf * 2 * TILE, j0, end); };
 
   f32x16 o[RB][DB];
   float m[RB], mc[RB], l[RB][2];  // reference score, its exponent, two partial sums
@@ -699,7 +729,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
       if (w.t0 < w.sink_tiles) {
         tile_at(w.t0, j0, end);
         sink_from = j0;
-        sink_to = min(min(w.t1, w.sink_tiles) * KT, w.sink_end);
+        sink_to = min(w.sink_start + min(w.t1, w.sink_tiles) * KT, w.sink_end);
       }
       if (w.t1 > w.sink_tiles) {
         from = w.start + (max(w.t0, w.sink_tiles) - w.sink_tiles) * KT;
@@ -712,10 +742,10 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Walk& w, 
         const int tx = w.token(rx), gx = static_cast<int>(rx - static_cast<uint32_t>(tx) * w.group);
         const int64_t ix = (w.q0 + tx) * a.q_heads + w.hk * w.group + gx;
         int lx, hx, sx;
-        seen_keys(tx + w.shift, w.lk, a.left, a.right, a.sinks, lx, hx, sx);
+        w.seen(a, rx, lx, hx, sx);
         float mx, lsum, ox[4];
         attend_row(a, static_cast<const T*>(a.q) + (w.q0 + tx) * a.q_row + (w.hk * w.group + gx) * a.q_head,
-                   DenseRows<T>{k, a.k_row}, DenseRows<T>{v, a.v_row}, lx, hx, sx, sink_from, sink_to, from, to, q_s, mx, lsum, ox);
+                   tiles.k_rows(), tiles.v_rows(), lx, hx, sx, sink_from, sink_to, from, to, q_s, mx, lsum, ox);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int d = lane + u * kWave;
@@ -777,7 +807,9 @@ __global__ void __launch_bounds__(kWave * WAVES, waves_per_simd<T>(DP, RB, WAVES
   const int tiles = w.sink_tiles + (w.end - w.start + KT - 1) / KT, each = (tiles + splits - 1) / splits;
   w.t0 = min(w.split * each, tiles);
   w.t1 = min(w.t0 + each, tiles);
-  attend_walk<T, DP, RB, KB, WAVES, ALIGNED>(a, w, k, v, lds);
+  DenseTiles<T, DP, KB, WAVES, ALIGNED> kv;
+  kv.begin(k, a.k_row, v, a.v_row, a.dim, __builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+  attend_walk<T, DP, RB, KB, WAVES>(a, w, kv, lds);
 }
 
 // Joins the splits of each row: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s,

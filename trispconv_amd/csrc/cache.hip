@@ -18,27 +18,36 @@ constexpr int kCus = 256;
 CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t prefix_rows, int q_heads, int k_heads,
                      int dim, int elem, int left, int right, int sinks) {
   CachePlan p;
-  const int64_t group = q_heads / k_heads, mean = n_q * group / samples;
+  const int64_t group = q_heads / k_heads, all = n_q * group, mean = all / samples;
   const int row_bytes = padded_dim(dim) * elem, kt = cache_keys(row_bytes);
   p.row_blocks = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
   while (p.row_blocks > cache_row_blocks(row_bytes)) p.row_blocks /= 2;
-  const int64_t rows = 16 * p.row_blocks;
+  // lists: of the rows that `tiles` are cut from; mean: rows of such a list
+  auto cut = [&](int64_t keys, int64_t lists, int64_t mean) {
+    CacheCut c;
+    auto tiles = [&](int64_t rows) { return all / rows + std::min(lists, n_q); };
+    if (sinks > 0) keys += kt;  // (a tile of their own)
+    if (mean <= 64) {
+      c.tiles = tiles(16 * p.row_blocks);
+      // about four workgroups per CU, of 256 keys and more
+      const int64_t most = std::max<int64_t>(1, 4 * kCus / std::max<int64_t>(1, c.tiles * k_heads));
+      const int64_t least = std::max<int64_t>(256, ceil_div(keys, std::min<int64_t>(most, kMostSplits / 2)));
+      c.chunk = static_cast<int>(align_up(std::min<int64_t>(least, 1ll << 30), 4 * kt));
+      c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
+      return c;
+    }
+    // as attend_cut
+    c.wave_rows = can_pair(padded_dim(dim), elem) && keys >= 4096 && tiles(256) * k_heads >= 2 * kCus ? 2 : 1;
+    c.tiles = tiles(128 * c.wave_rows);
+    c.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({keys / 256, 4 * kCus / (c.tiles * k_heads), kMostSplits / 2})));
+    return c;
+  };
   // keys that a tile of a sample's rows can see at most
   int64_t span = std::max<int64_t>(longest - prefix_rows, 0);
   if (left >= 0) span = std::min<int64_t>(span, (int64_t)left + n_q + sinks + kt);
-  auto cut = [&](int64_t keys, int64_t tiles) {
-    CacheCut c;
-    if (sinks > 0) keys += kt;  // (a tile of their own)
-    c.tiles = tiles;
-    // about four workgroups per CU, of 256 keys and more
-    const int64_t most = std::max<int64_t>(1, 4 * kCus / std::max<int64_t>(1, tiles * k_heads));
-    const int64_t least = std::max<int64_t>(256, ceil_div(keys, std::min<int64_t>(most, kMostSplits / 2)));
-    c.chunk = static_cast<int>(align_up(std::min<int64_t>(least, 1ll << 30), 4 * kt));
-    c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
-    return c;
-  };
-  p.own = cut(span, n_q * group / rows + std::min(samples, n_q));
-  if (prefix_rows) p.prefix = cut(prefix_rows, ceil_div(n_q * group, rows));
+  p.own = cut(span, samples, mean);
+  if (prefix_rows) p.prefix = cut(prefix_rows, 1, all);
   p.own.first_split = p.prefix.splits;
   return p;
 }

@@ -25,14 +25,15 @@ struct CacheArgs : AttendArgs {
 };
 
 // How the prefix's or the samples' own keys are cut: tiles of query rows (at
-// most), and chunks of `chunk` keys, numbered from first_split on.
+// most), and parts of the keys, numbered from first_split on.
 struct CacheCut {
   int64_t tiles = 0;
   int splits = 0, first_split = 0;
-  int chunk = 0;
+  int wave_rows = 0;  // rows of a workgroup of four waves in 128s, 0: the form for few rows
+  int chunk = 0;      // that form's keys of a part
 };
 struct CachePlan {
-  int row_blocks = 1;  // rows of a tile in 16s
+  int row_blocks = 1;  // that form's rows of a tile in 16s
   CacheCut prefix, own;
   int splits() const { return prefix.splits + own.splits; }
 };
@@ -147,32 +148,88 @@ __device__ __forceinline__ bool find_rows(const CacheArgs& a, int group, int row
   return false;
 }
 
-// A list of query rows (token, head of the group) and the keys that it walks.
-struct CacheRows {
-  int64_t q0;          // its first query
-  uint32_t rows;       // (queries) * group; the host keeps it within 32 bits
-  int group, hk;
-  int b, lq, lk;       // its sample; -1: the rows of all samples, each with a position of its own
-  int from, to;        // the keys of this part
-  __device__ int token(uint32_t r) const { return static_cast<int>(min(r, rows - 1) / static_cast<uint32_t>(group)); }
+// The query rows of one sample, or of all of them, each with a position of its own.
+struct CacheWalk : Walk {
+  const CacheArgs* args;
+  int b;  // the sample; -1: all
   __device__ int head(uint32_t r) const {
-    r = min(r, rows - 1);
-    return hk * group + static_cast<int>(r % static_cast<uint32_t>(group));
+    return hk * group + static_cast<int>(min(r, rows - 1) % static_cast<uint32_t>(group));
   }
-  // What row r sees: [lo, hi) and the sinks below both.
-  __device__ __forceinline__ void seen(const CacheArgs& a, uint32_t r, int& lo, int& hi, int& sink) const {
-    const int64_t t = q0 + token(r);
-    int p, keys = lk;
-    if (b >= 0) {
-      p = token(r) + lk - lq;
-    } else {
-      const int s = sample_of(a, t);
-      keys = kept(a, s);
+  __device__ __forceinline__ void seen(const AttendArgs& a, uint32_t r, int& lo, int& hi, int& sink) const {
+    int p = token(r) + shift, keys = lk;
+    if (b < 0) {
+      const int64_t t = q0 + token(r);
+      const int s = sample_of(*args, t);
+      keys = kept(*args, s);
       p = static_cast<int>(max(t - a.off_q[s + 1] + keys, -(int64_t)(1 << 30)));
     }
     seen_keys(p, keys, a.left, a.right, a.sinks, lo, hi, sink);
   }
+  __device__ __forceinline__ void bounds(const AttendArgs& a, uint32_t first, uint32_t last, int& lo_first,
+                                         int& hi_first, int& lo_last, int& hi_last) const {
+    if (b >= 0) return Walk::bounds(a, first, last, lo_first, hi_first, lo_last, hi_last);
+    lo_first = hi_first = kNoLimit, lo_last = hi_last = 0;
+    for (uint32_t r = first + threadIdx.x % kWave; r <= last; r += kWave) {
+      int lo, hi, sink;
+      seen(a, r, lo, hi, sink);
+      lo_first = min(lo_first, lo), lo_last = max(lo_last, lo);
+      hi_first = min(hi_first, hi), hi_last = max(hi_last, hi);
+    }
+#pragma unroll
+    for (int x = 1; x < kWave; x <<= 1) {
+      lo_first = min(lo_first, __shfl_xor(lo_first, x, kWave)), lo_last = max(lo_last, __shfl_xor(lo_last, x, kWave));
+      hi_first = min(hi_first, __shfl_xor(hi_first, x, kWave)), hi_last = max(hi_last, __shfl_xor(hi_last, x, kWave));
+    }
+    lo_first = __builtin_amdgcn_readfirstlane(lo_first), lo_last = __builtin_amdgcn_readfirstlane(lo_last);
+    hi_first = __builtin_amdgcn_readfirstlane(hi_first), hi_last = __builtin_amdgcn_readfirstlane(hi_last);
+  }
+  // Takes the x-th tile of `tile_rows` rows (the prefix's: of all samples) and the
+  // range of keys [from, to) of this part.  false: past the last tile.
+  __device__ __forceinline__ bool begin(const CacheArgs& a, bool prefix, int tile_rows, int x, int& from, int& to) {
+    args = &a;
+    int tile = x;
+    if (prefix) {
+      int64_t last;
+      sample_rows(a, q0, last);
+      rows = static_cast<uint32_t>((last - q0) * group);
+      b = -1, lk = shift = 0, from = 0, to = a.prefix_rows();
+      if ((int64_t)tile * tile_rows >= rows) return false;
+    } else {
+      int lq;
+      if (!find_rows(a, group, tile_rows, x, b, q0, lq, tile)) return false;
+      rows = static_cast<uint32_t>(lq) * group;
+      lk = kept(a, b), shift = lk - lq, from = a.prefix_rows(), to = lk;
+    }
+    row0 = static_cast<uint32_t>(tile) * tile_rows;
+    return true;
+  }
+  __device__ const int32_t* table() const {
+    return b < 0 ? args->prefix : args->pages.table + b * args->pages.table_row;
+  }
+  __device__ int entries() const { return b < 0 ? args->prefix_pages : args->pages.table_pages; }
+  // The key tiles of rows that see from lo_first on, up to hi_last at most: the
+  // window's begin at a multiple of `align`.  Returns how many there are.
+  __device__ __forceinline__ int place(int lo_first, int hi_last, int from, int to, int kt, int align) {
+    start = lo_first / align * align;
+    sink_end = min(args->sinks, hi_last);
+    if (args->sinks > start) start = sink_end = 0;
+    start = max(start, from), end = min(hi_last, to);
+    sink_start = from, sink_end = min(sink_end, to);
+    sink_tiles = max(sink_end - sink_start + kt - 1, 0) / kt;
+    return sink_tiles + max(end - start + kt - 1, 0) / kt;
+  }
+  // The first key of the window's first tile that a row sees (as a sink, or in
+  // its window): what lies before it in the tile is not read.
+  __device__ int first_seen(int lo_first) const {
+    return args->sinks > start ? start : max(start, min(lo_first, end - 1));
+  }
 };
+
+template <typename T>
+__device__ __forceinline__ PagedRows<T> paged_rows(const CacheArgs& a, const void* base, const PageStrides& at,
+                                                   const CacheWalk& w) {
+  return {static_cast<const T*>(base) + w.hk * at.head, at.page, at.row, w.table(), &a.pages};
+}
 
 // What 16-byte slot chunk c of row r of a V tile is stored in: the 16 lanes that
 // read b64 pieces of four rows, twice (16 bits), and the 64 that read words of
@@ -198,7 +255,7 @@ struct PagedStager {
   PageStrides k_at, v_at;
   const PageTable* pages;
   PageIds ids;
-  int dim, first, to;
+  int dim;
   bool whole_pages;  // tiles from multiples of KT on lie in one page
   uint32_t k_offset[ROUNDS], v_offset[ROUNDS];
 
@@ -208,10 +265,9 @@ struct PagedStager {
   __device__ static int v_chunk(int i) { return v_slot16<RB, !kIs16<T>>(slot(i) / CH, slot(i) % CH); }
   __device__ int there(int c) const { return c * kPer16<T> < dim ? c : 0; }
 
-  __device__ __forceinline__ void begin(const CacheArgs& a, int hk, const int32_t* table, int entries, int first_,
-                                        int to_) {
+  __device__ __forceinline__ void begin(const CacheArgs& a, int hk, const int32_t* table, int entries) {
     k = static_cast<const T*>(a.k) + hk * a.k_at.head, v = static_cast<const T*>(a.v) + hk * a.v_at.head;
-    k_at = a.k_at, v_at = a.v_at, pages = &a.pages, dim = a.dim, first = first_, to = to_;
+    k_at = a.k_at, v_at = a.v_at, pages = &a.pages, dim = a.dim;
     ids.begin(table, entries, a.pages.pages);
     whole_pages = a.pages.page_rows % KT == 0;
     if constexpr (ALIGNED) {
@@ -222,8 +278,8 @@ struct PagedStager {
       }
     }
   }
-  __device__ __forceinline__ void load(char* tile, int j0) {
-    const int j_first = max(j0, first), j_last = min(j0 + KT, to) - 1;
+  __device__ __forceinline__ void load(char* tile, int j0, int first, int to) {
+    const int j_first = first, j_last = min(j0 + KT, to) - 1;
     const int p_first = __builtin_amdgcn_readfirstlane(pages->page_of(j_first));
     ids.seek(p_first, __builtin_amdgcn_readfirstlane(pages->page_of(j_last)));
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(tile));
@@ -259,7 +315,7 @@ struct PagedStager {
   }
 };
 
-// Few query rows (16 NR) against many keys: the keys of a workgroup's chunk are
+// Few query rows (16 NR) against many keys (rows past the last are copies of it): the keys of a workgroup's chunk are
 // shared out over its waves, each with tiles of its own in LDS and no barrier
 // between them, and the waves' sums meet in LDS at the end.
 //
@@ -294,27 +350,13 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
   const bool is_prefix = blockIdx.x < prefix_blocks;
   const CacheCut& cut = is_prefix ? prefix : own;
   const int64_t id = is_prefix ? blockIdx.x : blockIdx.x - prefix_blocks;
-  CacheRows w;
+  const int split = static_cast<int>(id / cut.tiles / a.k_heads);
+  CacheWalk w;
   w.group = group;
   w.hk = static_cast<int>(id / cut.tiles % a.k_heads);
-  const int split = static_cast<int>(id / cut.tiles / a.k_heads);
-  int tile;
-  const int32_t* table;
-  if (is_prefix) {
-    int64_t last;
-    sample_rows(a, w.q0, last);
-    tile = static_cast<int>(id % cut.tiles);
-    w.rows = static_cast<uint32_t>((last - w.q0) * group);
-    if ((uint32_t)tile * ROWS >= w.rows) return;
-    w.b = -1, w.lq = w.lk = 0, w.from = 0, w.to = a.prefix_rows();
-    table = a.prefix;
-  } else {
-    if (!find_rows(a, group, ROWS, static_cast<int>(id % cut.tiles), w.b, w.q0, w.lq, tile)) return;
-    w.rows = static_cast<uint32_t>(w.lq) * group;
-    w.lk = kept(a, w.b), w.from = a.prefix_rows(), w.to = w.lk;
-    table = a.pages.table + w.b * a.pages.table_row;
-  }
-  const uint32_t row0 = static_cast<uint32_t>(tile) * ROWS;
+  int from, to;
+  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id % cut.tiles), from, to)) return;
+  const uint32_t row0 = w.row0;
 
   // rows past the last are copies of it
   int lo[NR], hi[NR], lo_min = kNoLimit, lo_max = 0, hi_min = kNoLimit, hi_max = 0;
@@ -333,14 +375,7 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
   lo_min = __builtin_amdgcn_readfirstlane(lo_min), lo_max = __builtin_amdgcn_readfirstlane(lo_max);
   hi_min = __builtin_amdgcn_readfirstlane(hi_min), hi_max = __builtin_amdgcn_readfirstlane(hi_max);
   // the window's tiles begin where pages of whole tiles have theirs
-  int start = lo_min;
-  if (a.pages.page_rows % KT == 0) start = start / KT * KT;
-  int sink_end = min(a.sinks, hi_max);
-  if (a.sinks > start) start = sink_end = 0;
-  start = max(start, w.from);
-  const int end = min(hi_max, w.to);
-  sink_end = min(sink_end, w.to);
-  const int sink_tiles = max(sink_end - w.from + KT - 1, 0) / KT, tiles = sink_tiles + max(end - start + KT - 1, 0) / KT;
+  const int tiles = w.place(lo_min, hi_max, from, to, KT, a.pages.page_rows % KT == 0 ? KT : 1);
   // this chunk's tiles, and this wave's
   const int chunk_tiles = cut.chunk / KT, c0 = min(split * (int64_t)chunk_tiles, (int64_t)tiles);
   const int c1 = split == cut.splits - 1 ? tiles : min(c0 + chunk_tiles, tiles), each = (c1 - c0 + WAVES - 1) / WAVES;
@@ -358,16 +393,13 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
   }
 
   Stager stager;
-  const int table_pages = is_prefix ? a.prefix_pages : a.pages.table_pages;
-  stager.begin(a, w.hk, table, table_pages, 0, 0);
+  stager.begin(a, w.hk, w.table(), w.entries());
   char* mine = lds + wave * kTileBuffers * TILE;
-  auto place = [&](int t) { return t < sink_tiles ? w.from + t * KT : start + (t - sink_tiles) * KT; };
+  auto place = [&](int t) { return t < w.sink_tiles ? w.sink_start + t * KT : w.start + (t - w.sink_tiles) * KT; };
+  const int first_seen = w.first_seen(lo_min);
   auto stage = [&](int t, int buf) {
-    const bool sinks = t < sink_tiles;
-    stager.first = sinks ? w.from : max(start, min(lo_min, end - 1));
-    if (!sinks && start == w.from) stager.first = start;
-    stager.to = sinks ? sink_end : end;
-    stager.load(mine + buf * TILE, place(t));
+    const int j0 = place(t);
+    stager.load(mine + buf * TILE, j0, t == w.sink_tiles ? first_seen : j0, t < w.sink_tiles ? w.sink_end : w.end);
   };
   if (t0 < t1) stage(t0, 0);
 
@@ -413,7 +445,7 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
     }
     const char* kt = mine + buf * TILE;
     const char* vt = kt + KT * RB;
-    const int j0 = place(t), last = t < sink_tiles ? sink_end : end;
+    const int j0 = place(t), last = t < w.sink_tiles ? w.sink_end : w.end;
     f32x4 s[NR][KB];
 #pragma unroll
     for (int x = 0; x < NR; ++x)
@@ -590,10 +622,10 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
     return;
   }
   // a value that is not finite, seen or not: key by key, of the seen ones only
-  PagedRows<T> kr{static_cast<const T*>(a.k) + w.hk * a.k_at.head, a.k_at.page, a.k_at.row, table, &a.pages};
-  PagedRows<T> vr{static_cast<const T*>(a.v) + w.hk * a.v_at.head, a.v_at.page, a.v_at.row, table, &a.pages};
-  const int s0 = min(w.from + c0 * KT, sink_end), s1 = min(w.from + c1 * KT, sink_end);
-  const int w0 = start + max(c0 - sink_tiles, 0) * KT, w1 = min(start + max(c1 - sink_tiles, 0) * KT, end);
+  const PagedRows<T> kr = paged_rows<T>(a, a.k, a.k_at, w), vr = paged_rows<T>(a, a.v, a.v_at, w);
+  const int s0 = min(w.sink_start + c0 * KT, w.sink_end), s1 = min(w.sink_start + c1 * KT, w.sink_end);
+  const int w0 = w.start + max(c0 - w.sink_tiles, 0) * KT;
+  const int w1 = min(w.start + max(c1 - w.sink_tiles, 0) * KT, w.end);
   float* q_s = reinterpret_cast<float*>(mine);
   for (int r = wave; r < ROWS && row0 + r < w.rows; r += WAVES) {
     int lo_r, hi_r, sink;
@@ -616,6 +648,123 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
   }
 }
 
+// Tiles of K and V for attend_walk, from pages.  Rows of a tile that no query sees
+// are those nearest to them again.
+template <typename T, int DP, int KB, int WAVES, bool ALIGNED>
+struct PagedTiles {
+  static constexpr int TILE = 32 * KB * DP * (int)sizeof(T), KT = 32 * KB;
+  using K = Stager<T, DP, KB, WAVES, ALIGNED, false>;
+  using V = Stager<T, DP, KB, WAVES, ALIGNED, true>;
+  // rows that a workgroup's instruction brings, or that share their offsets
+  static constexpr int UNIT = K::SAME ? K::THREADS / K::CH : KT;
+  K k;
+  V v;
+  const CacheArgs* args;
+  PageIds ids;
+  const int32_t* table;
+  int start, first;  // the window's first tile, and the first row of it that is seen
+  __device__ __forceinline__ void begin(const CacheArgs& a, const CacheWalk& w, int lo_first, int wave) {
+    args = &a, table = w.table();
+    k.begin(static_cast<const T*>(a.k) + w.hk * a.k_at.head, a.k_at.row, a.dim, wave);
+    v.begin(static_cast<const T*>(a.v) + w.hk * a.v_at.head, a.v_at.row, a.dim, wave);
+    ids.begin(table, w.entries(), a.pages.pages);
+    start = w.start, first = w.first_seen(lo_first);
+  }
+  __device__ __forceinline__ void clear(char* tile) const {
+    k.clear(tile);
+    v.clear(tile + TILE);
+  }
+  __device__ __forceinline__ void load(char* tile, int j0, int end) {
+    const PageTable& t = args->pages;
+    const int j_first = j0 == start ? first : j0, j_last = min(j0 + KT, end) - 1;
+    auto page_of = [&](int j) { return __builtin_amdgcn_readfirstlane(t.page_of(j)); };
+    ids.seek(page_of(j_first), page_of(j_last));
+    const uint32_t k_place = k.place(tile), v_place = v.place(tile + TILE);
+    if constexpr (ALIGNED)
+      if (t.page_rows % UNIT == 0 && j0 % UNIT == 0 && j_first == j0 && j_last == j0 + KT - 1 && k.dim >= DP) {
+        const T* kp = nullptr;
+        const T* vp = nullptr;
+#pragma unroll
+        for (int i = 0; i < K::ROUNDS; ++i) {
+          if (i == 0 || K::SAME) {
+            const int j = j0 + (K::SAME ? i * UNIT : 0), p = page_of(j);
+            const int64_t id = __builtin_amdgcn_readlane(ids.id, p - ids.from), r = j - p * t.page_rows;
+            kp = k.src + id * args->k_at.page + r * k.stride;
+            vp = v.src + id * args->v_at.page + r * v.stride;
+          }
+          load_to_lds(kp, k.offset[K::SAME ? 0 : i], k_place + i * WAVES * 1024);
+          load_to_lds(vp, v.offset[V::SAME ? 0 : i], v_place + i * WAVES * 1024);
+        }
+        return;
+      }
+#pragma unroll 2
+    for (int i = 0; i < K::ROUNDS; ++i) {
+      const int j = min(max(j0 + K::row(k.slot(i)), j_first), j_last), p = static_cast<int>(t.page_of(j));
+      const int64_t id = __shfl(ids.id, p - ids.from, kWave), r = j - p * t.page_rows;
+      const T* kp = k.src + id * args->k_at.page + r * k.stride;
+      const T* vp = v.src + id * args->v_at.page + r * v.stride;
+      if constexpr (ALIGNED) {
+        if (k.in(i)) load_to_lds_from(kp + K::chunk(k.slot(i)) * kPer16<T>, k_place + i * WAVES * 1024);
+        if (v.in(i)) load_to_lds_from(vp + V::chunk(v.slot(i)) * kPer16<T>, v_place + i * WAVES * 1024);
+      } else {
+        k.load_chunk(tile, kp, i);
+        v.load_chunk(tile + TILE, vp, i);
+      }
+    }
+  }
+  __device__ PagedRows<T> k_rows() const { return {k.src, args->k_at.page, k.stride, table, &args->pages}; }
+  __device__ PagedRows<T> v_rows() const { return {v.src, args->v_at.page, v.stride, table, &args->pages}; }
+};
+
+// Many query rows: attend_walk's tiles, over pages.
+template <typename T, int DP, int RB, int KB, bool ALIGNED>
+__global__ void __launch_bounds__(kWave * 4, waves_per_simd<T>(DP, RB, 4))
+    cache_tile_kernel(CacheArgs a, CacheCut cut, int is_prefix, int splits) {
+  constexpr int ROWS = 32 * RB * 4, KT = 32 * KB;
+  using Tiles = PagedTiles<T, DP, KB, 4, ALIGNED>;
+  extern __shared__ __align__(16) char lds[];  // as attend_kernel's
+  if (splits == 1) {  // (the join does it otherwise)
+    int64_t first, last;
+    sample_rows(a, first, last);
+    if (first > 0 || last < a.n_q)
+      zero_outside(static_cast<T*>(a.out), (int64_t)a.q_heads * a.dim, first, last, a.n_q);
+  }
+  // tiles of one head next to each other on one XCD, as in attend_kernel
+  const int64_t blocks = cut.tiles * a.k_heads * cut.splits, per = (blocks + 7) / 8;
+  const int64_t id = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  if (blockIdx.x / 8 >= per || id >= blocks) return;
+  CacheWalk w;
+  w.group = a.q_heads / a.k_heads;
+  w.hk = static_cast<int>(id / cut.splits / cut.tiles);
+  int from, to;
+  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id / cut.splits % cut.tiles), from, to)) return;
+  int lo_first, hi_first, lo_last, hi_last;
+  w.bounds(a, w.row0, w.row0 + ROWS - 1, lo_first, hi_first, lo_last, hi_last);
+  const int tiles = w.place(lo_first, hi_last, from, to, KT, a.pages.page_rows % Tiles::UNIT == 0 ? KT : 1);
+  const int split = static_cast<int>(id % cut.splits), each = (tiles + cut.splits - 1) / cut.splits;
+  w.t0 = min(split * each, tiles);
+  w.t1 = min(w.t0 + each, tiles);
+  w.split = cut.first_split + split;
+  w.splits = splits;
+  Tiles kv;
+  kv.begin(a, w, lo_first, __builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+  attend_walk<T, DP, RB, KB, 4>(a, w, kv, lds);
+}
+
+template <typename T, int DP, int RB, bool ALIGNED>
+int launch_many(const CacheArgs& a, const CacheCut& c, bool is_prefix, int splits, hipStream_t s) {
+  constexpr int KB = key_blocks<T>(DP);
+  constexpr int bytes = tile_buffers<T>(DP, 4) * 2 * 32 * KB * DP * (int)sizeof(T) + 4 * DP * 4 + KB * 4;
+  auto kernel = &cache_tile_kernel<T, DP, RB, KB, ALIGNED>;
+  if (bytes > 65536)
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  const int64_t blocks = align_up(c.tiles * a.k_heads * c.splits, 8);
+  TSC_REQUIRE(blocks * kWave * 4 < (1ll << 32), "cache_attention: too many tiles");
+  kernel<<<static_cast<unsigned>(blocks), kWave * 4, bytes, s>>>(a, c, is_prefix, splits);
+  TSC_LAUNCH_CHECK("cache_attention");
+  return 0;
+}
+
 template <typename T, int DP, int NR, bool ALIGNED>
 int launch_few(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
   constexpr int RB = DP * sizeof(T), WAVES = cache_waves(RB);
@@ -623,15 +772,25 @@ int launch_few(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
   auto kernel = &cache_few_kernel<T, DP, NR, ALIGNED>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
-  const int64_t blocks = (p.prefix.tiles * p.prefix.splits + p.own.tiles * p.own.splits) * a.k_heads;
+  const CacheCut prefix = p.prefix.wave_rows ? CacheCut{} : p.prefix, own = p.own.wave_rows ? CacheCut{} : p.own;
+  const int64_t blocks = (prefix.tiles * prefix.splits + own.tiles * own.splits) * a.k_heads;
+  if (!blocks) return 0;
   TSC_REQUIRE(blocks * kWave * WAVES < (1ll << 32), "cache_attention: too many tiles");
-  kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, p.prefix, p.own, p.splits());
+  kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, prefix, own, p.splits());
   TSC_LAUNCH_CHECK("cache_attention");
   return 0;
 }
 
 template <typename T, int DP, bool ALIGNED>
 int launch_rows(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
+  for (const CacheCut* c : {&p.prefix, &p.own}) {
+    if (!c->splits || !c->wave_rows) continue;
+    int rc = 0;
+    if constexpr (can_pair(DP, sizeof(T)))
+      if (c->wave_rows == 2) rc = launch_many<T, DP, 2, ALIGNED>(a, *c, c == &p.prefix, p.splits(), s);
+    if (c->wave_rows == 1) rc = launch_many<T, DP, 1, ALIGNED>(a, *c, c == &p.prefix, p.splits(), s);
+    if (rc) return rc;
+  }
   constexpr int MOST = cache_row_blocks(DP * sizeof(T));
   if constexpr (MOST >= 4)
     if (p.row_blocks == 4) return launch_few<T, DP, 4, ALIGNED>(a, p, s);
