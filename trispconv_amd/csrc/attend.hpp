@@ -234,11 +234,7 @@ struct Stager {
     if constexpr (ALIGNED) {
       const T* base = src + j0 * stride;
       if (j0 + 32 * KB <= end && dim >= DP) {
-#pragma unroll
-        for (int i = 0; i < ROUNDS; ++i) {
-          if (SAME) load_to_lds(base + i * (THREADS / CH) * stride, offset[0], at + i * WAVES * 1024);
-          else load_to_lds(base, offset[SAME ? 0 : i], at + i * WAVES * 1024);
-        }
+        load_whole(at, base);
       } else {
 #pragma unroll 2
         for (int i = 0; i < ROUNDS; ++i) {
@@ -252,6 +248,14 @@ struct Stager {
       for (int i = 0; i < ROUNDS; ++i) {
         load_chunk(tile, src + min(j0 + row(slot(i)), end - 1) * stride, i);
       }
+    }
+  }
+  // A tile whose rows are `stride` elements apart from base on.
+  __device__ __forceinline__ void load_whole(uint32_t at, const T* base) const {
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      if (SAME) load_to_lds(base + i * (THREADS / CH) * stride, offset[0], at + i * WAVES * 1024);
+      else load_to_lds(base, offset[SAME ? 0 : i], at + i * WAVES * 1024);
     }
   }
   // Round i's chunk of a row at any address, through registers.
@@ -373,6 +377,15 @@ struct Walk {
     seen(a, first, lo_first, hi_first, none);
     seen(a, last, lo_last, hi_last, none);
   }
+  // Both for a wave of N blocks of STEP rows, a lane of which has row `col` of each.
+  template <int N, int STEP>
+  __device__ __forceinline__ void wave(const AttendArgs& a, uint32_t first, int col, int lo[N], int hi[N],
+                                       int& lo_first, int& hi_first, int& lo_last, int& hi_last) const {
+    bounds(a, first, first + N * STEP - 1, lo_first, hi_first, lo_last, hi_last);
+    int none;
+#pragma unroll
+    for (int x = 0; x < N; ++x) seen(a, first + x * STEP + col, lo[x], hi[x], none);
+  }
 };
 
 // The weight of a key at its row's reference score (in log2), and what a lane's 16
@@ -425,16 +438,14 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, 
   constexpr int BUFFERS = tile_buffers<T>(DP, WAVES), TILE = KT * ROW_BYTES, STEPS = DP * (int)sizeof(T) / 32, DB = DP / 32;
   const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  int lo_first, hi_first, lo_last, hi_last, none;
   const uint32_t wave_row = w.row0 + wave * 32 * RB;
-  w.bounds(a, wave_row, wave_row + 32 * RB - 1, lo_first, hi_first, lo_last, hi_last);
-  int lo[RB], hi[RB];
+  int lo[RB], hi[RB], lo_first, hi_first, lo_last, hi_last;
+  w.template wave<RB, 32>(a, wave_row, col, lo, hi, lo_first, hi_first, lo_last, hi_last);
   int4v qf[RB][STEPS];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const uint32_t r = wave_row + rb * 32 + col;
     const int t = w.token(r), g = static_cast<int>(min(r, w.rows - 1) - static_cast<uint32_t>(t) * w.group);
-    w.seen(a, r, lo[rb], hi[rb], none);
     if (r >= w.rows) hi[rb] = 0;
     const T* q = static_cast<const T*>(a.q) + (w.q0 + t) * a.q_row + (w.hk * w.group + g) * a.q_head;
 #pragma unroll

@@ -27,20 +27,31 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     CacheCut c;
     auto tiles = [&](int64_t rows) { return all / rows + std::min(lists, n_q); };
     if (sinks > 0) keys += kt;  // (a tile of their own)
+    // workgroups that do something, and those that the CUs hold at once
+    auto units = [&](int64_t rows) { return std::max<int64_t>(1, lists * ceil_div(mean, rows)) * k_heads; };
     if (mean <= 64) {
-      c.tiles = tiles(16 * p.row_blocks);
-      // about four workgroups per CU, of 256 keys and more
-      const int64_t most = std::max<int64_t>(1, 4 * kCus / std::max<int64_t>(1, c.tiles * k_heads));
-      const int64_t least = std::max<int64_t>(256, ceil_div(keys, std::min<int64_t>(most, kMostSplits / 2)));
-      c.chunk = static_cast<int>(align_up(std::min<int64_t>(least, 1ll << 30), 4 * kt));
+      const int64_t rows = 16 * p.row_blocks;
+      c.tiles = tiles(rows);
+      // Parts of 256 to 2048 keys, one round of workgroups where that allows it: 64
+      // samples of up to 32k keys in parts of 2048 288 us, of 512 361, of 8192
+      // 291; 24 windows of 4096 in one round of 1024 28 us, in two of 768 33.
+      // Up to 1024 keys by themselves are not worth a join (14 us, in parts 17).
+      const int64_t want = std::max<int64_t>(1, cache_per_cu(row_bytes) * kCus / units(rows));
+      int64_t chunk = std::min<int64_t>(std::max<int64_t>(ceil_div(keys, want), 256), 2048);
+      if (!prefix_rows && keys <= 1024) chunk = keys;
+      chunk = std::max(chunk, ceil_div(keys, kMostSplits / 2));
+      c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), 4 * kt));
       c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
       return c;
     }
     // as attend_cut
-    c.wave_rows = can_pair(padded_dim(dim), elem) && keys >= 4096 && tiles(256) * k_heads >= 2 * kCus ? 2 : 1;
+    c.wave_rows = can_pair(padded_dim(dim), elem) && keys >= 4096 && units(256) >= 2 * kCus ? 2 : 1;
+    const int64_t work = units(128 * c.wave_rows);
     c.tiles = tiles(128 * c.wave_rows);
-    c.splits = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>({keys / 256, 4 * kCus / (c.tiles * k_heads), kMostSplits / 2})));
+    // One round of workgroups, of 256 keys and more (20k keys in 136 tiles, four
+    // workgroups a CU: 165 us in seven parts, 193 in four, 224 in three)
+    const int64_t slots = kCus * (row_bytes <= 128 ? 4 / c.wave_rows : row_bytes <= 256 ? 2 : 1);
+    c.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({keys / 256, slots / work, kMostSplits / 2})));
     return c;
   };
   // keys that a tile of a sample's rows can see at most

@@ -44,6 +44,10 @@ int launch_cache(const CacheArgs& a, const CachePlan& p, hipStream_t s);
 // Keys of a wave's tile, and waves of a workgroup: what the LDS has room for.
 constexpr int cache_keys(int row_bytes) { return row_bytes <= 512 ? 32 : 16; }
 constexpr int cache_waves(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
+// Workgroups of the form for few rows that a CU holds: what they have in LDS.
+constexpr int cache_per_cu(int row_bytes) {
+  return (160 << 10) / (cache_waves(row_bytes) * (4 * cache_keys(row_bytes) * row_bytes + 512));
+}
 // Rows of a tile in 16s at most: queries and sums stay in the registers.
 constexpr int cache_row_blocks(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
 
@@ -111,18 +115,6 @@ __device__ __forceinline__ int kept(const CacheArgs& a, int b) {
   return static_cast<int>(min(max((int64_t)a.pages.lengths[b], (int64_t)0), a.pages.most()));
 }
 
-// The sample of query row t (the last whose offset is not behind it); t is one
-// of the rows from the first sample's to the last one's.
-__device__ __forceinline__ int sample_of(const CacheArgs& a, int64_t t) {
-  int lo = 0, hi = a.samples;  // offsets up to t: [0, lo) are, [hi, ...) are not
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.off_q[mid] <= t) lo = mid + 1;
-    else hi = mid;
-  }
-  return max(lo - 1, 0);
-}
-
 // The sample and the tile of query rows within it of the x-th tile of all (as
 // find_tile).  false: past the last.
 __device__ __forceinline__ bool find_rows(const CacheArgs& a, int group, int rows, int x, int& b, int64_t& q0,
@@ -159,29 +151,70 @@ struct CacheWalk : Walk {
     int p = token(r) + shift, keys = lk;
     if (b < 0) {
       const int64_t t = q0 + token(r);
-      const int s = sample_of(*args, t);
+      const int s = first_past(a, t);
       keys = kept(*args, s);
-      p = static_cast<int>(max(t - a.off_q[s + 1] + keys, -(int64_t)(1 << 30)));
+      p = position(t, a.off_q[s + 1], keys);
     }
     seen_keys(p, keys, a.left, a.right, a.sinks, lo, hi, sink);
   }
-  __device__ __forceinline__ void bounds(const AttendArgs& a, uint32_t first, uint32_t last, int& lo_first,
-                                         int& hi_first, int& lo_last, int& hi_last) const {
-    if (b >= 0) return Walk::bounds(a, first, last, lo_first, hi_first, lo_last, hi_last);
-    lo_first = hi_first = kNoLimit, lo_last = hi_last = 0;
-    for (uint32_t r = first + threadIdx.x % kWave; r <= last; r += kWave) {
-      int lo, hi, sink;
-      seen(a, r, lo, hi, sink);
-      lo_first = min(lo_first, lo), lo_last = max(lo_last, lo);
-      hi_first = min(hi_first, hi), hi_last = max(hi_last, hi);
+  template <int N, int STEP>
+  __device__ __forceinline__ void wave(const AttendArgs& a, uint32_t first, int col, int lo[N], int hi[N],
+                                       int& lo_first, int& hi_first, int& lo_last, int& hi_last) const {
+    if (b >= 0) return Walk::wave<N, STEP>(a, first, col, lo, hi, lo_first, hi_first, lo_last, hi_last);
+    // the sample of the first row, then how many samples' ends each row is past
+    const int lane = threadIdx.x % kWave;
+    const int64_t t_last = q0 + token(first + N * STEP - 1);
+    int s = first_past(a, q0 + token(first));
+    int at[N], next[N];
+    int64_t t[N];
+#pragma unroll
+    for (int x = 0; x < N; ++x) t[x] = q0 + token(first + x * STEP + col), at[x] = s;
+    for (;; s += kWave) {
+      const int ends = a.off_q[min(s + lane, a.samples - 1) + 1];
+      int k = 0;
+      for (; k < kWave && s + k < a.samples - 1; ++k) {
+        const int e = __builtin_amdgcn_readlane(ends, k);
+        if (e > t_last) break;
+#pragma unroll
+        for (int x = 0; x < N; ++x) at[x] += t[x] >= e;
+      }
+      if (k < kWave) break;
     }
 #pragma unroll
-    for (int x = 1; x < kWave; x <<= 1) {
+    for (int x = 0; x < N; ++x) next[x] = a.off_q[at[x] + 1];
+    lo_first = hi_first = kNoLimit, lo_last = hi_last = 0;
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const int keys = kept(*args, at[x]);
+      int sink;
+      seen_keys(position(t[x], next[x], keys), keys, a.left, a.right, a.sinks, lo[x], hi[x], sink);
+      lo_first = min(lo_first, lo[x]), lo_last = max(lo_last, lo[x]);
+      hi_first = min(hi_first, hi[x]), hi_last = max(hi_last, hi[x]);
+    }
+#pragma unroll
+    for (int x = 1; x < STEP; x <<= 1) {
       lo_first = min(lo_first, __shfl_xor(lo_first, x, kWave)), lo_last = max(lo_last, __shfl_xor(lo_last, x, kWave));
       hi_first = min(hi_first, __shfl_xor(hi_first, x, kWave)), hi_last = max(hi_last, __shfl_xor(hi_last, x, kWave));
     }
     lo_first = __builtin_amdgcn_readfirstlane(lo_first), lo_last = __builtin_amdgcn_readfirstlane(lo_last);
     hi_first = __builtin_amdgcn_readfirstlane(hi_first), hi_last = __builtin_amdgcn_readfirstlane(hi_last);
+  }
+  __device__ static __forceinline__ int position(int64_t t, int end, int keys) {
+    return static_cast<int>(max(t - end + keys, -(int64_t)(1 << 30)));
+  }
+  // The first sample (the last at most) whose end is past row t, by the whole wave.
+  __device__ static __forceinline__ int first_past(const AttendArgs& a, int64_t t) {
+    int from = 0, n = a.samples;
+    while (n > 1) {
+      const int step = (n + kWave - 1) / kWave, lane = threadIdx.x % kWave;
+      const int s = min(from + (lane + 1) * step, from + n) - 1;  // the last of the lane's
+      const uint64_t past = __ballot(a.off_q[s + 1] > t);
+      const int l = past ? __builtin_ctzll(past) : kWave - 1;
+      const int next = min(from + l * step, from + n - 1);
+      n = min(step, from + n - next);
+      from = next;
+    }
+    return from;
   }
   // Takes the x-th tile of `tile_rows` rows (the prefix's: of all samples) and the
   // range of keys [from, to) of this part.  false: past the last tile.
@@ -359,21 +392,8 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
   const uint32_t row0 = w.row0;
 
   // rows past the last are copies of it
-  int lo[NR], hi[NR], lo_min = kNoLimit, lo_max = 0, hi_min = kNoLimit, hi_max = 0;
-#pragma unroll
-  for (int x = 0; x < NR; ++x) {
-    int sink;
-    w.seen(a, row0 + 16 * x + col, lo[x], hi[x], sink);
-    lo_min = min(lo_min, lo[x]), lo_max = max(lo_max, lo[x]);
-    hi_min = min(hi_min, hi[x]), hi_max = max(hi_max, hi[x]);
-  }
-#pragma unroll
-  for (int x = 1; x < 16; x <<= 1) {
-    lo_min = min(lo_min, __shfl_xor(lo_min, x, kWave)), lo_max = max(lo_max, __shfl_xor(lo_max, x, kWave));
-    hi_min = min(hi_min, __shfl_xor(hi_min, x, kWave)), hi_max = max(hi_max, __shfl_xor(hi_max, x, kWave));
-  }
-  lo_min = __builtin_amdgcn_readfirstlane(lo_min), lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-  hi_min = __builtin_amdgcn_readfirstlane(hi_min), hi_max = __builtin_amdgcn_readfirstlane(hi_max);
+  int lo[NR], hi[NR], lo_min, hi_min, lo_max, hi_max;
+  w.template wave<NR, 16>(a, row0, col, lo, hi, lo_min, hi_min, lo_max, hi_max);
   // the window's tiles begin where pages of whole tiles have theirs
   const int tiles = w.place(lo_min, hi_max, from, to, KT, a.pages.page_rows % KT == 0 ? KT : 1);
   // this chunk's tiles, and this wave's
@@ -655,7 +675,7 @@ struct PagedTiles {
   static constexpr int TILE = 32 * KB * DP * (int)sizeof(T), KT = 32 * KB;
   using K = Stager<T, DP, KB, WAVES, ALIGNED, false>;
   using V = Stager<T, DP, KB, WAVES, ALIGNED, true>;
-  // rows that a workgroup's instruction brings, or that share their offsets
+  // rows that an instruction of the workgroup brings
   static constexpr int UNIT = K::SAME ? K::THREADS / K::CH : KT;
   K k;
   V v;
@@ -678,25 +698,36 @@ struct PagedTiles {
     const PageTable& t = args->pages;
     const int j_first = j0 == start ? first : j0, j_last = min(j0 + KT, end) - 1;
     auto page_of = [&](int j) { return __builtin_amdgcn_readfirstlane(t.page_of(j)); };
-    ids.seek(page_of(j_first), page_of(j_last));
+    const int p_first = page_of(j_first), p_last = page_of(j_last);
+    ids.seek(p_first, p_last);
     const uint32_t k_place = k.place(tile), v_place = v.place(tile + TILE);
-    if constexpr (ALIGNED)
-      if (t.page_rows % UNIT == 0 && j0 % UNIT == 0 && j_first == j0 && j_last == j0 + KT - 1 && k.dim >= DP) {
-        const T* kp = nullptr;
-        const T* vp = nullptr;
-#pragma unroll
-        for (int i = 0; i < K::ROUNDS; ++i) {
-          if (i == 0 || K::SAME) {
-            const int j = j0 + (K::SAME ? i * UNIT : 0), p = page_of(j);
-            const int64_t id = __builtin_amdgcn_readlane(ids.id, p - ids.from), r = j - p * t.page_rows;
-            kp = k.src + id * args->k_at.page + r * k.stride;
-            vp = v.src + id * args->v_at.page + r * v.stride;
-          }
-          load_to_lds(kp, k.offset[K::SAME ? 0 : i], k_place + i * WAVES * 1024);
-          load_to_lds(vp, v.offset[V::SAME ? 0 : i], v_place + i * WAVES * 1024);
-        }
+    if (ALIGNED && j_first == j0 && j_last == j0 + KT - 1 && k.dim >= DP) {
+      auto row_at = [&](int j, int p, const T*& kp, const T*& vp) {
+        const int64_t id = __builtin_amdgcn_readlane(ids.id, p - ids.from), r = j - p * t.page_rows;
+        kp = k.src + id * args->k_at.page + r * k.stride;
+        vp = v.src + id * args->v_at.page + r * v.stride;
+      };
+      if (p_first == p_last) {
+        const T* kp;
+        const T* vp;
+        row_at(j0, p_first, kp, vp);
+        k.load_whole(k_place, kp);
+        v.load_whole(v_place, vp);
         return;
       }
+      if constexpr (K::SAME)
+        if (t.page_rows % UNIT == 0 && j0 % UNIT == 0) {
+#pragma unroll
+          for (int i = 0; i < K::ROUNDS; ++i) {
+            const T* kp;
+            const T* vp;
+            row_at(j0 + i * UNIT, page_of(j0 + i * UNIT), kp, vp);
+            load_to_lds(kp, k.offset[0], k_place + i * WAVES * 1024);
+            load_to_lds(vp, v.offset[0], v_place + i * WAVES * 1024);
+          }
+          return;
+        }
+    }
 #pragma unroll 2
     for (int i = 0; i < K::ROUNDS; ++i) {
       const int j = min(max(j0 + K::row(k.slot(i)), j_first), j_last), p = static_cast<int>(t.page_of(j));
@@ -738,8 +769,9 @@ __global__ void __launch_bounds__(kWave * 4, waves_per_simd<T>(DP, RB, 4))
   w.hk = static_cast<int>(id / cut.splits / cut.tiles);
   int from, to;
   if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id / cut.splits % cut.tiles), from, to)) return;
-  int lo_first, hi_first, lo_last, hi_last;
-  w.bounds(a, w.row0, w.row0 + ROWS - 1, lo_first, hi_first, lo_last, hi_last);
+  int lo_first = 0, hi_first, lo_last, hi_last = to;
+  // (the rows of all samples: every key of the prefix, most of them see it whole)
+  if (!is_prefix) w.bounds(a, w.row0, w.row0 + ROWS - 1, lo_first, hi_first, lo_last, hi_last);
   const int tiles = w.place(lo_first, hi_last, from, to, KT, a.pages.page_rows % Tiles::UNIT == 0 ? KT : 1);
   const int split = static_cast<int>(id % cut.splits), each = (tiles + cut.splits - 1) / cut.splits;
   w.t0 = min(split * each, tiles);
