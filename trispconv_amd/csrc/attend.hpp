@@ -706,9 +706,16 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, 
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int d = 32 * db + 8 * (i / 4) + 4 * half + i % 4;
-            if (d < a.dim) part[d] = o[rb][db][i];
+          for (int i = 0; i < 4; ++i) {
+            const int d = 32 * db + 8 * i + 4 * half;
+            const f32x4 x = {o[rb][db][4 * i], o[rb][db][4 * i + 1], o[rb][db][4 * i + 2], o[rb][db][4 * i + 3]};
+            if (d + 4 <= a.dim) {
+              __builtin_memcpy(part + d, &x, 16);
+            } else {
+#pragma unroll
+              for (int y = 0; y < 3; ++y)
+                if (d + y < a.dim) part[d + y] = x[y];
+            }
           }
       } else {
         T* out = static_cast<T*>(a.out) + item * a.dim;

@@ -25,7 +25,7 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
   // lists: of the rows that `tiles` are cut from; mean: rows of such a list
   auto cut = [&](int64_t keys, int64_t lists, int64_t mean) {
     CacheCut c;
-    auto tiles = [&](int64_t rows) { return all / rows + std::min(lists, n_q); };
+    auto tiles = [&](int64_t rows) { return lists == 1 ? ceil_div(all, rows) : all / rows + std::min(lists, n_q); };
     if (sinks > 0) keys += kt;  // (a tile of their own)
     // workgroups that do something, and those that the CUs hold at once
     auto units = [&](int64_t rows) { return std::max<int64_t>(1, lists * ceil_div(mean, rows)) * k_heads; };
@@ -48,10 +48,11 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     c.wave_rows = can_pair(padded_dim(dim), elem) && keys >= 4096 && units(256) >= 2 * kCus ? 2 : 1;
     const int64_t work = units(128 * c.wave_rows);
     c.tiles = tiles(128 * c.wave_rows);
-    // One round of workgroups, of 256 keys and more (20k keys in 136 tiles, four
-    // workgroups a CU: 165 us in seven parts, 193 in four, 224 in three)
+    // One round of workgroups, of 512 keys and more (20k keys in 136 tiles, four
+    // workgroups a CU: 151 us in seven parts, 166 in six, 239 in three; a prefix of
+    // 32k keys in 8 tiles: 50 us in 64 parts, 57 in 128 and 67 in 32)
     const int64_t slots = kCus * (row_bytes <= 128 ? 4 / c.wave_rows : row_bytes <= 256 ? 2 : 1);
-    c.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({keys / 256, slots / work, kMostSplits / 2})));
+    c.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({keys / 512, slots / work, kMostSplits / 2})));
     return c;
   };
   // keys that a tile of a sample's rows can see at most

@@ -118,12 +118,15 @@ __device__ __forceinline__ int kept(const CacheArgs& a, int b) {
 // The sample and the tile of query rows within it of the x-th tile of all (as
 // find_tile).  false: past the last.
 __device__ __forceinline__ bool find_rows(const CacheArgs& a, int group, int rows, int x, int& b, int64_t& q0,
-                                          int& lq, int& tile) {
+                                          int& lq, int& lk, int& tile) {
   const int lane = threadIdx.x % kWave;
   for (int b0 = 0; b0 < a.samples; b0 += kWave) {
     int64_t at = 0;
-    int len = 0;
-    if (b0 + lane < a.samples) sample_range(a.off_q, b0 + lane, a.n_q, at, len);
+    int len = 0, keys = 0;
+    if (b0 + lane < a.samples) {
+      sample_range(a.off_q, b0 + lane, a.n_q, at, len);
+      keys = kept(a, b0 + lane);
+    }
     const uint32_t tiles = static_cast<uint32_t>(((int64_t)len * group + rows - 1) / rows);
     const uint32_t inc = wave_inclusive(tiles);
     const uint64_t past = __ballot(inc > static_cast<uint32_t>(x));
@@ -132,6 +135,7 @@ __device__ __forceinline__ bool find_rows(const CacheArgs& a, int group, int row
       b = b0 + at_lane;
       tile = x - __builtin_amdgcn_readlane(inc - tiles, at_lane);
       lq = __builtin_amdgcn_readlane(len, at_lane);
+      lk = __builtin_amdgcn_readlane(keys, at_lane);
       q0 = __builtin_amdgcn_readlane(static_cast<int>(at), at_lane);
       return true;
     }
@@ -164,13 +168,15 @@ struct CacheWalk : Walk {
     // the sample of the first row, then how many samples' ends each row is past
     const int lane = threadIdx.x % kWave;
     const int64_t t_last = q0 + token(first + N * STEP - 1);
-    int s = first_past(a, q0 + token(first));
-    int at[N], next[N];
+    const int s0 = a.samples <= kWave ? 0 : first_past(a, q0 + token(first));
+    int at[N], next[N], keys[N];
     int64_t t[N];
 #pragma unroll
-    for (int x = 0; x < N; ++x) t[x] = q0 + token(first + x * STEP + col), at[x] = s;
-    for (;; s += kWave) {
-      const int ends = a.off_q[min(s + lane, a.samples - 1) + 1];
+    for (int x = 0; x < N; ++x) t[x] = q0 + token(first + x * STEP + col), at[x] = s0;
+    const int mine = min(s0 + lane, a.samples - 1);
+    int ends = a.off_q[mine + 1], s = s0;
+    const int kept_mine = kept(*args, mine);
+    for (;;) {
       int k = 0;
       for (; k < kWave && s + k < a.samples - 1; ++k) {
         const int e = __builtin_amdgcn_readlane(ends, k);
@@ -179,15 +185,19 @@ struct CacheWalk : Walk {
         for (int x = 0; x < N; ++x) at[x] += t[x] >= e;
       }
       if (k < kWave) break;
+      s += kWave;
+      ends = a.off_q[min(s + lane, a.samples - 1) + 1];
     }
 #pragma unroll
-    for (int x = 0; x < N; ++x) next[x] = a.off_q[at[x] + 1];
+    for (int x = 0; x < N; ++x) {
+      next[x] = s == s0 ? __shfl(ends, at[x] - s0, kWave) : a.off_q[at[x] + 1];
+      keys[x] = s == s0 ? __shfl(kept_mine, at[x] - s0, kWave) : kept(*args, at[x]);
+    }
     lo_first = hi_first = kNoLimit, lo_last = hi_last = 0;
 #pragma unroll
     for (int x = 0; x < N; ++x) {
-      const int keys = kept(*args, at[x]);
       int sink;
-      seen_keys(position(t[x], next[x], keys), keys, a.left, a.right, a.sinks, lo[x], hi[x], sink);
+      seen_keys(position(t[x], next[x], keys[x]), keys[x], a.left, a.right, a.sinks, lo[x], hi[x], sink);
       lo_first = min(lo_first, lo[x]), lo_last = max(lo_last, lo[x]);
       hi_first = min(hi_first, hi[x]), hi_last = max(hi_last, hi[x]);
     }
@@ -229,9 +239,9 @@ struct CacheWalk : Walk {
       if ((int64_t)tile * tile_rows >= rows) return false;
     } else {
       int lq;
-      if (!find_rows(a, group, tile_rows, x, b, q0, lq, tile)) return false;
+      if (!find_rows(a, group, tile_rows, x, b, q0, lq, lk, tile)) return false;
       rows = static_cast<uint32_t>(lq) * group;
-      lk = kept(a, b), shift = lk - lq, from = a.prefix_rows(), to = lk;
+      shift = lk - lq, from = a.prefix_rows(), to = lk;
     }
     row0 = static_cast<uint32_t>(tile) * tile_rows;
     return true;
@@ -760,20 +770,21 @@ __global__ void __launch_bounds__(kWave * 4, waves_per_simd<T>(DP, RB, 4))
     if (first > 0 || last < a.n_q)
       zero_outside(static_cast<T*>(a.out), (int64_t)a.q_heads * a.dim, first, last, a.n_q);
   }
-  // tiles of one head next to each other on one XCD, as in attend_kernel
+  // tiles that walk the same keys next to each other on one XCD (workgroups go
+  // round the eight in turn), so that its L2 reads them once
   const int64_t blocks = cut.tiles * a.k_heads * cut.splits, per = (blocks + 7) / 8;
   const int64_t id = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (blockIdx.x / 8 >= per || id >= blocks) return;
   CacheWalk w;
   w.group = a.q_heads / a.k_heads;
-  w.hk = static_cast<int>(id / cut.splits / cut.tiles);
+  w.hk = static_cast<int>(id / cut.tiles / cut.splits);
   int from, to;
-  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id / cut.splits % cut.tiles), from, to)) return;
+  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id % cut.tiles), from, to)) return;
   int lo_first = 0, hi_first, lo_last, hi_last = to;
   // (the rows of all samples: every key of the prefix, most of them see it whole)
   if (!is_prefix) w.bounds(a, w.row0, w.row0 + ROWS - 1, lo_first, hi_first, lo_last, hi_last);
   const int tiles = w.place(lo_first, hi_last, from, to, KT, a.pages.page_rows % Tiles::UNIT == 0 ? KT : 1);
-  const int split = static_cast<int>(id % cut.splits), each = (tiles + cut.splits - 1) / cut.splits;
+  const int split = static_cast<int>(id / cut.tiles % cut.splits), each = (tiles + cut.splits - 1) / cut.splits;
   w.t0 = min(split * each, tiles);
   w.t1 = min(w.t0 + each, tiles);
   w.split = cut.first_split + split;
