@@ -32,15 +32,17 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     if (mean <= 64) {
       const int64_t rows = 16 * p.row_blocks;
       c.tiles = tiles(rows);
-      // Parts of 256 to 2048 keys, one round of workgroups where that allows it: 64
-      // samples of up to 32k keys in parts of 2048 288 us, of 512 361, of 8192
-      // 291; 24 windows of 4096 in one round of 1024 28 us, in two of 768 33.
-      // Up to 1024 keys by themselves are not worth a join (14 us, in parts 17).
-      const int64_t want = std::max<int64_t>(1, cache_per_cu(row_bytes) * kCus / units(rows));
-      int64_t chunk = std::min<int64_t>(std::max<int64_t>(ceil_div(keys, want), 256), 2048);
+      // Parts of 256 to 2048 keys (4096 where a workgroup has a CU to itself), one
+      // round of workgroups where that allows it: 64 samples of up to 32k keys in
+      // parts of 2048 276 us, of 512 321, of 8192 295; 24 windows of 4096 in one
+      // round of 1024 27 us, in two of 768 30.  Up to 1024 keys by themselves are
+      // not worth a join (14 us, in parts 17).
+      const int per_cu = cache_per_cu(row_bytes);
+      const int64_t want = std::max<int64_t>(1, per_cu * kCus / units(rows));
+      int64_t chunk = std::min<int64_t>(std::max<int64_t>(ceil_div(keys, want), 256), 4096 / per_cu);
       if (!prefix_rows && keys <= 1024) chunk = keys;
       chunk = std::max(chunk, ceil_div(keys, kMostSplits / 2));
-      c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), 4 * kt));
+      c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), kt * cache_waves(row_bytes, p.row_blocks)));
       c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
       return c;
     }

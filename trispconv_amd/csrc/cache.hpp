@@ -41,19 +41,28 @@ struct CachePlan {
 template <typename T>
 int launch_cache(const CacheArgs& a, const CachePlan& p, hipStream_t s);
 
-// Keys of a wave's tile, and waves of a workgroup: what the LDS has room for.
+// The form for few rows: keys of a wave's tile, waves of a workgroup and the
+// tiles of K and V that each has in LDS, one in use and the others on their way.
+// Two workgroups share a CU's LDS, so that one walks while the other begins or
+// ends; rows of 256 bytes and more leave too few waves for that (32 x 16k keys,
+// heads of 128, bf16: 147 us with one workgroup of four waves, 152 with two of two;
+// heads of 64 in f32: 86 and 102; of 64 in bf16, 64 x 32k keys: 286 with one of
+// eight, 276 with two of four).
+constexpr int cache_per_cu(int row_bytes) { return row_bytes <= 192 ? 2 : 1; }
+constexpr int cache_lds(int row_bytes) { return (152 << 10) / cache_per_cu(row_bytes) - (4 << 10); }
 constexpr int cache_keys(int row_bytes) { return row_bytes <= 512 ? 32 : 16; }
-constexpr int cache_waves(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
-// Workgroups of the form for few rows that a CU holds: what they have in LDS.
-constexpr int cache_per_cu(int row_bytes) {
-  return (160 << 10) / (cache_waves(row_bytes) * (4 * cache_keys(row_bytes) * row_bytes + 512));
+constexpr int cache_tile(int row_bytes) { return 2 * cache_keys(row_bytes) * row_bytes; }
+constexpr int cache_waves(int row_bytes, int row_blocks) {
+  const int most = cache_lds(row_bytes) / (2 * cache_tile(row_bytes)), room = row_bytes * row_blocks <= 256 ? 8 : 4;
+  return most < room ? most : room;
+}
+constexpr int cache_buffers(int row_bytes, int row_blocks) {
+  return cache_lds(row_bytes) / (cache_waves(row_bytes, row_blocks) * cache_tile(row_bytes));
 }
 // Rows of a tile in 16s at most: queries and sums stay in the registers.
 constexpr int cache_row_blocks(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
 
 namespace {
-
-constexpr int kTileBuffers = 2;
 
 // c += a b for a 16x16 tile: lane l holds row (a) or column (b) l % 16, and of the
 // sum's terms the 16 bytes' elements of its quarter l / 16, the same for a and b.
@@ -79,6 +88,13 @@ __device__ __forceinline__ void load_to_lds_from(const void* p, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(m0) : "memory");
 }
 
+// The larger of a lane's value and that of the lane 16 away in its half.
+__device__ __forceinline__ float max_quarters(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
 // The keys or values of one head in the pages of one row of the table.  Page
 // numbers that there are not are cut to those there are.
 template <typename T>
@@ -94,6 +110,13 @@ struct PagedRows {
   }
 };
 
+// A loaded value that is waited for here, and not at its first use: there the
+// compiler would wait for all loads, those to LDS that it knows nothing of too.
+template <typename V>
+__device__ __forceinline__ void arrived(V& v) {
+  asm volatile("" : "+v"(v));
+}
+
 // 64 page numbers from `from` on, a lane each.
 struct PageIds {
   const int32_t* ids;
@@ -107,6 +130,7 @@ struct PageIds {
     if (from >= 0 && first >= from && last < from + kWave) return;
     from = first;
     id = min(max(ids[min(from + (int)(threadIdx.x % kWave), entries - 1)], 0), pages - 1);
+    arrived(id);
   }
 };
 
@@ -299,7 +323,9 @@ struct PagedStager {
   const PageTable* pages;
   PageIds ids;
   int dim;
-  bool whole_pages;  // tiles from multiples of KT on lie in one page
+  int page;           // whose first rows' addresses these are, -1: none
+  const T* k_base;
+  const T* v_base;
   uint32_t k_offset[ROUNDS], v_offset[ROUNDS];
 
   __device__ static int slot(int i) { return i * kWave + (int)(threadIdx.x % kWave); }
@@ -312,7 +338,7 @@ struct PagedStager {
     k = static_cast<const T*>(a.k) + hk * a.k_at.head, v = static_cast<const T*>(a.v) + hk * a.v_at.head;
     k_at = a.k_at, v_at = a.v_at, pages = &a.pages, dim = a.dim;
     ids.begin(table, entries, a.pages.pages);
-    whole_pages = a.pages.page_rows % KT == 0;
+    page = -1, k_base = v_base = nullptr;
     if constexpr (ALIGNED) {
 #pragma unroll
       for (int i = 0; i < ROUNDS; ++i) {
@@ -321,22 +347,33 @@ struct PagedStager {
       }
     }
   }
+  // Asks for the page numbers from row j on.
+  __device__ __forceinline__ void seek(int j) {
+    const int p = __builtin_amdgcn_readfirstlane(pages->page_of(j));
+    ids.seek(p, p);
+  }
   __device__ __forceinline__ void load(char* tile, int j0, int first, int to) {
     const int j_first = first, j_last = min(j0 + KT, to) - 1;
     const int p_first = __builtin_amdgcn_readfirstlane(pages->page_of(j_first));
-    ids.seek(p_first, __builtin_amdgcn_readfirstlane(pages->page_of(j_last)));
+    const int p_last = __builtin_amdgcn_readfirstlane(pages->page_of(j_last));
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(tile));
-    if (ALIGNED && whole_pages && j_first == j0 && j_last == j0 + KT - 1) {
-      const int64_t id = __builtin_amdgcn_readlane(ids.id, p_first - ids.from);
-      const int64_t r = j0 - p_first * pages->page_rows;
-      const T* kp = k + id * k_at.page + r * k_at.row;
-      const T* vp = v + id * v_at.page + r * v_at.row;
+    if (ALIGNED && p_first == p_last && j_first == j0 && j_last == j0 + KT - 1) {
+      if (p_first != page) {
+        page = p_first;
+        ids.seek(page, page);
+        const int64_t id = __builtin_amdgcn_readlane(ids.id, page - ids.from);
+        k_base = k + id * k_at.page, v_base = v + id * v_at.page;
+      }
+      const int64_t r = j0 - page * pages->page_rows;
+      const T* kp = k_base + r * k_at.row;
+      const T* vp = v_base + r * v_at.row;
 #pragma unroll
       for (int i = 0; i < ROUNDS; ++i) load_to_lds(kp, k_offset[i], at + i * 1024);
 #pragma unroll
       for (int i = 0; i < ROUNDS; ++i) load_to_lds(vp, v_offset[i], at + KT * RB + i * 1024);
       return;
     }
+    ids.seek(p_first, p_last);
 #pragma unroll 2
     for (int i = 0; i < ROUNDS; ++i) {
       const int j = min(max(j0 + row(i), j_first), j_last), p = static_cast<int>(pages->page_of(j));
@@ -364,29 +401,29 @@ struct PagedStager {
 //
 // Scores are kept transposed as in attend.hpp, S^T = K Q^T, in 16x16 tiles: a lane
 // has four keys of one row per 16, which are, as they stand, the right operand of
-// O^T = V^T e^S^T.  The reference is the running maximum; weights of 16-bit tensors
-// go into the product as two parts (value and remainder), so that they lose
-// nothing against f32: the walk is bound by memory, and the products are idle.
+// O^T = V^T e^S^T.  A row's reference is the largest of its first tile's scores and
+// moves only when weights outgrow it (kMostWeight).  Weights of 16-bit tensors go
+// into the product as two parts (value and remainder), so that they lose nothing
+// against f32: the walk is bound by memory, and the products are idle.
 template <typename T, int DP, int NR, bool ALIGNED>
-__global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
+__global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T), NR), (cache_waves(DP * sizeof(T), NR) + 3) / 4)
     cache_few_kernel(CacheArgs a, CacheCut prefix, CacheCut own, int splits) {
-  constexpr int RB = DP * sizeof(T), KT = cache_keys(RB), WAVES = cache_waves(RB), KB = KT / 16;
-  constexpr int STEPS = RB / 64, DB = DP / 16, TILE = 2 * KT * RB, ROWS = 16 * NR;
-  constexpr float LIFT = std::is_same_v<T, __half> ? 8.f : 0.f;  // small f16 weights stay normal
+  constexpr int RB = DP * sizeof(T), KT = cache_keys(RB), WAVES = cache_waves(RB, NR), KB = KT / 16;
+  constexpr int STEPS = RB / 64, DB = DP / 16, TILE = cache_tile(RB), ROWS = 16 * NR, BUFFERS = cache_buffers(RB, NR);
   using Stager = PagedStager<T, DP, KT, ALIGNED>;
-  static_assert(Stager::LOADS <= 63, "the wait counts to 63");
-  static_assert(ROWS * DP * 4 <= kTileBuffers * TILE, "a wave's sums take the place of its tiles");
-  extern __shared__ __align__(16) char lds[];  // the waves' tiles, then m and l of the waves' rows
-  float* ml = reinterpret_cast<float*>(lds + WAVES * kTileBuffers * TILE);
+  static_assert((BUFFERS - 1) * Stager::LOADS <= 63, "the wait counts to 63");
+  static_assert(ROWS * DP * 4 <= BUFFERS * TILE, "a wave's sums take the place of its tiles");
+  extern __shared__ __align__(16) char lds[];  // the waves' tiles, m and l of the waves' rows, a word a wave
+  float* ml = reinterpret_cast<float*>(lds + WAVES * BUFFERS * TILE);
   const int lane = threadIdx.x % kWave, col = lane % 16, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int group = a.q_heads / a.k_heads;
-  if (splits == 1) {  // (the join does it otherwise)
+  auto zero_others = [&] {
+    if (splits > 1) return;  // (the join does it)
     int64_t first, last;
     sample_rows(a, first, last);
     if (first > 0 || last < a.n_q)
       zero_outside(static_cast<T*>(a.out), (int64_t)a.q_heads * a.dim, first, last, a.n_q);
-  }
+  };
 
   // rows next to each other, then heads, then chunks
   const int64_t prefix_blocks = prefix.tiles * a.k_heads * prefix.splits;
@@ -395,10 +432,10 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
   const int64_t id = is_prefix ? blockIdx.x : blockIdx.x - prefix_blocks;
   const int split = static_cast<int>(id / cut.tiles / a.k_heads);
   CacheWalk w;
-  w.group = group;
+  w.group = a.q_heads / a.k_heads;
   w.hk = static_cast<int>(id / cut.tiles % a.k_heads);
   int from, to;
-  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id % cut.tiles), from, to)) return;
+  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id % cut.tiles), from, to)) return zero_others();
   const uint32_t row0 = w.row0;
 
   // rows past the last are copies of it
@@ -422,17 +459,6 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
     return;
   }
 
-  Stager stager;
-  stager.begin(a, w.hk, w.table(), w.entries());
-  char* mine = lds + wave * kTileBuffers * TILE;
-  auto place = [&](int t) { return t < w.sink_tiles ? w.sink_start + t * KT : w.start + (t - w.sink_tiles) * KT; };
-  const int first_seen = w.first_seen(lo_min);
-  auto stage = [&](int t, int buf) {
-    const int j0 = place(t);
-    stager.load(mine + buf * TILE, j0, t == w.sink_tiles ? first_seen : j0, t < w.sink_tiles ? w.sink_end : w.end);
-  };
-  if (t0 < t1) stage(t0, 0);
-
   int4v qf[NR][STEPS];
 #pragma unroll
   for (int x = 0; x < NR; ++x) {
@@ -454,6 +480,24 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
       qf[x][st] = y;
     }
   }
+  Stager stager;
+  stager.begin(a, w.hk, w.table(), w.entries());
+  char* mine = lds + wave * BUFFERS * TILE;
+  auto place = [&](int t) { return t < w.sink_tiles ? w.sink_start + t * KT : w.start + (t - w.sink_tiles) * KT; };
+  const int first_seen = w.first_seen(lo_min);
+  auto stage = [&](int t, int buf) {
+    const int j0 = place(t);
+    stager.load(mine + buf * TILE, j0, t == w.sink_tiles ? first_seen : j0, t < w.sink_tiles ? w.sink_end : w.end);
+  };
+  if (t0 < t1) stager.seek(place(t0));  // (while the queries are on their way)
+#pragma unroll
+  for (int x = 0; x < NR; ++x)
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) arrived(qf[x][st]);
+#pragma unroll
+  for (int i = 0; i < BUFFERS - 1; ++i)
+    if (t0 + i < t1) stage(t0 + i, i);
+  zero_others();
 
   f32x4 o[NR][DB];
   float m[NR], l[NR];  // reference; this lane's share of the sum
@@ -464,15 +508,19 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
     for (int db = 0; db < DB; ++db) o[x][db] = f32x4(0.f);
   }
   const float c = a.scale_log2;
-  for (int t = t0, buf = 0; t < t1; ++t, buf ^= 1) {
-    if (t + 1 < t1) {
+  for (int t = t0, buf = 0; t < t1; ++t, buf = buf + 1 == BUFFERS ? 0 : buf + 1) {
+    if (t + BUFFERS - 1 < t1) {
       // (what was read from that buffer has arrived)
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      stage(t + 1, buf ^ 1);
-      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(ALIGNED ? Stager::LOADS : 0) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      stage(t + BUFFERS - 1, buf == 0 ? BUFFERS - 1 : buf - 1);
     }
+    // all but the tiles behind this one
+    const int behind = min(t1 - 1 - t, BUFFERS - 1);
+    for_each_index(
+        [&](auto n) {
+          if (behind == n) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(ALIGNED ? n * Stager::LOADS : 0) : "memory");
+        },
+        std::make_integer_sequence<int, BUFFERS>{});
     const char* kt = mine + buf * TILE;
     const char* vt = kt + KT * RB;
     const int j0 = place(t), last = t < w.sink_tiles ? w.sink_end : w.end;
@@ -504,42 +552,44 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
           }
     }
     // weights, and their sums; a new reference rescales what is there
-    float top[NR];
-    bool moves = false;
-#pragma unroll
-    for (int x = 0; x < NR; ++x) {
-      top[x] = s[x][0][0];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[x] = fmaxf(top[x], s[x][kb][i]);
-      top[x] = fmaxf(top[x], __shfl_xor(top[x], 16, kWave));
-      top[x] = fmaxf(top[x], __shfl_xor(top[x], 32, kWave));
-      moves |= top[x] > m[x];
-    }
-    if (__any(moves)) {
+    float p[NR][KB][4], sum[NR];
+    auto weights = [&] {
 #pragma unroll
       for (int x = 0; x < NR; ++x) {
-        const float m_new = fmaxf(m[x], top[x]);
-        const float fix = m[x] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m[x] - m_new) * c);
-        m[x] = m_new;
+        const float base = m[x] == -__builtin_inff() ? 0.f : m[x];
+        sum[x] = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[x][kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][kb][i] - base, c, kLift<T>));
+            sum[x] += p[x][kb][i];
+          }
+      }
+    };
+    bool over = false;
+    weights();
+#pragma unroll
+    for (int x = 0; x < NR; ++x) over |= m[x] == -__builtin_inff() || sum[x] > kMostWeight<T>;
+    if (__any(over)) {
+#pragma unroll
+      for (int x = 0; x < NR; ++x) {
+        float top = m[x];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[x][kb][i]);
+        top = max_halves(max_quarters(top));
+        const float fix = m[x] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m[x] - top) * c);
+        m[x] = top;
         l[x] *= fix;
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[x][db] *= fix;
       }
+      weights();
     }
-    float p[NR][KB][4];
 #pragma unroll
-    for (int x = 0; x < NR; ++x) {
-      const float base = m[x] == -__builtin_inff() ? 0.f : m[x];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[x][kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][kb][i] - base, c, LIFT));
-          l[x] += p[x][kb][i];
-        }
-    }
+    for (int x = 0; x < NR; ++x) l[x] += sum[x];
     if constexpr (kIs16<T>) {
       static_assert(KB == 2, "a product of 32 keys");
       int4v ph[NR], pl[NR];  // the weights, and what their rounding leaves
@@ -605,8 +655,14 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
       ml[2 * (wave * ROWS + 16 * x + col) + 1] = l[x];
     }
   }
-  const int odd = __syncthreads_or(off != off);
-  if (!odd) {
+  int* odd = reinterpret_cast<int*>(ml + 2 * WAVES * ROWS);
+  if (lane == 0) odd[wave] = 0;
+  if (off != off) odd[wave] = 1;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int y = 0; y < WAVES; ++y) any |= odd[y];
+  if (!any) {
     float* sums = reinterpret_cast<float*>(mine);
 #pragma unroll
     for (int x = 0; x < NR; ++x) {
@@ -631,7 +687,7 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
       for (int y = 0; y < WAVES; ++y) {
         const float my = ml[2 * (y * ROWS + r)], ly = ml[2 * (y * ROWS + r) + 1];
         sum += my == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((my - all) * c) * ly;
-        v += *reinterpret_cast<const f32x4*>(lds + y * kTileBuffers * TILE + (r * DP + d) * 4);
+        v += *reinterpret_cast<const f32x4*>(lds + y * BUFFERS * TILE + (r * DP + d) * 4);
       }
       const int64_t item = item_of(row0 + r);
       const int cnt = min(4, a.dim - d);
@@ -639,7 +695,7 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)))
         const int64_t at = part * a.rows() + item;
         float* to = a.part + a.part_values(splits) + at * a.dim + d;
         if (d == 0) {
-          a.part[2 * at] = sum == 0.f ? -__builtin_inff() : all * c - LIFT;
+          a.part[2 * at] = sum == 0.f ? -__builtin_inff() : all * c - kLift<T>;
           a.part[2 * at + 1] = sum;
         }
         for (int i = 0; i < cnt; ++i) to[i] = v[i];
@@ -810,8 +866,8 @@ int launch_many(const CacheArgs& a, const CacheCut& c, bool is_prefix, int split
 
 template <typename T, int DP, int NR, bool ALIGNED>
 int launch_few(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
-  constexpr int RB = DP * sizeof(T), WAVES = cache_waves(RB);
-  constexpr int bytes = WAVES * (kTileBuffers * 2 * cache_keys(RB) * RB + 16 * NR * 8);
+  constexpr int RB = DP * sizeof(T), WAVES = cache_waves(RB, NR);
+  constexpr int bytes = WAVES * (cache_buffers(RB, NR) * cache_tile(RB) + 16 * NR * 8 + 4);
   auto kernel = &cache_few_kernel<T, DP, NR, ALIGNED>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
@@ -821,6 +877,67 @@ int launch_few(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
   TSC_REQUIRE(blocks * kWave * WAVES < (1ll << 32), "cache_attention: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, prefix, own, p.splits());
   TSC_LAUNCH_CHECK("cache_attention");
+  return 0;
+}
+
+// The join for few parts: a wave per row, VALUES / 4 lanes for its values and as
+// many parts at a time as that leaves room for.  (16k rows of 7 parts: a
+// workgroup per row 25 us.)
+constexpr int kFewParts = 16;
+
+template <typename T, int VALUES>
+__global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a, int splits) {
+  constexpr int LANES = VALUES / 4, GROUPS = kWave / LANES;
+  const int64_t item = blockIdx.x * (int64_t)4 + threadIdx.x / kWave, step = a.rows();
+  if (item >= step) return;
+  const int lane = threadIdx.x % kWave, c = lane % LANES, d = 4 * c;
+  const float* ml = a.part + 2 * item;
+  const float* o = a.part + a.part_values(splits) + item * a.dim + d;
+  float m = -__builtin_inff(), l = 0.f;
+  f32x4 sum = f32x4(0.f);
+#pragma unroll 4
+  for (int s = lane / LANES; s < splits; s += GROUPS) {
+    const float ms = ml[2 * s * step], ls = ml[2 * s * step + 1];
+    f32x4 x = f32x4(0.f);
+    const float* p = o + s * step * a.dim;
+    if (d + 4 <= a.dim) __builtin_memcpy(&x, p, 16);
+    else
+      for (int i = 0; i < 3; ++i) x[i] = d + i < a.dim ? p[i] : 0.f;
+    if (ls == 0.f) continue;  // (a part that saw nothing has no values)
+    const float m_new = fmaxf(m, ms);
+    const float f = m == -__builtin_inff() ? 0.f : exp2f(m - m_new), g = exp2f(ms - m_new);
+    m = m_new, l = f * l + g * ls, sum = f * sum + g * x;
+  }
+#pragma unroll
+  for (int x = LANES; x < kWave; x <<= 1) {
+    const float mx = __shfl_xor(m, x, kWave), lx = __shfl_xor(l, x, kWave), m_new = fmaxf(m, mx);
+    const float f = l == 0.f ? 0.f : exp2f(m - m_new), g = lx == 0.f ? 0.f : exp2f(mx - m_new);
+    f32x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __shfl_xor(sum[i], x, kWave);
+    m = m_new, l = f * l + g * lx;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = f * sum[i] + g * y[i];
+  }
+  if (lane >= LANES) return;
+  int64_t first, last;
+  sample_rows(a, first, last);
+  // (a row of no sample has no parts: what was read for it means nothing)
+  const bool none = l == 0.f || item < first * a.q_heads || item >= last * a.q_heads;
+  T* out = static_cast<T*>(a.out) + item * a.dim;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (d + i < a.dim) out[d + i] = from_f32<T>(none ? 0.f : sum[i] / l);
+}
+
+template <typename T>
+int launch_parts(const AttendArgs& a, int splits, hipStream_t s) {
+  if (splits > kFewParts) return launch_join<T>(a, splits, s);
+  const unsigned blocks = static_cast<unsigned>(ceil_div(a.rows(), 4));
+  if (a.dim <= 64) cache_join_kernel<T, 64><<<blocks, 256, 0, s>>>(a, splits);
+  else if (a.dim <= 128) cache_join_kernel<T, 128><<<blocks, 256, 0, s>>>(a, splits);
+  else cache_join_kernel<T, 256><<<blocks, 256, 0, s>>>(a, splits);
+  TSC_LAUNCH_CHECK("cache_attention_join");
   return 0;
 }
 
@@ -865,7 +982,7 @@ int launch_cache(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
   };
   const bool aligned = a.dim % e == 0 && whole(a.k, a.k_at) && whole(a.v, a.v_at);
   if (int rc = aligned ? launch_dims<T, true>(a, p, s) : launch_dims<T, false>(a, p, s)) return rc;
-  return p.splits() > 1 ? launch_join<T>(a, p.splits(), s) : 0;
+  return p.splits() > 1 ? launch_parts<T>(a, p.splits(), s) : 0;
 }
 
 }  // namespace tsc
