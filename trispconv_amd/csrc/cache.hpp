@@ -136,7 +136,7 @@ struct PageIds {
 
 // Positions of sample b.
 __device__ __forceinline__ int kept(const CacheArgs& a, int b) {
-  return static_cast<int>(min(max((int64_t)a.pages.lengths[b], (int64_t)0), a.pages.most()));
+  return a.pages.cut(a.pages.lengths[b]);
 }
 
 // The sample and the tile of query rows within it of the x-th tile of all (as
@@ -179,7 +179,7 @@ struct CacheWalk : Walk {
     int p = token(r) + shift, keys = lk;
     if (b < 0) {
       const int64_t t = q0 + token(r);
-      const int s = first_past(a, t);
+      const int s = first_past(a.off_q, a.samples, t);
       keys = kept(*args, s);
       p = position(t, a.off_q[s + 1], keys);
     }
@@ -189,39 +189,18 @@ struct CacheWalk : Walk {
   __device__ __forceinline__ void wave(const AttendArgs& a, uint32_t first, int col, int lo[N], int hi[N],
                                        int& lo_first, int& hi_first, int& lo_last, int& hi_last) const {
     if (b >= 0) return Walk::wave<N, STEP>(a, first, col, lo, hi, lo_first, hi_first, lo_last, hi_last);
-    // the sample of the first row, then how many samples' ends each row is past
-    const int lane = threadIdx.x % kWave;
-    const int64_t t_last = q0 + token(first + N * STEP - 1);
-    const int s0 = a.samples <= kWave ? 0 : first_past(a, q0 + token(first));
-    int at[N], next[N], keys[N];
+    int at[N], end[N], length[N];
     int64_t t[N];
 #pragma unroll
-    for (int x = 0; x < N; ++x) t[x] = q0 + token(first + x * STEP + col), at[x] = s0;
-    const int mine = min(s0 + lane, a.samples - 1);
-    int ends = a.off_q[mine + 1], s = s0;
-    const int kept_mine = kept(*args, mine);
-    for (;;) {
-      int k = 0;
-      for (; k < kWave && s + k < a.samples - 1; ++k) {
-        const int e = __builtin_amdgcn_readlane(ends, k);
-        if (e > t_last) break;
-#pragma unroll
-        for (int x = 0; x < N; ++x) at[x] += t[x] >= e;
-      }
-      if (k < kWave) break;
-      s += kWave;
-      ends = a.off_q[min(s + lane, a.samples - 1) + 1];
-    }
-#pragma unroll
-    for (int x = 0; x < N; ++x) {
-      next[x] = s == s0 ? __shfl(ends, at[x] - s0, kWave) : a.off_q[at[x] + 1];
-      keys[x] = s == s0 ? __shfl(kept_mine, at[x] - s0, kWave) : kept(*args, at[x]);
-    }
+    for (int x = 0; x < N; ++x) t[x] = q0 + token(first + x * STEP + col);
+    samples_of<N>(a.off_q, args->pages.lengths, a.samples, q0 + token(first), q0 + token(first + N * STEP - 1), t, at,
+                  end, length);
     lo_first = hi_first = kNoLimit, lo_last = hi_last = 0;
 #pragma unroll
     for (int x = 0; x < N; ++x) {
       int sink;
-      seen_keys(position(t[x], next[x], keys[x]), keys[x], a.left, a.right, a.sinks, lo[x], hi[x], sink);
+      const int keys = args->pages.cut(length[x]);
+      seen_keys(position(t[x], end[x], keys), keys, a.left, a.right, a.sinks, lo[x], hi[x], sink);
       lo_first = min(lo_first, lo[x]), lo_last = max(lo_last, lo[x]);
       hi_first = min(hi_first, hi[x]), hi_last = max(hi_last, hi[x]);
     }
@@ -235,20 +214,6 @@ struct CacheWalk : Walk {
   }
   __device__ static __forceinline__ int position(int64_t t, int end, int keys) {
     return static_cast<int>(max(t - end + keys, -(int64_t)(1 << 30)));
-  }
-  // The first sample (the last at most) whose end is past row t, by the whole wave.
-  __device__ static __forceinline__ int first_past(const AttendArgs& a, int64_t t) {
-    int from = 0, n = a.samples;
-    while (n > 1) {
-      const int step = (n + kWave - 1) / kWave, lane = threadIdx.x % kWave;
-      const int s = min(from + (lane + 1) * step, from + n) - 1;  // the last of the lane's
-      const uint64_t past = __ballot(a.off_q[s + 1] > t);
-      const int l = past ? __builtin_ctzll(past) : kWave - 1;
-      const int next = min(from + l * step, from + n - 1);
-      n = min(step, from + n - next);
-      from = next;
-    }
-    return from;
   }
   // Takes the x-th tile of `tile_rows` rows (the prefix's: of all samples) and the
   // range of keys [from, to) of this part.  false: past the last tile.

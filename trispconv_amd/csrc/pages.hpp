@@ -30,6 +30,10 @@ struct PageTable {
     return (static_cast<uint32_t>(static_cast<uint64_t>(t) * multiplier >> 32) + (t & whole)) >> shift;
   }
 
+  // A length as far as there is room for it.
+  __device__ __forceinline__ int cut(int length) const {
+    return static_cast<int>(min(max((int64_t)length, (int64_t)0), most()));
+  }
   // The checked arguments of an entry point; 0 or an error code.
   int set(const char* what, const int32_t* table_, int64_t table_row_, int64_t table_pages_, const int32_t* lengths_,
           int32_t samples_, int64_t pages_, int64_t page_rows_) {
@@ -53,5 +57,53 @@ struct PageTable {
     return 0;
   }
 };
+
+// The first sample (the last at most) whose end, off[s + 1], is past row t, by the
+// whole wave: 64 at a time.
+__device__ __forceinline__ int first_past(const int32_t* off, int samples, int64_t t) {
+  int from = 0, n = samples;
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave, lane = threadIdx.x % kWave;
+    const int s = min(from + (lane + 1) * step, from + n) - 1;  // the last of the lane's
+    const uint64_t past = __ballot(off[s + 1] > t);
+    const int l = past ? __builtin_ctzll(past) : kWave - 1;
+    const int next = min(from + l * step, from + n - 1);
+    n = min(step, from + n - next);
+    from = next;
+  }
+  return from;
+}
+
+// The samples at[x] of N rows t[x] a lane, all from t_first to t_last, with their
+// ends and lengths (as they are in `lengths`), by the whole wave: the sample of
+// the first row, then how many samples' ends each row is past.
+template <int N>
+__device__ __forceinline__ void samples_of(const int32_t* off, const int32_t* lengths, int samples, int64_t t_first,
+                                           int64_t t_last, const int64_t t[N], int at[N], int end[N], int length[N]) {
+  const int lane = threadIdx.x % kWave;
+  const int s0 = samples <= kWave ? 0 : first_past(off, samples, t_first);
+#pragma unroll
+  for (int x = 0; x < N; ++x) at[x] = s0;
+  const int mine = min(s0 + lane, samples - 1);
+  int ends = off[mine + 1], s = s0;
+  const int length_mine = lengths[mine];
+  for (;;) {
+    int k = 0;
+    for (; k < kWave && s + k < samples - 1; ++k) {
+      const int e = __builtin_amdgcn_readlane(ends, k);
+      if (e > t_last) break;
+#pragma unroll
+      for (int x = 0; x < N; ++x) at[x] += t[x] >= e;
+    }
+    if (k < kWave) break;
+    s += kWave;
+    ends = off[min(s + lane, samples - 1) + 1];
+  }
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    end[x] = s == s0 ? __shfl(ends, at[x] - s0, kWave) : off[at[x] + 1];
+    length[x] = s == s0 ? __shfl(length_mine, at[x] - s0, kWave) : lengths[at[x]];
+  }
+}
 
 }  // namespace tsc

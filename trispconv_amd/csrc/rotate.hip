@@ -48,27 +48,25 @@ struct RotateArgs {
   const int32_t* offsets;
 };
 
-// The page and its row that input row r goes to: r is one of the last rows of
+// The page and its row that an input row goes to: it is one of the last rows of
 // the sample whose offsets enclose it.  A page of -1: nowhere (a row of no
 // sample, a position or a page that there is not).
 struct Place {
   int32_t page, row;
 };
-__device__ __forceinline__ Place place_of(const RotateArgs& a, int64_t r) {
-  int lo = 0, hi = a.pages.samples + 1;  // offsets up to r: [0, lo) are, [hi, ...) are not
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.offsets[mid] <= r) lo = mid + 1;
-    else hi = mid;
-  }
-  const int b = lo - 1;
-  if (b < 0 || b >= a.pages.samples) return Place{-1, 0};
-  const int64_t pos = a.pages.lengths[b] - (a.offsets[b + 1] - r);
-  if (pos < 0 || pos >= a.pages.most()) return Place{-1, 0};
-  const uint32_t at = a.pages.page_of(static_cast<uint32_t>(pos));
-  const int32_t page = a.pages.table[b * a.pages.table_row + at];
+// For a row r of [first, last] a lane, by the whole wave.
+__device__ __forceinline__ Place place_of(const RotateArgs& a, int64_t first, int64_t last, int64_t r) {
+  if (a.pages.samples == 0) return Place{-1, 0};
+  const int64_t t[1] = {r};
+  int at[1], end[1], length[1];
+  const int begin = a.offsets[0];
+  samples_of<1>(a.offsets, a.pages.lengths, a.pages.samples, first, last, t, at, end, length);
+  const int64_t pos = (int64_t)length[0] - (end[0] - r);
+  if (r < begin || r >= end[0] || pos < 0 || pos >= a.pages.most()) return Place{-1, 0};
+  const uint32_t p = a.pages.page_of(static_cast<uint32_t>(pos));
+  const int32_t page = a.pages.table[at[0] * a.pages.table_row + p];
   if (page < 0 || page >= a.pages.pages) return Place{-1, 0};
-  return Place{page, static_cast<int32_t>(pos - (int64_t)at * a.pages.page_rows)};
+  return Place{page, static_cast<int32_t>(pos - (int64_t)p * a.pages.page_rows)};
 }
 
 // Cosine and sine of position p times a pair's speed, base^(-i/F) / 2 pi turns.
@@ -118,7 +116,7 @@ __device__ __forceinline__ void rotate_any_row(const RotateArgs& a, int64_t r, i
     }
   }
   Place to{0, 0};
-  if constexpr (PAGED) to = place_of(a, r);
+  if constexpr (PAGED) to = place_of(a, r, r, r);
   const int total = a.q_heads + a.k_heads;
   for (int h0 = 0; h0 < total; h0 += heads) {
     const int h = h0 + sub;
@@ -186,7 +184,10 @@ __global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
 // (or one after the other where pairs are neighbours), so that a pair never
 // leaves its lane.  Bound by memory: each vector is read and written once.
 // 500k rows of 12 + 12 heads of 64, bf16: 607 us, 5.07 TB/s (a large copy on
-// this card: 4.86).
+// this card: 4.86).  The paged form takes keys and values head by head, so that
+// what it writes of a page lies together (4 x 60k rows of 12 + 12 + 12 heads of
+// 64, f16: 445 us, 4.85 TB/s; row by row 553, and 25 more where each row searched
+// for its sample by itself).
 constexpr int kRows = 8, kMaxHalf = 128;
 
 template <typename T, int P, int LANES, bool PAGED>
@@ -207,8 +208,12 @@ __global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
   const int first = in ? (a.interleaved ? 2 * P * l : P * l) : 0, second = first + (a.interleaved ? P : half);
   for (int64_t r0 = blockIdx.x * (int64_t)kRows; r0 < a.n; r0 += (int64_t)gridDim.x * kRows) {
     const int rows = static_cast<int>(min((int64_t)kRows, a.n - r0));
-    if constexpr (PAGED)
-      if ((int)threadIdx.x >= 256 - rows) place[255 - threadIdx.x] = place_of(a, r0 + 255 - threadIdx.x);
+    if constexpr (PAGED) {
+      if (threadIdx.x >= 256 - kWave) {  // the last wave, which has the fewest angles
+        const int r = min((int)threadIdx.x - (256 - kWave), rows - 1);
+        place[r] = place_of(a, r0, r0 + rows - 1, r0 + r);
+      }
+    }
     for (int x = threadIdx.x; x < rows * half; x += 256) {
       const int r = x / half, j = x - r * half;
       float2 cs = make_float2(1.f, 0.f);
@@ -222,7 +227,15 @@ __global__ void __launch_bounds__(256) rotate_vector_kernel(RotateArgs a) {
     }
     __syncthreads();
     for (int v = threadIdx.x / LANES; v < rows * total; v += HEADS) {
-      const int r = v / total, h = v - r * total;
+      int r, h;
+      if (PAGED && v >= rows * a.q_heads) {
+        // head by head: its rows lie one behind the other in their page
+        const int u = v - rows * a.q_heads, n = rows == kRows ? u / kRows : u / rows;
+        h = a.q_heads + n, r = u - n * rows;
+      } else {
+        const int n = PAGED ? a.q_heads : total;
+        r = v / n, h = v - r * n;
+      }
       const bool is_q = h < a.q_heads;
       const int hh = is_q ? h : h - a.q_heads;
       const int64_t row = r0 + r;
