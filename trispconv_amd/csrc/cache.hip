@@ -42,7 +42,7 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
       int64_t chunk = std::min<int64_t>(std::max<int64_t>(ceil_div(keys, want), 256), 4096 / per_cu);
       if (!prefix_rows && keys <= 1024) chunk = keys;
       chunk = std::max(chunk, ceil_div(keys, kMostSplits / 2));
-      c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), kt * cache_waves(row_bytes, p.row_blocks)));
+      c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), kt * cache_waves(row_bytes)));
       c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
       return c;
     }
@@ -51,9 +51,12 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     const int64_t work = units(128 * c.wave_rows);
     c.tiles = tiles(128 * c.wave_rows);
     // One round of workgroups, of 512 keys and more (20k keys in 136 tiles, four
-    // workgroups a CU: 151 us in seven parts, 166 in six, 239 in three; a prefix of
-    // 32k keys in 8 tiles: 50 us in 64 parts, 57 in 128 and 67 in 32)
-    const int64_t slots = kCus * (row_bytes <= 128 ? 4 / c.wave_rows : row_bytes <= 256 ? 2 : 1);
+    // workgroups a CU: 141 us in seven parts, 166 in six, 239 in three); beside
+    // the samples' own keys one a CU (a prefix of 32k keys in 8 tiles: 42 us in 32
+    // parts, 45 in 64, 61 in 128)
+    const bool beside = lists == 1 && prefix_rows && all / samples <= 64 && row_bytes <= 128;
+    const int64_t per_cu = beside ? 1 : row_bytes <= 128 ? 4 / c.wave_rows : row_bytes <= 256 ? 2 : 1;
+    const int64_t slots = per_cu * kCus;
     c.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({keys / 512, slots / work, kMostSplits / 2})));
     return c;
   };
@@ -132,6 +135,12 @@ extern "C" int tsc_cache_attention(const void* q, int64_t q_row, int64_t q_head,
   a.q_sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
   a.out = out, a.part = static_cast<float*>(ws);
   a.prefix = prefix, a.prefix_pages = static_cast<int>(prefix_pages);
+  // (with 2^(l-1) < g <= 2^l: floor(2^32 (2^l - g) / g) + 1 and l - 1)
+  const uint64_t g = q_heads / k_heads;
+  int l = 0;
+  while ((1ull << l) < g) ++l;
+  a.group_mul = g == 1 ? 0 : static_cast<uint32_t>((((1ull << l) - g) << 32) / g + 1);
+  a.group_shift = l - 1;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case TSC_F32: return launch_cache<float>(a, p, s);

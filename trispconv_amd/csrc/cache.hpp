@@ -21,6 +21,10 @@ struct CacheArgs : AttendArgs {
   PageStrides k_at, v_at;
   const int32_t* prefix;  // its pages, or none
   int prefix_pages;
+  // r / group for any 32-bit r without a division: with t = umulhi(r, group_mul),
+  // (t + (r - t) / 2) >> group_shift; group_mul 0 for groups of one
+  uint32_t group_mul;
+  int group_shift;
   __host__ __device__ int prefix_rows() const { return prefix_pages * pages.page_rows; }
 };
 
@@ -52,12 +56,12 @@ constexpr int cache_per_cu(int row_bytes) { return row_bytes <= 192 ? 2 : 1; }
 constexpr int cache_lds(int row_bytes) { return (152 << 10) / cache_per_cu(row_bytes) - (4 << 10); }
 constexpr int cache_keys(int row_bytes) { return row_bytes <= 512 ? 32 : 16; }
 constexpr int cache_tile(int row_bytes) { return 2 * cache_keys(row_bytes) * row_bytes; }
-constexpr int cache_waves(int row_bytes, int row_blocks) {
-  const int most = cache_lds(row_bytes) / (2 * cache_tile(row_bytes)), room = row_bytes * row_blocks <= 256 ? 8 : 4;
-  return most < room ? most : room;
+constexpr int cache_waves(int row_bytes) {
+  const int most = cache_lds(row_bytes) / (2 * cache_tile(row_bytes));
+  return most < 4 ? most : 4;
 }
-constexpr int cache_buffers(int row_bytes, int row_blocks) {
-  return cache_lds(row_bytes) / (cache_waves(row_bytes, row_blocks) * cache_tile(row_bytes));
+constexpr int cache_buffers(int row_bytes) {
+  return cache_lds(row_bytes) / (cache_waves(row_bytes) * cache_tile(row_bytes));
 }
 // Rows of a tile in 16s at most: queries and sums stay in the registers.
 constexpr int cache_row_blocks(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
@@ -172,8 +176,13 @@ __device__ __forceinline__ bool find_rows(const CacheArgs& a, int group, int row
 struct CacheWalk : Walk {
   const CacheArgs* args;
   int b;  // the sample; -1: all
-  __device__ int head(uint32_t r) const {
-    return hk * group + static_cast<int>(min(r, rows - 1) % static_cast<uint32_t>(group));
+  __device__ __forceinline__ int token(uint32_t r) const {
+    r = min(r, rows - 1);
+    const uint32_t t = __umulhi(r, args->group_mul);
+    return static_cast<int>(args->group_mul ? (t + ((r - t) >> 1)) >> args->group_shift : r);
+  }
+  __device__ __forceinline__ int head(uint32_t r) const {
+    return hk * group + static_cast<int>(min(r, rows - 1) - static_cast<uint32_t>(token(r)) * group);
   }
   __device__ __forceinline__ void seen(const AttendArgs& a, uint32_t r, int& lo, int& hi, int& sink) const {
     int p = token(r) + shift, keys = lk;
@@ -185,10 +194,23 @@ struct CacheWalk : Walk {
     }
     seen_keys(p, keys, a.left, a.right, a.sinks, lo, hi, sink);
   }
+  __device__ __forceinline__ void bounds(const AttendArgs& a, uint32_t first, uint32_t last, int& lo_first,
+                                         int& hi_first, int& lo_last, int& hi_last) const {
+    int sink;
+    seen(a, first, lo_first, hi_first, sink);
+    seen(a, last, lo_last, hi_last, sink);
+  }
   template <int N, int STEP>
   __device__ __forceinline__ void wave(const AttendArgs& a, uint32_t first, int col, int lo[N], int hi[N],
                                        int& lo_first, int& hi_first, int& lo_last, int& hi_last) const {
-    if (b >= 0) return Walk::wave<N, STEP>(a, first, col, lo, hi, lo_first, hi_first, lo_last, hi_last);
+    if (b >= 0) {  // (later rows see later keys)
+      int sink;
+#pragma unroll
+      for (int x = 0; x < N; ++x) seen(a, first + x * STEP + col, lo[x], hi[x], sink);
+      lo_first = __builtin_amdgcn_readlane(lo[0], 0), hi_first = __builtin_amdgcn_readlane(hi[0], 0);
+      lo_last = __builtin_amdgcn_readlane(lo[N - 1], STEP - 1), hi_last = __builtin_amdgcn_readlane(hi[N - 1], STEP - 1);
+      return;
+    }
     int at[N], end[N], length[N];
     int64_t t[N];
 #pragma unroll
@@ -371,14 +393,14 @@ struct PagedStager {
 // into the product as two parts (value and remainder), so that they lose nothing
 // against f32: the walk is bound by memory, and the products are idle.
 template <typename T, int DP, int NR, bool ALIGNED>
-__global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T), NR), (cache_waves(DP * sizeof(T), NR) + 3) / 4)
-    cache_few_kernel(CacheArgs a, CacheCut prefix, CacheCut own, int splits) {
-  constexpr int RB = DP * sizeof(T), KT = cache_keys(RB), WAVES = cache_waves(RB, NR), KB = KT / 16;
-  constexpr int STEPS = RB / 64, DB = DP / 16, TILE = cache_tile(RB), ROWS = 16 * NR, BUFFERS = cache_buffers(RB, NR);
+__device__ __forceinline__ void cache_few(const CacheArgs& a, const CacheCut& cut, bool is_prefix, int splits,
+                                          int64_t id, char* lds) {
+  constexpr int RB = DP * sizeof(T), KT = cache_keys(RB), WAVES = cache_waves(RB), KB = KT / 16;
+  constexpr int STEPS = RB / 64, DB = DP / 16, TILE = cache_tile(RB), ROWS = 16 * NR, BUFFERS = cache_buffers(RB);
   using Stager = PagedStager<T, DP, KT, ALIGNED>;
   static_assert((BUFFERS - 1) * Stager::LOADS <= 63, "the wait counts to 63");
   static_assert(ROWS * DP * 4 <= BUFFERS * TILE, "a wave's sums take the place of its tiles");
-  extern __shared__ __align__(16) char lds[];  // the waves' tiles, m and l of the waves' rows, a word a wave
+  // lds: the waves' tiles, m and l of the waves' rows, a word a wave
   float* ml = reinterpret_cast<float*>(lds + WAVES * BUFFERS * TILE);
   const int lane = threadIdx.x % kWave, col = lane % 16, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -391,10 +413,6 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T), NR), (cache
   };
 
   // rows next to each other, then heads, then chunks
-  const int64_t prefix_blocks = prefix.tiles * a.k_heads * prefix.splits;
-  const bool is_prefix = blockIdx.x < prefix_blocks;
-  const CacheCut& cut = is_prefix ? prefix : own;
-  const int64_t id = is_prefix ? blockIdx.x : blockIdx.x - prefix_blocks;
   const int split = static_cast<int>(id / cut.tiles / a.k_heads);
   CacheWalk w;
   w.group = a.q_heads / a.k_heads;
@@ -699,6 +717,16 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T), NR), (cache
   }
 }
 
+template <typename T, int DP, int NR, bool ALIGNED>
+__global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)), (cache_waves(DP * sizeof(T)) + 3) / 4)
+    cache_few_kernel(CacheArgs a, CacheCut prefix, CacheCut own, int splits) {
+  extern __shared__ __align__(16) char lds[];
+  const int64_t prefix_blocks = prefix.tiles * a.k_heads * prefix.splits;
+  const bool is_prefix = blockIdx.x < prefix_blocks;
+  cache_few<T, DP, NR, ALIGNED>(a, is_prefix ? prefix : own, is_prefix, splits,
+                                blockIdx.x - (is_prefix ? 0 : prefix_blocks), lds);
+}
+
 // Tiles of K and V for attend_walk, from pages.  Rows of a tile that no query sees
 // are those nearest to them again.
 template <typename T, int DP, int KB, int WAVES, bool ALIGNED>
@@ -778,13 +806,12 @@ struct PagedTiles {
   __device__ PagedRows<T> v_rows() const { return {v.src, args->v_at.page, v.stride, table, &args->pages}; }
 };
 
-// Many query rows: attend_walk's tiles, over pages.
+// Many query rows: attend_walk's tiles, over pages.  lds: as attend_kernel's.
 template <typename T, int DP, int RB, int KB, bool ALIGNED>
-__global__ void __launch_bounds__(kWave * 4, waves_per_simd<T>(DP, RB, 4))
-    cache_tile_kernel(CacheArgs a, CacheCut cut, int is_prefix, int splits) {
+__device__ __forceinline__ void cache_many(const CacheArgs& a, const CacheCut& cut, bool is_prefix, int splits,
+                                           char* lds) {
   constexpr int ROWS = 32 * RB * 4, KT = 32 * KB;
   using Tiles = PagedTiles<T, DP, KB, 4, ALIGNED>;
-  extern __shared__ __align__(16) char lds[];  // as attend_kernel's
   if (splits == 1) {  // (the join does it otherwise)
     int64_t first, last;
     sample_rows(a, first, last);
@@ -815,10 +842,45 @@ __global__ void __launch_bounds__(kWave * 4, waves_per_simd<T>(DP, RB, 4))
   attend_walk<T, DP, RB, KB, 4>(a, w, kv, lds);
 }
 
+template <typename T, int DP, int RB, int KB, bool ALIGNED>
+__global__ void __launch_bounds__(kWave * 4, waves_per_simd<T>(DP, RB, 4))
+    cache_tile_kernel(CacheArgs a, CacheCut cut, int is_prefix, int splits) {
+  extern __shared__ __align__(16) char lds[];
+  cache_many<T, DP, RB, KB, ALIGNED>(a, cut, is_prefix, splits, lds);
+}
+
+// Many rows against the prefix and few against each sample's own keys, side by
+// side: either leaves CUs idle while it begins and ends (64 samples, 32k keys for
+// all and 1000 of their own: 27 and 15 us one after the other).
+template <typename T, int DP, int NR, bool ALIGNED>
+__global__ void __launch_bounds__(kWave * 4, 2)
+    cache_both_kernel(CacheArgs a, CacheCut prefix, CacheCut own, int splits, int prefix_blocks) {
+  extern __shared__ __align__(16) char lds[];
+  if ((int)blockIdx.x < prefix_blocks)
+    cache_many<T, DP, 1, key_blocks<T>(DP), ALIGNED>(a, prefix, true, splits, lds);
+  else
+    cache_few<T, DP, NR, ALIGNED>(a, own, false, splits, blockIdx.x - prefix_blocks, lds);
+}
+// Where both fit a CU twice.
+template <typename T>
+constexpr bool cache_both(int dp) {
+  return dp * (int)sizeof(T) <= 128 && cache_waves(dp * sizeof(T)) == 4;
+}
+
+template <typename T, int DP>
+constexpr int many_lds() {
+  constexpr int KB = key_blocks<T>(DP);
+  return tile_buffers<T>(DP, 4) * 2 * 32 * KB * DP * (int)sizeof(T) + 4 * DP * 4 + KB * 4;
+}
+template <typename T, int DP, int NR>
+constexpr int few_lds() {
+  constexpr int RB = DP * sizeof(T);
+  return cache_waves(RB) * (cache_buffers(RB) * cache_tile(RB) + 16 * NR * 8 + 4);
+}
+
 template <typename T, int DP, int RB, bool ALIGNED>
 int launch_many(const CacheArgs& a, const CacheCut& c, bool is_prefix, int splits, hipStream_t s) {
-  constexpr int KB = key_blocks<T>(DP);
-  constexpr int bytes = tile_buffers<T>(DP, 4) * 2 * 32 * KB * DP * (int)sizeof(T) + 4 * DP * 4 + KB * 4;
+  constexpr int KB = key_blocks<T>(DP), bytes = many_lds<T, DP>();
   auto kernel = &cache_tile_kernel<T, DP, RB, KB, ALIGNED>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
@@ -831,16 +893,29 @@ int launch_many(const CacheArgs& a, const CacheCut& c, bool is_prefix, int split
 
 template <typename T, int DP, int NR, bool ALIGNED>
 int launch_few(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
-  constexpr int RB = DP * sizeof(T), WAVES = cache_waves(RB, NR);
-  constexpr int bytes = WAVES * (cache_buffers(RB, NR) * cache_tile(RB) + 16 * NR * 8 + 4);
+  constexpr int WAVES = cache_waves(DP * sizeof(T)), bytes = few_lds<T, DP, NR>();
   auto kernel = &cache_few_kernel<T, DP, NR, ALIGNED>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
   const CacheCut prefix = p.prefix.wave_rows ? CacheCut{} : p.prefix, own = p.own.wave_rows ? CacheCut{} : p.own;
   const int64_t blocks = (prefix.tiles * prefix.splits + own.tiles * own.splits) * a.k_heads;
-  if (!blocks) return 0;
   TSC_REQUIRE(blocks * kWave * WAVES < (1ll << 32), "cache_attention: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, prefix, own, p.splits());
+  TSC_LAUNCH_CHECK("cache_attention");
+  return 0;
+}
+
+template <typename T, int DP, int NR, bool ALIGNED>
+int launch_both(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
+  constexpr int bytes = std::max(many_lds<T, DP>(), few_lds<T, DP, NR>());
+  auto kernel = &cache_both_kernel<T, DP, NR, ALIGNED>;
+  if (bytes > 65536)
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
+  const int64_t first = align_up(p.prefix.tiles * a.k_heads * p.prefix.splits, 8);
+  const int64_t blocks = first + p.own.tiles * a.k_heads * p.own.splits;
+  TSC_REQUIRE(blocks * kWave * 4 < (1ll << 32), "cache_attention: too many tiles");
+  kernel<<<static_cast<unsigned>(blocks), kWave * 4, bytes, s>>>(a, p.prefix, p.own, p.splits(),
+                                                                 static_cast<int>(first));
   TSC_LAUNCH_CHECK("cache_attention");
   return 0;
 }
@@ -906,8 +981,25 @@ int launch_parts(const AttendArgs& a, int splits, hipStream_t s) {
   return 0;
 }
 
+// f<NR>() for the plan's rows of a tile, of those that there are.
+template <int MOST, typename F>
+int with_row_blocks(int row_blocks, F&& f) {
+  if constexpr (MOST >= 4)
+    if (row_blocks == 4) return f(std::integral_constant<int, 4>{});
+  if constexpr (MOST >= 2)
+    if (row_blocks == 2) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 1>{});
+}
+
 template <typename T, int DP, bool ALIGNED>
 int launch_rows(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
+  constexpr int MOST = cache_row_blocks(DP * sizeof(T));
+  const bool few = !p.own.wave_rows || (p.prefix.splits && !p.prefix.wave_rows);
+  if (!p.own.wave_rows && p.prefix.wave_rows == 1 && cache_both<T>(DP))
+    return with_row_blocks<MOST>(p.row_blocks, [&](auto nr) {
+      if constexpr (cache_both<T>(DP)) return launch_both<T, DP, nr, ALIGNED>(a, p, s);
+      return 0;
+    });
   for (const CacheCut* c : {&p.prefix, &p.own}) {
     if (!c->splits || !c->wave_rows) continue;
     int rc = 0;
@@ -916,12 +1008,8 @@ int launch_rows(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
     if (c->wave_rows == 1) rc = launch_many<T, DP, 1, ALIGNED>(a, *c, c == &p.prefix, p.splits(), s);
     if (rc) return rc;
   }
-  constexpr int MOST = cache_row_blocks(DP * sizeof(T));
-  if constexpr (MOST >= 4)
-    if (p.row_blocks == 4) return launch_few<T, DP, 4, ALIGNED>(a, p, s);
-  if constexpr (MOST >= 2)
-    if (p.row_blocks == 2) return launch_few<T, DP, 2, ALIGNED>(a, p, s);
-  return launch_few<T, DP, 1, ALIGNED>(a, p, s);
+  if (!few) return 0;
+  return with_row_blocks<MOST>(p.row_blocks, [&](auto nr) { return launch_few<T, DP, nr, ALIGNED>(a, p, s); });
 }
 
 template <typename T, bool ALIGNED>
