@@ -272,6 +272,9 @@ struct Stager {
 template <typename T, int DP, int KB, int WAVES, bool ALIGNED>
 struct DenseTiles {
   static constexpr int TILE = 32 * KB * DP * (int)sizeof(T);  // bytes of K, and of V
+  static constexpr int BUFFERS = tile_buffers<T>(DP, WAVES);
+  static constexpr int LOADS = 0;  // a wave's loads of a tile, 0: every wait is for all of them
+  __device__ bool counted() const { return false; }
   Stager<T, DP, KB, WAVES, ALIGNED, false> k;
   Stager<T, DP, KB, WAVES, ALIGNED, true> v;
   __device__ __forceinline__ void begin(const T* k_, int64_t k_row, const T* v_, int64_t v_row, int dim, int wave) {
@@ -435,18 +438,19 @@ constexpr float kFar = 0x1p24f;  // exponents from here on have no fractions in 
 template <typename T, int DP, int RB, int KB, int WAVES, typename Tiles, typename Rows>
 __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, Tiles& tiles, char* lds) {
   constexpr int KT = 32 * KB, ROW_BYTES = DP * sizeof(T);
-  constexpr int BUFFERS = tile_buffers<T>(DP, WAVES), TILE = KT * ROW_BYTES, STEPS = DP * (int)sizeof(T) / 32, DB = DP / 32;
+  constexpr int BUFFERS = Tiles::BUFFERS, TILE = KT * ROW_BYTES, STEPS = DP * (int)sizeof(T) / 32, DB = DP / 32;
   const int lane = threadIdx.x % kWave, half = lane / 32, col = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t wave_row = w.row0 + wave * 32 * RB;
   int lo[RB], hi[RB], lo_first, hi_first, lo_last, hi_last;
+  // rows past the last are copies of it, waves of such rows only see nothing
   w.template wave<RB, 32>(a, wave_row, col, lo, hi, lo_first, hi_first, lo_last, hi_last);
+  if (wave_row >= w.rows) hi_last = 0;
   int4v qf[RB][STEPS];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const uint32_t r = wave_row + rb * 32 + col;
     const int t = w.token(r), g = static_cast<int>(min(r, w.rows - 1) - static_cast<uint32_t>(t) * w.group);
-    if (r >= w.rows) hi[rb] = 0;
     const T* q = static_cast<const T*>(a.q) + (w.q0 + t) * a.q_row + (w.hk * w.group + g) * a.q_head;
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
@@ -608,8 +612,7 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, 
   for (;;) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      // (rows past the last need none: their scores are all -inf)
-      m[rb] = wave_row + rb * 32 + col < w.rows ? -__builtin_inff() : 0.f;
+      m[rb] = -__builtin_inff();
       mc[rb] = l[rb][0] = l[rb][1] = 0.f;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[rb][db] = f32x16(0.f);
@@ -628,7 +631,16 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, 
       }
     }
     for (int t = w.t0; t < w.t1; ++t, buf = buf + 1 == BUFFERS ? 0 : buf + 1) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (Tiles::LOADS && tiles.counted()) {  // all but the tiles behind this one
+        const int behind = min(w.t1 - 1 - t, BUFFERS - 2);
+        for_each_index(
+            [&](auto n) {
+              if (behind == n) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(n * Tiles::LOADS) : "memory");
+            },
+            std::make_integer_sequence<int, BUFFERS - 1>{});
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
       __syncthreads();
       const int j0_now = j0, end_now = end;
       if (t + 1 < w.t1) {
@@ -663,14 +675,12 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, 
         for (int kb = 0; kb < KB; ++kb) {
           const int jk = j0_now + kb * 32;
           if (jk >= min(hi_last, end_now) || (jk + 32 <= lo_first && jk >= a.sinks)) continue;
-          const bool whole = jk + 32 <= min(end_now, hi_first) && (jk >= lo_last || jk + 32 <= a.sinks) &&
-                             wave_row + 32 * RB <= w.rows;
+          const bool whole = jk + 32 <= min(end_now, hi_first) && (jk >= lo_last || jk + 32 <= a.sinks);
           key_step(whole, kt, vt, kb, j0_now, end_now);
         }
       } else {
         if (j0_now >= hi_last || (j0_now + KT <= lo_first && j0_now >= a.sinks)) continue;
-        const bool whole = j0_now + KT <= min(end_now, hi_first) &&
-                           (j0_now >= lo_last || j0_now + KT <= a.sinks) && wave_row + 32 * RB <= w.rows;
+        const bool whole = j0_now + KT <= min(end_now, hi_first) && (j0_now >= lo_last || j0_now + KT <= a.sinks);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) key_step(whole, kt, vt, kb, j0_now, end_now);
       }

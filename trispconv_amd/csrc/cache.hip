@@ -14,6 +14,36 @@ namespace {
 
 constexpr int kCus = 256;
 
+// The form for many rows (of `lists` lists): 64 rows a wave or 32, and the parts,
+// by what they cost by this account (in us): rounds of workgroups over the slots that the CUs have,
+// each walking its part at what a key costs there; a round that leaves slots free
+// gains up to 30%; more parts have more sums to write and join.  20k keys, 18
+// tiles of 256 rows on 4 heads: 128 us in seven parts of one round, 155 in eight;
+// 141 with 128 rows.  2 x 32k keys, 64 tiles: 615 us in two parts, 833 in one
+// (half the slots), 671 with 128 rows.
+CacheCut many_cut(int64_t rows, int64_t lists, int64_t heads, int64_t keys_of_row, int64_t keys_per_tile_row, int dim, int elem) {
+  const int row_bytes = padded_dim(dim) * elem;
+  CacheCut best;
+  double least = 0;
+  for (int w = can_pair(padded_dim(dim), elem) ? 2 : 1; w >= 1; --w) {
+    const int per_cu = many_per_cu(row_bytes, w);
+    const int64_t keys = keys_of_row + keys_per_tile_row * 128 * w;
+    const double key = (w == 2 ? 0.0375 : row_bytes <= 128 ? 0.0336 : 0.0375 * row_bytes / 256) * (elem == 4 ? 4 : 1);
+    // (lists of few tiles round up one by one; of many, some are shorter than others)
+    const int64_t each = rows / lists, tile = 128 * w;
+    const int64_t units = (each < 2 * tile ? lists * ceil_div(each, tile) : ceil_div(rows, tile)) * heads;
+    for (int64_t parts = 1; parts == 1 || (parts <= keys / 512 && parts <= 16); ++parts) {
+      const int64_t a_cu = ceil_div(units * parts, kCus), rest = a_cu % per_cu;
+      const double rounds = a_cu / per_cu + (rest ? 0.7 + 0.3 * rest / per_cu : 0);
+      const double us = rounds * (4 + keys * key / parts) +
+                        (parts > 1 ? 6 + parts * rows * heads * (dim + 2) * 8 / 4e6 : 0);
+      if (best.wave_rows && us >= least) continue;
+      least = us, best.wave_rows = w, best.splits = static_cast<int>(parts);
+    }
+  }
+  return best;
+}
+
 // longest: positions a sample may have, prefix_rows of them shared.
 CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t prefix_rows, int q_heads, int k_heads,
                      int dim, int elem, int left, int right, int sinks) {
@@ -22,49 +52,50 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
   const int row_bytes = padded_dim(dim) * elem, kt = cache_keys(row_bytes);
   p.row_blocks = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
   while (p.row_blocks > cache_row_blocks(row_bytes)) p.row_blocks /= 2;
-  // lists: of the rows that `tiles` are cut from; mean: rows of such a list
-  auto cut = [&](int64_t keys, int64_t lists, int64_t mean) {
+  const int64_t rows = 16 * p.row_blocks;
+  // own keys that rows of a sample can see at most: each of them, and with every
+  // row more of the tile
+  int64_t span = std::max<int64_t>(longest - prefix_rows, 0), per_row = 0;
+  if (left >= 0) {
+    const int64_t seen = (int64_t)left + sinks + kt + (right >= 0 ? right : n_q);
+    if (seen < span) span = seen, per_row = right >= 0;
+  }
+  // Few rows against `keys`: parts of 256 to 2048 keys (4096 where a workgroup has
+  // a CU to itself), one round of workgroups where that allows it: 64 samples of up
+  // to 32k keys in parts of 2048 276 us, of 512 321, of 8192 295; 24 windows of
+  // 4096 in one round of 1024 27 us, in two of 768 30.  Up to 1024 keys by
+  // themselves are not worth a join (13 us, in parts 17).
+  auto few = [&](int64_t keys, int64_t tiles, int64_t units) {
     CacheCut c;
-    auto tiles = [&](int64_t rows) { return lists == 1 ? ceil_div(all, rows) : all / rows + std::min(lists, n_q); };
     if (sinks > 0) keys += kt;  // (a tile of their own)
-    // workgroups that do something, and those that the CUs hold at once
-    auto units = [&](int64_t rows) { return std::max<int64_t>(1, lists * ceil_div(mean, rows)) * k_heads; };
-    if (mean <= 64) {
-      const int64_t rows = 16 * p.row_blocks;
-      c.tiles = tiles(rows);
-      // Parts of 256 to 2048 keys (4096 where a workgroup has a CU to itself), one
-      // round of workgroups where that allows it: 64 samples of up to 32k keys in
-      // parts of 2048 276 us, of 512 321, of 8192 295; 24 windows of 4096 in one
-      // round of 1024 27 us, in two of 768 30.  Up to 1024 keys by themselves are
-      // not worth a join (14 us, in parts 17).
-      const int per_cu = cache_per_cu(row_bytes);
-      const int64_t want = std::max<int64_t>(1, per_cu * kCus / units(rows));
-      int64_t chunk = std::min<int64_t>(std::max<int64_t>(ceil_div(keys, want), 256), 4096 / per_cu);
-      if (!prefix_rows && keys <= 1024) chunk = keys;
-      chunk = std::max(chunk, ceil_div(keys, kMostSplits / 2));
-      c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), kt * cache_waves(row_bytes)));
-      c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
-      return c;
-    }
-    // as attend_cut
-    c.wave_rows = can_pair(padded_dim(dim), elem) && keys >= 4096 && units(256) >= 2 * kCus ? 2 : 1;
-    const int64_t work = units(128 * c.wave_rows);
-    c.tiles = tiles(128 * c.wave_rows);
-    // One round of workgroups, of 512 keys and more (20k keys in 136 tiles, four
-    // workgroups a CU: 141 us in seven parts, 166 in six, 239 in three); beside
-    // the samples' own keys one a CU (a prefix of 32k keys in 8 tiles: 42 us in 32
-    // parts, 45 in 64, 61 in 128)
-    const bool beside = lists == 1 && prefix_rows && all / samples <= 64 && row_bytes <= 128;
-    const int64_t per_cu = beside ? 1 : row_bytes <= 128 ? 4 / c.wave_rows : row_bytes <= 256 ? 2 : 1;
-    const int64_t slots = per_cu * kCus;
-    c.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({keys / 512, slots / work, kMostSplits / 2})));
+    const int per_cu = cache_per_cu(row_bytes);
+    const int64_t want = std::max<int64_t>(1, per_cu * kCus / std::max<int64_t>(1, units * k_heads));
+    int64_t chunk = std::min<int64_t>(std::max<int64_t>(ceil_div(keys, want), 256), 4096 / per_cu);
+    if (!prefix_rows && keys <= 1024) chunk = keys;
+    chunk = std::max(chunk, ceil_div(keys, kMostSplits / 2));
+    c.tiles = tiles;
+    c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), kt * cache_waves(row_bytes)));
+    c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
     return c;
   };
-  // keys that a tile of a sample's rows can see at most
-  int64_t span = std::max<int64_t>(longest - prefix_rows, 0);
-  if (left >= 0) span = std::min<int64_t>(span, (int64_t)left + n_q + sinks + kt);
-  p.own = cut(span, samples, mean);
-  if (prefix_rows) p.prefix = cut(prefix_rows, 1, all);
+  if (mean <= 64) {
+    p.own = few(span + per_row * rows, all / rows + std::min(samples, n_q), samples * ceil_div(mean, rows));
+  } else {
+    p.own = many_cut(all, samples, k_heads, span, per_row, dim, elem);
+    p.own.tiles = all / (128 * p.own.wave_rows) + std::min(samples, n_q);
+  }
+  if (prefix_rows && all <= 64) {
+    p.prefix = few(prefix_rows, ceil_div(all, rows), ceil_div(all, rows));
+  } else if (prefix_rows && mean <= 64 && row_bytes <= 128) {
+    // beside the samples' own keys (cache_both_kernel), one workgroup a CU and 512
+    // keys at least: 32k keys in 8 tiles 42 us in 32 parts, 45 in 64, 61 in 128
+    p.prefix.wave_rows = 1, p.prefix.tiles = ceil_div(all, 128);
+    p.prefix.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({prefix_rows / 512, kCus / (p.prefix.tiles * k_heads), kMostSplits / 2})));
+  } else if (prefix_rows) {
+    p.prefix = many_cut(all, 1, k_heads, prefix_rows, 0, dim, elem);
+    p.prefix.tiles = ceil_div(all, 128 * p.prefix.wave_rows);
+  }
   p.own.first_split = p.prefix.splits;
   return p;
 }

@@ -63,6 +63,15 @@ constexpr int cache_waves(int row_bytes) {
 constexpr int cache_buffers(int row_bytes) {
   return cache_lds(row_bytes) / (cache_waves(row_bytes) * cache_tile(row_bytes));
 }
+// The form for many rows: key blocks of a tile and its buffers (8k rows, 16 heads of
+// 64, bf16: 333 us with three, 364 with two; rows of 256 bytes have no room for
+// more at two workgroups a CU, and halved tiles cost them 30%).
+constexpr int many_key_blocks(int row_bytes) { return row_bytes <= 512 ? 2 : 1; }
+constexpr int many_buffers(int row_bytes) { return row_bytes <= 192 ? 3 : 2; }
+// Its workgroups a CU (row_blocks: 32s of rows a wave).
+constexpr int many_per_cu(int row_bytes, int row_blocks) {
+  return row_bytes <= 128 ? 4 - row_blocks : row_bytes <= 256 ? 2 : 1;
+}
 // Rows of a tile in 16s at most: queries and sums stay in the registers.
 constexpr int cache_row_blocks(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
 
@@ -141,6 +150,20 @@ struct PageIds {
 // Positions of sample b.
 __device__ __forceinline__ int kept(const CacheArgs& a, int b) {
   return a.pages.cut(a.pages.lengths[b]);
+}
+
+// Tiles of `rows` query rows of all samples.
+__device__ __forceinline__ int64_t count_tiles(const CacheArgs& a, int group, int rows) {
+  const int lane = threadIdx.x % kWave;
+  int64_t all = 0;
+  for (int b0 = 0; b0 < a.samples; b0 += kWave) {
+    int64_t at = 0;
+    int len = 0;
+    if (b0 + lane < a.samples) sample_range(a.off_q, b0 + lane, a.n_q, at, len);
+    const uint32_t inc = wave_inclusive(static_cast<uint32_t>(((int64_t)len * group + rows - 1) / rows));
+    all += __builtin_amdgcn_readlane(inc, kWave - 1);
+  }
+  return all;
 }
 
 // The sample and the tile of query rows within it of the x-th tile of all (as
@@ -731,11 +754,13 @@ __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)), (cache_wav
 // are those nearest to them again.
 template <typename T, int DP, int KB, int WAVES, bool ALIGNED>
 struct PagedTiles {
-  static constexpr int TILE = 32 * KB * DP * (int)sizeof(T), KT = 32 * KB;
+  static constexpr int TILE = 32 * KB * DP * (int)sizeof(T), KT = 32 * KB, BUFFERS = many_buffers(DP * sizeof(T));
   using K = Stager<T, DP, KB, WAVES, ALIGNED, false>;
   using V = Stager<T, DP, KB, WAVES, ALIGNED, true>;
   // rows that an instruction of the workgroup brings
   static constexpr int UNIT = K::SAME ? K::THREADS / K::CH : KT;
+  static constexpr int LOADS = ALIGNED ? K::ROUNDS + V::ROUNDS : 0;
+  static_assert((BUFFERS - 2) * LOADS <= 63, "the wait counts to 63");
   K k;
   V v;
   const CacheArgs* args;
@@ -749,6 +774,8 @@ struct PagedTiles {
     ids.begin(table, w.entries(), a.pages.pages);
     start = w.start, first = w.first_seen(lo_first);
   }
+  // (where chunks are left out, a wave may have fewer loads)
+  __device__ bool counted() const { return k.dim >= DP; }
   __device__ __forceinline__ void clear(char* tile) const {
     k.clear(tile);
     v.clear(tile + TILE);
@@ -818,32 +845,55 @@ __device__ __forceinline__ void cache_many(const CacheArgs& a, const CacheCut& c
     if (first > 0 || last < a.n_q)
       zero_outside(static_cast<T*>(a.out), (int64_t)a.q_heads * a.dim, first, last, a.n_q);
   }
-  // tiles that walk the same keys next to each other on one XCD (workgroups go
-  // round the eight in turn), so that its L2 reads them once
-  const int64_t blocks = cut.tiles * a.k_heads * cut.splits, per = (blocks + 7) / 8;
-  const int64_t id = (blockIdx.x % 8) * per + blockIdx.x / 8;
-  if (blockIdx.x / 8 >= per || id >= blocks) return;
+  // Tiles that walk the same keys next to each other on one XCD (workgroups go
+  // round the eight in turn), so that its L2 reads them once.  The tiles that
+  // there are, not those that there might be, are shared out evenly: one more
+  // than an XCD holds at once and all wait for it (8k rows, 16 heads on 4: 317 us,
+  // with 65 for 64 places 467).
   CacheWalk w;
   w.group = a.q_heads / a.k_heads;
-  w.hk = static_cast<int>(id / cut.tiles / cut.splits);
+  const int64_t there = is_prefix ? cut.tiles : count_tiles(a, w.group, ROWS), units = there * a.k_heads;
+  // Of the host's parts as many as make the fewest rounds of them (a_cu: a CU's).
+  int parts = is_prefix ? cut.splits : 1;
+  int64_t a_cu = (units + 255) / 256;
+  for (int n = 2; n <= cut.splits && !is_prefix; ++n) {
+    const int64_t next = (units * n + 255) / 256, per_cu = many_per_cu(DP * sizeof(T), RB);
+    if ((next + per_cu - 1) / per_cu * parts < (a_cu + per_cu - 1) / per_cu * n) parts = n, a_cu = next;
+  }
+  const int64_t blocks = units * parts, per = (blocks + 7) / 8;
+  int64_t id = blockIdx.x / 8 < per ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+  if (id >= units * cut.splits) return;
+  const bool idle = id >= blocks;  // a part that is not made says so
+  if (idle) id -= blocks;
+  const int64_t rest = id / there;
+  const int split = static_cast<int>(idle ? parts + rest / a.k_heads : rest % parts);
+  w.hk = static_cast<int>(idle ? rest % a.k_heads : rest / parts);
+  w.split = cut.first_split + split;
+  w.splits = splits;
   int from, to;
-  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id % cut.tiles), from, to)) return;
+  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id % there), from, to)) return;
+  if (idle) {
+    for (uint32_t r = w.row0 + threadIdx.x; r < w.row0 + ROWS && r < w.rows; r += kWave * 4) {
+      const int64_t at = w.split * a.rows() + (w.q0 + w.token(r)) * a.q_heads + w.head(r);
+      a.part[2 * at] = -__builtin_inff();
+      a.part[2 * at + 1] = 0.f;
+    }
+    return;
+  }
   int lo_first = 0, hi_first, lo_last, hi_last = to;
   // (the rows of all samples: every key of the prefix, most of them see it whole)
   if (!is_prefix) w.bounds(a, w.row0, w.row0 + ROWS - 1, lo_first, hi_first, lo_last, hi_last);
   const int tiles = w.place(lo_first, hi_last, from, to, KT, a.pages.page_rows % Tiles::UNIT == 0 ? KT : 1);
-  const int split = static_cast<int>(id / cut.tiles % cut.splits), each = (tiles + cut.splits - 1) / cut.splits;
+  const int each = (tiles + parts - 1) / parts;
   w.t0 = min(split * each, tiles);
   w.t1 = min(w.t0 + each, tiles);
-  w.split = cut.first_split + split;
-  w.splits = splits;
   Tiles kv;
   kv.begin(a, w, lo_first, __builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
   attend_walk<T, DP, RB, KB, 4>(a, w, kv, lds);
 }
 
 template <typename T, int DP, int RB, int KB, bool ALIGNED>
-__global__ void __launch_bounds__(kWave * 4, waves_per_simd<T>(DP, RB, 4))
+__global__ void __launch_bounds__(kWave * 4, many_per_cu(DP * sizeof(T), RB))
     cache_tile_kernel(CacheArgs a, CacheCut cut, int is_prefix, int splits) {
   extern __shared__ __align__(16) char lds[];
   cache_many<T, DP, RB, KB, ALIGNED>(a, cut, is_prefix, splits, lds);
@@ -857,7 +907,7 @@ __global__ void __launch_bounds__(kWave * 4, 2)
     cache_both_kernel(CacheArgs a, CacheCut prefix, CacheCut own, int splits, int prefix_blocks) {
   extern __shared__ __align__(16) char lds[];
   if ((int)blockIdx.x < prefix_blocks)
-    cache_many<T, DP, 1, key_blocks<T>(DP), ALIGNED>(a, prefix, true, splits, lds);
+    cache_many<T, DP, 1, many_key_blocks(DP * sizeof(T)), ALIGNED>(a, prefix, true, splits, lds);
   else
     cache_few<T, DP, NR, ALIGNED>(a, own, false, splits, blockIdx.x - prefix_blocks, lds);
 }
@@ -869,8 +919,8 @@ constexpr bool cache_both(int dp) {
 
 template <typename T, int DP>
 constexpr int many_lds() {
-  constexpr int KB = key_blocks<T>(DP);
-  return tile_buffers<T>(DP, 4) * 2 * 32 * KB * DP * (int)sizeof(T) + 4 * DP * 4 + KB * 4;
+  constexpr int RB = DP * sizeof(T), KB = many_key_blocks(RB);
+  return many_buffers(RB) * 2 * 32 * KB * RB + 4 * DP * 4 + KB * 4;
 }
 template <typename T, int DP, int NR>
 constexpr int few_lds() {
@@ -880,7 +930,7 @@ constexpr int few_lds() {
 
 template <typename T, int DP, int RB, bool ALIGNED>
 int launch_many(const CacheArgs& a, const CacheCut& c, bool is_prefix, int splits, hipStream_t s) {
-  constexpr int KB = key_blocks<T>(DP), bytes = many_lds<T, DP>();
+  constexpr int KB = many_key_blocks(DP * sizeof(T)), bytes = many_lds<T, DP>();
   auto kernel = &cache_tile_kernel<T, DP, RB, KB, ALIGNED>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
