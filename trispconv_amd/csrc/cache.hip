@@ -69,10 +69,12 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     CacheCut c;
     if (sinks > 0) keys += kt;  // (a tile of their own)
     const int per_cu = cache_per_cu(row_bytes);
-    const int64_t want = std::max<int64_t>(1, per_cu * kCus / std::max<int64_t>(1, units * k_heads));
+    const int64_t slots = per_cu * kCus, lists = std::max<int64_t>(1, units * k_heads);
+    const int64_t want = std::max<int64_t>(1, slots / lists);
     int64_t chunk = std::min<int64_t>(std::max<int64_t>(ceil_div(keys, want), 256), 4096 / per_cu);
     if (!prefix_rows && keys <= 1024) chunk = keys;
-    chunk = std::max(chunk, ceil_div(keys, kMostSplits / 2));
+    // (and no more than 16 rounds are worth their parts' memory)
+    chunk = std::max({chunk, ceil_div(keys, kMostSplits / 2), ceil_div(keys, std::max<int64_t>(1, 16 * slots / lists))});
     c.tiles = tiles;
     c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), kt * cache_waves(row_bytes)));
     c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));

@@ -975,12 +975,8 @@ int launch_both(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
 // workgroup per row 25 us.)
 constexpr int kFewParts = 16;
 
-template <typename T, int VALUES>
-__global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a, int splits) {
-  constexpr int LANES = VALUES / 4, GROUPS = kWave / LANES;
-  const int64_t item = blockIdx.x * (int64_t)4 + threadIdx.x / kWave, step = a.rows();
-  if (item >= step) return;
-  const int lane = threadIdx.x % kWave, c = lane % LANES, d = 4 * c;
+template <typename T, int LANES, int GROUPS>
+__device__ __forceinline__ void join_row(const AttendArgs& a, int splits, int64_t item, int64_t step, int lane, int d) {
   const float* ml = a.part + 2 * item;
   const float* o = a.part + a.part_values(splits) + item * a.dim + d;
   float m = -__builtin_inff(), l = 0.f;
@@ -1020,10 +1016,20 @@ __global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a, int split
     if (d + i < a.dim) out[d + i] = from_f32<T>(none ? 0.f : sum[i] / l);
 }
 
+template <typename T, int VALUES>
+__global__ void __launch_bounds__(256) cache_join_kernel(AttendArgs a, int splits) {
+  constexpr int LANES = VALUES / 4, GROUPS = kWave / LANES;
+  const int64_t step = a.rows();
+  const int lane = threadIdx.x % kWave, c = lane % LANES, d = 4 * c;
+  for (int64_t item = blockIdx.x * (int64_t)4 + threadIdx.x / kWave; item < step; item += gridDim.x * (int64_t)4)
+    join_row<T, LANES, GROUPS>(a, splits, item, step, lane, d);
+}
+
 template <typename T>
 int launch_parts(const AttendArgs& a, int splits, hipStream_t s) {
-  if (splits > kFewParts) return launch_join<T>(a, splits, s);
-  const unsigned blocks = static_cast<unsigned>(ceil_div(a.rows(), 4));
+  // (a launch holds fewer than 2^32 threads)
+  if (splits > kFewParts && a.rows() < (1 << 20)) return launch_join<T>(a, splits, s);
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(ceil_div(a.rows(), 4), 1 << 22));
   if (a.dim <= 64) cache_join_kernel<T, 64><<<blocks, 256, 0, s>>>(a, splits);
   else if (a.dim <= 128) cache_join_kernel<T, 128><<<blocks, 256, 0, s>>>(a, splits);
   else cache_join_kernel<T, 256><<<blocks, 256, 0, s>>>(a, splits);
