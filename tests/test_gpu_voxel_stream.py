@@ -141,3 +141,17 @@ def test_a_step_without_voxels():
     cache = _cache(layers=1)
     assert _step([block], _input((0, 0, 0)), cache).features.shape == (0, 32)
     assert cache.rows() == [0, 0, 0]
+
+
+def test_document_example():
+    """The stream shown in the boundary document, as written there."""
+    import re
+    from pathlib import Path
+    text = (Path(__file__).resolve().parent.parent / "INTEGRATION.md").read_text()
+    block = re.findall(r"```python\n(.*?)```", text.split("## Streams of voxels", 1)[1], flags=re.S)[0]
+    names: dict = {}
+    exec(compile(block, "INTEGRATION.md", "exec"), names)
+    for i, rows in enumerate([(300, 0, 171), (5, 1, 1)]):
+        y = names["step"](_input(rows, channels=16, dtype=torch.float16, seed=i))
+        assert y.features.shape == (sum(rows), 128) and torch.isfinite(y.features).all()
+    assert names["cache"].rows() == [305, 1, 172]

@@ -274,6 +274,9 @@ struct DenseTiles {
   static constexpr int TILE = 32 * KB * DP * (int)sizeof(T);  // bytes of K, and of V
   static constexpr int BUFFERS = tile_buffers<T>(DP, WAVES);
   static constexpr int LOADS = 0;  // a wave's loads of a tile, 0: every wait is for all of them
+  static constexpr bool STRAIGHT = false;  // 32-row waves take whole tiles without a branch too
+  // (16-byte stores of parts put ten more registers of heads of 64 into scratch)
+  static constexpr bool WIDE_PARTS = false;
   __device__ bool counted() const { return false; }
   Stager<T, DP, KB, WAVES, ALIGNED, false> k;
   Stager<T, DP, KB, WAVES, ALIGNED, true> v;
@@ -671,6 +674,12 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, 
       // or by the tile where a wave has so many rows that it sees nearly all
       // (the blocks of keys then follow each other without a branch)
       if constexpr (RB == 1) {
+        if (Tiles::STRAIGHT && j0_now + KT <= min(end_now, min(hi_first, hi_last)) &&
+            (j0_now >= lo_last || j0_now + KT <= a.sinks)) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) key_step(true, kt, vt, kb, j0_now, end_now);
+          continue;
+        }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const int jk = j0_now + kb * 32;
@@ -719,11 +728,11 @@ __device__ __forceinline__ void attend_walk(const AttendArgs& a, const Rows& w, 
           for (int i = 0; i < 4; ++i) {
             const int d = 32 * db + 8 * i + 4 * half;
             const f32x4 x = {o[rb][db][4 * i], o[rb][db][4 * i + 1], o[rb][db][4 * i + 2], o[rb][db][4 * i + 3]};
-            if (d + 4 <= a.dim) {
+            if (Tiles::WIDE_PARTS && d + 4 <= a.dim) {
               __builtin_memcpy(part + d, &x, 16);
             } else {
 #pragma unroll
-              for (int y = 0; y < 3; ++y)
+              for (int y = 0; y < 4; ++y)
                 if (d + y < a.dim) part[d + y] = x[y];
             }
           }

@@ -405,9 +405,13 @@ struct PagedStager {
   }
 };
 
-// Few query rows (16 NR) against many keys (rows past the last are copies of it): the keys of a workgroup's chunk are
-// shared out over its waves, each with tiles of its own in LDS and no barrier
-// between them, and the waves' sums meet in LDS at the end.
+// Few query rows (16 NR; rows past the last are copies of it) against many keys:
+// the keys of a workgroup's chunk are shared out over its waves, each with tiles
+// of its own in LDS and no barrier between them, and the waves' sums meet in LDS
+// at the end.  Bound by memory: 64 samples of 14k to 33k keys, 16 heads on 4 of 64,
+// bf16, 1.53 GB in 276 us, 5.5 TB/s (a large copy on this card: 4.87).  Small
+// calls are bound by what comes before the first tile: arguments, offsets, page
+// numbers and keys are dependent reads, 4 of the 12 us of 4 x 900 keys.
 //
 // Scores are kept transposed as in attend.hpp, S^T = K Q^T, in 16x16 tiles: a lane
 // has four keys of one row per 16, which are, as they stand, the right operand of
@@ -761,6 +765,10 @@ struct PagedTiles {
   static constexpr int UNIT = K::SAME ? K::THREADS / K::CH : KT;
   static constexpr int LOADS = ALIGNED ? K::ROUNDS + V::ROUNDS : 0;
   static_assert((BUFFERS - 2) * LOADS <= 63, "the wait counts to 63");
+  // (2 x 2048 rows over 32k keys, heads of 128, bf16: 1153 us, 1199 with the branch;
+  // 1-2% slower for heads of 64, and those of 256 have no registers left)
+  static constexpr bool STRAIGHT = kIs16<T> && DP == 128;
+  static constexpr bool WIDE_PARTS = true;
   K k;
   V v;
   const CacheArgs* args;
@@ -833,7 +841,10 @@ struct PagedTiles {
   __device__ PagedRows<T> v_rows() const { return {v.src, args->v_at.page, v.stride, table, &args->pages}; }
 };
 
-// Many query rows: attend_walk's tiles, over pages.  lds: as attend_kernel's.
+// Many query rows: attend_walk's tiles, over pages.  lds: as attend_kernel's.  Bound
+// as attend_walk is, by vector instructions and products that overlap little: 2 x
+// 2048 rows over 32k keys, 16 heads on 4, bf16, 1153 us with heads of 128 (0.88
+// PFLOP/s; a library product's rate on this card 1.13), 616 us with heads of 64 (0.82).
 template <typename T, int DP, int RB, int KB, bool ALIGNED>
 __device__ __forceinline__ void cache_many(const CacheArgs& a, const CacheCut& cut, bool is_prefix, int splits,
                                            char* lds) {
