@@ -134,9 +134,12 @@ def test_cache_extend():
 def test_cache_share_and_drop():
     c = _cache()
     c.extend([20, 0, 0])
-    for bad in ((0, [1], 20), (0, [1], 24), (0, [1, 1], 16), (0, [0], 8), (1, [2], 8), (0, [1], -8)):
+    for bad in ((0, [1], 20), (0, [1], 24), (0, [1, 1], 16), (0, [0], 8), (1, [2], 8), (0, [1], -8),
+                (0, [2, -1], 8), (0, [3], 8), (-3, [1], 8)):
         with pytest.raises(ValueError):
             c.share(*bad)
+    with pytest.raises(ValueError):
+        c.drop([0, 3])
     c.share(0, [1, 2], 16)
     assert c.rows() == [20, 16, 16] and c.free_pages() == 5
     assert _entries(c, 1) == _entries(c, 2) == _entries(c, 0)[:2]

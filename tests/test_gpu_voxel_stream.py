@@ -123,6 +123,10 @@ def test_captured_step():
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
+        for refused in (lambda: captured.extend([1, 1, 1]), lambda: captured.drop([0]),
+                        lambda: captured.share(0, [], 16)):
+            with pytest.raises(RuntimeError, match="captured"):
+                refused()
         out = block(inputs, captured, 0).features
     for i, x in enumerate(parts):
         if i:

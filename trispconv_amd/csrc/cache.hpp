@@ -1097,7 +1097,7 @@ int launch_cache(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
   const int64_t e = kPer16<T>;
   // 16-byte pieces at 16-byte addresses, rows of a tile within 32-bit offsets
   auto whole = [&](const void* base, const PageStrides& at) {
-    return at.row < (1 << 24) && at.row % e == 0 && at.page % e == 0 && at.head % e == 0 &&
+    return at.row >= 0 && at.row < (1 << 24) && at.row % e == 0 && at.page % e == 0 && at.head % e == 0 &&
            reinterpret_cast<uintptr_t>(base) % 16 == 0;
   };
   const bool aligned = a.dim % e == 0 && whole(a.k, a.k_at) && whole(a.v, a.v_at);

@@ -212,25 +212,50 @@ class VoxelCache:
         self._pages: List[List[int]] = [[] for _ in range(samples)]
         self._users = [0] * pages
         self._free = list(range(pages - 1, -1, -1))
-        self._common = 0
+        self._used = 0           # the longest row of the table
+        self._first = None       # a sample that keeps something
+        self._common = 0         # pages that all those begin with
 
-    def _publish(self, pages_changed: bool) -> None:
-        """The host's state to the device."""
-        if pages_changed:
+    def _give(self, b: int, pages: List[int]) -> None:
+        """Appends pages to sample b's."""
+        at = len(self._pages[b])
+        self._entries[b, at:at + len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        self._pages[b] = self._pages[b] + pages
+
+    def _publish(self, pages: bool, samples: bool) -> None:
+        """The host's state to the device; whether a sample's pages have changed, and
+        whether they can begin differently now (new pages at an end cannot)."""
+        if pages:
             self.table.copy_(self._entries)
-            held = [p for p in self._pages if p]
-            n = 0
+            self._used = max(len(p) for p in self._pages)
+        if samples:
+            held = [b for b, p in enumerate(self._pages) if p]
+            self._first, self._common = (held[0] if held else None), 0
             if len(held) > 1:
-                for column in zip(*held):
-                    if len(set(column)) > 1:
-                        break
-                    n += 1
-            self._common = n
+                first, *others = (self._pages[b] for b in held)
+                n = min(len(p) for p in (first, *others))
+                for p in others:
+                    n = next((i for i in range(n) if p[i] != first[i]), n)
+                self._common = n
         kept = torch.tensor(self._kept, dtype=torch.int32)
         if self.lengths.is_cuda:
             self.lengths.copy_(kept.pin_memory(), non_blocking=True)
         else:
             self.lengths.copy_(kept)
+
+    def _capturing(self) -> bool:
+        return self.table.is_cuda and torch.cuda.is_current_stream_capturing()
+
+    def _check_steps(self) -> None:
+        if self._capturing():
+            raise RuntimeError("VoxelCache: rows are given and dropped between the replays of a "
+                               "captured step, not in it")
+
+    def _check_samples(self, samples: Sequence[int]) -> List[int]:
+        samples = list(samples)
+        if any(not 0 <= b < self.samples for b in samples):
+            raise ValueError(f"VoxelCache: samples {samples}, there are {self.samples}")
+        return samples
 
     def rows(self) -> List[int]:
         """The rows that each sample keeps."""
@@ -242,6 +267,7 @@ class VoxelCache:
     def extend(self, rows: Union[Sequence[int], torch.Tensor]) -> None:
         """Room for ``rows[b]`` new rows behind what sample b keeps, for instance
         ``order.offsets.diff()``.  A ValueError leaves everything as it was."""
+        self._check_steps()
         rows = rows.tolist() if isinstance(rows, torch.Tensor) else [int(n) for n in rows]
         if len(rows) != self.samples or any(n < 0 for n in rows):
             raise ValueError(f"VoxelCache: {rows} new rows for {self.samples} samples")
@@ -252,54 +278,52 @@ class VoxelCache:
         need = [-(-n // self.page_rows) - len(p) for n, p in zip(kept, self._pages)]
         if sum(need) > len(self._free):
             raise ValueError(f"VoxelCache: {sum(need)} pages are needed, {len(self._free)} are free")
+        new = any(n and not p for n, p in zip(need, self._pages))
         for b, n in enumerate(need):
-            for _ in range(n):
-                page = self._free.pop()
-                self._users[page] = 1
-                self._entries[b, len(self._pages[b])] = page
-                self._pages[b].append(page)
+            if n:
+                pages = [self._free.pop() for _ in range(n)]
+                for page in pages:
+                    self._users[page] = 1
+                self._give(b, pages)
         self._kept = kept
-        self._publish(sum(need) > 0)
+        self._publish(sum(need) > 0, new)
 
     def share(self, source: int, targets: Sequence[int], rows: int) -> None:
         """Lets samples that keep nothing begin with the first ``rows`` rows of
         ``source``, in the same pages: whole pages, so a multiple of page_rows."""
+        self._check_steps()
+        targets = self._check_samples([source, *targets])[1:]
         if rows % self.page_rows or not 0 <= rows <= self._kept[source]:
             raise ValueError(f"VoxelCache: {rows} rows of sample {source}, which keeps "
                              f"{self._kept[source]}, are not whole pages of {self.page_rows}")
-        targets = list(targets)
         if len(set(targets)) < len(targets) or any(self._kept[b] for b in targets):
             raise ValueError(f"VoxelCache: samples {targets} must be different and keep nothing")
         pages = self._pages[source][:rows // self.page_rows]
+        for page in pages:
+            self._users[page] += len(targets)
         for b in targets:
-            for i, page in enumerate(pages):
-                self._users[page] += 1
-                self._entries[b, i] = page
-            self._pages[b] = list(pages)
+            self._give(b, pages)
             self._kept[b] = rows
-        self._publish(True)
+        self._publish(True, True)
 
     def drop(self, samples: Sequence[int]) -> None:
         """Forgets what these samples keep; pages that no other sample has are free again."""
-        for b in samples:
+        self._check_steps()
+        for b in self._check_samples(samples):
             for page in reversed(self._pages[b]):
                 self._users[page] -= 1
                 if not self._users[page]:
                     self._free.append(page)
             self._pages[b], self._kept[b] = [], 0
-        self._publish(True)
+        self._publish(True, True)
 
     def _tables(self) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         """The table as far as it is used, and the pages that all samples begin
         with; a captured step takes the whole table, which later steps fill."""
-        if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+        if self._capturing():
             return self.table, None
-        used = max(len(p) for p in self._pages)
-        table = self.table[:, :used]
-        if not self._common:
-            return table, None
-        first = next(b for b, p in enumerate(self._pages) if p)
-        return table, self.table[first, :self._common]
+        table = self.table[:, :self._used]
+        return table, self.table[self._first, :self._common] if self._common else None
 
     def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                positions: torch.Tensor, offsets: torch.Tensor,
