@@ -112,27 +112,26 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     return out
 
 
-def _position_rows(positions: torch.Tensor, q: torch.Tensor,
-                   what: str) -> Tuple[torch.Tensor, int, bool]:
-    """Checked positions, their row stride and whether they are float32."""
-    in_f32 = positions.dtype is torch.float32
-    if positions.dim() != 2 or positions.shape[0] != q.shape[0] or \
-            positions.get_device() != q.get_device() or \
-            not (in_f32 or positions.dtype is torch.int32):
-        raise ValueError(f"{what}: positions must be ({q.shape[0]}, axes) int32 or float32 on "
-                         f"{q.device}")
+def _position_rows(positions: torch.Tensor, q: torch.Tensor, n: int,
+                   what: str) -> Tuple[torch.Tensor, int, int, bool]:
+    """Checked positions of q's n rows, their axes, their row stride and whether
+    they are float32."""
+    dtype, shape = positions.dtype, positions.shape
+    in_f32 = dtype is torch.float32
+    if len(shape) != 2 or shape[0] != n or positions.get_device() != q.get_device() or \
+            not (in_f32 or dtype is torch.int32):
+        raise ValueError(f"{what}: positions must be ({n}, axes) int32 or float32 on {q.device}")
     positions, (row, _) = _rows_of(positions)
-    return positions, row, in_f32
+    return positions, shape[1], row, in_f32
 
 
 def _head_gains(q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
-                q: torch.Tensor, hk: int, what: str):
+                q: torch.Tensor, hq: int, hk: int, dim: int, what: str):
     """Checked gains, and their arguments of a C entry: two pointers, the
     dtype's code and whether each has a gain per head."""
     qg_ptr = kg_ptr = None
     qg_heads = kg_heads = g_code = 0
     if q_weight is not None or k_weight is not None:
-        hq, dim = q.shape[1:]
         device = q.get_device()
         g_dtype = (k_weight if q_weight is None else q_weight).dtype
         g_code = L.dtype_code(g_dtype)
@@ -176,13 +175,13 @@ def norm_rotate_heads(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     _same(k, q, what, "k")
     n, hq, dim = q.shape
     hk = k.shape[1]
-    positions, p_row, in_f32 = _position_rows(positions, q, what)
-    q_weight, k_weight, gains = _head_gains(q_weight, k_weight, q, hk, what)
+    positions, axes, p_row, in_f32 = _position_rows(positions, q, n, what)
+    q_weight, k_weight, gains = _head_gains(q_weight, k_weight, q, hq, hk, dim, what)
     (q, (q_row, q_head, _)), (k, (k_row, k_head, _)) = _rows_of(q), _rows_of(k)
-    q_out, k_out = q.new_empty((n, hq, dim)), q.new_empty((n, hk, dim))
+    q_out, k_out = q.new_empty(n, hq, dim), q.new_empty(n, hk, dim)
     rc = L.lib().tsc_norm_rotate_heads(
         q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, positions.data_ptr(), p_row,
-        in_f32, positions.shape[1], *gains, eps, base, interleaved, code, n, hq, hk, dim,
+        in_f32, axes, *gains, eps, base, interleaved, code, n, hq, hk, dim,
         q_out.data_ptr(), k_out.data_ptr(), L.stream_of(q))
     if rc:
         L.check(rc, what)
