@@ -81,7 +81,13 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     return c;
   };
   if (mean <= 64) {
-    p.own = few(span + per_row * rows, all / rows + std::min(samples, n_q), samples * ceil_div(mean, rows));
+    // Tiles at most: those of every query by itself, or all rows' and one more a
+    // sample; then an odd number, so that those that there are, the first, meet all
+    // XCDs (4 samples of 4 rows over 8k keys, 16 heads on 4: 18.6 us, with 8 22.0; one
+    // of 16 rows over 30k keys 31, with 8 41).
+    const int64_t each = n_q * ceil_div(group, rows);
+    p.own = few(span + per_row * rows, std::min(each, (all / rows + std::min(samples, n_q)) | 1),
+                samples * ceil_div(mean, rows));
   } else {
     p.own = many_cut(all, samples, k_heads, span, per_row, dim, elem);
     p.own.tiles = all / (128 * p.own.wave_rows) + std::min(samples, n_q);

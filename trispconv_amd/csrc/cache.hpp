@@ -72,8 +72,19 @@ constexpr int many_buffers(int row_bytes) { return row_bytes <= 192 ? 3 : 2; }
 constexpr int many_per_cu(int row_bytes, int row_blocks) {
   return row_bytes <= 128 ? 4 - row_blocks : row_bytes <= 256 ? 2 : 1;
 }
-// Rows of a tile in 16s at most: queries and sums stay in the registers.
-constexpr int cache_row_blocks(int row_bytes) { return row_bytes <= 256 ? 4 : row_bytes <= 512 ? 2 : 1; }
+// Waves a SIMD that the compiler leaves registers for.  With two, a wave's half of the
+// file holds the products' sums as well; a wave with all of it keeps them in the
+// other half and moves them over and back for every tile (few rows, `values` a lane
+// of a quarter: 8 samples of 16 rows over 32k keys, 16 heads on 4 of 64, bf16, 92 us,
+// before 154; 4 x 1000 keys 11.4, before 12.1; four samples of 512 rows over 8k keys,
+// heads of 128, f32, 1057 us, before 1097).  More do not fit (16 rows, heads of 256,
+// bf16: 532 us, in half the file 2855).
+constexpr int few_per_simd(int values) { return values <= 384 ? 2 : 1; }
+constexpr int many_per_simd(int dim, int per_cu) { return dim <= 128 && per_cu < 2 ? 2 : per_cu; }
+// Rows of a tile in 16s at most: queries and sums stay in the registers (8 samples of
+// 16 rows over 32k keys, 16 heads on 4: of 128, bf16, 199 us in 32s, 203 in 64s; of 64,
+// f32, 271 and 324; of 256, bf16, 532 in 32s, 636 in 16s).
+constexpr int cache_row_blocks(int row_bytes) { return row_bytes <= 192 ? 4 : row_bytes <= 512 ? 2 : 1; }
 
 namespace {
 
@@ -745,7 +756,7 @@ __device__ __forceinline__ void cache_few(const CacheArgs& a, const CacheCut& cu
 }
 
 template <typename T, int DP, int NR, bool ALIGNED>
-__global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)), (cache_waves(DP * sizeof(T)) + 3) / 4)
+__global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)), few_per_simd(NR * DP))
     cache_few_kernel(CacheArgs a, CacheCut prefix, CacheCut own, int splits) {
   extern __shared__ __align__(16) char lds[];
   const int64_t prefix_blocks = prefix.tiles * a.k_heads * prefix.splits;
@@ -904,7 +915,7 @@ __device__ __forceinline__ void cache_many(const CacheArgs& a, const CacheCut& c
 }
 
 template <typename T, int DP, int RB, int KB, bool ALIGNED>
-__global__ void __launch_bounds__(kWave * 4, many_per_cu(DP * sizeof(T), RB))
+__global__ void __launch_bounds__(kWave * 4, many_per_simd(DP, many_per_cu(DP * sizeof(T), RB)))
     cache_tile_kernel(CacheArgs a, CacheCut cut, int is_prefix, int splits) {
   extern __shared__ __align__(16) char lds[];
   cache_many<T, DP, RB, KB, ALIGNED>(a, cut, is_prefix, splits, lds);
