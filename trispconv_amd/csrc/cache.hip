@@ -78,6 +78,9 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     c.tiles = tiles;
     c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), kt * cache_waves(row_bytes)));
     c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
+    // (the table may have room for far more than is kept, in a captured step above all:
+    // 4 x 4000 keys with room for 65536 each, 10.7 us, in parts of 2048 19.9)
+    if (c.splits > 1 && c.splits <= want) c.chunk = -1;
     return c;
   };
   if (mean <= 64) {

@@ -34,7 +34,7 @@ struct CacheCut {
   int64_t tiles = 0;
   int splits = 0, first_split = 0;
   int wave_rows = 0;  // rows of a workgroup of four waves in 128s, 0: the form for few rows
-  int chunk = 0;      // that form's keys of a part
+  int chunk = 0;      // that form's keys of a part; -1: a tile's shared out evenly, 256 at least
 };
 struct CachePlan {
   int row_blocks = 1;  // that form's rows of a tile in 16s
@@ -465,7 +465,12 @@ __device__ __forceinline__ void cache_few(const CacheArgs& a, const CacheCut& cu
   // the window's tiles begin where pages of whole tiles have theirs
   const int tiles = w.place(lo_min, hi_max, from, to, KT, a.pages.page_rows % KT == 0 ? KT : 1);
   // this chunk's tiles, and this wave's
-  const int chunk_tiles = cut.chunk / KT, c0 = min(split * (int64_t)chunk_tiles, (int64_t)tiles);
+  int chunk_tiles = cut.chunk / KT;
+  if (cut.chunk < 0) {
+    const float share = static_cast<float>(tiles) * __builtin_amdgcn_rcpf(static_cast<float>(cut.splits * WAVES));
+    chunk_tiles = max(static_cast<int>(ceilf(share)) * WAVES, 256 / KT / WAVES * WAVES);
+  }
+  const int c0 = min(split * (int64_t)chunk_tiles, (int64_t)tiles);
   const int c1 = split == cut.splits - 1 ? tiles : min(c0 + chunk_tiles, tiles), each = (c1 - c0 + WAVES - 1) / WAVES;
   const int t0 = min(c0 + wave * each, c1), t1 = min(t0 + each, c1);
   auto item_of = [&](uint32_t r) { return (w.q0 + w.token(r)) * a.q_heads + w.head(r); };
