@@ -75,7 +75,7 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     if (!prefix_rows && keys <= 1024) chunk = keys;
     // (and no more than 16 rounds are worth their parts' memory)
     chunk = std::max({chunk, ceil_div(keys, kMostSplits / 2), ceil_div(keys, std::max<int64_t>(1, 16 * slots / lists))});
-    c.tiles = tiles;
+    c.tiles = static_cast<int>(std::min<int64_t>(tiles, 1 << 30));  // (more than a launch takes)
     c.chunk = static_cast<int>(align_up(std::max<int64_t>(chunk, 1), kt * cache_waves(row_bytes)));
     c.splits = static_cast<int>(std::max<int64_t>(1, ceil_div(keys, c.chunk)));
     // (the table may have room for far more than is kept, in a captured step above all:
@@ -93,19 +93,19 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
                 samples * ceil_div(mean, rows));
   } else {
     p.own = many_cut(all, samples, k_heads, span, per_row, dim, elem);
-    p.own.tiles = all / (128 * p.own.wave_rows) + std::min(samples, n_q);
+    p.own.tiles = static_cast<int>(std::min<int64_t>(all / (128 * p.own.wave_rows) + std::min(samples, n_q), 1 << 30));
   }
   if (prefix_rows && all <= 64) {
     p.prefix = few(prefix_rows, ceil_div(all, rows), ceil_div(all, rows));
   } else if (prefix_rows && mean <= 64 && row_bytes <= 128) {
     // beside the samples' own keys (cache_both_kernel), one workgroup a CU and 512
     // keys at least: 32k keys in 8 tiles 42 us in 32 parts, 45 in 64, 61 in 128
-    p.prefix.wave_rows = 1, p.prefix.tiles = ceil_div(all, 128);
+    p.prefix.wave_rows = 1, p.prefix.tiles = static_cast<int>(ceil_div(all, 128));
     p.prefix.splits = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>({prefix_rows / 512, kCus / (p.prefix.tiles * k_heads), kMostSplits / 2})));
+        1, std::min<int64_t>({prefix_rows / 512, kCus / ((int64_t)p.prefix.tiles * k_heads), kMostSplits / 2})));
   } else if (prefix_rows) {
     p.prefix = many_cut(all, 1, k_heads, prefix_rows, 0, dim, elem);
-    p.prefix.tiles = ceil_div(all, 128 * p.prefix.wave_rows);
+    p.prefix.tiles = static_cast<int>(ceil_div(all, 128 * p.prefix.wave_rows));
   }
   p.own.first_split = p.prefix.splits;
   return p;

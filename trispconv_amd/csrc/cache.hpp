@@ -31,8 +31,7 @@ struct CacheArgs : AttendArgs {
 // How the prefix's or the samples' own keys are cut: tiles of query rows (at
 // most), and parts of the keys, numbered from first_split on.
 struct CacheCut {
-  int64_t tiles = 0;
-  int splits = 0, first_split = 0;
+  int tiles = 0, splits = 0, first_split = 0;
   int wave_rows = 0;  // rows of a workgroup of four waves in 128s, 0: the form for few rows
   int chunk = 0;      // that form's keys of a part; -1: a tile's shared out evenly, 256 at least
 };
@@ -432,7 +431,7 @@ struct PagedStager {
 // against f32: the walk is bound by memory, and the products are idle.
 template <typename T, int DP, int NR, bool ALIGNED>
 __device__ __forceinline__ void cache_few(const CacheArgs& a, const CacheCut& cut, bool is_prefix, int splits,
-                                          int64_t id, char* lds) {
+                                          uint32_t id, char* lds) {
   constexpr int RB = DP * sizeof(T), KT = cache_keys(RB), WAVES = cache_waves(RB), KB = KT / 16;
   constexpr int STEPS = RB / 64, DB = DP / 16, TILE = cache_tile(RB), ROWS = 16 * NR, BUFFERS = cache_buffers(RB);
   using Stager = PagedStager<T, DP, KT, ALIGNED>;
@@ -451,12 +450,13 @@ __device__ __forceinline__ void cache_few(const CacheArgs& a, const CacheCut& cu
   };
 
   // rows next to each other, then heads, then chunks
-  const int split = static_cast<int>(id / cut.tiles / a.k_heads);
+  const uint32_t rest = id / cut.tiles;
+  const int split = rest / a.k_heads;
   CacheWalk w;
   w.group = a.q_heads / a.k_heads;
-  w.hk = static_cast<int>(id / cut.tiles % a.k_heads);
+  w.hk = rest - split * a.k_heads;
   int from, to;
-  if (!w.begin(a, is_prefix, ROWS, static_cast<int>(id % cut.tiles), from, to)) return zero_others();
+  if (!w.begin(a, is_prefix, ROWS, id - rest * cut.tiles, from, to)) return zero_others();
   const uint32_t row0 = w.row0;
 
   // rows past the last are copies of it
@@ -764,7 +764,7 @@ template <typename T, int DP, int NR, bool ALIGNED>
 __global__ void __launch_bounds__(kWave* cache_waves(DP * sizeof(T)), few_per_simd(NR * DP))
     cache_few_kernel(CacheArgs a, CacheCut prefix, CacheCut own, int splits) {
   extern __shared__ __align__(16) char lds[];
-  const int64_t prefix_blocks = prefix.tiles * a.k_heads * prefix.splits;
+  const uint32_t prefix_blocks = prefix.tiles * a.k_heads * prefix.splits;
   const bool is_prefix = blockIdx.x < prefix_blocks;
   cache_few<T, DP, NR, ALIGNED>(a, is_prefix ? prefix : own, is_prefix, splits,
                                 blockIdx.x - (is_prefix ? 0 : prefix_blocks), lds);
@@ -879,20 +879,21 @@ __device__ __forceinline__ void cache_many(const CacheArgs& a, const CacheCut& c
   // with 65 for 64 places 467).
   CacheWalk w;
   w.group = a.q_heads / a.k_heads;
-  const int64_t there = is_prefix ? cut.tiles : count_tiles(a, w.group, ROWS), units = there * a.k_heads;
+  const uint32_t there = is_prefix ? cut.tiles : min(count_tiles(a, w.group, ROWS), (int64_t)cut.tiles);
+  const uint32_t units = there * a.k_heads;
   // Of the host's parts as many as make the fewest rounds of them (a_cu: a CU's).
   int parts = is_prefix ? cut.splits : 1;
-  int64_t a_cu = (units + 255) / 256;
+  uint32_t a_cu = (units + 255) / 256;
   for (int n = 2; n <= cut.splits && !is_prefix; ++n) {
-    const int64_t next = (units * n + 255) / 256, per_cu = many_per_cu(DP * sizeof(T), RB);
+    const uint32_t next = (units * n + 255) / 256, per_cu = many_per_cu(DP * sizeof(T), RB);
     if ((next + per_cu - 1) / per_cu * parts < (a_cu + per_cu - 1) / per_cu * n) parts = n, a_cu = next;
   }
-  const int64_t blocks = units * parts, per = (blocks + 7) / 8;
-  int64_t id = blockIdx.x / 8 < per ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+  const uint32_t blocks = units * parts, per = (blocks + 7) / 8;
+  uint32_t id = blockIdx.x / 8 < per ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
   if (id >= units * cut.splits) return;
   const bool idle = id >= blocks;  // a part that is not made says so
   if (idle) id -= blocks;
-  const int64_t rest = id / there;
+  const uint32_t rest = id / there;
   const int split = static_cast<int>(idle ? parts + rest / a.k_heads : rest % parts);
   w.hk = static_cast<int>(idle ? rest % a.k_heads : rest / parts);
   w.split = cut.first_split + split;
@@ -961,7 +962,7 @@ int launch_many(const CacheArgs& a, const CacheCut& c, bool is_prefix, int split
   auto kernel = &cache_tile_kernel<T, DP, RB, KB, ALIGNED>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
-  const int64_t blocks = align_up(c.tiles * a.k_heads * c.splits, 8);
+  const int64_t blocks = align_up((int64_t)c.tiles * a.k_heads * c.splits, 8);
   TSC_REQUIRE(blocks * kWave * 4 < (1ll << 32), "cache_attention: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * 4, bytes, s>>>(a, c, is_prefix, splits);
   TSC_LAUNCH_CHECK("cache_attention");
@@ -975,7 +976,7 @@ int launch_few(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
   const CacheCut prefix = p.prefix.wave_rows ? CacheCut{} : p.prefix, own = p.own.wave_rows ? CacheCut{} : p.own;
-  const int64_t blocks = (prefix.tiles * prefix.splits + own.tiles * own.splits) * a.k_heads;
+  const int64_t blocks = ((int64_t)prefix.tiles * prefix.splits + (int64_t)own.tiles * own.splits) * a.k_heads;
   TSC_REQUIRE(blocks * kWave * WAVES < (1ll << 32), "cache_attention: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * WAVES, bytes, s>>>(a, prefix, own, p.splits());
   TSC_LAUNCH_CHECK("cache_attention");
@@ -988,8 +989,8 @@ int launch_both(const CacheArgs& a, const CachePlan& p, hipStream_t s) {
   auto kernel = &cache_both_kernel<T, DP, NR, ALIGNED>;
   if (bytes > 65536)
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes)) return rc;
-  const int64_t first = align_up(p.prefix.tiles * a.k_heads * p.prefix.splits, 8);
-  const int64_t blocks = first + p.own.tiles * a.k_heads * p.own.splits;
+  const int64_t first = align_up((int64_t)p.prefix.tiles * a.k_heads * p.prefix.splits, 8);
+  const int64_t blocks = first + (int64_t)p.own.tiles * a.k_heads * p.own.splits;
   TSC_REQUIRE(blocks * kWave * 4 < (1ll << 32), "cache_attention: too many tiles");
   kernel<<<static_cast<unsigned>(blocks), kWave * 4, bytes, s>>>(a, p.prefix, p.own, p.splits(),
                                                                  static_cast<int>(first));
