@@ -68,6 +68,31 @@ def test_rows_a_step(rows, dtype):
         _check([rows] * 3, [rows + 500, rows + 1, rows], 4, 2, 64, dtype, 64, window, sinks)
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.float16, 32), (torch.bfloat16, 64),
+                                       (torch.bfloat16, 128), (torch.float32, 256)])
+@pytest.mark.parametrize("lq,lk,prefix", [([1, 1, 1, 1, 0], [2600, 1, 700, 257, 300], 0),
+                                          ([3, 0, 16], [513, 20, 1500], 0), ([1, 2], [900, 300], 4)])
+def test_tables_with_far_more_room(dtype, dim, lq, lk, prefix):
+    """Parts follow what is kept, not the 40,000 positions that the table has room for."""
+    q, k, v, table = _case(lq, lk, 4, 2, dim, dtype, 32, prefix)
+    wide = torch.full((len(lk), 1250), 1 << 30, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    for window, sinks in (((None, 0), 0), ((400, 0), 5)):
+        say("cache_attention, room", lq, lk, dim, dtype, prefix, window, sinks)
+        check(_run(q, k, v, wide, lq, lk, window, sinks, prefix),
+              *attend_pages64(q, k, v, table, lq, lk, window, sinks), what=f"{lq} {lk} {window}")
+
+
+@pytest.mark.parametrize("samples,rows,keys,hq,hk,dim", [(1, 16, 5000, 16, 4, 64), (4, 4, 900, 16, 4, 64),
+                                                         (4, 2, 700, 32, 2, 96), (3, 16, 600, 16, 4, 128),
+                                                         (2, 32, 600, 4, 2, 256), (9, 5, 333, 24, 3, 32)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tiles_of_some_rows(samples, rows, keys, hq, hk, dim, dtype):
+    """Tiles of 16, 32 and 64 rows, whole and not, of one sample and of several."""
+    _check([rows] * samples, [keys - 7 * b for b in range(samples)], hq, hk, dim, dtype, 64)
+    _check([rows, *[1] * (samples - 1)], [keys] * samples, hq, hk, dim, dtype, 64, window=(300, 2), sinks=9)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("window,sinks", [((None, None), 0), ((0, 0), 0), ((63, 0), 0), ((64, 0), 16),
                                           ((100, 0), 70), ((100, 0), 1000), ((5, None), 2),
