@@ -64,7 +64,8 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
   // a CU to itself), one round of workgroups where that allows it: 64 samples of up
   // to 32k keys in parts of 2048 276 us, of 512 321, of 8192 295; 24 windows of
   // 4096 in one round of 1024 27 us, in two of 768 30.  Up to 1024 keys by
-  // themselves are not worth a join (13 us, in parts 17).
+  // themselves are not worth a join (4 x 1000: 12 us, in parts 10 on the GPU, but the
+  // host takes 16 with the second launch and the workspace).
   auto few = [&](int64_t keys, int64_t tiles, int64_t units) {
     CacheCut c;
     if (sinks > 0) keys += kt;  // (a tile of their own)

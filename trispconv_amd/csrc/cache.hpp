@@ -421,7 +421,7 @@ struct PagedStager {
 // at the end.  Bound by memory: 64 samples of 14k to 33k keys, 16 heads on 4 of 64,
 // bf16, 1.53 GB in 276 us, 5.5 TB/s (a large copy on this card: 4.87).  Small
 // calls are bound by what comes before the first tile: arguments, offsets, page
-// numbers and keys are dependent reads, 4 of the 12 us of 4 x 900 keys.
+// numbers and keys are dependent reads, 6 of the 11 us of 4 x 900 keys.
 //
 // Scores are kept transposed as in attend.hpp, S^T = K Q^T, in 16x16 tiles: a lane
 // has four keys of one row per 16, which are, as they stand, the right operand of
@@ -859,8 +859,8 @@ struct PagedTiles {
 
 // Many query rows: attend_walk's tiles, over pages.  lds: as attend_kernel's.  Bound
 // as attend_walk is, by vector instructions and products that overlap little: 2 x
-// 2048 rows over 32k keys, 16 heads on 4, bf16, 1153 us with heads of 128 (0.88
-// PFLOP/s; a library product's rate on this card 1.13), 616 us with heads of 64 (0.82).
+// 2048 rows over 32k keys, 16 heads on 4, bf16, 1123 us with heads of 128 (0.90
+// PFLOP/s; a library product's rate on this card 1.13), 594 us with heads of 64 (0.85).
 template <typename T, int DP, int RB, int KB, bool ALIGNED>
 __device__ __forceinline__ void cache_many(const CacheArgs& a, const CacheCut& cut, bool is_prefix, int splits,
                                            char* lds) {
