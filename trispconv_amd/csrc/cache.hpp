@@ -223,7 +223,7 @@ struct CacheWalk : Walk {
       const int64_t t = q0 + token(r);
       const int s = first_past(a.off_q, a.samples, t);
       keys = kept(*args, s);
-      p = position(t, a.off_q[s + 1], keys);
+      p = position(a, t, a.off_q[s + 1], keys);
     }
     seen_keys(p, keys, a.left, a.right, a.sinks, lo, hi, sink);
   }
@@ -255,7 +255,7 @@ struct CacheWalk : Walk {
     for (int x = 0; x < N; ++x) {
       int sink;
       const int keys = args->pages.cut(length[x]);
-      seen_keys(position(t[x], end[x], keys), keys, a.left, a.right, a.sinks, lo[x], hi[x], sink);
+      seen_keys(position(a, t[x], end[x], keys), keys, a.left, a.right, a.sinks, lo[x], hi[x], sink);
       lo_first = min(lo_first, lo[x]), lo_last = max(lo_last, lo[x]);
       hi_first = min(hi_first, hi[x]), hi_last = max(hi_last, hi[x]);
     }
@@ -267,8 +267,10 @@ struct CacheWalk : Walk {
     lo_first = __builtin_amdgcn_readfirstlane(lo_first), lo_last = __builtin_amdgcn_readfirstlane(lo_last);
     hi_first = __builtin_amdgcn_readfirstlane(hi_first), hi_last = __builtin_amdgcn_readfirstlane(hi_last);
   }
-  __device__ static __forceinline__ int position(int64_t t, int end, int keys) {
-    return static_cast<int>(max(t - end + keys, -(int64_t)(1 << 30)));
+  // Row t's position in a sample whose rows end at `end`, or with the call's (as
+  // sample_range has them).
+  __device__ static __forceinline__ int position(const AttendArgs& a, int64_t t, int end, int keys) {
+    return static_cast<int>(max(t - min((int64_t)end, a.n_q) + keys, -(int64_t)(1 << 30)));
   }
   // Takes the x-th tile of `tile_rows` rows (the prefix's: of all samples) and the
   // range of keys [from, to) of this part.  false: past the last tile.

@@ -61,7 +61,8 @@ __device__ __forceinline__ Place place_of(const RotateArgs& a, int64_t first, in
   int at[1], end[1], length[1];
   const int begin = a.offsets[0];
   samples_of<1>(a.offsets, a.pages.lengths, a.pages.samples, first, last, t, at, end, length);
-  const int64_t pos = (int64_t)length[0] - (end[0] - r);
+  // (an end past the last row is cut to it)
+  const int64_t pos = (int64_t)length[0] - (min((int64_t)end[0], a.n) - r);
   if (r < begin || r >= end[0] || pos < 0 || pos >= a.pages.most()) return Place{-1, 0};
   const uint32_t p = a.pages.page_of(static_cast<uint32_t>(pos));
   const int32_t page = a.pages.table[at[0] * a.pages.table_row + p];
