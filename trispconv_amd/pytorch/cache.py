@@ -276,10 +276,11 @@ class VoxelCache:
         """Room for ``rows[b]`` new rows behind what sample b keeps, for instance
         ``order.offsets.diff()``.  A ValueError leaves everything as it was."""
         self._check_steps()
-        rows = rows.tolist() if isinstance(rows, torch.Tensor) else [int(n) for n in rows]
-        if len(rows) != self.samples or any(n < 0 for n in rows):
+        rows = rows.tolist() if isinstance(rows, torch.Tensor) else list(rows)
+        new_rows = [int(n) for n in rows]
+        if len(rows) != self.samples or any(n < 0 or n != r for n, r in zip(new_rows, rows)):
             raise ValueError(f"VoxelCache: {rows} new rows for {self.samples} samples")
-        kept = [a + b for a, b in zip(self._kept, rows)]
+        kept = [a + b for a, b in zip(self._kept, new_rows)]
         if max(kept) > self.positions:
             raise ValueError(f"VoxelCache: {max(kept)} rows of a sample, it has room for "
                              f"{self.positions}")
