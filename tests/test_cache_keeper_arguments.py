@@ -27,3 +27,24 @@ def test_whole_rows_of_any_type_count_as_integers():
     assert all(type(n) is int for n in c.rows())
     c.extend([9, 0, 0])
     assert c.rows() == [14, 2, 10] and c.free_pages() == 3
+
+
+def test_samples_and_rows_as_tensors():
+    """Elements of tensors name samples and rows as integers do: the same twice is
+    found, and nothing of the keeper changes with a tensor later."""
+    c = _cache()
+    c.extend([16, 0, 0])
+    with pytest.raises(ValueError):
+        c.share(0, torch.tensor([1, 1]), 8)
+    assert c.rows() == [16, 0, 0] and c.free_pages() == 6
+    rows = torch.tensor([8, 8])
+    c.share(torch.tensor(0), torch.tensor([1, 2]), rows[0])
+    rows += 5
+    assert c.rows() == [16, 8, 8] and all(type(n) is int for n in c.rows())
+    c.extend([0, 1, 0])
+    c.drop(torch.tensor([0, 2]))
+    assert c.rows() == [0, 9, 0] == c.lengths.tolist() and c.free_pages() == 6
+    for bad in ((0.5, [1], 8), (1, [0.0], 8), (1, [0], 8.0)):
+        with pytest.raises(TypeError):
+            c.share(*bad)
+    assert c.rows() == [0, 9, 0] and c.free_pages() == 6

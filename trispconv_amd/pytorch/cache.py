@@ -15,6 +15,7 @@ them; a VoxelBlock called with one streams.
 """
 from __future__ import annotations
 
+from operator import index
 from typing import Callable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -260,7 +261,7 @@ class VoxelCache:
                                "captured step, not in it")
 
     def _check_samples(self, samples: Sequence[int]) -> List[int]:
-        samples = list(samples)
+        samples = [index(b) for b in samples]
         if any(not 0 <= b < self.samples for b in samples):
             raise ValueError(f"VoxelCache: samples {samples}, there are {self.samples}")
         return samples
@@ -301,7 +302,8 @@ class VoxelCache:
         """Lets samples that keep nothing begin with the first ``rows`` rows of
         ``source``, in the same pages: whole pages, so a multiple of page_rows."""
         self._check_steps()
-        targets = self._check_samples([source, *targets])[1:]
+        source, *targets = self._check_samples([source, *targets])
+        rows = index(rows)
         if rows % self.page_rows or not 0 <= rows <= self._kept[source]:
             raise ValueError(f"VoxelCache: {rows} rows of sample {source}, which keeps "
                              f"{self._kept[source]}, are not whole pages of {self.page_rows}")
