@@ -13,8 +13,9 @@ pytestmark = [pytest.mark.gpu, needs_gpu]
 
 @pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.float32, 64), (torch.bfloat16, 32)])
 @pytest.mark.parametrize("lq", [[2], [1, 2], [7, 1, 31], [100, 40]])
+@pytest.mark.parametrize("unseen", [1.0, float("nan")])
 @pytest.mark.parametrize("prefix", [0, 2])
-def test_attention(prefix, lq, dtype, dim):
+def test_attention(prefix, unseen, lq, dtype, dim):
     """The last sample's offset is past the last row, the first one's before the
     first: with a prefix (read for all rows at once) and without, what those of
     the rows that there are say."""
@@ -25,6 +26,8 @@ def test_attention(prefix, lq, dtype, dim):
     table, pages = tables(lk, page, prefix)
     q = torch.randn(sum(lq), 4, dim, generator=g).to(dtype)
     k, v = (torch.randn(pages, page, 2, dim, generator=g).to(dtype) for _ in range(2))
+    if prefix:
+        k[table[0, 1], 80 - page], v[table[0, 1], 80 - page] = unseen, unseen
     want = attend_pages64(q, k, v, table, lq, lk, (40, 0), 3)
     for past in (0, 3, 1 << 20):
         off = offsets_of(lq)

@@ -208,7 +208,11 @@ __device__ __forceinline__ bool find_rows(const CacheArgs& a, int group, int row
 // The query rows of one sample, or of all of them, each with a position of its own.
 struct CacheWalk : Walk {
   const CacheArgs* args;
-  int b;  // the sample; -1: all
+  // The sample; -1: all, and lk is where their rows end: what the offsets name past
+  // that is cut off, as sample_range does.  (The arguments' n_q instead takes
+  // cache_tile_kernel scalar registers in the walk: 512 to 2 rows over 15k to 20k
+  // keys 136 us, with lk 128.)
+  int b;
   __device__ __forceinline__ int token(uint32_t r) const {
     r = min(r, rows - 1);
     const uint32_t t = __umulhi(r, args->group_mul);
@@ -223,7 +227,7 @@ struct CacheWalk : Walk {
       const int64_t t = q0 + token(r);
       const int s = first_past(a.off_q, a.samples, t);
       keys = kept(*args, s);
-      p = position(a, t, a.off_q[s + 1], keys);
+      p = position(t, min(a.off_q[s + 1], lk), keys);
     }
     seen_keys(p, keys, a.left, a.right, a.sinks, lo, hi, sink);
   }
@@ -255,7 +259,7 @@ struct CacheWalk : Walk {
     for (int x = 0; x < N; ++x) {
       int sink;
       const int keys = args->pages.cut(length[x]);
-      seen_keys(position(a, t[x], end[x], keys), keys, a.left, a.right, a.sinks, lo[x], hi[x], sink);
+      seen_keys(position(t[x], min(end[x], lk), keys), keys, a.left, a.right, a.sinks, lo[x], hi[x], sink);
       lo_first = min(lo_first, lo[x]), lo_last = max(lo_last, lo[x]);
       hi_first = min(hi_first, hi[x]), hi_last = max(hi_last, hi[x]);
     }
@@ -267,10 +271,9 @@ struct CacheWalk : Walk {
     lo_first = __builtin_amdgcn_readfirstlane(lo_first), lo_last = __builtin_amdgcn_readfirstlane(lo_last);
     hi_first = __builtin_amdgcn_readfirstlane(hi_first), hi_last = __builtin_amdgcn_readfirstlane(hi_last);
   }
-  // Row t's position in a sample whose rows end at `end`, or with the call's (as
-  // sample_range has them).
-  __device__ static __forceinline__ int position(const AttendArgs& a, int64_t t, int end, int keys) {
-    return static_cast<int>(max(t - min((int64_t)end, a.n_q) + keys, -(int64_t)(1 << 30)));
+  // Row t's position in a sample whose rows end at `end`.
+  __device__ static __forceinline__ int position(int64_t t, int end, int keys) {
+    return static_cast<int>(max(t - end + keys, -(int64_t)(1 << 30)));
   }
   // Takes the x-th tile of `tile_rows` rows (the prefix's: of all samples) and the
   // range of keys [from, to) of this part.  false: past the last tile.
@@ -281,7 +284,7 @@ struct CacheWalk : Walk {
       int64_t last;
       sample_rows(a, q0, last);
       rows = static_cast<uint32_t>((last - q0) * group);
-      b = -1, lk = shift = 0, from = 0, to = a.prefix_rows();
+      b = -1, lk = static_cast<int>(last), shift = 0, from = 0, to = a.prefix_rows();
       if ((int64_t)tile * tile_rows >= rows) return false;
     } else {
       int lq;
