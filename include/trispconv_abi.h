@@ -523,13 +523,14 @@ TSC_API int tsc_window_attention(const void* q, int64_t q_row, int64_t q_head, c
  * int32; table_pages entries a sample), and lengths[b] (device int32) is how
  * many positions the sample has, its new rows among them: of the Lq rows
  * offsets[b] .. offsets[b+1] (as above) row i stands at position
- * lengths[b] - Lq + i.  Lengths over the table's room, or negative, are cut.
+ * lengths[b] - Lq + i.
  *
  * tsc_norm_rotate_append is tsc_norm_rotate_heads with the keys written to their
  * rows of k_pages, and the values v (n, k_heads, dim; copied as they are) to
  * those of v_pages.  Nothing else of the pages is written.  A row of no sample,
- * or one whose position or page there is not, writes its q_out only.  No two
- * samples' new rows may share a page's row.
+ * or one whose position or page there is not, writes its q_out only: a length
+ * over the table's room is taken as it is, and rows past the room are left out.
+ * No two samples' new rows may share a page's row.
  * ------------------------------------------------------------------------ */
 TSC_API int tsc_norm_rotate_append(
     const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
@@ -544,10 +545,15 @@ TSC_API int tsc_norm_rotate_append(
 
 /* tsc_window_attention of the new rows q (n_q, q_heads, dim) over what their
  * samples keep: query i of Lq stands at p = i + Lk - Lq of its sample's Lk =
- * lengths[b] positions.  prefix_pages > 0: the first prefix_pages * page_rows
- * positions of every sample are the pages prefix[0 ..] (device int32; these
- * entries of the table are not read), and are read once for all samples.  Pages
- * that a query sees have to be there; other numbers are cut to those there are.
+ * lengths[b] positions; a length over the table's room, or negative, is cut
+ * first.  prefix_pages > 0: the first prefix_pages * page_rows positions of every
+ * sample are the pages prefix[0 ..] (device int32; these entries of the table are
+ * not read), and are read once for all samples.  Pages that a query sees have to
+ * be there; other numbers are cut to those there are.  For f16 and bf16 the
+ * softmax weights are rounded to the type for the product with the values where a
+ * sample has over 64 rows (queries times the heads that share a key head) in the
+ * mean, and for a prefix of over 64 such rows in all; with fewer they are two
+ * values of the type.
  * Rows of out before the first sample and behind the last are 0.
  * `longest` of the workspace query: table_pages * page_rows; its prefix_rows:
  * prefix_pages * page_rows. */

@@ -20,7 +20,9 @@ constexpr int kCus = 256;
 // gains up to 30%; more parts have more sums to write and join.  20k keys, 18
 // tiles of 256 rows on 4 heads: 128 us in seven parts of one round, 155 in eight;
 // 141 with 128 rows.  2 x 32k keys, 64 tiles: 615 us in two parts, 833 in one
-// (half the slots), 671 with 128 rows.
+// (half the slots), 671 with 128 rows.  Parts have 512 keys at least, which leaves
+// CUs idle over short caches (4 x 17 rows, 16 heads on 4 of 64: 1000 keys 23 us in 16
+// workgroups, 4000 keys 24; shorter parts are not measured).
 CacheCut many_cut(int64_t rows, int64_t lists, int64_t heads, int64_t keys_of_row, int64_t keys_per_tile_row, int dim, int elem) {
   const int row_bytes = padded_dim(dim) * elem;
   CacheCut best;
@@ -84,6 +86,11 @@ CachePlan cache_plan(int64_t samples, int64_t n_q, int64_t longest, int64_t pref
     if (c.splits > 1 && c.splits <= want) c.chunk = -1;
     return c;
   };
+  // One form for all samples, by their mean rows.  On the border, 4 samples of 16 and
+  // of 17 rows, 16 heads on 4 of 64, over 300, 1000 and 4000 keys: bf16 16, 24 and 25
+  // us, and 15, 23 and 24; f32 17, 32 and 44, and 31, 48 and 54 (a tile of 128 rows
+  // half full).  Rows far from the mean pay for it: one sample of 2048 rows and 63 of
+  // one over 32k keys take 1152 us, by themselves 333 and 365.
   if (mean <= 64) {
     // Tiles at most: those of every query by itself, or all rows' and one more a
     // sample; then an odd number, so that those that there are, the first, meet all

@@ -432,8 +432,10 @@ struct PagedStager {
 // has four keys of one row per 16, which are, as they stand, the right operand of
 // O^T = V^T e^S^T.  A row's reference is the largest of its first tile's scores and
 // moves only when weights outgrow it (kMostWeight).  Weights of 16-bit tensors go
-// into the product as two parts (value and remainder), so that they lose nothing
-// against f32: the walk is bound by memory, and the products are idle.
+// into the product as two parts, value and remainder, which leave out 2^-16 of a
+// bf16 weight and 2^-22 of an f16 one at most: errors against 64 bits are those of
+// f32 weights (bf16 0.0017), with one part 0.0024.  The walk is bound by memory, and
+// the products are idle.
 template <typename T, int DP, int NR, bool ALIGNED>
 __device__ __forceinline__ void cache_few(const CacheArgs& a, const CacheCut& cut, bool is_prefix, int splits,
                                           uint32_t id, char* lds) {
@@ -914,7 +916,9 @@ __device__ __forceinline__ void cache_many(const CacheArgs& a, const CacheCut& c
     return;
   }
   int lo_first = 0, hi_first, lo_last, hi_last = to;
-  // (the rows of all samples: every key of the prefix, most of them see it whole)
+  // (the rows of all samples: every key of the prefix, most of them see it whole.  In
+  // a window they walk it whole too: 64 samples of one row behind 32k shared keys, 16
+  // heads on 4 of 64, a window of 4096, 45 us, without a shared prefix 31)
   if (!is_prefix) w.bounds(a, w.row0, w.row0 + ROWS - 1, lo_first, hi_first, lo_last, hi_last);
   const int tiles = w.place(lo_first, hi_last, from, to, KT, a.pages.page_rows % Tiles::UNIT == 0 ? KT : 1);
   const int each = (tiles + parts - 1) / parts;

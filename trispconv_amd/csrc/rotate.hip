@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(256) rotate_any_kernel(RotateArgs a, int lp) {
 // 500k rows of 12 + 12 heads of 64, bf16: 607 us, 5.07 TB/s (a large copy on
 // this card: 4.86).  The paged form takes keys and values head by head, so that
 // what it writes of a page lies together (4 x 60k rows of 12 + 12 + 12 heads of
-// 64, f16: 445 us, 4.85 TB/s; row by row 553, and 25 more where each row searched
-// for its sample by itself).
+// 64, f16: 470 us, 4.6 TB/s; row by row a quarter more, and
+// another 25 us where each row searched for its sample by itself).
 constexpr int kRows = 8, kMaxHalf = 128;
 
 template <typename T, int P, int LANES, bool PAGED>

@@ -78,7 +78,8 @@ def norm_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positi
     to offsets[b+1], the last of its lengths[b] positions, and position t is row
     t % R of page table[b, t // R].  offsets (B + 1,), lengths (B,) and table
     (B, pages) are int32 on the GPU.  Nothing else in the pages is written; a row
-    of no sample, or one whose position or page there is not, is written nowhere.
+    of no sample, or one whose position or page there is not, is written nowhere
+    (with a length over the table's room those that are past it).
     No row of a page may be that of two new rows, and no input may lie in the pages.
     """
     what = "norm_rotate_append"
@@ -133,8 +134,15 @@ def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     what they hold, means nothing.  prefix (int32 on the GPU, page numbers):
     every sample's first positions lie in these pages; they are then read once
     for the queries of all samples, and the table's entries for them not at all.
-    A query that sees no key gives zeros, as rows outside every sample do.
-    Scores, maxima and sums are float32.
+    A query that sees no key gives zeros, as rows outside every sample do.  Lengths
+    over the table's room, and negative ones, are cut before anything else.
+
+    Scores, maxima and sums are float32.  For float16 and bfloat16 the softmax
+    weights are rounded to that type for the product with the values where a
+    sample has over 64 rows (queries times Hq / heads) in the mean, and for a
+    prefix of over 64 such rows in all; with fewer they go into it as two values
+    of the type.  The same step may therefore differ in its last bits with and
+    without ``prefix``.
     """
     what = "cache_attention"
     if not q.is_cuda:
@@ -300,7 +308,13 @@ class VoxelCache:
 
     def share(self, source: int, targets: Sequence[int], rows: int) -> None:
         """Lets samples that keep nothing begin with the first ``rows`` rows of
-        ``source``, in the same pages: whole pages, so a multiple of page_rows."""
+        ``source``, in the same pages: whole pages, so a multiple of page_rows.
+
+        Pages that all samples share are read once for all of them.  With over 64
+        rows of queries and heads that share a key head they are read whole, though
+        a window sees less of them: one row each of 64 samples behind 32,768 shared
+        ones takes 45 us, from unshared pages 160; in a window of 4096 45, unshared 31
+        (16 heads on 4 of 64, bf16)."""
         self._check_steps()
         source, *targets = self._check_samples([source, *targets])
         rows = index(rows)
