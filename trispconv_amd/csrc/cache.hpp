@@ -867,7 +867,7 @@ struct PagedTiles {
 // Many query rows: attend_walk's tiles, over pages.  lds: as attend_kernel's.  Bound
 // as attend_walk is, by vector instructions and products that overlap little: 2 x
 // 2048 rows over 32k keys, 16 heads on 4, bf16, 1123 us with heads of 128 (0.90
-// PFLOP/s; a library product's rate on this card 1.13), 594 us with heads of 64 (0.85).
+// PFLOP/s; a library product's rate on this card 1.13), 619 us with heads of 64 (0.82).
 template <typename T, int DP, int RB, int KB, bool ALIGNED>
 __device__ __forceinline__ void cache_many(const CacheArgs& a, const CacheCut& cut, bool is_prefix, int splits,
                                            char* lds) {
